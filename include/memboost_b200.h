@@ -378,6 +378,113 @@ mb_status mb_gptq_quantize_rows(const float* W, int64_t M, int64_t K, int64_t ro
                                 int blocksize, int scalar_division, float* Q_rows,
                                 void* workspace, size_t workspace_bytes, mb_stream_t stream);
 
+/* ---------------------------------------------------------------------------
+ * 8-bit rows and their product -- no counterpart in the reference.
+ *
+ * Rows of activations (tokens) or weights (output channels) are held as
+ * int8 codes with one fp32 scale a row: with a = max_k |x[r, k]|,
+ *   scales[r] = a / 127 rounded to fp32,
+ *   codes[r, k] = x[r, k] / scales[r] rounded to the nearest integer, ties to
+ *                 even, in [-127, 127].
+ * A row with a / 127 = 0 in fp32 has scale 0 and codes 0.  A row that holds a
+ * NaN or an infinity has scale NaN and codes 0: whatever is computed from it
+ * is NaN.
+ * Strides count elements between the starts of rows; codes begin on 16-byte
+ * boundaries (base and stride), every other buffer on its element's size.
+ * ------------------------------------------------------------------------- */
+typedef enum { MB_FP16 = 0, MB_BF16 = 1, MB_FP32 = 2 } mb_dtype;
+
+/* x: [rows, K]; codes: [rows, K] with codes_stride >= K; scales: [rows]. */
+mb_status mb_int8_quantize(const void* x, mb_dtype x_type, int64_t rows, int64_t K,
+                           int64_t x_stride, int8_t* codes, int64_t codes_stride, float* scales,
+                           mb_stream_t stream);
+
+/* out[r, k] = codes[r, k] * scales[r], rounded to fp32 and then to out_type. */
+mb_status mb_int8_dequantize(const int8_t* codes, int64_t codes_stride, const float* scales,
+                             int64_t rows, int64_t K, void* out, mb_dtype out_type,
+                             int64_t out_stride, mb_stream_t stream);
+
+/* Largest K of mb_int8_matmul: 127 * 127 * K stays below 2^31, so the int32
+ * sums are exact. */
+#define MB_INT8_MAX_K 131072
+
+/* out[m, n] = a_scales[m] * b_scales[n] * sum_k a_codes[m, k] b_codes[n, k]
+ *             + bias[n]
+ * (bias may be NULL): a = the tokens, b = the weights (an output channel a
+ * row).  The sum is a whole number and exact; it is rounded to fp32,
+ * multiplied by the two scales and added to the bias in fp32, and rounded
+ * once more to out_type.  If a wait inside the kernel ran out (2 s), the
+ * outputs it concerns are NaN. */
+mb_status mb_int8_matmul(const int8_t* a_codes, int64_t a_stride, const float* a_scales, int64_t M,
+                         const int8_t* b_codes, int64_t b_stride, const float* b_scales, int64_t N,
+                         int64_t K, const void* bias, mb_dtype bias_type, void* out,
+                         mb_dtype out_type, int64_t out_stride, mb_stream_t stream);
+
+/* ---------------------------------------------------------------------------
+ * Quantised key/value cache -- no counterpart in the reference.
+ *
+ * Keys and values live in pages of page_size tokens:
+ *   codes   [pages, kv_heads, page_size, head_dim * bits / 8] bytes
+ *   scales  bits == 8: fp32 [pages, kv_heads, page_size]
+ *           bits == 4: fp16 [pages, kv_heads, page_size, head_dim / 32, 2]
+ * A slot is page * page_size + the token's place in the page.
+ * 8 bits: a token's head is a row as above.  4 bits: each 32 channels have an
+ * fp16 pair (s, m), m = their minimum and s = (maximum - minimum) / 15 rounded
+ * to fp16, and codes (x - m) / s rounded to the nearest, ties to even, in
+ * [0, 15] (0 where s is 0); the even channel is the low half of a byte; a
+ * value reads m + s * code.  32 channels with a NaN or an infinity, or whose
+ * minimum is beyond fp16, read NaN.
+ * Contiguous, 16-byte aligned; page_size a multiple of 16; head_dim a
+ * multiple of 16 (8 bits) or 32 (4 bits), at most 256.
+ * ------------------------------------------------------------------------- */
+typedef struct mb_kv_cache {
+  void* k_codes;
+  void* v_codes;
+  void* k_scales;
+  void* v_scales;
+  int64_t pages;
+  int32_t page_size;
+  int32_t kv_heads;
+  int32_t head_dim;
+  int32_t bits; /* 8 or 4 */
+} mb_kv_cache;
+
+/* Workspace bytes of mb_cache_write (0 for few tokens). */
+size_t mb_cache_write_workspace_size(int64_t tokens);
+
+/* Quantises token t of k and v ([tokens, kv_heads, head_dim], the strides of
+ * tokens and heads in elements, channels contiguous) into slots[t].  Tokens
+ * whose slot is outside [0, pages * page_size) are left out; of several
+ * tokens with the same slot the last one is kept. */
+mb_status mb_cache_write(const mb_kv_cache* cache, const void* k, int64_t k_token_stride,
+                         int64_t k_head_stride, const void* v, int64_t v_token_stride,
+                         int64_t v_head_stride, mb_dtype type, int64_t tokens,
+                         const int64_t* slots, void* workspace, size_t workspace_bytes,
+                         mb_stream_t stream);
+
+/* The values at slots[t], to k_out and v_out ([tokens, kv_heads, head_dim],
+ * contiguous).  A slot outside the cache reads 0. */
+mb_status mb_cache_read(const mb_kv_cache* cache, const int64_t* slots, int64_t tokens,
+                        void* k_out, void* v_out, mb_dtype out_type, mb_stream_t stream);
+
+/* Workspace bytes of mb_cache_attention. */
+size_t mb_cache_attention_workspace_size(const mb_kv_cache* cache, int64_t batch, int64_t heads,
+                                         int64_t table_width);
+
+/* One query token a sequence over the cache:
+ *   out[b, h] = sum_t softmax_t(scale * q[b, h] . k[t]) v[t],  t < lengths[b],
+ * token t at place t % page_size of page page_table[b, t / page_size], its
+ * head h / (heads / kv_heads).  q [batch, heads, head_dim] with strides in
+ * elements (channels contiguous), out contiguous, both of `type` (fp16 or
+ * bf16).  A length beyond the table counts as the table's, tokens of a page
+ * outside [0, pages) are left out, and a sequence with no token gives 0.
+ * scale is finite. */
+mb_status mb_cache_attention(const mb_kv_cache* cache, const void* q, int64_t q_batch_stride,
+                             int64_t q_head_stride, mb_dtype type, int64_t batch, int64_t heads,
+                             const int32_t* page_table, int64_t table_stride,
+                             int64_t table_width, const int32_t* lengths, float scale, void* out,
+                             void* workspace, size_t workspace_bytes, mb_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -100,8 +100,39 @@ _lib.mb_gptq_quantize.restype = ctypes.c_int
 _lib.mb_gptq_quantize.argtypes = [_P, _I64, _I64, _P, _P, ctypes.c_int, ctypes.c_int, _P, _P,
                                   ctypes.c_size_t, _P]
 
+
+
+class KVCache(ctypes.Structure):
+    """mb_kv_cache: a quantised key/value cache's buffers and sizes."""
+    _fields_ = [("k_codes", _P), ("v_codes", _P), ("k_scales", _P), ("v_scales", _P),
+                ("pages", _I64), ("page_size", ctypes.c_int32), ("kv_heads", ctypes.c_int32),
+                ("head_dim", ctypes.c_int32), ("bits", ctypes.c_int32)]
+
+
+_CACHE = ctypes.POINTER(KVCache)
+_lib.mb_int8_quantize.restype = ctypes.c_int
+_lib.mb_int8_quantize.argtypes = [_P, ctypes.c_int, _I64, _I64, _I64, _P, _I64, _P, _P]
+_lib.mb_int8_dequantize.restype = ctypes.c_int
+_lib.mb_int8_dequantize.argtypes = [_P, _I64, _P, _I64, _I64, _P, ctypes.c_int, _I64, _P]
+_lib.mb_int8_matmul.restype = ctypes.c_int
+_lib.mb_int8_matmul.argtypes = [_P, _I64, _P, _I64, _P, _I64, _P, _I64, _I64, _P, ctypes.c_int,
+                                _P, ctypes.c_int, _I64, _P]
+_lib.mb_cache_write_workspace_size.restype = ctypes.c_size_t
+_lib.mb_cache_write_workspace_size.argtypes = [_I64]
+_lib.mb_cache_write.restype = ctypes.c_int
+_lib.mb_cache_write.argtypes = [_CACHE, _P, _I64, _I64, _P, _I64, _I64, ctypes.c_int, _I64, _P,
+                                _P, ctypes.c_size_t, _P]
+_lib.mb_cache_read.restype = ctypes.c_int
+_lib.mb_cache_read.argtypes = [_CACHE, _P, _I64, _P, _P, ctypes.c_int, _P]
+_lib.mb_cache_attention_workspace_size.restype = ctypes.c_size_t
+_lib.mb_cache_attention_workspace_size.argtypes = [_CACHE, _I64, _I64, _I64]
+_lib.mb_cache_attention.restype = ctypes.c_int
+_lib.mb_cache_attention.argtypes = [_CACHE, _P, _I64, _I64, ctypes.c_int, _I64, _I64, _P, _I64,
+                                    _I64, _P, ctypes.c_float, _P, _P, ctypes.c_size_t, _P]
+
 GROUP_SIZE_1ST = 16
 GROUP_SIZE_2ND = 256
+INT8_MAX_K = 131072  # MB_INT8_MAX_K: the int32 sums of 127 * 127 * K are exact
 
 # mb_gptq_quantize's evaluation of (w - gmin) / sc: the IEEE quotient
 # (PyTorch on CPU tensors) or a product with the fp32 reciprocal (PyTorch on
@@ -755,3 +786,256 @@ class QuantizeBatch:
                     torch.cuda.current_stream(self.device).synchronize()
             res.append([*self.out[i], self.vals[i][:k], self.cols[i][:k], self.row_ptrs[i]])
         return res
+
+
+# ---- 8-bit rows and their product; quantised key/value cache ----
+
+_DTYPES = {torch.float16: 0, torch.bfloat16: 1, torch.float32: 2}
+_DTYPES_16 = {torch.float16: 0, torch.bfloat16: 1}
+
+
+def _dtype(dt: torch.dtype, name: str, known=_DTYPES) -> int:
+    code = known.get(dt)
+    if code is None:
+        raise RuntimeError(f"{name} must be " + " or ".join(
+            str(d).replace("torch.", "") for d in known))
+    return code
+
+
+def _rows_2d(x: torch.Tensor, name: str) -> torch.Tensor:
+    """x as [rows, K] with contiguous columns (its own memory where its
+    strides allow)."""
+    if x.dim() == 0:
+        raise RuntimeError(f"{name} must have at least one dimension")
+    K = x.shape[-1]
+    if x.dim() != 2:
+        x = x.reshape(-1, K) if K > 0 else x.new_empty((0, 0))
+    return x if x.stride(1) == 1 or K <= 1 else x.contiguous()
+
+
+def _row_stride(x: torch.Tensor) -> int:
+    """Elements between rows (of a single row: its length)."""
+    return x.stride(0) if x.shape[0] > 1 else x.shape[1]
+
+
+def _int8_operand(codes: torch.Tensor, scales: torch.Tensor, name: str):
+    """Checks an Int8Tensor's parts; returns (scales, row stride of codes)."""
+    if codes.dtype != torch.int8 or codes.dim() != 2:
+        raise RuntimeError(f"{name}.codes must be 2D int8")
+    if not codes.is_cuda:
+        raise RuntimeError(f"{name}.codes must be on CUDA")
+    rows, K = codes.shape
+    if scales.dtype != torch.float32 or tuple(scales.shape) != (rows,) \
+            or scales.device != codes.device:
+        raise RuntimeError(f"{name}.scales must be float32 [rows] on the device of its codes")
+    stride = codes.stride(0) if rows > 1 else (K + 15) // 16 * 16
+    if (K > 1 and codes.stride(1) != 1) or stride % 16 != 0 or stride < K \
+            or codes.data_ptr() % 16 != 0:
+        raise RuntimeError(f"{name}.codes must have contiguous rows that begin on 16-byte "
+                           "boundaries (as quantize_int8 returns them)")
+    return scales.contiguous(), stride
+
+
+def int8_quantize(x: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor) -> None:
+    """Rows of x [rows, K] to codes and scales (``mb_int8_quantize``)."""
+    _check(_lib.mb_int8_quantize(_ptr(x), _DTYPES[x.dtype], x.shape[0], x.shape[1],
+                                 _row_stride(x), _ptr(codes), codes.stride(0), _ptr(scales),
+                                 _stream(x.device)))
+
+
+def quantize_int8(x: torch.Tensor):
+    """(codes, scales) of the rows of x ([..., K], the leading dimensions
+    flattened)."""
+    from .formats import int8_rows
+    _dtype(x.dtype, "x")
+    if not x.is_cuda:
+        raise RuntimeError("x must be on CUDA")
+    with torch.cuda.device(x.device):
+        x = _rows_2d(x, "x")
+        rows, K = x.shape
+        codes = int8_rows(rows, K, x.device)
+        scales = torch.empty((rows,), dtype=torch.float32, device=x.device)
+        if rows > 0 and K > 0:
+            int8_quantize(x, codes, scales)
+        else:
+            scales.zero_()
+    return codes, scales
+
+
+def dequantize_int8(codes: torch.Tensor, scales: torch.Tensor, dtype: torch.dtype,
+                    out: torch.Tensor | None = None) -> torch.Tensor:
+    scales, stride = _int8_operand(codes, scales, "t")
+    code = _dtype(dtype, "dtype")
+    rows, K = codes.shape
+    with torch.cuda.device(codes.device):
+        if out is None:
+            out = torch.empty((rows, K), dtype=dtype, device=codes.device)
+        elif out.dtype != dtype or tuple(out.shape) != (rows, K) or out.device != codes.device \
+                or not out.is_contiguous():
+            raise RuntimeError("out must be a contiguous [rows, K] tensor of dtype on the device "
+                               "of t")
+        if rows > 0 and K > 0:
+            _check(_lib.mb_int8_dequantize(_ptr(codes), stride, _ptr(scales), rows, K, _ptr(out),
+                                           code, K, _stream(codes.device)))
+    return out
+
+
+def int8_matmul(x, w_codes: torch.Tensor, w_scales: torch.Tensor,
+                bias: torch.Tensor | None = None, out_dtype: torch.dtype | None = None,
+                out: torch.Tensor | None = None) -> torch.Tensor:
+    """[..., N] = x W^T + bias; x a floating tensor [..., K] (quantised a row
+    at a time here) or a pair (codes, scales)."""
+    w_scales, w_stride = _int8_operand(w_codes, w_scales, "w")
+    N, K = w_codes.shape
+    dev = w_codes.device
+    given = isinstance(x, tuple)
+    xs = x[0] if given else x
+    if xs.device != dev:
+        raise RuntimeError("x must be on the device of w")
+    if xs.dim() == 0 or xs.shape[-1] != K:
+        raise RuntimeError(f"x must have {K} columns as w")
+    if K == 0 or K > INT8_MAX_K:
+        raise RuntimeError(f"w must have 1 to {INT8_MAX_K} columns")
+    if given:
+        a_scales, a_stride = _int8_operand(x[0], x[1], "x")
+    else:
+        _dtype(x.dtype, "x")
+    if out_dtype is None:
+        out_dtype = torch.float16 if given else x.dtype
+    out_code = _dtype(out_dtype, "out_dtype")
+    bias_code = 0
+    if bias is not None:
+        bias_code = _dtype(bias.dtype, "bias")
+        if tuple(bias.shape) != (N,) or bias.device != dev:
+            raise RuntimeError(f"bias must be [{N}] on the device of w")
+    shape = tuple(xs.shape[:-1]) + (N,)
+    if out is not None and (out.dtype != out_dtype or tuple(out.shape) != shape
+                            or out.device != dev or not out.is_contiguous()):
+        raise RuntimeError("out must be a contiguous tensor of x's leading dimensions and N "
+                           "columns, of out_dtype, on the device of w")
+    with torch.cuda.device(dev):
+        if out is None:
+            out = torch.empty(shape, dtype=out_dtype, device=dev)
+        M = out.numel() // N if N > 0 else 0
+        if M == 0:
+            return out
+        if given:
+            a_codes = x[0]
+        else:
+            a_codes, a_scales = quantize_int8(x)
+            a_stride = a_codes.stride(0)
+        if bias is not None:
+            bias = bias.contiguous()
+        _check(_lib.mb_int8_matmul(_ptr(a_codes), a_stride, _ptr(a_scales), M, _ptr(w_codes),
+                                   w_stride, _ptr(w_scales), N, K, _ptr(bias), bias_code,
+                                   _ptr(out), out_code, N, _stream(dev)))
+    return out
+
+
+def _cache_struct(cache) -> KVCache:
+    """mb_kv_cache of a QuantizedCache, its parts checked against each other."""
+    kc, vc, ks, vs = cache.k_codes, cache.v_codes, cache.k_scales, cache.v_scales
+    if kc.dim() != 4 or kc.dtype not in (torch.int8, torch.uint8):
+        raise RuntimeError("k_codes must be 4D int8 (8 bits) or uint8 (4 bits)")
+    if not kc.is_cuda:
+        raise RuntimeError("k_codes must be on CUDA")
+    bits = 8 if kc.dtype == torch.int8 else 4
+    pages, heads, page, width = kc.shape
+    dim = width * 8 // bits
+    rows = (pages, heads, page)
+    want = (torch.float32, rows) if bits == 8 else (torch.float16, rows + (dim // 32, 2))
+    for t, dt, shape, name in ((kc, kc.dtype, kc.shape, "k_codes"),
+                               (vc, kc.dtype, kc.shape, "v_codes"),
+                               (ks,) + want + ("k_scales",), (vs,) + want + ("v_scales",)):
+        if t.dtype != dt or tuple(t.shape) != tuple(shape):
+            raise RuntimeError(f"{name} must be {str(dt).replace('torch.', '')} {list(shape)}")
+        if t.device != kc.device:
+            raise RuntimeError(f"{name} must be on the same CUDA device as k_codes")
+        if not t.is_contiguous():
+            raise RuntimeError(f"{name} must be contiguous")
+    return KVCache(kc.data_ptr(), vc.data_ptr(), ks.data_ptr(), vs.data_ptr(), pages, page, heads,
+                   dim, bits)
+
+
+def _slots(slots: torch.Tensor, tokens: int | None, dev) -> torch.Tensor:
+    if slots.dim() != 1 or slots.dtype != torch.int64 or slots.device != dev:
+        raise RuntimeError("slots must be 1D int64 on the device of the cache")
+    if tokens is not None and slots.shape[0] != tokens:
+        raise RuntimeError("slots must hold a slot for each token")
+    return slots.contiguous()
+
+
+def cache_write(cache, k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor) -> None:
+    c = _cache_struct(cache)
+    dev = cache.k_codes.device
+    code = _dtype(k.dtype, "k", _DTYPES_16)
+    for t, name in ((k, "k"), (v, "v")):
+        if t.dim() != 3 or tuple(t.shape[1:]) != (c.kv_heads, c.head_dim):
+            raise RuntimeError(f"{name} must be [tokens, {c.kv_heads}, {c.head_dim}]")
+        if t.device != dev or t.dtype != k.dtype:
+            raise RuntimeError(f"{name} must be on the device of the cache and of k's dtype")
+    if k.shape[0] != v.shape[0]:
+        raise RuntimeError("k and v must hold the same number of tokens")
+    tokens = k.shape[0]
+    slots = _slots(slots, tokens, dev)
+    if tokens == 0:
+        return
+    with torch.cuda.device(dev):
+        k, v = (t if t.stride(2) == 1 else t.contiguous() for t in (k, v))
+        n = int(_lib.mb_cache_write_workspace_size(tokens))
+        ws = torch.empty(n, dtype=torch.uint8, device=dev) if n else None
+        _check(_lib.mb_cache_write(ctypes.byref(c), _ptr(k), k.stride(0), k.stride(1), _ptr(v),
+                                   v.stride(0), v.stride(1), code, tokens, _ptr(slots), _ptr(ws),
+                                   n, _stream(dev)))
+
+
+def cache_read(cache, slots: torch.Tensor, dtype: torch.dtype):
+    c = _cache_struct(cache)
+    dev = cache.k_codes.device
+    code = _dtype(dtype, "dtype")
+    slots = _slots(slots, None, dev)
+    tokens = slots.shape[0]
+    with torch.cuda.device(dev):
+        k, v = (torch.empty((tokens, c.kv_heads, c.head_dim), dtype=dtype, device=dev)
+                for _ in range(2))
+        if tokens > 0:
+            _check(_lib.mb_cache_read(ctypes.byref(c), _ptr(slots), tokens, _ptr(k), _ptr(v),
+                                      code, _stream(dev)))
+    return k, v
+
+
+def cache_attention(q: torch.Tensor, cache, page_table: torch.Tensor, lengths: torch.Tensor,
+                    scale: float, out: torch.Tensor | None = None) -> torch.Tensor:
+    c = _cache_struct(cache)
+    dev = cache.k_codes.device
+    code = _dtype(q.dtype, "q", _DTYPES_16)
+    if q.dim() != 3 or q.shape[2] != c.head_dim or q.device != dev:
+        raise RuntimeError(f"q must be [batch, heads, {c.head_dim}] on the device of the cache")
+    batch, heads = q.shape[:2]
+    if heads == 0 or heads % c.kv_heads != 0:
+        raise RuntimeError(f"q's heads must be a multiple of the cache's {c.kv_heads}")
+    if page_table.dim() != 2 or page_table.dtype != torch.int32 or page_table.device != dev \
+            or page_table.shape[0] != batch:
+        raise RuntimeError("page_table must be int32 [batch, pages] on the device of the cache")
+    if tuple(lengths.shape) != (batch,) or lengths.dtype != torch.int32 or lengths.device != dev:
+        raise RuntimeError("lengths must be int32 [batch] on the device of the cache")
+    if out is not None and (out.dtype != q.dtype or out.shape != q.shape or out.device != dev
+                            or not out.is_contiguous()):
+        raise RuntimeError("out must be a contiguous tensor of q's shape, dtype and device")
+    with torch.cuda.device(dev):
+        if out is None:
+            out = torch.empty((batch, heads, c.head_dim), dtype=q.dtype, device=dev)
+        if batch == 0:
+            return out
+        q = q if q.stride(2) == 1 else q.contiguous()
+        width = page_table.shape[1]
+        if width > 1 and page_table.stride(1) != 1:
+            page_table = page_table.contiguous()
+        lengths = lengths.contiguous()
+        n = int(_lib.mb_cache_attention_workspace_size(ctypes.byref(c), batch, heads, width))
+        ws = torch.empty(n, dtype=torch.uint8, device=dev) if n else None
+        _check(_lib.mb_cache_attention(ctypes.byref(c), _ptr(q), q.stride(0), q.stride(1), code,
+                                       batch, heads, _ptr(page_table), page_table.stride(0),
+                                       width, _ptr(lengths), float(scale), _ptr(out), _ptr(ws), n,
+                                       _stream(dev)))
+    return out

@@ -1,0 +1,196 @@
+// Rows to 8-bit codes with one fp32 scale each, and back (no counterpart in
+// the reference): scale = max|x| / 127, code = x / scale to the nearest.
+//
+// Both directions are bound by memory: 3 bytes a value for the 16-bit types.
+// A row is read once: its threads keep the first 32 values each in registers
+// between the maximum and the codes (rows longer than that are read a second
+// time past it, from L2).
+#include <algorithm>
+
+#include "mb_codes.cuh"
+
+namespace mb {
+namespace {
+
+constexpr int kRowChunks = 4;  // 8-value pieces a thread keeps
+
+// T threads a row; CTAs of max(T, 256) threads.
+template <typename X, int T>
+__global__ void __launch_bounds__(T < 256 ? 256 : T)
+    int8_quantize_kernel(const X* __restrict__ x, int64_t rows, int64_t K, int64_t x_stride,
+                         bool x_vec, int8_t* __restrict__ codes, int64_t codes_stride,
+                         float* __restrict__ scales) {
+  constexpr int kRows = T < 256 ? 256 / T : 1;
+  __shared__ uint32_t part[kRows][(T + 31) / 32];
+  const int tid = threadIdx.x % T, sub = threadIdx.x / T;
+  const int64_t row = (int64_t)blockIdx.x * kRows + sub;
+  const bool live = row < rows;
+  const X* xr = x + (live ? row : 0) * x_stride;
+  const int64_t n8 = live ? ceil_div(K, 8) : 0;
+
+  float v[kRowChunks][8];
+  uint32_t m = 0;
+#pragma unroll
+  for (int j = 0; j < kRowChunks; ++j) {
+    const int64_t c = tid + (int64_t)j * T;
+    if (c < n8) load8(xr + 8 * c, x_vec, (int)min64(8, K - 8 * c), v[j]);
+  }
+#pragma unroll
+  for (int j = 0; j < kRowChunks; ++j)
+    if (tid + (int64_t)j * T < n8) m = max(m, abs_bits_max(v[j]));
+  for (int64_t c = tid + (int64_t)kRowChunks * T; c < n8; c += T) {
+    float u[8];
+    load8(xr + 8 * c, x_vec, (int)min64(8, K - 8 * c), u);
+    m = max(m, abs_bits_max(u));
+  }
+  m = __reduce_max_sync(0xffffffffu, m);
+  if constexpr (T > 32) {
+    if ((threadIdx.x & 31) == 0) part[sub][tid / 32] = m;
+    __syncthreads();
+    for (int w = 0; w < T / 32; ++w) m = max(m, part[sub][w]);
+  }
+  if (!live) return;
+  const RowScale r = row_scale(m);
+  if (tid == 0) scales[row] = r.scale;
+  int8_t* cr = codes + row * codes_stride;
+  const auto put = [&](int64_t c, const float(&u)[8]) {
+    const uint2 q = codes8(u, r);
+    if (8 * c + 8 <= K) {
+      *reinterpret_cast<uint2*>(cr + 8 * c) = q;
+    } else {
+      for (int i = 0; i < (int)(K - 8 * c); ++i)
+        cr[8 * c + i] = (int8_t)((i < 4 ? q.x : q.y) >> (8 * (i & 3)));
+    }
+  };
+#pragma unroll
+  for (int j = 0; j < kRowChunks; ++j) {
+    const int64_t c = tid + (int64_t)j * T;
+    if (c < n8) put(c, v[j]);
+  }
+  for (int64_t c = tid + (int64_t)kRowChunks * T; c < n8; c += T) {
+    float u[8];
+    load8(xr + 8 * c, x_vec, (int)min64(8, K - 8 * c), u);
+    put(c, u);
+  }
+}
+
+// A thread decodes 16 codes.
+template <typename Y>
+__global__ void __launch_bounds__(256)
+    int8_dequantize_kernel(const int8_t* __restrict__ codes, int64_t codes_stride,
+                           const float* __restrict__ scales, uint32_t pieces, uint32_t total,
+                           int64_t K, Y* __restrict__ out, int64_t out_stride, bool out_vec) {
+  const uint32_t i = blockIdx.x * 256u + threadIdx.x;
+  if (i >= total) return;
+  const uint32_t row = i / pieces, p = i - row * pieces;
+  const int64_t c0 = 16 * (int64_t)p;
+  const uint4 q = *reinterpret_cast<const uint4*>(codes + row * codes_stride + c0);
+  const float s = scales[row];
+  const uint32_t w[4] = {q.x, q.y, q.z, q.w};
+  Y* o = out + row * out_stride + c0;
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    float v[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+      v[e] = __fmul_rn((float)(int)(int8_t)(w[2 * h + e / 4] >> (8 * (e & 3))), s);
+    const int n = (int)min64(8, K - c0 - 8 * h);
+    if (n > 0) store8(o + 8 * h, out_vec, n, v);
+  }
+}
+
+template <typename X, int T>
+void launch_quantize(const void* x, int64_t rows, int64_t K, int64_t x_stride, bool x_vec,
+                     int8_t* codes, int64_t codes_stride, float* scales, cudaStream_t stream) {
+  constexpr int kThreads = T < 256 ? 256 : T;
+  const unsigned grid = (unsigned)ceil_div(rows, kThreads / T);
+  int8_quantize_kernel<X, T><<<grid, kThreads, 0, stream>>>(
+      static_cast<const X*>(x), rows, K, x_stride, x_vec, codes, codes_stride, scales);
+}
+
+template <typename X>
+void dispatch_quantize(const void* x, int64_t rows, int64_t K, int64_t x_stride, bool x_vec,
+                       int8_t* codes, int64_t codes_stride, float* scales, cudaStream_t stream) {
+  if (K <= 32 * 8 * kRowChunks)
+    launch_quantize<X, 32>(x, rows, K, x_stride, x_vec, codes, codes_stride, scales, stream);
+  else if (K <= 256 * 8 * kRowChunks)
+    launch_quantize<X, 256>(x, rows, K, x_stride, x_vec, codes, codes_stride, scales, stream);
+  else
+    launch_quantize<X, 512>(x, rows, K, x_stride, x_vec, codes, codes_stride, scales, stream);
+}
+
+}  // namespace
+}  // namespace mb
+
+using namespace mb;
+
+extern "C" mb_status mb_int8_quantize(const void* x, mb_dtype x_type, int64_t rows, int64_t K,
+                                      int64_t x_stride, int8_t* codes, int64_t codes_stride,
+                                      float* scales, mb_stream_t stream_) {
+  clear_error();
+  MB_REQUIRE(x && codes && scales, "int8_quantize pointers must not be null");
+  MB_REQUIRE(dtype_known(x_type), "unknown type of x");
+  MB_REQUIRE(rows > 0 && K > 0, "rows and K must be positive");
+  MB_REQUIRE(rows < (int64_t(1) << 31), "too many rows");
+  MB_REQUIRE(rows == 1 || codes_stride >= K, "codes_stride must be at least K");
+  MB_REQUIRE(aligned(codes, 16) && codes_stride % 16 == 0,
+             "codes must begin on 16-byte boundaries");
+  MB_REQUIRE(aligned(x, dtype_size(x_type)) && aligned(scales, 4), "misaligned x or scales");
+  cudaStream_t stream = reinterpret_cast<cudaStream_t>(stream_);
+  const bool vec = aligned(x, 16) && (rows == 1 || x_stride * dtype_size(x_type) % 16 == 0);
+  switch (x_type) {
+    case MB_FP16:
+      dispatch_quantize<__half>(x, rows, K, x_stride, vec, codes, codes_stride, scales, stream);
+      break;
+    case MB_BF16:
+      dispatch_quantize<__nv_bfloat16>(x, rows, K, x_stride, vec, codes, codes_stride, scales,
+                                       stream);
+      break;
+    default:
+      dispatch_quantize<float>(x, rows, K, x_stride, vec, codes, codes_stride, scales, stream);
+  }
+  MB_LAUNCH_CHECK("int8_quantize_kernel");
+  return MB_OK;
+}
+
+extern "C" mb_status mb_int8_dequantize(const int8_t* codes, int64_t codes_stride,
+                                        const float* scales, int64_t rows, int64_t K, void* out,
+                                        mb_dtype out_type, int64_t out_stride,
+                                        mb_stream_t stream_) {
+  clear_error();
+  MB_REQUIRE(codes && scales && out, "int8_dequantize pointers must not be null");
+  MB_REQUIRE(dtype_known(out_type), "unknown type of out");
+  MB_REQUIRE(rows > 0 && K > 0, "rows and K must be positive");
+  MB_REQUIRE(K < (int64_t(1) << 31), "K too large");
+  MB_REQUIRE(rows == 1 || (codes_stride >= K && out_stride >= K),
+             "strides must be at least K");
+  MB_REQUIRE(aligned(codes, 16) && codes_stride % 16 == 0,
+             "codes must begin on 16-byte boundaries");
+  MB_REQUIRE(aligned(out, dtype_size(out_type)) && aligned(scales, 4), "misaligned out or scales");
+  cudaStream_t stream = reinterpret_cast<cudaStream_t>(stream_);
+  const size_t size = dtype_size(out_type);
+  const bool vec = aligned(out, 16) && (rows == 1 || out_stride * size % 16 == 0);
+  const int64_t pieces = ceil_div(K, 16);
+  // a launch counts its 16-code pieces in 32 bits
+  const int64_t most = std::max<int64_t>(1, (int64_t(1) << 31) / pieces);
+  for (int64_t r0 = 0; r0 < rows; r0 += most) {
+    const int64_t n = min64(most, rows - r0);
+    const uint32_t total = (uint32_t)(n * pieces);
+    const unsigned grid = (unsigned)ceil_div(total, 256);
+    const int8_t* c = codes + r0 * codes_stride;
+    uint8_t* o = static_cast<uint8_t*>(out) + (size_t)(r0 * out_stride) * size;
+    const auto go = [&](auto* typed) {
+      int8_dequantize_kernel<<<grid, 256, 0, stream>>>(c, codes_stride, scales + r0,
+                                                       (uint32_t)pieces, total, K, typed,
+                                                       out_stride, vec);
+    };
+    if (out_type == MB_FP16)
+      go(reinterpret_cast<__half*>(o));
+    else if (out_type == MB_BF16)
+      go(reinterpret_cast<__nv_bfloat16*>(o));
+    else
+      go(reinterpret_cast<float*>(o));
+    MB_LAUNCH_CHECK("int8_dequantize_kernel");
+  }
+  return MB_OK;
+}

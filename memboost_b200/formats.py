@@ -172,3 +172,106 @@ class QuantizedTensor:
             fields["packed_2bit"] = p2
             fields["packed_4bit"] = p4.reshape(M, 2 * ng)
         return cls(**fields, M=M, K=K)
+
+
+@dataclass
+class Int8Tensor:
+    """Rows (tokens or output channels) in 8 bits: ``codes`` int8 [rows, K],
+    whose rows begin on 16-byte boundaries (``quantize_int8`` lays them out
+    so), and ``scales`` fp32 [rows]; row r stands for codes[r] * scales[r]."""
+
+    codes: torch.Tensor
+    scales: torch.Tensor
+
+    @property
+    def shape(self) -> torch.Size:
+        return self.codes.shape
+
+    @property
+    def device(self) -> torch.device:
+        return self.codes.device
+
+    def to(self, device) -> "Int8Tensor":
+        codes = int8_rows(self.codes.shape[0], self.codes.shape[1], device)
+        codes.copy_(self.codes)
+        return Int8Tensor(codes, self.scales.to(device))
+
+
+def int8_rows(rows: int, K: int, device) -> torch.Tensor:
+    """Uninitialised int8 [rows, K] whose rows begin on 16-byte boundaries."""
+    return torch.empty((rows, (K + 15) // 16 * 16), dtype=torch.int8, device=device)[:, :K]
+
+
+CACHE_GROUP_4BIT = 32  # channels that share a 4-bit cache scale and minimum
+
+
+@dataclass
+class QuantizedCache:
+    """Paged keys and values in 8 or 4 bits.
+
+      k_codes, v_codes    int8 [pages, kv_heads, page_size, head_dim]       (8 bits)
+                          uint8 [pages, kv_heads, page_size, head_dim / 2]  (4 bits,
+                          the even channel in the low half of a byte)
+      k_scales, v_scales  fp32 [pages, kv_heads, page_size]                 (8 bits)
+                          fp16 [pages, kv_heads, page_size, head_dim / 32, 2]
+                          (4 bits: scale and minimum of 32 channels)
+
+    Slot page * page_size + i is place i of a page."""
+
+    k_codes: torch.Tensor
+    v_codes: torch.Tensor
+    k_scales: torch.Tensor
+    v_scales: torch.Tensor
+
+    @classmethod
+    def allocate(cls, pages: int, page_size: int, kv_heads: int, head_dim: int, bits: int = 8,
+                 device=None) -> "QuantizedCache":
+        """A cache of zeros.  page_size is a multiple of 16, head_dim of 16
+        (8 bits) or 32 (4 bits) and at most 256."""
+        if bits not in (4, 8):
+            raise RuntimeError("bits must be 8 or 4")
+        if pages <= 0 or kv_heads <= 0:
+            raise RuntimeError("pages and kv_heads must be positive")
+        if page_size <= 0 or page_size % 16 != 0:
+            raise RuntimeError("page_size must be a multiple of 16")
+        step = 16 if bits == 8 else CACHE_GROUP_4BIT
+        if not 0 < head_dim <= 256 or head_dim % step != 0:
+            raise RuntimeError(f"head_dim must be a multiple of {step} up to 256")
+        device = torch.device("cuda", torch.cuda.current_device()) if device is None \
+            else torch.device(device)
+        rows = (pages, kv_heads, page_size)
+        if bits == 8:
+            codes, scales = (rows + (head_dim,), torch.int8), (rows, torch.float32)
+        else:
+            codes = (rows + (head_dim // 2,), torch.uint8)
+            scales = (rows + (head_dim // CACHE_GROUP_4BIT, 2), torch.float16)
+        return cls(*(torch.zeros(s, dtype=t, device=device)
+                     for s, t in (codes, codes, scales, scales)))
+
+    @property
+    def bits(self) -> int:
+        return 8 if self.k_codes.dtype == torch.int8 else 4
+
+    @property
+    def pages(self) -> int:
+        return self.k_codes.shape[0]
+
+    @property
+    def kv_heads(self) -> int:
+        return self.k_codes.shape[1]
+
+    @property
+    def page_size(self) -> int:
+        return self.k_codes.shape[2]
+
+    @property
+    def head_dim(self) -> int:
+        return self.k_codes.shape[3] * 8 // self.bits
+
+    @property
+    def device(self) -> torch.device:
+        return self.k_codes.device
+
+    @property
+    def nbytes(self) -> int:
+        return sum(t.nbytes for t in (self.k_codes, self.v_codes, self.k_scales, self.v_scales))

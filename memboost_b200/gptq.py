@@ -26,8 +26,8 @@ import torch.nn as nn
 import torch.nn.functional as F
 
 from . import _C
-from .formats import GROUP_SIZE_1ST, QuantizedTensor
-from .ops import dequantize, quantize
+from .formats import GROUP_SIZE_1ST, Int8Tensor, QuantizedTensor
+from .ops import dequantize, int8_matmul, quantize, quantize_int8
 
 GROUP_SIZE = GROUP_SIZE_1ST
 GPTQ_DIV_TRUE = _C.GPTQ_DIV_TRUE
@@ -141,6 +141,27 @@ class QuantizedLinear(nn.Module):
 
     def forward(self, x: torch.Tensor) -> torch.Tensor:
         return F.linear(x.to(torch.float16), dequantize(self.q_weight))
+
+
+class Int8Linear(nn.Module):
+    """Linear layer with its weight in 8 bits, a scale for each output
+    channel, and its input quantised a token at a time: int8_matmul on the
+    tensor cores instead of QuantizedLinear's fp16 product, without expanding
+    the weight in each call.  No counterpart in the reference."""
+
+    def __init__(self, weight: Int8Tensor, bias: torch.Tensor | None = None):
+        super().__init__()
+        self.out_features, self.in_features = weight.shape
+        self.weight = weight
+        self.bias = bias
+
+    @classmethod
+    def from_quantized(cls, q_weight: QuantizedTensor) -> "Int8Linear":
+        """Of a 2/4-bit weight: its dequantised matrix in 8 bits."""
+        return cls(quantize_int8(dequantize(q_weight)))
+
+    def forward(self, x: torch.Tensor) -> torch.Tensor:
+        return int8_matmul(x, self.weight, bias=self.bias)
 
 
 def make_quantized_linear(W_fp32: torch.Tensor, h_diag: torch.Tensor, Hinv_cho: torch.Tensor,

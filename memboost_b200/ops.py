@@ -2,12 +2,13 @@
 sm_100a kernels of libmemboost_b200.so."""
 from __future__ import annotations
 
-from typing import Optional
+import math
+from typing import Optional, Union
 
 import torch
 
 from . import _C
-from .formats import QuantizedTensor
+from .formats import Int8Tensor, QuantizedCache, QuantizedTensor
 
 
 def pack_2bit(values: torch.Tensor) -> torch.Tensor:
@@ -88,3 +89,61 @@ def qgemv(qtensor: QuantizedTensor, x: torch.Tensor, add_outliers: bool = True,
     return _C.qgemv(qtensor.packed_2bit, qtensor.packed_4bit, qtensor.scales_1st,
                     qtensor.zeros_1st, qtensor.group_precision, qtensor.outlier_row_ptrs, cols,
                     vals, qtensor.M, qtensor.K, x.reshape(-1), out)
+
+
+def quantize_int8(x: torch.Tensor) -> Int8Tensor:
+    """Rows of x ([..., K] fp16, bf16 or fp32 CUDA; the leading dimensions
+    flattened) in 8 bits: a token's activations, or an output channel's
+    weights.  scale = max|row| / 127 in fp32, code = x / scale to the nearest
+    integer (ties to even).  A row of zeros has scale 0; a row that holds a NaN
+    or an infinity has scale NaN, and whatever is computed from it is NaN."""
+    return Int8Tensor(*_C.quantize_int8(x))
+
+
+def dequantize_int8(t: Int8Tensor, dtype: torch.dtype = torch.float16,
+                    out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """[rows, K] = codes * scales in ``dtype`` (fp16, bf16 or fp32)."""
+    return _C.dequantize_int8(t.codes, t.scales, dtype, out)
+
+
+def int8_matmul(x: Union[torch.Tensor, Int8Tensor], w: Int8Tensor,
+                bias: Optional[torch.Tensor] = None, out_dtype: Optional[torch.dtype] = None,
+                out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """[..., N] = x W^T + bias with both operands in 8 bits: W [N, K] with a
+    scale for each output channel, x [..., K] with a scale for each token --
+    quantised here if x is a floating tensor, as quantize_int8 does.  The
+    integer sums are exact (K up to 131072); the result is rounded once to
+    ``out_dtype`` (x's dtype; fp16 for an Int8Tensor)."""
+    given = (x.codes, x.scales) if isinstance(x, Int8Tensor) else x
+    return _C.int8_matmul(given, w.codes, w.scales, bias, out_dtype, out)
+
+
+def cache_write(cache: QuantizedCache, k: torch.Tensor, v: torch.Tensor,
+                slots: torch.Tensor) -> None:
+    """Quantise tokens' keys and values ([tokens, kv_heads, head_dim] fp16 or
+    bf16) into ``slots`` (int64 [tokens]) of the cache.  Tokens whose slot is
+    outside the cache (a padding token's -1) are left out; of several tokens
+    with the same slot the last is kept."""
+    _C.cache_write(cache, k, v, slots)
+
+
+def cache_read(cache: QuantizedCache, slots: torch.Tensor, dtype: torch.dtype = torch.float16
+               ) -> tuple[torch.Tensor, torch.Tensor]:
+    """(k, v) [tokens, kv_heads, head_dim] in ``dtype`` as ``slots`` (int64
+    [tokens]) of the cache hold them; a slot outside the cache reads 0."""
+    return _C.cache_read(cache, slots, dtype)
+
+
+def cache_attention(q: torch.Tensor, cache: QuantizedCache, page_table: torch.Tensor,
+                    lengths: torch.Tensor, scale: Optional[float] = None,
+                    out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Attention of one query token a sequence, q [batch, heads, head_dim]
+    (fp16 or bf16; heads a multiple of the cache's), over the tokens t <
+    lengths[b] of the cache, token t in page page_table[b, t // page_size]
+    (int32 [batch, pages]; lengths int32 [batch]).  ``scale`` defaults to
+    1 / sqrt(head_dim).  The cache is read as it is held, never expanded in
+    memory.  Tokens of a page outside the cache are left out; a sequence
+    without tokens gives zeros."""
+    if scale is None:
+        scale = 1.0 / math.sqrt(cache.head_dim)
+    return _C.cache_attention(q, cache, page_table, lengths, scale, out)
