@@ -1,80 +1,322 @@
 // out = (a_scales b_scales^T) o (A B^T) + bias for 8-bit codes A (tokens) and
-// B (weights, an output channel a row): the sums are whole numbers, exact in
-// int32 (127^2 K < 2^31), scaled once at the end.
+// B (weights, an output channel a row), on the tcgen05 tensor cores: the sums
+// are whole numbers, exact in int32 (127^2 K < 2^31), scaled once at the end.
 //
-// 64 x 64 outputs a CTA, 64-byte pieces of both operands in shared memory,
-// four products an instruction.
+// The weights are the 128-row operand (accumulator row = TMEM lane = output
+// channel), the tokens the columns, so the same kernel serves one token and
+// thousands: a tile is 128 channels by kN tokens.  Both operands are read by
+// TMA in 128-byte steps of K with the 128-byte swizzle ("K-major"); rows and
+// columns past the matrices read 0.  A warp issues the loads, a warp the
+// products, and the four warps then drain the accumulator: a thread owns a
+// channel, so its scale and bias are registers and a warp writes 32
+// consecutive channels of a token.
+//
+// Few tiles (few tokens): K is split over the CTAs of a cluster, which add
+// their int32 parts through distributed shared memory -- whole numbers, so
+// the result does not depend on the split.
+#include <cstring>
+
 #include "mb_codes.cuh"
+#include "mb_tma.cuh"
 
 namespace mb {
 namespace {
 
-constexpr int kTile = 64, kStep = 64;
+constexpr int kChannels = 128;            // tile rows: output channels
+constexpr int kStepK = 128;               // bytes of K a stage
+constexpr int kWeightBytes = kChannels * kStepK;
+constexpr int kThreads = 192;             // warps 0-3 drain, 4 loads, 5 multiplies
 
-template <typename T>
-__device__ __forceinline__ float load_as_float(const void* p, int64_t i) {
-  return to_float<T>(static_cast<const T*>(p)[i]);
+// tokens a tile -> stages that fill shared memory for the blocks an SM holds
+template <int kN>
+struct Shape {
+  static constexpr int kStage = kWeightBytes + kN * kStepK;
+  static constexpr int kStages = kN == 256 ? 4 : kN == 128 ? 6 : 5;
+  static constexpr int kRing = kStages * kStage;
+  // int32 parts of a split: [kN tokens][128 channels], in the ring's memory
+  static_assert(kN * kChannels * 4 <= kRing, "the parts reuse the ring");
+  static constexpr int kSmem = kRing + 1024;
+  static constexpr uint32_t kTmem = kN < 32 ? 32 : kN;
+};
+
+// Shared-memory descriptor of a K-major operand written by TMA with the
+// 128-byte swizzle: rows of 128 bytes, 8-row atoms of 1024 bytes.
+__device__ __forceinline__ uint64_t umma_desc_k_sw128(uint32_t saddr) {
+  uint64_t d = 0;
+  d |= (uint64_t)((saddr >> 4) & 0x3FFFu);
+  d |= (uint64_t)1 << 16;                         // (unused with this swizzle)
+  d |= (uint64_t)((1024u >> 4) & 0x3FFFu) << 32;  // between 8-row groups
+  d |= (uint64_t)1 << 46;                         // descriptor version (sm_100)
+  d |= (uint64_t)2 << 61;                         // 128-byte swizzle
+  return d;
 }
 
-__device__ __forceinline__ float bias_at(const void* bias, int type, int64_t n) {
-  if (bias == nullptr) return 0.0f;
-  return type == MB_FP16 ? load_as_float<__half>(bias, n)
-         : type == MB_BF16 ? load_as_float<__nv_bfloat16>(bias, n)
-                           : load_as_float<float>(bias, n);
+// Instruction descriptor, kind::i8: int32 accumulate, signed 8-bit operands,
+// both K-major, M = 128.
+__host__ __device__ constexpr uint32_t int8_idesc(int n) {
+  return (2u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(n >> 3) << 17) |
+         ((uint32_t)(kChannels >> 4) << 24);
 }
 
-template <typename Y>
-__global__ void __launch_bounds__(256)
-    int8_matmul_kernel(const int8_t* __restrict__ a, int64_t a_stride,
-                       const float* __restrict__ a_scales, int64_t M,
-                       const int8_t* __restrict__ b, int64_t b_stride,
-                       const float* __restrict__ b_scales, int64_t N, int64_t K,
-                       const void* __restrict__ bias, int bias_type, Y* __restrict__ out,
-                       int64_t out_stride) {
-  __shared__ int sa[kStep / 4][kTile + 1], sb[kStep / 4][kTile + 1];
-  const int64_t m0 = (int64_t)blockIdx.y * kTile, n0 = (int64_t)blockIdx.x * kTile;
-  const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
-  int acc[4][4] = {};
-  for (int64_t k0 = 0; k0 < K; k0 += kStep) {
-    // a thread brings 16 bytes of one row of each operand
-    const int r = threadIdx.x >> 2, c = (threadIdx.x & 3) * 16;
-    const auto fetch = [&](const int8_t* p, int64_t stride, int64_t row, int64_t rows,
-                           int(*s)[kTile + 1]) {
-      int w[4] = {0, 0, 0, 0};
-      if (row < rows) {
-#pragma unroll
-        for (int e = 0; e < 16; ++e)
-          if (k0 + c + e < K)
-            w[e / 4] |= (int)(uint8_t)p[row * stride + k0 + c + e] << (8 * (e & 3));
+__device__ __forceinline__ void umma_i8(uint32_t tmem_d, uint64_t a, uint64_t b, uint32_t idesc,
+                                        uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::i8 [%0], %1, %2, %3, p;\n\t}" ::"r"(tmem_d),
+      "l"(a), "l"(b), "r"(idesc), "r"(accumulate));
+}
+
+__device__ __forceinline__ void umma_commit(uint64_t* bar) {
+  asm volatile(
+      "tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(
+          smem_u32(bar))
+      : "memory");
+}
+
+__device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
+      "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]),
+        "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]),
+        "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+      : "r"(taddr));
+  asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+}
+
+__device__ __forceinline__ uint32_t cluster_rank() {
+  uint32_t r;
+  asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+  return r;
+}
+__device__ __forceinline__ uint32_t cluster_size() {
+  uint32_t r;
+  asm("mov.u32 %0, %%cluster_nctarank;" : "=r"(r));
+  return r;
+}
+__device__ __forceinline__ void cluster_sync() {
+  asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+  asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+// Shared-memory address of the same place in the cluster's CTA `rank`.
+__device__ __forceinline__ uint32_t cluster_address(uint32_t saddr, uint32_t rank) {
+  uint32_t d;
+  asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(d) : "r"(saddr), "r"(rank));
+  return d;
+}
+__device__ __forceinline__ int load_cluster(uint32_t saddr) {
+  int v;
+  asm volatile("ld.shared::cluster.s32 %0, [%1];" : "=r"(v) : "r"(saddr) : "memory");
+  return v;
+}
+
+struct Epilogue {
+  const float* a_scales;
+  const float* b_scales;
+  const void* bias;
+  void* out;
+  int64_t out_stride;
+  int bias_type, out_type;
+};
+
+__device__ __forceinline__ float bias_at(const Epilogue& e, int64_t n) {
+  if (e.bias == nullptr) return 0.0f;
+  return e.bias_type == MB_FP16   ? __half2float(static_cast<const __half*>(e.bias)[n])
+         : e.bias_type == MB_BF16 ? __bfloat162float(static_cast<const __nv_bfloat16*>(e.bias)[n])
+                                  : static_cast<const float*>(e.bias)[n];
+}
+
+__device__ __forceinline__ void put(const Epilogue& e, int64_t m, int64_t n, float y) {
+  const int64_t i = m * e.out_stride + n;
+  if (e.out_type == MB_FP16)
+    static_cast<__half*>(e.out)[i] = __float2half_rn(y);
+  else if (e.out_type == MB_BF16)
+    static_cast<__nv_bfloat16*>(e.out)[i] = __float2bfloat16_rn(y);
+  else
+    static_cast<float*>(e.out)[i] = y;
+}
+
+// Grid: x = cluster (a tile's K parts) fastest, then channel tiles; y = token
+// tiles.
+template <int kN>
+__global__ void __launch_bounds__(kThreads, 1)
+    int8_matmul_kernel(const __grid_constant__ CUtensorMap tokens,
+                       const __grid_constant__ CUtensorMap weights, int64_t M, int64_t N,
+                       int64_t K, Epilogue e) {
+  using S = Shape<kN>;
+  extern __shared__ uint8_t raw[];
+  uint8_t* ring = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(raw) + 1023) &
+                                             ~(uintptr_t)1023);
+  __shared__ uint64_t full[S::kStages], empty[S::kStages], done;
+  __shared__ uint32_t tmem_slot, failed;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t parts = cluster_size(), part = cluster_rank();
+  const int64_t n0 = (int64_t)(blockIdx.x / parts) * kChannels, m0 = (int64_t)blockIdx.y * kN;
+  const int all = (int)ceil_div(K, kStepK);
+  const int k0 = (int)((int64_t)all * part / parts), k1 = (int)((int64_t)all * (part + 1) / parts);
+  const int steps = k1 - k0;
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < S::kStages; ++s) {
+      mbar_init(&full[s], 1);
+      mbar_init(&empty[s], 1);
+    }
+    mbar_init(&done, 1);
+    failed = 0;
+    fence_mbar_init();
+  }
+  if (warp == 0) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(
+                     smem_u32(&tmem_slot)),
+                 "r"(S::kTmem));
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+  }
+  asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+  __syncthreads();
+  asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+  const uint32_t tmem = tmem_slot;
+
+  if (warp == 4 && lane == 0) {
+    int issued = 0;
+    bool ok = true;
+    for (int i = 0; i < steps; ++i) {
+      const int s = i % S::kStages;
+      if (i >= S::kStages && !mbar_wait(&empty[s], (uint32_t)((i / S::kStages - 1) & 1))) {
+        ok = false;
+        break;
       }
-#pragma unroll
-      for (int e = 0; e < 4; ++e) s[c / 4 + e][r] = w[e];
-    };
-    fetch(a, a_stride, m0 + r, M, sa);
-    fetch(b, b_stride, n0 + r, N, sb);
-    __syncthreads();
-#pragma unroll
-    for (int k = 0; k < kStep / 4; ++k) {
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-#pragma unroll
-        for (int j = 0; j < 4; ++j)
-          acc[i][j] = __dp4a(sa[k][ty + 16 * i], sb[k][tx + 16 * j], acc[i][j]);
+      uint8_t* at = ring + s * S::kStage;
+      mbar_arrive_expect_tx(&full[s], S::kStage);
+      tma_load_2d(at, &weights, &full[s], (k0 + i) * kStepK, (int)n0);
+      tma_load_2d(at + kWeightBytes, &tokens, &full[s], (k0 + i) * kStepK, (int)m0);
+      ++issued;
     }
-    __syncthreads();
-  }
+    // every load has landed before the CTA can exit or reuse the ring
+    for (int i = issued > S::kStages ? issued - S::kStages : 0; i < issued; ++i)
+      if (!mbar_wait(&full[i % S::kStages], (uint32_t)((i / S::kStages) & 1))) ok = false;
+    if (!ok) atomicExch(&failed, 1u);
+  } else if (warp == 5 && lane == 0) {
+    bool ok = true;
+    for (int i = 0; i < steps; ++i) {
+      const int s = i % S::kStages;
+      if (!mbar_wait(&full[s], (uint32_t)((i / S::kStages) & 1))) {
+        ok = false;
+        break;
+      }
+      asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+      const uint32_t w = smem_u32(ring + s * S::kStage), t = w + kWeightBytes;
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const int64_t m = m0 + ty + 16 * i;
-    if (m >= M) continue;
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const int64_t n = n0 + tx + 16 * j;
-      if (n >= N) continue;
-      const float y = __fmul_rn(__fmul_rn((float)acc[i][j], a_scales[m]), b_scales[n]);
-      out[m * out_stride + n] = from_float<Y>(__fadd_rn(y, bias_at(bias, bias_type, n)));
+      for (int k = 0; k < kStepK / 32; ++k)
+        umma_i8(tmem, umma_desc_k_sw128(w + 32 * k), umma_desc_k_sw128(t + 32 * k),
+                int8_idesc(kN), (i > 0 || k > 0) ? 1u : 0u);
+      umma_commit(&empty[s]);
     }
+    umma_commit(&done);
+    if (!ok) atomicExch(&failed, 1u);
   }
+  __syncwarp();
+  if (!mbar_wait(&done, 0)) atomicExch(&failed, 1u);
+  asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+  __syncthreads();  // `failed` is final; the ring is free
+
+  const int64_t n = n0 + 32 * warp + lane;  // warps 0-3: this thread's channel
+  const uint32_t lanes = tmem + ((uint32_t)(32 * (warp & 3)) << 16);
+  if (parts == 1) {
+    if (warp < 4) {
+      const bool live = n < N;
+      const float sb = live ? e.b_scales[n] : 0.0f, bias = live ? bias_at(e, n) : 0.0f;
+#pragma unroll 1
+      for (int c = 0; c < kN && m0 + c < M; c += 16) {
+        uint32_t v[16];
+        tmem_ld16(lanes + c, v);
+        if (!live) continue;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          const int64_t m = m0 + c + i;
+          if (m >= M) break;
+          const float sa = failed ? __uint_as_float(0x7FC00000u) : e.a_scales[m];
+          put(e, m, n, __fadd_rn(__fmul_rn(__fmul_rn((float)(int)v[i], sa), sb), bias));
+        }
+      }
+    }
+  } else {
+    int* own = reinterpret_cast<int*>(ring);  // [token][channel]
+    const int columns = (int)min64(kN, M - m0);
+    if (warp < 4) {
+#pragma unroll 1
+      for (int c = 0; c < columns; c += 16) {
+        uint32_t v[16];
+        if (steps > 0) tmem_ld16(lanes + c, v);
+#pragma unroll
+        for (int i = 0; i < 16; ++i)
+          own[(c + i) * kChannels + 32 * warp + lane] = steps > 0 ? (int)v[i] : 0;
+      }
+    }
+    cluster_sync();
+    const uint32_t base = smem_u32(own), fail = smem_u32(&failed);
+    bool bad = false;
+    for (uint32_t r = 0; r < parts; ++r) bad |= load_cluster(cluster_address(fail, r)) != 0;
+    // this CTA's share of the tile's tokens, a channel a thread
+    if (warp < 4 && n < N) {
+      const float sb = e.b_scales[n], bias = bias_at(e, n);
+      for (int c = (int)part; c < columns; c += (int)parts) {
+        int sum = 0;
+        for (uint32_t r = 0; r < parts; ++r)
+          sum += load_cluster(cluster_address(base + (c * kChannels + 32 * warp + lane) * 4, r));
+        const float sa = bad ? __uint_as_float(0x7FC00000u) : e.a_scales[m0 + c];
+        put(e, m0 + c, n, __fadd_rn(__fmul_rn(__fmul_rn((float)sum, sa), sb), bias));
+      }
+    }
+    cluster_sync();  // no CTA leaves while another reads its part
+  }
+  asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+  __syncthreads();
+  if (warp == 0)
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem),
+                 "r"(S::kTmem));
+}
+
+// [rows, K] codes, boxes of 128 bytes by box_rows.
+bool codes_map(CUtensorMap* map, const int8_t* codes, int64_t stride, int64_t rows, int64_t K,
+               uint32_t box_rows) {
+  auto enc = tensor_map_encoder();
+  if (enc == nullptr) return false;
+  std::memset(map, 0, sizeof(*map));
+  const cuuint64_t dims[2] = {(cuuint64_t)K, (cuuint64_t)rows};
+  const cuuint64_t strides[1] = {(cuuint64_t)stride};
+  const cuuint32_t box[2] = {kStepK, box_rows};
+  const cuuint32_t ones[2] = {1, 1};
+  return enc(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<int8_t*>(codes), dims, strides, box,
+             ones, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+             CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) ==
+         CUDA_SUCCESS;
+}
+
+template <int kN>
+mb_status launch(const int8_t* a_codes, int64_t a_stride, int64_t M, const int8_t* b_codes,
+                 int64_t b_stride, int64_t N, int64_t K, const Epilogue& e, int parts,
+                 cudaStream_t stream) {
+  using S = Shape<kN>;
+  static std::atomic<uint64_t> attr_done{0};
+  MB_CUDA_TRY(set_smem_limit_once(int8_matmul_kernel<kN>, S::kSmem, attr_done));
+  CUtensorMap tokens, weights;
+  if (!codes_map(&tokens, a_codes, a_stride, M, K, kN) ||
+      !codes_map(&weights, b_codes, b_stride, N, K, kChannels))
+    return set_error(MB_ERR_CUDA, "cuTensorMapEncodeTiled rejected the codes");
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)(ceil_div(N, kChannels) * parts), (unsigned)ceil_div(M, kN));
+  cfg.blockDim = dim3(kThreads);
+  cfg.dynamicSmemBytes = S::kSmem;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = (unsigned)parts;
+  attr[0].val.clusterDim.y = 1;
+  attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  MB_CUDA_TRY(cudaLaunchKernelEx(&cfg, int8_matmul_kernel<kN>, tokens, weights, M, N, K, e));
+  return MB_OK;
 }
 
 }  // namespace
@@ -94,7 +336,7 @@ extern "C" mb_status mb_int8_matmul(const int8_t* a_codes, int64_t a_stride, con
              "unknown type of out or bias");
   MB_REQUIRE(M > 0 && N > 0 && K > 0, "M, N and K must be positive");
   MB_REQUIRE(K <= MB_INT8_MAX_K, "K too large: the int32 sums would not be exact");
-  MB_REQUIRE(M < (int64_t(1) << 31) && N < (int64_t(1) << 31), "M or N too large");
+  MB_REQUIRE(M <= (int64_t(1) << 23) && N < (int64_t(1) << 31) - 128, "M or N too large");
   MB_REQUIRE((M == 1 || a_stride >= K) && (N == 1 || b_stride >= K) && (M == 1 || out_stride >= N),
              "strides must be at least the length of a row");
   MB_REQUIRE(aligned(a_codes, 16) && aligned(b_codes, 16) && a_stride % 16 == 0 &&
@@ -103,20 +345,21 @@ extern "C" mb_status mb_int8_matmul(const int8_t* a_codes, int64_t a_stride, con
   MB_REQUIRE(aligned(out, dtype_size(out_type)) && aligned(a_scales, 4) && aligned(b_scales, 4) &&
                  (bias == nullptr || aligned(bias, dtype_size(bias_type))),
              "misaligned out, scales or bias");
+  // the stride of a single row is not read, but TMA wants one
+  if (M == 1) a_stride = ceil_div(K, 16) * 16;
+  if (N == 1) b_stride = ceil_div(K, 16) * 16;
   cudaStream_t stream = reinterpret_cast<cudaStream_t>(stream_);
-  const dim3 grid((unsigned)ceil_div(N, kTile), (unsigned)ceil_div(M, kTile));
-  MB_REQUIRE(grid.y <= 65535u, "M too large");
-  const auto go = [&](auto* typed) {
-    int8_matmul_kernel<<<grid, 256, 0, stream>>>(a_codes, a_stride, a_scales, M, b_codes, b_stride,
-                                                 b_scales, N, K, bias, (int)bias_type, typed,
-                                                 out_stride);
-  };
-  if (out_type == MB_FP16)
-    go(static_cast<__half*>(out));
-  else if (out_type == MB_BF16)
-    go(static_cast<__nv_bfloat16*>(out));
-  else
-    go(static_cast<float*>(out));
-  MB_LAUNCH_CHECK("int8_matmul_kernel");
-  return MB_OK;
+  const Epilogue e{a_scales, b_scales, bias, out, out_stride, (int)bias_type, (int)out_type};
+  const int kn = M <= 16 ? 16 : M <= 32 ? 32 : M <= 64 ? 64 : M <= 128 ? 128 : 256;
+  // K parts: until the tiles fill the SMs, each part at least two steps
+  const int64_t tiles = ceil_div(N, kChannels) * ceil_div(M, kn), steps = ceil_div(K, kStepK);
+  int parts = 1;
+  while (parts < 8 && tiles * parts * 2 <= 148 && steps >= 4 * parts) parts *= 2;
+  switch (kn) {
+    case 16: return launch<16>(a_codes, a_stride, M, b_codes, b_stride, N, K, e, parts, stream);
+    case 32: return launch<32>(a_codes, a_stride, M, b_codes, b_stride, N, K, e, parts, stream);
+    case 64: return launch<64>(a_codes, a_stride, M, b_codes, b_stride, N, K, e, parts, stream);
+    case 128: return launch<128>(a_codes, a_stride, M, b_codes, b_stride, N, K, e, parts, stream);
+    default: return launch<256>(a_codes, a_stride, M, b_codes, b_stride, N, K, e, parts, stream);
+  }
 }
