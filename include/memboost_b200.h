@@ -420,6 +420,16 @@ mb_status mb_int8_matmul(const int8_t* a_codes, int64_t a_stride, const float* a
                          int64_t K, const void* bias, mb_dtype bias_type, void* out,
                          mb_dtype out_type, int64_t out_stride, mb_stream_t stream);
 
+/* mb_int8_quantize of the tokens x [M, K] into the workspace and
+ * mb_int8_matmul of their codes: out = x W^T + bias with both in 8 bits.
+ * workspace: 16-byte aligned, mb_int8_linear_workspace_size(M, K) bytes. */
+size_t mb_int8_linear_workspace_size(int64_t M, int64_t K);
+mb_status mb_int8_linear(const void* x, mb_dtype x_type, int64_t x_stride, int64_t M,
+                         const int8_t* b_codes, int64_t b_stride, const float* b_scales, int64_t N,
+                         int64_t K, const void* bias, mb_dtype bias_type, void* out,
+                         mb_dtype out_type, int64_t out_stride, void* workspace,
+                         size_t workspace_bytes, mb_stream_t stream);
+
 /* ---------------------------------------------------------------------------
  * Quantised key/value cache -- no counterpart in the reference.
  *

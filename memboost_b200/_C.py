@@ -11,6 +11,7 @@ CUDA device first, and return CPU tensors as the reference does).
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes
 import os
 
@@ -117,6 +118,11 @@ _lib.mb_int8_dequantize.argtypes = [_P, _I64, _P, _I64, _I64, _P, ctypes.c_int, 
 _lib.mb_int8_matmul.restype = ctypes.c_int
 _lib.mb_int8_matmul.argtypes = [_P, _I64, _P, _I64, _P, _I64, _P, _I64, _I64, _P, ctypes.c_int,
                                 _P, ctypes.c_int, _I64, _P]
+_lib.mb_int8_linear_workspace_size.restype = ctypes.c_size_t
+_lib.mb_int8_linear_workspace_size.argtypes = [_I64, _I64]
+_lib.mb_int8_linear.restype = ctypes.c_int
+_lib.mb_int8_linear.argtypes = [_P, ctypes.c_int, _I64, _I64, _P, _I64, _P, _I64, _I64, _P,
+                                ctypes.c_int, _P, ctypes.c_int, _I64, _P, ctypes.c_size_t, _P]
 _lib.mb_cache_write_workspace_size.restype = ctypes.c_size_t
 _lib.mb_cache_write_workspace_size.argtypes = [_I64]
 _lib.mb_cache_write.restype = ctypes.c_int
@@ -789,9 +795,21 @@ class QuantizeBatch:
 
 
 # ---- 8-bit rows and their product; quantised key/value cache ----
+#
+# A call of these takes a few microseconds on the GPU, so the host's side of it
+# is kept short: the checks are attribute comparisons whose messages are put
+# together only where one fails, pointers go to ctypes as integers, the stream
+# is read as a handle and the device is only switched where it has to be.
 
 _DTYPES = {torch.float16: 0, torch.bfloat16: 1, torch.float32: 2}
 _DTYPES_16 = {torch.float16: 0, torch.bfloat16: 1}
+_SAME_DEVICE = contextlib.nullcontext()
+_raw_stream = torch._C._cuda_getCurrentRawStream  # torch.cuda.current_stream's handle
+
+
+def _on(index: int):
+    """Context with device ``index`` current."""
+    return _SAME_DEVICE if torch.cuda.current_device() == index else torch.cuda.device(index)
 
 
 def _dtype(dt: torch.dtype, name: str, known=_DTYPES) -> int:
@@ -802,63 +820,60 @@ def _dtype(dt: torch.dtype, name: str, known=_DTYPES) -> int:
     return code
 
 
-def _rows_2d(x: torch.Tensor, name: str) -> torch.Tensor:
-    """x as [rows, K] with contiguous columns (its own memory where its
-    strides allow)."""
+def _rows_of(x: torch.Tensor):
+    """(x with contiguous columns, rows, K, elements between rows) of x taken
+    as [rows, K]."""
     if x.dim() == 0:
-        raise RuntimeError(f"{name} must have at least one dimension")
+        raise RuntimeError("x must have at least one dimension")
     K = x.shape[-1]
-    if x.dim() != 2:
-        x = x.reshape(-1, K) if K > 0 else x.new_empty((0, 0))
-    return x if x.stride(1) == 1 or K <= 1 else x.contiguous()
-
-
-def _row_stride(x: torch.Tensor) -> int:
-    """Elements between rows (of a single row: its length)."""
-    return x.stride(0) if x.shape[0] > 1 else x.shape[1]
+    if not x.is_contiguous():
+        if x.dim() != 2:
+            x = x.reshape(-1, K) if x.numel() > 0 else x.contiguous()
+        if x.dim() == 2 and K > 1 and x.stride(1) != 1:
+            x = x.contiguous()
+        if x.dim() == 2 and x.shape[0] > 1 and x.stride(0) >= K:
+            return x, x.shape[0], K, x.stride(0)
+        x = x.contiguous()  # rows that overlap, as an expanded tensor's
+    return x, (x.numel() // K if K > 0 else 0), K, K
 
 
 def _int8_operand(codes: torch.Tensor, scales: torch.Tensor, name: str):
-    """Checks an Int8Tensor's parts; returns (scales, row stride of codes)."""
-    if codes.dtype != torch.int8 or codes.dim() != 2:
+    """Checks an Int8Tensor's parts; returns (scales, bytes between the rows
+    of codes)."""
+    if codes.dtype is not torch.int8 or codes.dim() != 2:
         raise RuntimeError(f"{name}.codes must be 2D int8")
     if not codes.is_cuda:
         raise RuntimeError(f"{name}.codes must be on CUDA")
     rows, K = codes.shape
-    if scales.dtype != torch.float32 or tuple(scales.shape) != (rows,) \
-            or scales.device != codes.device:
+    if scales.dtype is not torch.float32 or scales.dim() != 1 or scales.shape[0] != rows \
+            or scales.get_device() != codes.get_device():
         raise RuntimeError(f"{name}.scales must be float32 [rows] on the device of its codes")
-    stride = codes.stride(0) if rows > 1 else (K + 15) // 16 * 16
-    if (K > 1 and codes.stride(1) != 1) or stride % 16 != 0 or stride < K \
-            or codes.data_ptr() % 16 != 0:
+    stride, step = codes.stride()
+    if rows <= 1:
+        stride = (K + 15) // 16 * 16
+    if (K > 1 and step != 1) or stride % 16 != 0 or stride < K or codes.data_ptr() % 16 != 0:
         raise RuntimeError(f"{name}.codes must have contiguous rows that begin on 16-byte "
                            "boundaries (as quantize_int8 returns them)")
-    return scales.contiguous(), stride
-
-
-def int8_quantize(x: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor) -> None:
-    """Rows of x [rows, K] to codes and scales (``mb_int8_quantize``)."""
-    _check(_lib.mb_int8_quantize(_ptr(x), _DTYPES[x.dtype], x.shape[0], x.shape[1],
-                                 _row_stride(x), _ptr(codes), codes.stride(0), _ptr(scales),
-                                 _stream(x.device)))
+    return (scales if scales.is_contiguous() else scales.contiguous()), stride
 
 
 def quantize_int8(x: torch.Tensor):
     """(codes, scales) of the rows of x ([..., K], the leading dimensions
-    flattened)."""
-    from .formats import int8_rows
-    _dtype(x.dtype, "x")
+    flattened), by ``mb_int8_quantize``."""
+    code = _dtype(x.dtype, "x")
     if not x.is_cuda:
         raise RuntimeError("x must be on CUDA")
-    with torch.cuda.device(x.device):
-        x = _rows_2d(x, "x")
-        rows, K = x.shape
-        codes = int8_rows(rows, K, x.device)
-        scales = torch.empty((rows,), dtype=torch.float32, device=x.device)
-        if rows > 0 and K > 0:
-            int8_quantize(x, codes, scales)
-        else:
-            scales.zero_()
+    dev = x.device
+    with _on(dev.index):
+        x, rows, K, stride = _rows_of(x)
+        pitch = (K + 15) // 16 * 16
+        codes = torch.empty((rows, pitch), dtype=torch.int8, device=dev)
+        if pitch != K:
+            codes = codes[:, :K]
+        scales = torch.empty((rows,), dtype=torch.float32, device=dev)
+        if rows > 0:
+            _check(_lib.mb_int8_quantize(x.data_ptr(), code, rows, K, stride, codes.data_ptr(),
+                                         pitch, scales.data_ptr(), _raw_stream(dev.index)))
     return codes, scales
 
 
@@ -867,30 +882,31 @@ def dequantize_int8(codes: torch.Tensor, scales: torch.Tensor, dtype: torch.dtyp
     scales, stride = _int8_operand(codes, scales, "t")
     code = _dtype(dtype, "dtype")
     rows, K = codes.shape
-    with torch.cuda.device(codes.device):
+    dev = codes.device
+    with _on(dev.index):
         if out is None:
-            out = torch.empty((rows, K), dtype=dtype, device=codes.device)
-        elif out.dtype != dtype or tuple(out.shape) != (rows, K) or out.device != codes.device \
+            out = torch.empty((rows, K), dtype=dtype, device=dev)
+        elif out.dtype != dtype or out.shape != codes.shape or out.device != dev \
                 or not out.is_contiguous():
             raise RuntimeError("out must be a contiguous [rows, K] tensor of dtype on the device "
                                "of t")
         if rows > 0 and K > 0:
-            _check(_lib.mb_int8_dequantize(_ptr(codes), stride, _ptr(scales), rows, K, _ptr(out),
-                                           code, K, _stream(codes.device)))
+            _check(_lib.mb_int8_dequantize(codes.data_ptr(), stride, scales.data_ptr(), rows, K,
+                                           out.data_ptr(), code, K, _raw_stream(dev.index)))
     return out
 
 
 def int8_matmul(x, w_codes: torch.Tensor, w_scales: torch.Tensor,
                 bias: torch.Tensor | None = None, out_dtype: torch.dtype | None = None,
                 out: torch.Tensor | None = None) -> torch.Tensor:
-    """[..., N] = x W^T + bias; x a floating tensor [..., K] (quantised a row
-    at a time here) or a pair (codes, scales)."""
+    """[..., N] = x W^T + bias; x a floating tensor [..., K] (``mb_int8_linear``
+    quantises its rows) or a pair (codes, scales) (``mb_int8_matmul``)."""
     w_scales, w_stride = _int8_operand(w_codes, w_scales, "w")
     N, K = w_codes.shape
     dev = w_codes.device
-    given = isinstance(x, tuple)
+    given = type(x) is tuple
     xs = x[0] if given else x
-    if xs.device != dev:
+    if xs.get_device() != dev.index:
         raise RuntimeError("x must be on the device of w")
     if xs.dim() == 0 or xs.shape[-1] != K:
         raise RuntimeError(f"x must have {K} columns as w")
@@ -899,70 +915,96 @@ def int8_matmul(x, w_codes: torch.Tensor, w_scales: torch.Tensor,
     if given:
         a_scales, a_stride = _int8_operand(x[0], x[1], "x")
     else:
-        _dtype(x.dtype, "x")
+        x_code = _dtype(x.dtype, "x")
     if out_dtype is None:
         out_dtype = torch.float16 if given else x.dtype
     out_code = _dtype(out_dtype, "out_dtype")
-    bias_code = 0
+    bias_ptr, bias_code = None, 0
     if bias is not None:
         bias_code = _dtype(bias.dtype, "bias")
-        if tuple(bias.shape) != (N,) or bias.device != dev:
+        if bias.dim() != 1 or bias.shape[0] != N or bias.get_device() != dev.index:
             raise RuntimeError(f"bias must be [{N}] on the device of w")
-    shape = tuple(xs.shape[:-1]) + (N,)
-    if out is not None and (out.dtype != out_dtype or tuple(out.shape) != shape
-                            or out.device != dev or not out.is_contiguous()):
+    shape = xs.shape[:-1] + (N,)
+    if out is not None and (out.dtype != out_dtype or out.shape != shape or out.device != dev
+                            or not out.is_contiguous()):
         raise RuntimeError("out must be a contiguous tensor of x's leading dimensions and N "
                            "columns, of out_dtype, on the device of w")
-    with torch.cuda.device(dev):
+    with _on(dev.index):
         if out is None:
             out = torch.empty(shape, dtype=out_dtype, device=dev)
-        M = out.numel() // N if N > 0 else 0
-        if M == 0:
+        if out.numel() == 0:
             return out
-        if given:
-            a_codes = x[0]
-        else:
-            a_codes, a_scales = quantize_int8(x)
-            a_stride = a_codes.stride(0)
         if bias is not None:
             bias = bias.contiguous()
-        _check(_lib.mb_int8_matmul(_ptr(a_codes), a_stride, _ptr(a_scales), M, _ptr(w_codes),
-                                   w_stride, _ptr(w_scales), N, K, _ptr(bias), bias_code,
-                                   _ptr(out), out_code, N, _stream(dev)))
+            bias_ptr = bias.data_ptr()
+        if given:
+            M = xs.shape[0]
+            _check(_lib.mb_int8_matmul(xs.data_ptr(), a_stride, a_scales.data_ptr(), M,
+                                       w_codes.data_ptr(), w_stride, w_scales.data_ptr(), N, K,
+                                       bias_ptr, bias_code, out.data_ptr(), out_code, N,
+                                       _raw_stream(dev.index)))
+        else:
+            x, M, _, x_stride = _rows_of(x)
+            n = M * ((K + 15) // 16 * 16 + 4)  # mb_int8_linear_workspace_size
+            ws = torch.empty((n,), dtype=torch.uint8, device=dev)
+            _check(_lib.mb_int8_linear(x.data_ptr(), x_code, x_stride, M, w_codes.data_ptr(),
+                                       w_stride, w_scales.data_ptr(), N, K, bias_ptr, bias_code,
+                                       out.data_ptr(), out_code, N, ws.data_ptr(), n,
+                                       _raw_stream(dev.index)))
     return out
+
+
+def _cache_fault(cache) -> str:
+    """What is wrong with the parts of a QuantizedCache."""
+    kc = cache.k_codes
+    if kc.dim() != 4 or kc.dtype not in (torch.int8, torch.uint8):
+        return "k_codes must be 4D int8 (8 bits) or uint8 (4 bits)"
+    if not kc.is_cuda:
+        return "k_codes must be on CUDA"
+    rows, width = tuple(kc.shape[:3]), kc.shape[3]
+    want = (torch.float32, rows) if kc.dtype == torch.int8 \
+        else (torch.float16, rows + (width // 16, 2))
+    for t, dt, shape, name in ((kc, kc.dtype, kc.shape, "k_codes"),
+                               (cache.v_codes, kc.dtype, kc.shape, "v_codes"),
+                               (cache.k_scales,) + want + ("k_scales",),
+                               (cache.v_scales,) + want + ("v_scales",)):
+        if t.dtype != dt or tuple(t.shape) != tuple(shape):
+            return f"{name} must be {str(dt).replace('torch.', '')} {list(shape)}"
+        if t.device != kc.device:
+            return f"{name} must be on the same CUDA device as k_codes"
+        if not t.is_contiguous():
+            return f"{name} must be contiguous"
+    return "not a cache"
 
 
 def _cache_struct(cache) -> KVCache:
     """mb_kv_cache of a QuantizedCache, its parts checked against each other."""
     kc, vc, ks, vs = cache.k_codes, cache.v_codes, cache.k_scales, cache.v_scales
-    if kc.dim() != 4 or kc.dtype not in (torch.int8, torch.uint8):
-        raise RuntimeError("k_codes must be 4D int8 (8 bits) or uint8 (4 bits)")
-    if not kc.is_cuda:
-        raise RuntimeError("k_codes must be on CUDA")
-    bits = 8 if kc.dtype == torch.int8 else 4
-    pages, heads, page, width = kc.shape
-    dim = width * 8 // bits
-    rows = (pages, heads, page)
-    want = (torch.float32, rows) if bits == 8 else (torch.float16, rows + (dim // 32, 2))
-    for t, dt, shape, name in ((kc, kc.dtype, kc.shape, "k_codes"),
-                               (vc, kc.dtype, kc.shape, "v_codes"),
-                               (ks,) + want + ("k_scales",), (vs,) + want + ("v_scales",)):
-        if t.dtype != dt or tuple(t.shape) != tuple(shape):
-            raise RuntimeError(f"{name} must be {str(dt).replace('torch.', '')} {list(shape)}")
-        if t.device != kc.device:
-            raise RuntimeError(f"{name} must be on the same CUDA device as k_codes")
-        if not t.is_contiguous():
-            raise RuntimeError(f"{name} must be contiguous")
-    return KVCache(kc.data_ptr(), vc.data_ptr(), ks.data_ptr(), vs.data_ptr(), pages, page, heads,
-                   dim, bits)
+    shape, dev = kc.shape, kc.get_device()
+    ok = dev >= 0 and len(shape) == 4 and vc.shape == shape and vc.dtype == kc.dtype \
+        and dev == vc.get_device() == ks.get_device() == vs.get_device() \
+        and kc.is_contiguous() and vc.is_contiguous() and ks.is_contiguous() and vs.is_contiguous()
+    if ok and kc.dtype is torch.int8:
+        bits, dim = 8, shape[3]
+        ok = ks.dtype is torch.float32 and vs.dtype is torch.float32 \
+            and ks.shape == shape[:3] and vs.shape == shape[:3]
+    elif ok and kc.dtype is torch.uint8:
+        bits, dim = 4, shape[3] * 2
+        groups = shape[:3] + (dim // 32, 2)
+        ok = ks.dtype is torch.float16 and vs.dtype is torch.float16 \
+            and ks.shape == groups and vs.shape == groups
+    else:
+        ok = False
+    if not ok:
+        raise RuntimeError(_cache_fault(cache))
+    return KVCache(kc.data_ptr(), vc.data_ptr(), ks.data_ptr(), vs.data_ptr(), shape[0], shape[2],
+                   shape[1], dim, bits)
 
 
-def _slots(slots: torch.Tensor, tokens: int | None, dev) -> torch.Tensor:
-    if slots.dim() != 1 or slots.dtype != torch.int64 or slots.device != dev:
+def _slots(slots: torch.Tensor, dev: int) -> torch.Tensor:
+    if slots.dim() != 1 or slots.dtype is not torch.int64 or slots.get_device() != dev:
         raise RuntimeError("slots must be 1D int64 on the device of the cache")
-    if tokens is not None and slots.shape[0] != tokens:
-        raise RuntimeError("slots must hold a slot for each token")
-    return slots.contiguous()
+    return slots if slots.is_contiguous() else slots.contiguous()
 
 
 def cache_write(cache, k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor) -> None:
@@ -970,37 +1012,47 @@ def cache_write(cache, k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor) ->
     dev = cache.k_codes.device
     code = _dtype(k.dtype, "k", _DTYPES_16)
     for t, name in ((k, "k"), (v, "v")):
-        if t.dim() != 3 or tuple(t.shape[1:]) != (c.kv_heads, c.head_dim):
+        shape = t.shape
+        if len(shape) != 3 or shape[1] != c.kv_heads or shape[2] != c.head_dim:
             raise RuntimeError(f"{name} must be [tokens, {c.kv_heads}, {c.head_dim}]")
-        if t.device != dev or t.dtype != k.dtype:
+        if t.get_device() != dev.index or t.dtype is not k.dtype:
             raise RuntimeError(f"{name} must be on the device of the cache and of k's dtype")
-    if k.shape[0] != v.shape[0]:
-        raise RuntimeError("k and v must hold the same number of tokens")
     tokens = k.shape[0]
-    slots = _slots(slots, tokens, dev)
+    if v.shape[0] != tokens:
+        raise RuntimeError("k and v must hold the same number of tokens")
+    slots = _slots(slots, dev.index)
+    if slots.shape[0] != tokens:
+        raise RuntimeError("slots must hold a slot for each token")
     if tokens == 0:
         return
-    with torch.cuda.device(dev):
-        k, v = (t if t.stride(2) == 1 else t.contiguous() for t in (k, v))
-        n = int(_lib.mb_cache_write_workspace_size(tokens))
-        ws = torch.empty(n, dtype=torch.uint8, device=dev) if n else None
-        _check(_lib.mb_cache_write(ctypes.byref(c), _ptr(k), k.stride(0), k.stride(1), _ptr(v),
-                                   v.stride(0), v.stride(1), code, tokens, _ptr(slots), _ptr(ws),
-                                   n, _stream(dev)))
+    with _on(dev.index):
+        ks, vs = k.stride(), v.stride()
+        if ks[2] != 1:
+            k = k.contiguous()
+            ks = k.stride()
+        if vs[2] != 1:
+            v = v.contiguous()
+            vs = v.stride()
+        n = _lib.mb_cache_write_workspace_size(tokens)
+        ws = torch.empty((n,), dtype=torch.uint8, device=dev) if n else None
+        _check(_lib.mb_cache_write(ctypes.byref(c), k.data_ptr(), ks[0], ks[1], v.data_ptr(),
+                                   vs[0], vs[1], code, tokens, slots.data_ptr(),
+                                   ws.data_ptr() if n else None, n, _raw_stream(dev.index)))
 
 
 def cache_read(cache, slots: torch.Tensor, dtype: torch.dtype):
     c = _cache_struct(cache)
     dev = cache.k_codes.device
     code = _dtype(dtype, "dtype")
-    slots = _slots(slots, None, dev)
+    slots = _slots(slots, dev.index)
     tokens = slots.shape[0]
-    with torch.cuda.device(dev):
-        k, v = (torch.empty((tokens, c.kv_heads, c.head_dim), dtype=dtype, device=dev)
-                for _ in range(2))
+    with _on(dev.index):
+        shape = (tokens, c.kv_heads, c.head_dim)
+        k = torch.empty(shape, dtype=dtype, device=dev)
+        v = torch.empty(shape, dtype=dtype, device=dev)
         if tokens > 0:
-            _check(_lib.mb_cache_read(ctypes.byref(c), _ptr(slots), tokens, _ptr(k), _ptr(v),
-                                      code, _stream(dev)))
+            _check(_lib.mb_cache_read(ctypes.byref(c), slots.data_ptr(), tokens, k.data_ptr(),
+                                      v.data_ptr(), code, _raw_stream(dev.index)))
     return k, v
 
 
@@ -1009,33 +1061,42 @@ def cache_attention(q: torch.Tensor, cache, page_table: torch.Tensor, lengths: t
     c = _cache_struct(cache)
     dev = cache.k_codes.device
     code = _dtype(q.dtype, "q", _DTYPES_16)
-    if q.dim() != 3 or q.shape[2] != c.head_dim or q.device != dev:
+    shape = q.shape
+    if len(shape) != 3 or shape[2] != c.head_dim or q.get_device() != dev.index:
         raise RuntimeError(f"q must be [batch, heads, {c.head_dim}] on the device of the cache")
-    batch, heads = q.shape[:2]
+    batch, heads = shape[0], shape[1]
     if heads == 0 or heads % c.kv_heads != 0:
         raise RuntimeError(f"q's heads must be a multiple of the cache's {c.kv_heads}")
-    if page_table.dim() != 2 or page_table.dtype != torch.int32 or page_table.device != dev \
-            or page_table.shape[0] != batch:
+    if page_table.dim() != 2 or page_table.dtype is not torch.int32 \
+            or page_table.get_device() != dev.index or page_table.shape[0] != batch:
         raise RuntimeError("page_table must be int32 [batch, pages] on the device of the cache")
-    if tuple(lengths.shape) != (batch,) or lengths.dtype != torch.int32 or lengths.device != dev:
+    if lengths.dim() != 1 or lengths.shape[0] != batch or lengths.dtype is not torch.int32 \
+            or lengths.get_device() != dev.index:
         raise RuntimeError("lengths must be int32 [batch] on the device of the cache")
-    if out is not None and (out.dtype != q.dtype or out.shape != q.shape or out.device != dev
+    if out is not None and (out.dtype != q.dtype or out.shape != shape or out.device != dev
                             or not out.is_contiguous()):
         raise RuntimeError("out must be a contiguous tensor of q's shape, dtype and device")
-    with torch.cuda.device(dev):
+    with _on(dev.index):
         if out is None:
-            out = torch.empty((batch, heads, c.head_dim), dtype=q.dtype, device=dev)
+            out = torch.empty(shape, dtype=q.dtype, device=dev)
         if batch == 0:
             return out
-        q = q if q.stride(2) == 1 else q.contiguous()
+        qs = q.stride()
+        if qs[2] != 1:
+            q = q.contiguous()
+            qs = q.stride()
         width = page_table.shape[1]
-        if width > 1 and page_table.stride(1) != 1:
+        table_stride, step = page_table.stride()
+        if step != 1 and width > 1:
             page_table = page_table.contiguous()
-        lengths = lengths.contiguous()
-        n = int(_lib.mb_cache_attention_workspace_size(ctypes.byref(c), batch, heads, width))
-        ws = torch.empty(n, dtype=torch.uint8, device=dev) if n else None
-        _check(_lib.mb_cache_attention(ctypes.byref(c), _ptr(q), q.stride(0), q.stride(1), code,
-                                       batch, heads, _ptr(page_table), page_table.stride(0),
-                                       width, _ptr(lengths), float(scale), _ptr(out), _ptr(ws), n,
-                                       _stream(dev)))
+            table_stride = width
+        if not lengths.is_contiguous():
+            lengths = lengths.contiguous()
+        cache_ref = ctypes.byref(c)
+        n = _lib.mb_cache_attention_workspace_size(cache_ref, batch, heads, width)
+        ws = torch.empty((n,), dtype=torch.uint8, device=dev) if n else None
+        _check(_lib.mb_cache_attention(cache_ref, q.data_ptr(), qs[0], qs[1], code, batch, heads,
+                                       page_table.data_ptr(), table_stride, width,
+                                       lengths.data_ptr(), scale, out.data_ptr(),
+                                       ws.data_ptr() if n else None, n, _raw_stream(dev.index)))
     return out

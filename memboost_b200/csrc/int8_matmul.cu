@@ -363,3 +363,28 @@ extern "C" mb_status mb_int8_matmul(const int8_t* a_codes, int64_t a_stride, con
     default: return launch<256>(a_codes, a_stride, M, b_codes, b_stride, N, K, e, parts, stream);
   }
 }
+
+extern "C" size_t mb_int8_linear_workspace_size(int64_t M, int64_t K) {
+  if (M <= 0 || K <= 0) return 0;
+  return (size_t)M * ((size_t)ceil_div(K, 16) * 16 + sizeof(float));
+}
+
+extern "C" mb_status mb_int8_linear(const void* x, mb_dtype x_type, int64_t x_stride, int64_t M,
+                                    const int8_t* b_codes, int64_t b_stride, const float* b_scales,
+                                    int64_t N, int64_t K, const void* bias, mb_dtype bias_type,
+                                    void* out, mb_dtype out_type, int64_t out_stride,
+                                    void* workspace, size_t workspace_bytes, mb_stream_t stream) {
+  clear_error();
+  MB_REQUIRE(M > 0 && K > 0, "M, N and K must be positive");
+  MB_REQUIRE(M <= (int64_t(1) << 23) && K <= MB_INT8_MAX_K, "M or K too large");
+  if (workspace == nullptr || !aligned(workspace, 16) ||
+      workspace_bytes < mb_int8_linear_workspace_size(M, K))
+    return set_error(MB_ERR_WORKSPACE, "int8_linear workspace missing, misaligned or too small");
+  const int64_t pitch = ceil_div(K, 16) * 16;
+  int8_t* codes = static_cast<int8_t*>(workspace);
+  float* scales = reinterpret_cast<float*>(codes + M * pitch);
+  const mb_status st = mb_int8_quantize(x, x_type, M, K, x_stride, codes, pitch, scales, stream);
+  if (st != MB_OK) return st;
+  return mb_int8_matmul(codes, pitch, scales, M, b_codes, b_stride, b_scales, N, K, bias,
+                        bias_type, out, out_type, out_stride, stream);
+}

@@ -89,7 +89,9 @@ def test_rows_of_zeros_nan_infinity_and_tiny():
 @pytest.mark.parametrize("dtype", TYPES, ids=IDS)
 def test_rows_strides(dtype):
     x = _x(40, 121, dtype, seed=3).cuda()
-    for view in (x[:, 1:], x[::3, 5:70], x[1:, :64], x.t(), x[7], x.view(4, 10, 121)):
+    for view in (x[:, 1:], x[::3, 5:70], x[1:, :64], x.t(), x[7], x.view(4, 10, 121),
+                 x[:1].expand(5, 121), x[:, :1].expand(40, 30), x.view(4, 10, 121)[:, ::2],
+                 x.view(4, 10, 121).transpose(0, 1), x[:, :1], x.t()[:, :1]):
         t = mb.quantize_int8(view)
         _check_rows(t, view.reshape(-1, view.shape[-1]))
 

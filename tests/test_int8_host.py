@@ -149,6 +149,23 @@ def test_matmul_entry_refusals(change, words):
                                       None), words)
 
 
+def test_linear_entry_refusals():
+    lib = _c()._lib
+    n = lib.mb_int8_linear_workspace_size(3, 33)
+    assert n == 3 * (48 + 4) and lib.mb_int8_linear_workspace_size(0, 33) == 0
+
+    def call(x=P, t=0, M=3, K=33, b=P, ws=P, nbytes=n, out=P):
+        return lib.mb_int8_linear(x, t, 33, M, b, 48, P, 4, K, None, 0, out, 0, 4, ws, nbytes, None)
+
+    _refused(call(M=0), "positive")
+    _refused(call(K=131073), "too large")
+    _refused(call(nbytes=n - 1), "workspace")
+    _refused(call(ws=None), "workspace")
+    _refused(call(ws=P + 8), "workspace")
+    _refused(call(x=None), "null")
+    _refused(call(t=5), "unknown type")
+
+
 CACHE = dict(k_codes=P, v_codes=P, k_scales=P, v_scales=P, pages=4, page_size=16, kv_heads=2,
              head_dim=64, bits=8)
 
