@@ -228,12 +228,12 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll 1
       for (int c = 0; c < kN && m0 + c < M; c += 16) {
         uint32_t v[16];
+        __syncwarp();
         tmem_ld16(lanes + c, v);
-        if (!live) continue;
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
           const int64_t m = m0 + c + i;
-          if (m >= M) break;
+          if (m >= M || !live) break;
           const float sa = failed ? __uint_as_float(0x7FC00000u) : e.a_scales[m];
           put(e, m, n, __fadd_rn(__fmul_rn(__fmul_rn((float)(int)v[i], sa), sb), bias));
         }
@@ -274,6 +274,196 @@ __global__ void __launch_bounds__(kThreads, 1)
   if (warp == 0)
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem),
                  "r"(S::kTmem));
+}
+
+// ---------------------------------------------------------------------------
+// Many tokens: pairs of CTAs (tcgen05 cta_group::2), persistent.
+// ---------------------------------------------------------------------------
+// A pair's tile is 256 channels by 256 tokens; each CTA loads its 128
+// channels and half of the tokens, and keeps the sums of its channels with
+// all 256 tokens (256 TMEM columns, twice: the products of the next tile run
+// while the last one is drained).  A stage is 32 KB a CTA instead of the 48
+// KB of a lone CTA's 128 x 256 tile: shared memory is read 8 KB (the 128
+// weights' 32 bytes, half the tokens') instead of 12 for the same products.
+constexpr int kPairTokens = 256;                       // tokens a tile
+constexpr int kPairStage = kWeightBytes + kPairTokens / 2 * kStepK;  // of one CTA
+constexpr int kPairStages = 6;
+constexpr int kPairSmem = kPairStages * kPairStage + 1024;
+constexpr int kPairGroup = 8;                          // token tiles taken together
+
+__host__ __device__ constexpr uint32_t pair_idesc() {
+  return (2u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(kPairTokens >> 3) << 17) |
+         ((uint32_t)(2 * kChannels >> 4) << 24);
+}
+
+// A load whose bytes count on the pair's first CTA's barrier.
+__device__ __forceinline__ void pair_load(void* dst, const CUtensorMap* map, uint32_t bar, int x,
+                                          int y) {
+  asm volatile(
+      "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes"
+      " [%0], [%1, {%3, %4}], [%2];" ::"r"(smem_u32(dst)),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(bar), "r"(x), "r"(y)
+      : "memory");
+}
+
+__device__ __forceinline__ void pair_umma_i8(uint32_t tmem_d, uint64_t a, uint64_t b,
+                                             uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::2.kind::i8 [%0], %1, %2, %3, p;\n\t}" ::"r"(tmem_d),
+      "l"(a), "l"(b), "r"(pair_idesc()), "r"(accumulate));
+}
+
+// Arrives on the barrier of both CTAs once the products issued so far are done.
+__device__ __forceinline__ void pair_commit(uint64_t* bar) {
+  asm volatile(
+      "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 "
+      "[%0], %1;" ::"r"(smem_u32(bar)),
+      "h"((uint16_t)3)
+      : "memory");
+}
+
+__device__ __forceinline__ void arrive_cluster(uint32_t bar) {
+  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar)
+               : "memory");
+}
+
+// Tile -> (channel tile, token tile): kPairGroup token tiles by all channel
+// tiles, tokens fastest, so that the tiles in flight share operands in L2.
+__device__ __forceinline__ void pair_tile(uint32_t t, uint32_t channel_tiles, uint32_t token_tiles,
+                                          uint32_t& cn, uint32_t& cm) {
+  const uint32_t per = channel_tiles * kPairGroup, group = t / per, in = t - group * per;
+  const uint32_t first = group * kPairGroup, high = min(token_tiles - first, (uint32_t)kPairGroup);
+  cn = in / high;
+  cm = first + in - cn * high;
+}
+
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
+    int8_matmul_pair_kernel(const __grid_constant__ CUtensorMap tokens,
+                            const __grid_constant__ CUtensorMap weights, int64_t M, int64_t N,
+                            int64_t K, Epilogue e) {
+  extern __shared__ uint8_t raw[];
+  uint8_t* ring = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(raw) + 1023) &
+                                             ~(uintptr_t)1023);
+  __shared__ uint64_t full[kPairStages], empty[kPairStages], drain[2], drained[2];
+  __shared__ uint32_t tmem_slot;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t rank = cluster_rank();
+  const uint32_t channel_tiles = (uint32_t)ceil_div(N, 2 * kChannels);
+  const uint32_t token_tiles = (uint32_t)ceil_div(M, kPairTokens);
+  const uint32_t tiles = channel_tiles * token_tiles;
+  const uint32_t first = blockIdx.x / 2, stride = gridDim.x / 2;
+  const int steps = (int)ceil_div(K, kStepK);
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < kPairStages; ++s) {
+      mbar_init(&full[s], 1);
+      mbar_init(&empty[s], 1);
+    }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&drain[i], 1);
+      mbar_init(&drained[i], 8);  // four warps of both CTAs
+    }
+    fence_mbar_init();
+  }
+  if (warp == 0) {
+    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(
+                     smem_u32(&tmem_slot)),
+                 "r"(2 * kPairTokens));
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;");
+  }
+  asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+  __syncthreads();
+  cluster_sync();
+  asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+  const uint32_t tmem = tmem_slot;
+
+  if (warp == 4 && lane == 0) {
+    int i = 0;
+    bool ok = true;
+    for (uint32_t t = first; t < tiles && ok; t += stride) {
+      uint32_t cn, cm;
+      pair_tile(t, channel_tiles, token_tiles, cn, cm);
+      const int n0 = (int)(cn * 2 + rank) * kChannels;
+      const int m0 = (int)(cm * kPairTokens + rank * (kPairTokens / 2));
+      for (int k = 0; k < steps; ++k, ++i) {
+        const int s = i % kPairStages;
+        if (i >= kPairStages && !mbar_wait(&empty[s], (uint32_t)((i / kPairStages - 1) & 1))) {
+          ok = false;
+          break;
+        }
+        uint8_t* at = ring + s * kPairStage;
+        const uint32_t bar = cluster_address(smem_u32(&full[s]), 0);
+        if (rank == 0) mbar_arrive_expect_tx(&full[s], 2 * kPairStage);
+        pair_load(at, &weights, bar, k * kStepK, n0);
+        pair_load(at + kWeightBytes, &tokens, bar, k * kStepK, m0);
+      }
+    }
+    // Both CTAs' last loads are read by products before anyone leaves.
+    for (int b = i > kPairStages ? i - kPairStages : 0; b < i; ++b)
+      mbar_wait(&empty[b % kPairStages], (uint32_t)((b / kPairStages) & 1));
+  } else if (warp == 5 && lane == 0 && rank == 0) {
+    int i = 0, a = 0;
+    bool ok = true;
+    for (uint32_t t = first; t < tiles && ok; t += stride, ++a) {
+      const int buf = a & 1;
+      if (a >= 2 && !mbar_wait(&drained[buf], (uint32_t)((a / 2 - 1) & 1))) break;
+      asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+      for (int k = 0; k < steps; ++k, ++i) {
+        const int s = i % kPairStages;
+        if (!mbar_wait(&full[s], (uint32_t)((i / kPairStages) & 1))) {
+          ok = false;
+          break;
+        }
+        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+        const uint32_t w = smem_u32(ring + s * kPairStage), x = w + kWeightBytes;
+#pragma unroll
+        for (int q = 0; q < kStepK / 32; ++q)
+          pair_umma_i8(tmem + buf * kPairTokens, umma_desc_k_sw128(w + 32 * q),
+                       umma_desc_k_sw128(x + 32 * q), (k > 0 || q > 0) ? 1u : 0u);
+        pair_commit(&empty[s]);
+      }
+      if (ok) pair_commit(&drain[buf]);
+    }
+  } else if (warp < 4) {
+    int a = 0;
+    bool ok = true;
+    for (uint32_t t = first; t < tiles; t += stride, ++a) {
+      const int buf = a & 1;
+      uint32_t cn, cm;
+      pair_tile(t, channel_tiles, token_tiles, cn, cm);
+      const int64_t n = (int64_t)(cn * 2 + rank) * kChannels + 32 * warp + lane;
+      const int64_t m0 = (int64_t)cm * kPairTokens;
+      const bool live = n < N;
+      const float sb = live ? e.b_scales[n] : 0.0f, bias = live ? bias_at(e, n) : 0.0f;
+      ok = ok && mbar_wait(&drain[buf], (uint32_t)((a / 2) & 1));
+      asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+      __syncwarp();
+      const uint32_t at = tmem + buf * kPairTokens + ((uint32_t)(32 * warp) << 16);
+#pragma unroll 1
+      for (int c = 0; c < kPairTokens && m0 + c < M; c += 16) {
+        uint32_t v[16];
+        __syncwarp();
+        tmem_ld16(at + c, v);
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          const int64_t m = m0 + c + i;
+          if (m >= M || !live) break;
+          const float sa = ok ? e.a_scales[m] : __uint_as_float(0x7FC00000u);
+          put(e, m, n, __fadd_rn(__fmul_rn(__fmul_rn((float)(int)v[i], sa), sb), bias));
+        }
+      }
+      asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+      __syncwarp();
+      if (lane == 0) arrive_cluster(cluster_address(smem_u32(&drained[buf]), 0));
+    }
+  }
+  __syncwarp();
+  __syncthreads();
+  cluster_sync();  // no CTA leaves while the other's barriers or products need it
+  if (warp == 0)
+    asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem),
+                 "r"(2 * kPairTokens));
 }
 
 // [rows, K] codes, boxes of 128 bytes by box_rows.
@@ -319,6 +509,23 @@ mb_status launch(const int8_t* a_codes, int64_t a_stride, int64_t M, const int8_
   return MB_OK;
 }
 
+mb_status launch_pairs(const int8_t* a_codes, int64_t a_stride, int64_t M, const int8_t* b_codes,
+                       int64_t b_stride, int64_t N, int64_t K, const Epilogue& e,
+                       cudaStream_t stream) {
+  static std::atomic<uint64_t> attr_done{0};
+  MB_CUDA_TRY(set_smem_limit_once(int8_matmul_pair_kernel, kPairSmem, attr_done));
+  CUtensorMap tokens, weights;
+  if (!codes_map(&tokens, a_codes, a_stride, M, K, kPairTokens / 2) ||
+      !codes_map(&weights, b_codes, b_stride, N, K, kChannels))
+    return set_error(MB_ERR_CUDA, "cuTensorMapEncodeTiled rejected the codes");
+  const int64_t tiles = ceil_div(N, 2 * kChannels) * ceil_div(M, kPairTokens);
+  MB_REQUIRE(tiles < (int64_t(1) << 31), "M or N too large");
+  int8_matmul_pair_kernel<<<(unsigned)(2 * min64(tiles, 74)), kThreads, kPairSmem, stream>>>(
+      tokens, weights, M, N, K, e);
+  MB_LAUNCH_CHECK("int8_matmul_pair_kernel");
+  return MB_OK;
+}
+
 }  // namespace
 }  // namespace mb
 
@@ -350,6 +557,9 @@ extern "C" mb_status mb_int8_matmul(const int8_t* a_codes, int64_t a_stride, con
   if (N == 1) b_stride = ceil_div(K, 16) * 16;
   cudaStream_t stream = reinterpret_cast<cudaStream_t>(stream_);
   const Epilogue e{a_scales, b_scales, bias, out, out_stride, (int)bias_type, (int)out_type};
+  // pairs where their tiles give every pair of SMs work
+  if (ceil_div(N, 2 * kChannels) * ceil_div(M, kPairTokens) >= 74)
+    return launch_pairs(a_codes, a_stride, M, b_codes, b_stride, N, K, e, stream);
   const int kn = M <= 16 ? 16 : M <= 32 ? 32 : M <= 64 ? 64 : M <= 128 ? 128 : 256;
   // K parts: until the tiles fill the SMs, each part at least two steps
   const int64_t tiles = ceil_div(N, kChannels) * ceil_div(M, kn), steps = ceil_div(K, kStepK);

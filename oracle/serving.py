@@ -27,8 +27,8 @@ def dequantize_rows(codes, scales):
 
 
 def matmul(a_codes, a_scales, b_codes, b_scales, bias=None):
-    """(y, |scaled sums|) in 64 bits; the integer sums are exact in int64."""
-    acc = (a_codes.astype(np.int64) @ b_codes.astype(np.int64).T).astype(np.float64)
+    """(y, |scaled sums|) in 64 bits; the integer sums (below 2^31) are exact."""
+    acc = a_codes.astype(np.float64) @ b_codes.astype(np.float64).T
     y = acc * a_scales.astype(np.float64)[:, None] * b_scales.astype(np.float64)[None, :]
     mag = np.abs(y)
     return (y if bias is None else y + np.asarray(bias, np.float64)), mag

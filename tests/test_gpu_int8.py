@@ -124,7 +124,8 @@ def _check_product(y, a, w, bias=None):
 SIZES = [(1, 1, 1), (1, 16, 16), (2, 8, 33), (3, 130, 64), (17, 4096, 1000), (16, 257, 128),
          (33, 65, 129), (64, 64, 4096), (65, 4100, 40), (100, 1000, 1001), (129, 129, 257),
          (128, 256, 512), (257, 513, 300), (300, 40, 2050), (1, 5000, 11008), (520, 768, 1024),
-         (1000, 3, 70), (7, 40, 20000)]
+         (1000, 3, 70), (7, 40, 20000), (2300, 2100, 300),
+         (4100, 1300, 40), (300, 19100, 1700), (2049, 2561, 2049)]
 
 
 @pytest.mark.parametrize("dtype", TYPES, ids=IDS)
