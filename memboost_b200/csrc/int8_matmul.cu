@@ -116,7 +116,7 @@ struct Epilogue {
   const void* bias;
   void* out;
   int64_t out_stride;
-  int bias_type, out_type;
+  int bias_type;
 };
 
 __device__ __forceinline__ float bias_at(const Epilogue& e, int64_t n) {
@@ -126,19 +126,39 @@ __device__ __forceinline__ float bias_at(const Epilogue& e, int64_t n) {
                                   : static_cast<const float*>(e.bias)[n];
 }
 
-__device__ __forceinline__ void put(const Epilogue& e, int64_t m, int64_t n, float y) {
-  const int64_t i = m * e.out_stride + n;
-  if (e.out_type == MB_FP16)
-    static_cast<__half*>(e.out)[i] = __float2half_rn(y);
-  else if (e.out_type == MB_BF16)
-    static_cast<__nv_bfloat16*>(e.out)[i] = __float2bfloat16_rn(y);
-  else
-    static_cast<float*>(e.out)[i] = y;
+__device__ __forceinline__ float scaled(int sum, float sa, float sb, float bias) {
+  return fmaf(__fmul_rn((float)sum, sa), sb, bias);
+}
+
+// A channel's (a lane's) sums with 16 tokens, `count` of which exist: sa in
+// shared memory (16-byte aligned), o the first token's place, the tokens
+// `stride` apart.  A warp writes 32 consecutive channels a token.
+template <typename Y>
+__device__ __forceinline__ void put16(const uint32_t (&v)[16], const float* sa, float sb,
+                                      float bias, Y* o, int64_t stride, int count) {
+  if (count >= 16) {
+#pragma unroll
+    for (int i = 0; i < 16; i += 4) {
+      const float4 s = *reinterpret_cast<const float4*>(sa + i);
+      o[0] = from_float<Y>(scaled((int)v[i], s.x, sb, bias));
+      o += stride;
+      o[0] = from_float<Y>(scaled((int)v[i + 1], s.y, sb, bias));
+      o += stride;
+      o[0] = from_float<Y>(scaled((int)v[i + 2], s.z, sb, bias));
+      o += stride;
+      o[0] = from_float<Y>(scaled((int)v[i + 3], s.w, sb, bias));
+      o += stride;
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 16; ++i)
+      if (i < count) o[i * stride] = from_float<Y>(scaled((int)v[i], sa[i], sb, bias));
+  }
 }
 
 // Grid: x = cluster (a tile's K parts) fastest, then channel tiles; y = token
 // tiles.
-template <int kN>
+template <int kN, typename Y>
 __global__ void __launch_bounds__(kThreads, 1)
     int8_matmul_kernel(const __grid_constant__ CUtensorMap tokens,
                        const __grid_constant__ CUtensorMap weights, int64_t M, int64_t N,
@@ -149,6 +169,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                                              ~(uintptr_t)1023);
   __shared__ uint64_t full[S::kStages], empty[S::kStages], done;
   __shared__ uint32_t tmem_slot, failed;
+  __shared__ __align__(16) float a_scale[kN];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint32_t parts = cluster_size(), part = cluster_rank();
   const int64_t n0 = (int64_t)(blockIdx.x / parts) * kChannels, m0 = (int64_t)blockIdx.y * kN;
@@ -215,56 +236,53 @@ __global__ void __launch_bounds__(kThreads, 1)
     if (!ok) atomicExch(&failed, 1u);
   }
   __syncwarp();
+  if (warp < 4)
+    for (int i = threadIdx.x; i < kN; i += 128) a_scale[i] = m0 + i < M ? e.a_scales[m0 + i] : 0.0f;
   if (!mbar_wait(&done, 0)) atomicExch(&failed, 1u);
   asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
   __syncthreads();  // `failed` is final; the ring is free
 
   const int64_t n = n0 + 32 * warp + lane;  // warps 0-3: this thread's channel
+  const bool live = warp < 4 && n < N;
   const uint32_t lanes = tmem + ((uint32_t)(32 * (warp & 3)) << 16);
+  const int columns = (int)min64(kN, M - m0);
+  float sb = live ? e.b_scales[n] : 0.0f;
+  const float bias = live ? bias_at(e, n) : 0.0f;
+  Y* o = static_cast<Y*>(e.out) + m0 * e.out_stride + n;
   if (parts == 1) {
-    if (warp < 4) {
-      const bool live = n < N;
-      const float sb = live ? e.b_scales[n] : 0.0f, bias = live ? bias_at(e, n) : 0.0f;
-#pragma unroll 1
-      for (int c = 0; c < kN && m0 + c < M; c += 16) {
-        uint32_t v[16];
-        __syncwarp();
-        tmem_ld16(lanes + c, v);
-#pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          const int64_t m = m0 + c + i;
-          if (m >= M || !live) break;
-          const float sa = failed ? __uint_as_float(0x7FC00000u) : e.a_scales[m];
-          put(e, m, n, __fadd_rn(__fmul_rn(__fmul_rn((float)(int)v[i], sa), sb), bias));
-        }
-      }
-    }
-  } else {
-    int* own = reinterpret_cast<int*>(ring);  // [token][channel]
-    const int columns = (int)min64(kN, M - m0);
+    if (failed) sb = __uint_as_float(0x7FC00000u);
     if (warp < 4) {
 #pragma unroll 1
       for (int c = 0; c < columns; c += 16) {
         uint32_t v[16];
-        if (steps > 0) tmem_ld16(lanes + c, v);
+        __syncwarp();
+        tmem_ld16(lanes + c, v);
+        if (live)
+          put16<Y>(v, a_scale + c, sb, bias, o + c * e.out_stride, e.out_stride, columns - c);
+      }
+    }
+  } else {
+    int* own = reinterpret_cast<int*>(ring);  // [token][channel]
+    if (warp < 4) {
+#pragma unroll 1
+      for (int c = 0; c < columns; c += 16) {
+        uint32_t v[16];
+        tmem_ld16(lanes + c, v);
 #pragma unroll
-        for (int i = 0; i < 16; ++i)
-          own[(c + i) * kChannels + 32 * warp + lane] = steps > 0 ? (int)v[i] : 0;
+        for (int i = 0; i < 16; ++i) own[(c + i) * kChannels + 32 * warp + lane] = (int)v[i];
       }
     }
     cluster_sync();
     const uint32_t base = smem_u32(own), fail = smem_u32(&failed);
-    bool bad = false;
-    for (uint32_t r = 0; r < parts; ++r) bad |= load_cluster(cluster_address(fail, r)) != 0;
+    for (uint32_t r = 0; r < parts; ++r)
+      if (load_cluster(cluster_address(fail, r)) != 0) sb = __uint_as_float(0x7FC00000u);
     // this CTA's share of the tile's tokens, a channel a thread
-    if (warp < 4 && n < N) {
-      const float sb = e.b_scales[n], bias = bias_at(e, n);
+    if (live) {
       for (int c = (int)part; c < columns; c += (int)parts) {
         int sum = 0;
         for (uint32_t r = 0; r < parts; ++r)
           sum += load_cluster(cluster_address(base + (c * kChannels + 32 * warp + lane) * 4, r));
-        const float sa = bad ? __uint_as_float(0x7FC00000u) : e.a_scales[m0 + c];
-        put(e, m0 + c, n, __fadd_rn(__fmul_rn(__fmul_rn((float)sum, sa), sb), bias));
+        o[c * e.out_stride] = from_float<Y>(scaled(sum, a_scale[c], sb, bias));
       }
     }
     cluster_sync();  // no CTA leaves while another reads its part
@@ -338,6 +356,7 @@ __device__ __forceinline__ void pair_tile(uint32_t t, uint32_t channel_tiles, ui
   cm = first + in - cn * high;
 }
 
+template <typename Y>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     int8_matmul_pair_kernel(const __grid_constant__ CUtensorMap tokens,
                             const __grid_constant__ CUtensorMap weights, int64_t M, int64_t N,
@@ -347,6 +366,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
                                              ~(uintptr_t)1023);
   __shared__ uint64_t full[kPairStages], empty[kPairStages], drain[2], drained[2];
   __shared__ uint32_t tmem_slot;
+  __shared__ __align__(16) float a_scale[2][kPairTokens];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint32_t rank = cluster_rank();
   const uint32_t channel_tiles = (uint32_t)ceil_div(N, 2 * kChannels);
@@ -435,23 +455,25 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
       const int64_t n = (int64_t)(cn * 2 + rank) * kChannels + 32 * warp + lane;
       const int64_t m0 = (int64_t)cm * kPairTokens;
       const bool live = n < N;
-      const float sb = live ? e.b_scales[n] : 0.0f, bias = live ? bias_at(e, n) : 0.0f;
+      float sb = live ? e.b_scales[n] : 0.0f;
+      const float bias = live ? bias_at(e, n) : 0.0f;
+      for (int i = threadIdx.x; i < kPairTokens; i += 128)
+        a_scale[buf][i] = m0 + i < M ? e.a_scales[m0 + i] : 0.0f;
+      // the four warps: the scales are there; those of two tiles ago are read
+      asm volatile("bar.sync 1, 128;" ::: "memory");
       ok = ok && mbar_wait(&drain[buf], (uint32_t)((a / 2) & 1));
+      if (!ok) sb = __uint_as_float(0x7FC00000u);
       asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-      __syncwarp();
       const uint32_t at = tmem + buf * kPairTokens + ((uint32_t)(32 * warp) << 16);
+      const int columns = (int)min64(kPairTokens, M - m0);
+      Y* o = static_cast<Y*>(e.out) + m0 * e.out_stride + n;
 #pragma unroll 1
-      for (int c = 0; c < kPairTokens && m0 + c < M; c += 16) {
+      for (int c = 0; c < columns; c += 16) {
         uint32_t v[16];
         __syncwarp();
         tmem_ld16(at + c, v);
-#pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          const int64_t m = m0 + c + i;
-          if (m >= M || !live) break;
-          const float sa = ok ? e.a_scales[m] : __uint_as_float(0x7FC00000u);
-          put(e, m, n, __fadd_rn(__fmul_rn(__fmul_rn((float)(int)v[i], sa), sb), bias));
-        }
+        if (live)
+          put16<Y>(v, a_scale[buf] + c, sb, bias, o + c * e.out_stride, e.out_stride, columns - c);
       }
       asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
       __syncwarp();
@@ -482,13 +504,13 @@ bool codes_map(CUtensorMap* map, const int8_t* codes, int64_t stride, int64_t ro
          CUDA_SUCCESS;
 }
 
-template <int kN>
+template <int kN, typename Y>
 mb_status launch(const int8_t* a_codes, int64_t a_stride, int64_t M, const int8_t* b_codes,
                  int64_t b_stride, int64_t N, int64_t K, const Epilogue& e, int parts,
                  cudaStream_t stream) {
   using S = Shape<kN>;
   static std::atomic<uint64_t> attr_done{0};
-  MB_CUDA_TRY(set_smem_limit_once(int8_matmul_kernel<kN>, S::kSmem, attr_done));
+  MB_CUDA_TRY(set_smem_limit_once(int8_matmul_kernel<kN, Y>, S::kSmem, attr_done));
   CUtensorMap tokens, weights;
   if (!codes_map(&tokens, a_codes, a_stride, M, K, kN) ||
       !codes_map(&weights, b_codes, b_stride, N, K, kChannels))
@@ -505,25 +527,51 @@ mb_status launch(const int8_t* a_codes, int64_t a_stride, int64_t M, const int8_
   attr[0].val.clusterDim.z = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  MB_CUDA_TRY(cudaLaunchKernelEx(&cfg, int8_matmul_kernel<kN>, tokens, weights, M, N, K, e));
+  MB_CUDA_TRY(cudaLaunchKernelEx(&cfg, int8_matmul_kernel<kN, Y>, tokens, weights, M, N, K, e));
   return MB_OK;
 }
 
+template <typename Y>
 mb_status launch_pairs(const int8_t* a_codes, int64_t a_stride, int64_t M, const int8_t* b_codes,
                        int64_t b_stride, int64_t N, int64_t K, const Epilogue& e,
                        cudaStream_t stream) {
   static std::atomic<uint64_t> attr_done{0};
-  MB_CUDA_TRY(set_smem_limit_once(int8_matmul_pair_kernel, kPairSmem, attr_done));
+  MB_CUDA_TRY(set_smem_limit_once(int8_matmul_pair_kernel<Y>, kPairSmem, attr_done));
   CUtensorMap tokens, weights;
   if (!codes_map(&tokens, a_codes, a_stride, M, K, kPairTokens / 2) ||
       !codes_map(&weights, b_codes, b_stride, N, K, kChannels))
     return set_error(MB_ERR_CUDA, "cuTensorMapEncodeTiled rejected the codes");
   const int64_t tiles = ceil_div(N, 2 * kChannels) * ceil_div(M, kPairTokens);
   MB_REQUIRE(tiles < (int64_t(1) << 31), "M or N too large");
-  int8_matmul_pair_kernel<<<(unsigned)(2 * min64(tiles, 74)), kThreads, kPairSmem, stream>>>(
+  int8_matmul_pair_kernel<Y><<<(unsigned)(2 * min64(tiles, 74)), kThreads, kPairSmem, stream>>>(
       tokens, weights, M, N, K, e);
   MB_LAUNCH_CHECK("int8_matmul_pair_kernel");
   return MB_OK;
+}
+
+template <typename Y>
+mb_status dispatch(const int8_t* a_codes, int64_t a_stride, int64_t M, const int8_t* b_codes,
+                   int64_t b_stride, int64_t N, int64_t K, const Epilogue& e,
+                   cudaStream_t stream) {
+  // pairs where their tiles give every pair of SMs work
+  if (ceil_div(N, 2 * kChannels) * ceil_div(M, kPairTokens) >= 74)
+    return launch_pairs<Y>(a_codes, a_stride, M, b_codes, b_stride, N, K, e, stream);
+  const int kn = M <= 16 ? 16 : M <= 32 ? 32 : M <= 64 ? 64 : M <= 128 ? 128 : 256;
+  // K parts: until the tiles fill the SMs, each part at least two steps
+  const int64_t tiles = ceil_div(N, kChannels) * ceil_div(M, kn), steps = ceil_div(K, kStepK);
+  int parts = 1;
+  while (parts < 8 && tiles * parts * 2 <= 148 && steps >= 4 * parts) parts *= 2;
+  const auto go = [&](auto size) {
+    return launch<decltype(size)::value, Y>(a_codes, a_stride, M, b_codes, b_stride, N, K, e,
+                                            parts, stream);
+  };
+  switch (kn) {
+    case 16: return go(std::integral_constant<int, 16>{});
+    case 32: return go(std::integral_constant<int, 32>{});
+    case 64: return go(std::integral_constant<int, 64>{});
+    case 128: return go(std::integral_constant<int, 128>{});
+    default: return go(std::integral_constant<int, 256>{});
+  }
 }
 
 }  // namespace
@@ -556,21 +604,14 @@ extern "C" mb_status mb_int8_matmul(const int8_t* a_codes, int64_t a_stride, con
   if (M == 1) a_stride = ceil_div(K, 16) * 16;
   if (N == 1) b_stride = ceil_div(K, 16) * 16;
   cudaStream_t stream = reinterpret_cast<cudaStream_t>(stream_);
-  const Epilogue e{a_scales, b_scales, bias, out, out_stride, (int)bias_type, (int)out_type};
-  // pairs where their tiles give every pair of SMs work
-  if (ceil_div(N, 2 * kChannels) * ceil_div(M, kPairTokens) >= 74)
-    return launch_pairs(a_codes, a_stride, M, b_codes, b_stride, N, K, e, stream);
-  const int kn = M <= 16 ? 16 : M <= 32 ? 32 : M <= 64 ? 64 : M <= 128 ? 128 : 256;
-  // K parts: until the tiles fill the SMs, each part at least two steps
-  const int64_t tiles = ceil_div(N, kChannels) * ceil_div(M, kn), steps = ceil_div(K, kStepK);
-  int parts = 1;
-  while (parts < 8 && tiles * parts * 2 <= 148 && steps >= 4 * parts) parts *= 2;
-  switch (kn) {
-    case 16: return launch<16>(a_codes, a_stride, M, b_codes, b_stride, N, K, e, parts, stream);
-    case 32: return launch<32>(a_codes, a_stride, M, b_codes, b_stride, N, K, e, parts, stream);
-    case 64: return launch<64>(a_codes, a_stride, M, b_codes, b_stride, N, K, e, parts, stream);
-    case 128: return launch<128>(a_codes, a_stride, M, b_codes, b_stride, N, K, e, parts, stream);
-    default: return launch<256>(a_codes, a_stride, M, b_codes, b_stride, N, K, e, parts, stream);
+  const Epilogue e{a_scales, b_scales, bias, out, out_stride, (int)bias_type};
+  switch (out_type) {
+    case MB_FP16:
+      return dispatch<__half>(a_codes, a_stride, M, b_codes, b_stride, N, K, e, stream);
+    case MB_BF16:
+      return dispatch<__nv_bfloat16>(a_codes, a_stride, M, b_codes, b_stride, N, K, e, stream);
+    default:
+      return dispatch<float>(a_codes, a_stride, M, b_codes, b_stride, N, K, e, stream);
   }
 }
 
