@@ -2,9 +2,11 @@
 // the reference): scale = max|x| / 127, code = x / scale to the nearest.
 //
 // Both directions are bound by memory: 3 bytes a value for the 16-bit types.
-// A row is read once: its threads keep the first 32 values each in registers
-// between the maximum and the codes (rows longer than that are read a second
-// time past it, from L2).
+// A row is read once: its threads keep what they loaded in registers between
+// the maximum and the codes (a row too long for that is read a second time
+// past it, from L2).  With many rows a warp takes a row alone, so nothing
+// waits at a barrier and each lane has up to 16 loads in flight; with few,
+// more threads share a row to shorten the call.
 #include <algorithm>
 
 #include "mb_codes.cuh"
@@ -12,64 +14,65 @@
 namespace mb {
 namespace {
 
-constexpr int kRowChunks = 4;  // 8-value pieces a thread keeps
-
-// T threads a row; CTAs of max(T, 256) threads.
-template <typename X, int T>
-__global__ void __launch_bounds__(T < 256 ? 256 : T)
+// T threads a row, kPieces pieces of 8 values a thread kept in registers;
+// CTAs of max(T, 128) threads.
+template <typename X, int T, int kPieces>
+__global__ void __launch_bounds__(T < 128 ? 128 : T)
     int8_quantize_kernel(const X* __restrict__ x, int64_t rows, int64_t K, int64_t x_stride,
                          bool x_vec, int8_t* __restrict__ codes, int64_t codes_stride,
                          float* __restrict__ scales) {
-  constexpr int kRows = T < 256 ? 256 / T : 1;
-  __shared__ uint32_t part[kRows][(T + 31) / 32];
+  constexpr int kRows = T < 128 ? 128 / T : 1;
   const int tid = threadIdx.x % T, sub = threadIdx.x / T;
   const int64_t row = (int64_t)blockIdx.x * kRows + sub;
-  const bool live = row < rows;
-  const X* xr = x + (live ? row : 0) * x_stride;
-  const int64_t n8 = live ? ceil_div(K, 8) : 0;
+  if (T <= 32 && row >= rows) return;  // whole warps; longer rows have a CTA each
+  const X* xr = x + row * x_stride;
+  const int n8 = (int)ceil_div(K, 8), k = (int)K;
 
-  float v[kRowChunks][8];
+  Raw8<X> v[kPieces];
   uint32_t m = 0;
 #pragma unroll
-  for (int j = 0; j < kRowChunks; ++j) {
-    const int64_t c = tid + (int64_t)j * T;
-    if (c < n8) load8(xr + 8 * c, x_vec, (int)min64(8, K - 8 * c), v[j]);
+  for (int j = 0; j < kPieces; ++j) {
+    const int c = tid + j * T;
+    if (c < n8) v[j].load(xr + 8 * c, x_vec, k - 8 * c);
   }
 #pragma unroll
-  for (int j = 0; j < kRowChunks; ++j)
-    if (tid + (int64_t)j * T < n8) m = max(m, abs_bits_max(v[j]));
-  for (int64_t c = tid + (int64_t)kRowChunks * T; c < n8; c += T) {
-    float u[8];
-    load8(xr + 8 * c, x_vec, (int)min64(8, K - 8 * c), u);
-    m = max(m, abs_bits_max(u));
+  for (int j = 0; j < kPieces; ++j)
+    if (tid + j * T < n8) m = v[j].abs_max(m);
+  for (int c = tid + kPieces * T; c < n8; c += T) {
+    Raw8<X> u;
+    u.load(xr + 8 * c, x_vec, k - 8 * c);
+    m = u.abs_max(m);
   }
-  m = __reduce_max_sync(0xffffffffu, m);
+  m = __reduce_max_sync(0xffffffffu, Raw8<X>::abs_max_bits(m));
   if constexpr (T > 32) {
-    if ((threadIdx.x & 31) == 0) part[sub][tid / 32] = m;
+    __shared__ uint32_t part[T / 32];
+    if ((threadIdx.x & 31) == 0) part[tid / 32] = m;
     __syncthreads();
-    for (int w = 0; w < T / 32; ++w) m = max(m, part[sub][w]);
+#pragma unroll
+    for (int w = 0; w < T / 32; ++w) m = max(m, part[w]);
   }
-  if (!live) return;
   const RowScale r = row_scale(m);
   if (tid == 0) scales[row] = r.scale;
   int8_t* cr = codes + row * codes_stride;
-  const auto put = [&](int64_t c, const float(&u)[8]) {
-    const uint2 q = codes8(u, r);
-    if (8 * c + 8 <= K) {
+  const auto put = [&](int c, const Raw8<X>& u) {
+    float f[8];
+    u.floats(f);
+    const uint2 q = codes8(f, r);
+    if (8 * c + 8 <= k) {
       *reinterpret_cast<uint2*>(cr + 8 * c) = q;
     } else {
-      for (int i = 0; i < (int)(K - 8 * c); ++i)
+      for (int i = 0; i < k - 8 * c; ++i)
         cr[8 * c + i] = (int8_t)((i < 4 ? q.x : q.y) >> (8 * (i & 3)));
     }
   };
 #pragma unroll
-  for (int j = 0; j < kRowChunks; ++j) {
-    const int64_t c = tid + (int64_t)j * T;
+  for (int j = 0; j < kPieces; ++j) {
+    const int c = tid + j * T;
     if (c < n8) put(c, v[j]);
   }
-  for (int64_t c = tid + (int64_t)kRowChunks * T; c < n8; c += T) {
-    float u[8];
-    load8(xr + 8 * c, x_vec, (int)min64(8, K - 8 * c), u);
+  for (int c = tid + kPieces * T; c < n8; c += T) {
+    Raw8<X> u;
+    u.load(xr + 8 * c, x_vec, k - 8 * c);
     put(c, u);
   }
 }
@@ -99,24 +102,32 @@ __global__ void __launch_bounds__(256)
   }
 }
 
-template <typename X, int T>
+template <typename X, int T, int kPieces>
 void launch_quantize(const void* x, int64_t rows, int64_t K, int64_t x_stride, bool x_vec,
                      int8_t* codes, int64_t codes_stride, float* scales, cudaStream_t stream) {
-  constexpr int kThreads = T < 256 ? 256 : T;
+  constexpr int kThreads = T < 128 ? 128 : T;
   const unsigned grid = (unsigned)ceil_div(rows, kThreads / T);
-  int8_quantize_kernel<X, T><<<grid, kThreads, 0, stream>>>(
+  int8_quantize_kernel<X, T, kPieces><<<grid, kThreads, 0, stream>>>(
       static_cast<const X*>(x), rows, K, x_stride, x_vec, codes, codes_stride, scales);
 }
 
 template <typename X>
 void dispatch_quantize(const void* x, int64_t rows, int64_t K, int64_t x_stride, bool x_vec,
                        int8_t* codes, int64_t codes_stride, float* scales, cudaStream_t stream) {
-  if (K <= 32 * 8 * kRowChunks)
-    launch_quantize<X, 32>(x, rows, K, x_stride, x_vec, codes, codes_stride, scales, stream);
-  else if (K <= 256 * 8 * kRowChunks)
-    launch_quantize<X, 256>(x, rows, K, x_stride, x_vec, codes, codes_stride, scales, stream);
+  const auto go = [&](auto threads, auto pieces) {
+    launch_quantize<X, decltype(threads)::value, decltype(pieces)::value>(
+        x, rows, K, x_stride, x_vec, codes, codes_stride, scales, stream);
+  };
+  constexpr int kDeep = sizeof(X) == 4 ? 8 : 16;  // pieces that leave registers for 16 warps
+  using std::integral_constant;
+  if (K <= 32 * 8 * 4)
+    go(integral_constant<int, 32>{}, integral_constant<int, 4>{});
+  else if (rows < 148 * 8)
+    go(integral_constant<int, 512>{}, integral_constant<int, 4>{});
+  else if (K <= 32 * 8 * kDeep)
+    go(integral_constant<int, 32>{}, integral_constant<int, kDeep>{});
   else
-    launch_quantize<X, 512>(x, rows, K, x_stride, x_vec, codes, codes_stride, scales, stream);
+    go(integral_constant<int, 128>{}, integral_constant<int, kDeep>{});
 }
 
 }  // namespace
@@ -132,6 +143,7 @@ extern "C" mb_status mb_int8_quantize(const void* x, mb_dtype x_type, int64_t ro
   MB_REQUIRE(dtype_known(x_type), "unknown type of x");
   MB_REQUIRE(rows > 0 && K > 0, "rows and K must be positive");
   MB_REQUIRE(rows < (int64_t(1) << 31), "too many rows");
+  MB_REQUIRE(K < (int64_t(1) << 31) - 8192, "K too large");
   MB_REQUIRE(rows == 1 || codes_stride >= K, "codes_stride must be at least K");
   MB_REQUIRE(aligned(codes, 16) && codes_stride % 16 == 0,
              "codes must begin on 16-byte boundaries");

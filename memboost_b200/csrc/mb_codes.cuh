@@ -4,6 +4,8 @@
 
 #include <cuda_bf16.h>
 
+#include <type_traits>
+
 #include "mb_common.cuh"
 
 namespace mb {
@@ -77,6 +79,69 @@ __device__ __forceinline__ void store8(T* __restrict__ p, bool vec, int n, const
   }
 }
 
+// Eight consecutive values as they are held (16 or 32 bytes), loaded as load8
+// does; 0 past n.
+template <typename T>
+struct Raw8 {
+  static constexpr int kWords = sizeof(T) * 2;
+  uint32_t w[kWords];
+
+  __device__ __forceinline__ void load(const T* __restrict__ p, bool vec, int n) {
+    if (vec && n >= 8) {
+#pragma unroll
+      for (int i = 0; i < kWords / 4; ++i) {
+        const uint4 u = reinterpret_cast<const uint4*>(p)[i];
+        w[4 * i] = u.x; w[4 * i + 1] = u.y; w[4 * i + 2] = u.z; w[4 * i + 3] = u.w;
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < kWords; ++i) w[i] = 0u;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        if (i >= n) break;
+        if constexpr (sizeof(T) == 4)
+          w[i] = __float_as_uint(p[i]);
+        else
+          w[i / 2] |= (uint32_t)reinterpret_cast<const uint16_t*>(p)[i] << (16 * (i & 1));
+      }
+    }
+  }
+
+  __device__ __forceinline__ void floats(float (&v)[8]) const {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      if constexpr (sizeof(T) == 4)
+        v[i] = __uint_as_float(w[i]);
+      else if constexpr (std::is_same_v<T, __half>)
+        v[i] = __half2float(__ushort_as_half((uint16_t)(w[i / 2] >> (16 * (i & 1)))));
+      else  // bf16 is the upper half of an fp32
+        v[i] = __uint_as_float(i & 1 ? w[i / 2] & 0xFFFF0000u : w[i / 2] << 16);
+    }
+  }
+
+  // max(m, |values|), two 16-bit magnitudes a word for the 16-bit types: as
+  // bits, finite < infinity < NaN, so a NaN is not lost
+  __device__ __forceinline__ uint32_t abs_max(uint32_t m) const {
+#pragma unroll
+    for (int i = 0; i < kWords; ++i) {
+      if constexpr (sizeof(T) == 4)
+        m = max(m, w[i] & 0x7FFFFFFFu);
+      else
+        m = __vmaxu2(m, w[i] & 0x7FFF7FFFu);
+    }
+    return m;
+  }
+
+  // what abs_max gathered, as the bits of an fp32
+  __device__ __forceinline__ static uint32_t abs_max_bits(uint32_t m) {
+    if constexpr (sizeof(T) == 4) return m;
+    const uint32_t h = max(m & 0xFFFFu, m >> 16);
+    return __float_as_uint(std::is_same_v<T, __half> ? __half2float(__ushort_as_half((uint16_t)h))
+                                                     : __uint_as_float(h << 16)) &
+           0x7FFFFFFFu;
+  }
+};
+
 // max of |v| as bits: finite < infinity < NaN, so a NaN is not lost.
 __device__ __forceinline__ uint32_t abs_bits_max(const float (&v)[8]) {
   uint32_t m = 0;
@@ -107,27 +172,44 @@ __device__ __forceinline__ RowScale row_scale(uint32_t amax_bits) {
 constexpr float kRoundMagic = 12582912.0f;  // 1.5 * 2^23: x + magic rounds x to an integer
 // Distance from the rounded value up to which the fp32 quotient decides: its
 // error is below 127 * 2^-23 = 1.6e-5.
-constexpr float kRoundSafe = 0.4999f;
+constexpr float kRoundSafe = 0.49998f;
 
 // Codes of eight values, x / scale to the nearest integer, ties to even, of
-// the exact quotient.  The product x * inv (one rounding of inv, the sum with
-// the magic number rounds once) decides unless some value comes within 1e-4
-// of a border: those eight take the 64-bit quotient, whose error (2^-46 of a
-// code) no 24-bit x and scale can turn into a wrong side.
+// the exact quotient.  The product x * inv (inv rounds once, the sum with the
+// magic number once) decides, unless one of the eight comes within 2e-5 of a
+// border (one in 6000 warps' steps or so).  Then the remainder x - t * scale
+// says for each whether t is the nearest: it is exact for |t| >= 2 (a
+// multiple of scale's last place, below 2^24 of them) and for t = 0; for
+// |t| = 1 its rounding can at most turn a remainder just above scale / 2 into
+// the tie, which leaves the odd t as well.
 __device__ __forceinline__ uint2 codes8(const float (&x)[8], RowScale r) {
   uint32_t y[8];
-  float far = 1.0f;
   if (r.inv != 0.0f) {
-    far = 0.0f;
+    float far = 0.0f;
+    const uint64_t inv = f2_pack(r.inv, r.inv), magic = f2_pack(kRoundMagic, kRoundMagic);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const float m = fmaf(x[i], r.inv, kRoundMagic);
-      const float t = m - kRoundMagic;
-      far = fmaxf(far, fabsf(fmaf(x[i], r.inv, -t)));
-      y[i] = __float_as_uint(m);
+    for (int i = 0; i < 8; i += 2) {
+      const uint64_t v = f2_pack(x[i], x[i + 1]);
+      const uint64_t m = f2_fma(v, inv, magic);
+      // magic - m = -(the rounded value), exactly
+      float d0, d1, m0, m1;
+      f2_unpack(f2_fma(v, inv, f2_sub(magic, m)), d0, d1);
+      f2_unpack(m, m0, m1);
+      far = fmaxf(far, fmaxf(fabsf(d0), fabsf(d1)));
+      y[i] = __float_as_uint(m0);
+      y[i + 1] = __float_as_uint(m1);
     }
-  }
-  if (far > kRoundSafe) {
+    if (far > kRoundSafe) {
+      const float half = 0.5f * r.scale;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const float t = __uint_as_float(y[i]) - kRoundMagic;
+        const float rest = fmaf(-t, r.scale, x[i]);
+        if (fabsf(rest) > half || (fabsf(rest) == half && (y[i] & 1u)))
+          y[i] += rest > 0.0f ? 1u : ~0u;
+      }
+    }
+  } else {
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
       double q = 0.0;
