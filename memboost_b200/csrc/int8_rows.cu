@@ -1,12 +1,12 @@
 // Rows to 8-bit codes with one fp32 scale each, and back (no counterpart in
 // the reference): scale = max|x| / 127, code = x / scale to the nearest.
 //
-// Both directions are bound by memory: 3 bytes a value for the 16-bit types.
-// A row is read once: its threads keep what they loaded in registers between
-// the maximum and the codes (a row too long for that is read a second time
-// past it, from L2).  With many rows a warp takes a row alone, so nothing
-// waits at a barrier and each lane has up to 16 loads in flight; with few,
-// more threads share a row to shorten the call.
+// Both directions are bound by memory: 3 bytes a value for the 16-bit types
+// (8192 x 11008 bf16: 46 us = 5.9 TB/s to codes).  A row is read once: its
+// threads keep what they loaded in registers between the maximum and the
+// codes, 4 or 6 16-byte loads each in flight (with 16 the registers leave too
+// few warps: 70 us).  A row too long for 1024 threads' registers is read a
+// second time past them, from L2.
 #include <algorithm>
 
 #include "mb_codes.cuh"
@@ -15,41 +15,42 @@ namespace mb {
 namespace {
 
 // T threads a row, kPieces pieces of 8 values a thread kept in registers;
-// CTAs of max(T, 128) threads.
-template <typename X, int T, int kPieces>
+// CTAs of max(T, 128) threads.  kWhole: rows of whole 8-value pieces that begin on 16-byte boundaries.
+template <typename X, int T, int kPieces, bool kWhole>
 __global__ void __launch_bounds__(T < 128 ? 128 : T)
     int8_quantize_kernel(const X* __restrict__ x, int64_t rows, int64_t K, int64_t x_stride,
-                         bool x_vec, int8_t* __restrict__ codes, int64_t codes_stride,
+                         int8_t* __restrict__ codes, int64_t codes_stride,
                          float* __restrict__ scales) {
   constexpr int kRows = T < 128 ? 128 / T : 1;
   const int tid = threadIdx.x % T, sub = threadIdx.x / T;
   const int64_t row = (int64_t)blockIdx.x * kRows + sub;
-  if (T <= 32 && row >= rows) return;  // whole warps; longer rows have a CTA each
+  if (T == 32 && row >= rows) return;  // a warp without a row
   const X* xr = x + row * x_stride;
-  const int n8 = (int)ceil_div(K, 8), k = (int)K;
+  const int k = row < rows ? (int)K : 0, n8 = (k + 7) / 8;
 
   Raw8<X> v[kPieces];
   uint32_t m = 0;
 #pragma unroll
   for (int j = 0; j < kPieces; ++j) {
     const int c = tid + j * T;
-    if (c < n8) v[j].load(xr + 8 * c, x_vec, k - 8 * c);
+    if (c < n8) v[j].load(xr + 8 * c, kWhole, kWhole ? 8 : k - 8 * c);
   }
 #pragma unroll
   for (int j = 0; j < kPieces; ++j)
     if (tid + j * T < n8) m = v[j].abs_max(m);
   for (int c = tid + kPieces * T; c < n8; c += T) {
     Raw8<X> u;
-    u.load(xr + 8 * c, x_vec, k - 8 * c);
+    u.load(xr + 8 * c, kWhole, kWhole ? 8 : k - 8 * c);
     m = u.abs_max(m);
   }
   m = __reduce_max_sync(0xffffffffu, Raw8<X>::abs_max_bits(m));
   if constexpr (T > 32) {
-    __shared__ uint32_t part[T / 32];
-    if ((threadIdx.x & 31) == 0) part[tid / 32] = m;
+    __shared__ uint32_t part[kRows][T / 32];
+    if ((threadIdx.x & 31) == 0) part[sub][tid / 32] = m;
     __syncthreads();
 #pragma unroll
-    for (int w = 0; w < T / 32; ++w) m = max(m, part[w]);
+    for (int w = 0; w < T / 32; ++w) m = max(m, part[sub][w]);
+    if (row >= rows) return;
   }
   const RowScale r = row_scale(m);
   if (tid == 0) scales[row] = r.scale;
@@ -58,7 +59,7 @@ __global__ void __launch_bounds__(T < 128 ? 128 : T)
     float f[8];
     u.floats(f);
     const uint2 q = codes8(f, r);
-    if (8 * c + 8 <= k) {
+    if (kWhole || 8 * c + 8 <= k) {
       *reinterpret_cast<uint2*>(cr + 8 * c) = q;
     } else {
       for (int i = 0; i < k - 8 * c; ++i)
@@ -72,62 +73,86 @@ __global__ void __launch_bounds__(T < 128 ? 128 : T)
   }
   for (int c = tid + kPieces * T; c < n8; c += T) {
     Raw8<X> u;
-    u.load(xr + 8 * c, x_vec, k - 8 * c);
+    u.load(xr + 8 * c, kWhole, kWhole ? 8 : k - 8 * c);
     put(c, u);
   }
 }
 
-// A thread decodes 16 codes.
+// A thread decodes two pieces of 8 codes, 256 pieces apart: neighbouring
+// lanes store neighbouring 16 bytes.
+constexpr uint32_t kDecodeThreads = 256, kDecodePieces = 2 * kDecodeThreads;
+
 template <typename Y>
-__global__ void __launch_bounds__(256)
+__global__ void __launch_bounds__(kDecodeThreads)
     int8_dequantize_kernel(const int8_t* __restrict__ codes, int64_t codes_stride,
                            const float* __restrict__ scales, uint32_t pieces, uint32_t total,
                            int64_t K, Y* __restrict__ out, int64_t out_stride, bool out_vec) {
-  const uint32_t i = blockIdx.x * 256u + threadIdx.x;
-  if (i >= total) return;
-  const uint32_t row = i / pieces, p = i - row * pieces;
-  const int64_t c0 = 16 * (int64_t)p;
-  const uint4 q = *reinterpret_cast<const uint4*>(codes + row * codes_stride + c0);
-  const float s = scales[row];
-  const uint32_t w[4] = {q.x, q.y, q.z, q.w};
-  Y* o = out + row * out_stride + c0;
+  const uint32_t i0 = blockIdx.x * kDecodePieces + threadIdx.x;
+  uint2 q[2];
+  float s[2];
+  uint32_t row[2], c0[2];
 #pragma unroll
   for (int h = 0; h < 2; ++h) {
+    const uint32_t i = i0 + h * kDecodeThreads;
+    if (i >= total) break;
+    row[h] = i / pieces;
+    c0[h] = 8 * (i - row[h] * pieces);
+    q[h] = *reinterpret_cast<const uint2*>(codes + row[h] * codes_stride + c0[h]);
+    s[h] = scales[row[h]];
+  }
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    if (i0 + h * kDecodeThreads >= total) break;
     float v[8];
 #pragma unroll
     for (int e = 0; e < 8; ++e)
-      v[e] = __fmul_rn((float)(int)(int8_t)(w[2 * h + e / 4] >> (8 * (e & 3))), s);
-    const int n = (int)min64(8, K - c0 - 8 * h);
-    if (n > 0) store8(o + 8 * h, out_vec, n, v);
+      v[e] = __fmul_rn((float)(int)(int8_t)((e < 4 ? q[h].x : q[h].y) >> (8 * (e & 3))), s[h]);
+    store8(out + row[h] * out_stride + c0[h], out_vec, (int)min64(8, K - c0[h]), v);
   }
 }
 
 template <typename X, int T, int kPieces>
-void launch_quantize(const void* x, int64_t rows, int64_t K, int64_t x_stride, bool x_vec,
+void launch_quantize(const void* x, int64_t rows, int64_t K, int64_t x_stride, bool whole,
                      int8_t* codes, int64_t codes_stride, float* scales, cudaStream_t stream) {
   constexpr int kThreads = T < 128 ? 128 : T;
   const unsigned grid = (unsigned)ceil_div(rows, kThreads / T);
-  int8_quantize_kernel<X, T, kPieces><<<grid, kThreads, 0, stream>>>(
-      static_cast<const X*>(x), rows, K, x_stride, x_vec, codes, codes_stride, scales);
+  const auto go = [&](auto kernel) {
+    kernel<<<grid, kThreads, 0, stream>>>(static_cast<const X*>(x), rows, K, x_stride, codes,
+                                          codes_stride, scales);
+  };
+  whole ? go(int8_quantize_kernel<X, T, kPieces, true>)
+        : go(int8_quantize_kernel<X, T, kPieces, false>);
 }
 
 template <typename X>
-void dispatch_quantize(const void* x, int64_t rows, int64_t K, int64_t x_stride, bool x_vec,
+void dispatch_quantize(const void* x, int64_t rows, int64_t K, int64_t x_stride, bool whole,
                        int8_t* codes, int64_t codes_stride, float* scales, cudaStream_t stream) {
   const auto go = [&](auto threads, auto pieces) {
     launch_quantize<X, decltype(threads)::value, decltype(pieces)::value>(
-        x, rows, K, x_stride, x_vec, codes, codes_stride, scales, stream);
+        x, rows, K, x_stride, whole, codes, codes_stride, scales, stream);
   };
-  constexpr int kDeep = sizeof(X) == 4 ? 8 : 16;  // pieces that leave registers for 16 warps
   using std::integral_constant;
-  if (K <= 32 * 8 * 4)
-    go(integral_constant<int, 32>{}, integral_constant<int, 4>{});
-  else if (rows < 148 * 8)
-    go(integral_constant<int, 512>{}, integral_constant<int, 4>{});
-  else if (K <= 32 * 8 * kDeep)
-    go(integral_constant<int, 32>{}, integral_constant<int, kDeep>{});
-  else
-    go(integral_constant<int, 128>{}, integral_constant<int, kDeep>{});
+  const auto kept = [&](auto threads, int64_t pieces) {
+    pieces <= 4 ? go(threads, integral_constant<int, 4>{})
+                : go(threads, integral_constant<int, 6>{});
+  };
+  // As few threads as hold the row in 6 pieces each; for fewer rows than fill
+  // the GPU up to 256, which shorten the call (8 x 4096: 1.6 us against 4.3
+  // with 32, 8192 x 4096: 18.4 us with 128, 23.4 with 256, 28.9 with 32).
+  const int64_t n8 = ceil_div(K, 8);
+  int threads = 32;
+  while (threads < 1024 && ceil_div(n8, threads) > 6) threads *= 2;
+  if (rows < 4 * 148)
+    while (threads < 256 && n8 > threads) threads *= 2;
+  const int64_t pieces = ceil_div(n8, threads);
+  switch (threads) {
+    case 32: return kept(integral_constant<int, 32>{}, pieces);
+    case 64: return kept(integral_constant<int, 64>{}, pieces);
+    case 128: return kept(integral_constant<int, 128>{}, pieces);
+    case 256: return kept(integral_constant<int, 256>{}, pieces);
+    case 512: return kept(integral_constant<int, 512>{}, pieces);
+    default: return kept(integral_constant<int, 1024>{}, pieces);
+  }
 }
 
 }  // namespace
@@ -149,7 +174,8 @@ extern "C" mb_status mb_int8_quantize(const void* x, mb_dtype x_type, int64_t ro
              "codes must begin on 16-byte boundaries");
   MB_REQUIRE(aligned(x, dtype_size(x_type)) && aligned(scales, 4), "misaligned x or scales");
   cudaStream_t stream = reinterpret_cast<cudaStream_t>(stream_);
-  const bool vec = aligned(x, 16) && (rows == 1 || x_stride * dtype_size(x_type) % 16 == 0);
+  const bool vec = K % 8 == 0 && aligned(x, 16) &&
+                   (rows == 1 || x_stride * dtype_size(x_type) % 16 == 0);
   switch (x_type) {
     case MB_FP16:
       dispatch_quantize<__half>(x, rows, K, x_stride, vec, codes, codes_stride, scales, stream);
@@ -182,17 +208,17 @@ extern "C" mb_status mb_int8_dequantize(const int8_t* codes, int64_t codes_strid
   cudaStream_t stream = reinterpret_cast<cudaStream_t>(stream_);
   const size_t size = dtype_size(out_type);
   const bool vec = aligned(out, 16) && (rows == 1 || out_stride * size % 16 == 0);
-  const int64_t pieces = ceil_div(K, 16);
-  // a launch counts its 16-code pieces in 32 bits
+  const int64_t pieces = ceil_div(K, 8);
+  // a launch counts its 8-code pieces in 32 bits
   const int64_t most = std::max<int64_t>(1, (int64_t(1) << 31) / pieces);
   for (int64_t r0 = 0; r0 < rows; r0 += most) {
     const int64_t n = min64(most, rows - r0);
     const uint32_t total = (uint32_t)(n * pieces);
-    const unsigned grid = (unsigned)ceil_div(total, 256);
+    const unsigned grid = (unsigned)ceil_div(total, kDecodePieces);
     const int8_t* c = codes + r0 * codes_stride;
     uint8_t* o = static_cast<uint8_t*>(out) + (size_t)(r0 * out_stride) * size;
     const auto go = [&](auto* typed) {
-      int8_dequantize_kernel<<<grid, 256, 0, stream>>>(c, codes_stride, scales + r0,
+      int8_dequantize_kernel<<<grid, kDecodeThreads, 0, stream>>>(c, codes_stride, scales + r0,
                                                        (uint32_t)pieces, total, K, typed,
                                                        out_stride, vec);
     };
