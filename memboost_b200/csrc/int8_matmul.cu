@@ -27,17 +27,19 @@ constexpr int kStepK = 128;               // bytes of K a stage
 constexpr int kWeightBytes = kChannels * kStepK;
 constexpr int kThreads = 192;             // warps 0-3 drain, 4 loads, 5 multiplies
 
-// tokens a tile -> stages that fill shared memory for the blocks an SM holds
+// Shared memory of a tile of kN tokens: a ring of stages (128 bytes of K of
+// both operands), whose memory the int32 parts of a split reuse ([kN tokens]
+// [128 channels]).
 template <int kN>
 struct Shape {
   static constexpr int kStage = kWeightBytes + kN * kStepK;
-  static constexpr int kStages = kN == 256 ? 4 : kN == 128 ? 6 : 5;
-  static constexpr int kRing = kStages * kStage;
-  // int32 parts of a split: [kN tokens][128 channels], in the ring's memory
-  static_assert(kN * kChannels * 4 <= kRing, "the parts reuse the ring");
-  static constexpr int kSmem = kRing + 1024;
   static constexpr uint32_t kTmem = kN < 32 ? 32 : kN;
+  static constexpr int smem(int stages) { return stages * kStage + 1024; }
+  static constexpr int kLeast = (kN * kChannels * 4 + kStage - 1) / kStage;  // stages
 };
+constexpr int kMaxStages = 12;
+constexpr int kMostSmem = 227 * 1024 - 2048;  // a CTA's, less what is declared statically
+constexpr int kSms = 148;
 
 // Shared-memory descriptor of a K-major operand written by TMA with the
 // 128-byte swizzle: rows of 128 bytes, 8-row atoms of 1024 bytes.
@@ -162,12 +164,12 @@ template <int kN, typename Y>
 __global__ void __launch_bounds__(kThreads, 1)
     int8_matmul_kernel(const __grid_constant__ CUtensorMap tokens,
                        const __grid_constant__ CUtensorMap weights, int64_t M, int64_t N,
-                       int64_t K, Epilogue e) {
+                       int64_t K, int stages, Epilogue e) {
   using S = Shape<kN>;
   extern __shared__ uint8_t raw[];
   uint8_t* ring = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(raw) + 1023) &
                                              ~(uintptr_t)1023);
-  __shared__ uint64_t full[S::kStages], empty[S::kStages], done;
+  __shared__ uint64_t full[kMaxStages], empty[kMaxStages], done;
   __shared__ uint32_t tmem_slot, failed;
   __shared__ __align__(16) float a_scale[kN];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -178,7 +180,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   const int steps = k1 - k0;
 
   if (threadIdx.x == 0) {
-    for (int s = 0; s < S::kStages; ++s) {
+    for (int s = 0; s < stages; ++s) {
       mbar_init(&full[s], 1);
       mbar_init(&empty[s], 1);
     }
@@ -198,30 +200,39 @@ __global__ void __launch_bounds__(kThreads, 1)
   const uint32_t tmem = tmem_slot;
 
   if (warp == 4 && lane == 0) {
-    int issued = 0;
-    bool ok = true;
-    for (int i = 0; i < steps; ++i) {
-      const int s = i % S::kStages;
-      if (i >= S::kStages && !mbar_wait(&empty[s], (uint32_t)((i / S::kStages - 1) & 1))) {
-        ok = false;
+    const auto weights_of = [&](int i, int s) {
+      mbar_arrive_expect_tx(&full[s], S::kStage);
+      tma_load_2d(ring + s * S::kStage, &weights, &full[s], (k0 + i) * kStepK, (int)n0);
+    };
+    const auto tokens_of = [&](int i, int s) {
+      tma_load_2d(ring + s * S::kStage + kWeightBytes, &tokens, &full[s], (k0 + i) * kStepK,
+                  (int)m0);
+    };
+    // the weights do not wait for the kernel that quantises the tokens
+    int i = 0;
+    for (; i < steps && i < stages; ++i) weights_of(i, i);
+    grid_dependency_wait();
+    for (int f = 0; f < i; ++f) tokens_of(f, f);
+    int s = i == stages ? 0 : i;
+    uint32_t phase = 0;
+    for (; i < steps; ++i) {
+      if (!mbar_wait(&empty[s], phase)) {
+        atomicExch(&failed, 1u);
         break;
       }
-      uint8_t* at = ring + s * S::kStage;
-      mbar_arrive_expect_tx(&full[s], S::kStage);
-      tma_load_2d(at, &weights, &full[s], (k0 + i) * kStepK, (int)n0);
-      tma_load_2d(at + kWeightBytes, &tokens, &full[s], (k0 + i) * kStepK, (int)m0);
-      ++issued;
+      weights_of(i, s);
+      tokens_of(i, s);
+      if (++s == stages) s = 0, phase ^= 1u;
     }
     // every load has landed before the CTA can exit or reuse the ring
-    for (int i = issued > S::kStages ? issued - S::kStages : 0; i < issued; ++i)
-      if (!mbar_wait(&full[i % S::kStages], (uint32_t)((i / S::kStages) & 1))) ok = false;
-    if (!ok) atomicExch(&failed, 1u);
+    for (int f = max(0, i - stages); f < i; ++f)
+      if (!mbar_wait(&full[f % stages], (uint32_t)((f / stages) & 1))) atomicExch(&failed, 1u);
   } else if (warp == 5 && lane == 0) {
-    bool ok = true;
+    int s = 0;
+    uint32_t phase = 0;
     for (int i = 0; i < steps; ++i) {
-      const int s = i % S::kStages;
-      if (!mbar_wait(&full[s], (uint32_t)((i / S::kStages) & 1))) {
-        ok = false;
+      if (!mbar_wait(&full[s], phase)) {
+        atomicExch(&failed, 1u);
         break;
       }
       asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
@@ -231,11 +242,12 @@ __global__ void __launch_bounds__(kThreads, 1)
         umma_i8(tmem, umma_desc_k_sw128(w + 32 * k), umma_desc_k_sw128(t + 32 * k),
                 int8_idesc(kN), (i > 0 || k > 0) ? 1u : 0u);
       umma_commit(&empty[s]);
+      if (++s == stages) s = 0, phase ^= 1u;
     }
     umma_commit(&done);
-    if (!ok) atomicExch(&failed, 1u);
   }
   __syncwarp();
+  grid_dependency_wait();
   if (warp < 4)
     for (int i = threadIdx.x; i < kN; i += 128) a_scale[i] = m0 + i < M ? e.a_scales[m0 + i] : 0.0f;
   if (!mbar_wait(&done, 0)) atomicExch(&failed, 1u);
@@ -398,6 +410,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
   asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
   const uint32_t tmem = tmem_slot;
 
+  grid_dependency_wait();
   if (warp == 4 && lane == 0) {
     int i = 0;
     bool ok = true;
@@ -504,74 +517,128 @@ bool codes_map(CUtensorMap* map, const int8_t* codes, int64_t stride, int64_t ro
          CUDA_SUCCESS;
 }
 
+// A product: its operands and how it is launched.
+struct Product {
+  const int8_t* a_codes;
+  int64_t a_stride, M;
+  const int8_t* b_codes;
+  int64_t b_stride, N, K;
+  Epilogue e;
+  bool chained;  // right behind the kernel that writes the tokens' codes
+  cudaStream_t stream;
+};
+
 template <int kN, typename Y>
-mb_status launch(const int8_t* a_codes, int64_t a_stride, int64_t M, const int8_t* b_codes,
-                 int64_t b_stride, int64_t N, int64_t K, const Epilogue& e, int parts,
-                 cudaStream_t stream) {
+mb_status launch_tiles(const Product& p, int parts, int stages) {
   using S = Shape<kN>;
   static std::atomic<uint64_t> attr_done{0};
-  MB_CUDA_TRY(set_smem_limit_once(int8_matmul_kernel<kN, Y>, S::kSmem, attr_done));
+  MB_CUDA_TRY(set_smem_limit_once(int8_matmul_kernel<kN, Y>, kMostSmem, attr_done));
   CUtensorMap tokens, weights;
-  if (!codes_map(&tokens, a_codes, a_stride, M, K, kN) ||
-      !codes_map(&weights, b_codes, b_stride, N, K, kChannels))
+  if (!codes_map(&tokens, p.a_codes, p.a_stride, p.M, p.K, kN) ||
+      !codes_map(&weights, p.b_codes, p.b_stride, p.N, p.K, kChannels))
     return set_error(MB_ERR_CUDA, "cuTensorMapEncodeTiled rejected the codes");
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)(ceil_div(N, kChannels) * parts), (unsigned)ceil_div(M, kN));
-  cfg.blockDim = dim3(kThreads);
-  cfg.dynamicSmemBytes = S::kSmem;
-  cfg.stream = stream;
-  cudaLaunchAttribute attr[1];
+  cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeClusterDimension;
   attr[0].val.clusterDim.x = (unsigned)parts;
   attr[0].val.clusterDim.y = 1;
   attr[0].val.clusterDim.z = 1;
+  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[1].val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)(ceil_div(p.N, kChannels) * parts), (unsigned)ceil_div(p.M, kN));
+  cfg.blockDim = dim3(kThreads);
+  cfg.dynamicSmemBytes = (size_t)S::smem(stages);
+  cfg.stream = p.stream;
   cfg.attrs = attr;
-  cfg.numAttrs = 1;
-  MB_CUDA_TRY(cudaLaunchKernelEx(&cfg, int8_matmul_kernel<kN, Y>, tokens, weights, M, N, K, e));
+  cfg.numAttrs = p.chained ? 2 : 1;
+  MB_CUDA_TRY(cudaLaunchKernelEx(&cfg, int8_matmul_kernel<kN, Y>, tokens, weights, p.M, p.N, p.K,
+                                 stages, p.e));
   return MB_OK;
 }
 
 template <typename Y>
-mb_status launch_pairs(const int8_t* a_codes, int64_t a_stride, int64_t M, const int8_t* b_codes,
-                       int64_t b_stride, int64_t N, int64_t K, const Epilogue& e,
-                       cudaStream_t stream) {
+mb_status launch_pairs(const Product& p) {
   static std::atomic<uint64_t> attr_done{0};
   MB_CUDA_TRY(set_smem_limit_once(int8_matmul_pair_kernel<Y>, kPairSmem, attr_done));
   CUtensorMap tokens, weights;
-  if (!codes_map(&tokens, a_codes, a_stride, M, K, kPairTokens / 2) ||
-      !codes_map(&weights, b_codes, b_stride, N, K, kChannels))
+  if (!codes_map(&tokens, p.a_codes, p.a_stride, p.M, p.K, kPairTokens / 2) ||
+      !codes_map(&weights, p.b_codes, p.b_stride, p.N, p.K, kChannels))
     return set_error(MB_ERR_CUDA, "cuTensorMapEncodeTiled rejected the codes");
-  const int64_t tiles = ceil_div(N, 2 * kChannels) * ceil_div(M, kPairTokens);
+  const int64_t tiles = ceil_div(p.N, 2 * kChannels) * ceil_div(p.M, kPairTokens);
   MB_REQUIRE(tiles < (int64_t(1) << 31), "M or N too large");
-  int8_matmul_pair_kernel<Y><<<(unsigned)(2 * min64(tiles, 74)), kThreads, kPairSmem, stream>>>(
-      tokens, weights, M, N, K, e);
-  MB_LAUNCH_CHECK("int8_matmul_pair_kernel");
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)(2 * min64(tiles, kSms / 2)));
+  cfg.blockDim = dim3(kThreads);
+  cfg.dynamicSmemBytes = kPairSmem;
+  cfg.stream = p.stream;
+  cfg.attrs = attr;
+  cfg.numAttrs = p.chained ? 1 : 0;
+  MB_CUDA_TRY(cudaLaunchKernelEx(&cfg, int8_matmul_pair_kernel<Y>, tokens, weights, p.M, p.N, p.K,
+                                 p.e));
   return MB_OK;
 }
 
-template <typename Y>
-mb_status dispatch(const int8_t* a_codes, int64_t a_stride, int64_t M, const int8_t* b_codes,
-                   int64_t b_stride, int64_t N, int64_t K, const Epilogue& e,
-                   cudaStream_t stream) {
-  // pairs where their tiles give every pair of SMs work
-  if (ceil_div(N, 2 * kChannels) * ceil_div(M, kPairTokens) >= 74)
-    return launch_pairs<Y>(a_codes, a_stride, M, b_codes, b_stride, N, K, e, stream);
-  const int kn = M <= 16 ? 16 : M <= 32 ? 32 : M <= 64 ? 64 : M <= 128 ? 128 : 256;
+template <int kN, typename Y>
+mb_status split_tiles(const Product& p) {
+  using S = Shape<kN>;
   // K parts: until the tiles fill the SMs, each part at least two steps
-  const int64_t tiles = ceil_div(N, kChannels) * ceil_div(M, kn), steps = ceil_div(K, kStepK);
+  const int64_t tiles = ceil_div(p.N, kChannels) * ceil_div(p.M, kN);
+  const int64_t steps = ceil_div(p.K, kStepK);
   int parts = 1;
-  while (parts < 8 && tiles * parts * 2 <= 148 && steps >= 4 * parts) parts *= 2;
-  const auto go = [&](auto size) {
-    return launch<decltype(size)::value, Y>(a_codes, a_stride, M, b_codes, b_stride, N, K, e,
-                                            parts, stream);
-  };
-  switch (kn) {
-    case 16: return go(std::integral_constant<int, 16>{});
-    case 32: return go(std::integral_constant<int, 32>{});
-    case 64: return go(std::integral_constant<int, 64>{});
-    case 128: return go(std::integral_constant<int, 128>{});
-    default: return go(std::integral_constant<int, 256>{});
+  while (parts < 8 && tiles * parts * 2 <= kSms && steps >= 4 * parts) parts *= 2;
+  int stages = kN == 256 ? 4 : kN == 128 ? 6 : 5;
+  return launch_tiles<kN, Y>(p, parts, stages);
+}
+
+template <typename Y>
+mb_status dispatch(const Product& p) {
+  // pairs where their tiles give every pair of SMs work
+  if (ceil_div(p.N, 2 * kChannels) * ceil_div(p.M, kPairTokens) >= kSms / 2)
+    return launch_pairs<Y>(p);
+  if (p.M <= 16) return split_tiles<16, Y>(p);
+  if (p.M <= 32) return split_tiles<32, Y>(p);
+  if (p.M <= 64) return split_tiles<64, Y>(p);
+  if (p.M <= 128) return split_tiles<128, Y>(p);
+  return split_tiles<256, Y>(p);
+}
+
+mb_status multiply(const int8_t* a_codes, int64_t a_stride, const float* a_scales, int64_t M,
+                   const int8_t* b_codes, int64_t b_stride, const float* b_scales, int64_t N,
+                   int64_t K, const void* bias, mb_dtype bias_type, void* out, mb_dtype out_type,
+                   int64_t out_stride, bool chained, mb_stream_t stream) {
+  // the stride of a single row is not read, but TMA wants one
+  if (M == 1) a_stride = ceil_div(K, 16) * 16;
+  if (N == 1) b_stride = ceil_div(K, 16) * 16;
+  const Product p{a_codes, a_stride, M, b_codes, b_stride, N, K,
+                  Epilogue{a_scales, b_scales, bias, out, out_stride, (int)bias_type},
+                  chained, reinterpret_cast<cudaStream_t>(stream)};
+  switch (out_type) {
+    case MB_FP16: return dispatch<__half>(p);
+    case MB_BF16: return dispatch<__nv_bfloat16>(p);
+    default: return dispatch<float>(p);
   }
+}
+
+// What mb_int8_matmul and mb_int8_linear ask of the weights and the output.
+mb_status check_product(int64_t M, const int8_t* b_codes, int64_t b_stride, const float* b_scales,
+                        int64_t N, int64_t K, const void* bias, mb_dtype bias_type, void* out,
+                        mb_dtype out_type, int64_t out_stride) {
+  MB_REQUIRE(b_codes && b_scales && out, "int8_matmul pointers must not be null");
+  MB_REQUIRE(dtype_known(out_type) && (bias == nullptr || dtype_known(bias_type)),
+             "unknown type of out or bias");
+  MB_REQUIRE(M > 0 && N > 0 && K > 0, "M, N and K must be positive");
+  MB_REQUIRE(K <= MB_INT8_MAX_K, "K too large: the int32 sums would not be exact");
+  MB_REQUIRE(M <= (int64_t(1) << 23) && N < (int64_t(1) << 31) - 256, "M or N too large");
+  MB_REQUIRE((N == 1 || b_stride >= K) && (M == 1 || out_stride >= N),
+             "strides must be at least the length of a row");
+  MB_REQUIRE(aligned(b_codes, 16) && b_stride % 16 == 0, "codes must begin on 16-byte boundaries");
+  MB_REQUIRE(aligned(out, dtype_size(out_type)) && aligned(b_scales, 4) &&
+                 (bias == nullptr || aligned(bias, dtype_size(bias_type))),
+             "misaligned out, scales or bias");
+  return MB_OK;
 }
 
 }  // namespace
@@ -583,36 +650,18 @@ extern "C" mb_status mb_int8_matmul(const int8_t* a_codes, int64_t a_stride, con
                                     int64_t M, const int8_t* b_codes, int64_t b_stride,
                                     const float* b_scales, int64_t N, int64_t K, const void* bias,
                                     mb_dtype bias_type, void* out, mb_dtype out_type,
-                                    int64_t out_stride, mb_stream_t stream_) {
+                                    int64_t out_stride, mb_stream_t stream) {
   clear_error();
-  MB_REQUIRE(a_codes && a_scales && b_codes && b_scales && out,
-             "int8_matmul pointers must not be null");
-  MB_REQUIRE(dtype_known(out_type) && (bias == nullptr || dtype_known(bias_type)),
-             "unknown type of out or bias");
-  MB_REQUIRE(M > 0 && N > 0 && K > 0, "M, N and K must be positive");
-  MB_REQUIRE(K <= MB_INT8_MAX_K, "K too large: the int32 sums would not be exact");
-  MB_REQUIRE(M <= (int64_t(1) << 23) && N < (int64_t(1) << 31) - 128, "M or N too large");
-  MB_REQUIRE((M == 1 || a_stride >= K) && (N == 1 || b_stride >= K) && (M == 1 || out_stride >= N),
-             "strides must be at least the length of a row");
-  MB_REQUIRE(aligned(a_codes, 16) && aligned(b_codes, 16) && a_stride % 16 == 0 &&
-                 b_stride % 16 == 0,
-             "codes must begin on 16-byte boundaries");
-  MB_REQUIRE(aligned(out, dtype_size(out_type)) && aligned(a_scales, 4) && aligned(b_scales, 4) &&
-                 (bias == nullptr || aligned(bias, dtype_size(bias_type))),
-             "misaligned out, scales or bias");
-  // the stride of a single row is not read, but TMA wants one
-  if (M == 1) a_stride = ceil_div(K, 16) * 16;
-  if (N == 1) b_stride = ceil_div(K, 16) * 16;
-  cudaStream_t stream = reinterpret_cast<cudaStream_t>(stream_);
-  const Epilogue e{a_scales, b_scales, bias, out, out_stride, (int)bias_type};
-  switch (out_type) {
-    case MB_FP16:
-      return dispatch<__half>(a_codes, a_stride, M, b_codes, b_stride, N, K, e, stream);
-    case MB_BF16:
-      return dispatch<__nv_bfloat16>(a_codes, a_stride, M, b_codes, b_stride, N, K, e, stream);
-    default:
-      return dispatch<float>(a_codes, a_stride, M, b_codes, b_stride, N, K, e, stream);
-  }
+  if (const mb_status st = check_product(M, b_codes, b_stride, b_scales, N, K, bias, bias_type,
+                                         out, out_type, out_stride);
+      st != MB_OK)
+    return st;
+  MB_REQUIRE(a_codes && a_scales, "int8_matmul pointers must not be null");
+  MB_REQUIRE(M == 1 || a_stride >= K, "strides must be at least the length of a row");
+  MB_REQUIRE(aligned(a_codes, 16) && a_stride % 16 == 0, "codes must begin on 16-byte boundaries");
+  MB_REQUIRE(aligned(a_scales, 4), "misaligned out, scales or bias");
+  return multiply(a_codes, a_stride, a_scales, M, b_codes, b_stride, b_scales, N, K, bias,
+                  bias_type, out, out_type, out_stride, false, stream);
 }
 
 extern "C" size_t mb_int8_linear_workspace_size(int64_t M, int64_t K) {
@@ -626,8 +675,10 @@ extern "C" mb_status mb_int8_linear(const void* x, mb_dtype x_type, int64_t x_st
                                     void* out, mb_dtype out_type, int64_t out_stride,
                                     void* workspace, size_t workspace_bytes, mb_stream_t stream) {
   clear_error();
-  MB_REQUIRE(M > 0 && K > 0, "M, N and K must be positive");
-  MB_REQUIRE(M <= (int64_t(1) << 23) && K <= MB_INT8_MAX_K, "M or K too large");
+  if (const mb_status st = check_product(M, b_codes, b_stride, b_scales, N, K, bias, bias_type,
+                                         out, out_type, out_stride);
+      st != MB_OK)
+    return st;
   if (workspace == nullptr || !aligned(workspace, 16) ||
       workspace_bytes < mb_int8_linear_workspace_size(M, K))
     return set_error(MB_ERR_WORKSPACE, "int8_linear workspace missing, misaligned or too small");
@@ -636,6 +687,6 @@ extern "C" mb_status mb_int8_linear(const void* x, mb_dtype x_type, int64_t x_st
   float* scales = reinterpret_cast<float*>(codes + M * pitch);
   const mb_status st = mb_int8_quantize(x, x_type, M, K, x_stride, codes, pitch, scales, stream);
   if (st != MB_OK) return st;
-  return mb_int8_matmul(codes, pitch, scales, M, b_codes, b_stride, b_scales, N, K, bias,
-                        bias_type, out, out_type, out_stride, stream);
+  return multiply(codes, pitch, scales, M, b_codes, b_stride, b_scales, N, K, bias, bias_type, out,
+                  out_type, out_stride, true, stream);
 }

@@ -10,6 +10,7 @@
 #include <algorithm>
 
 #include "mb_codes.cuh"
+#include "mb_tma.cuh"
 
 namespace mb {
 namespace {
@@ -21,6 +22,7 @@ __global__ void __launch_bounds__(T < 128 ? 128 : T)
     int8_quantize_kernel(const X* __restrict__ x, int64_t rows, int64_t K, int64_t x_stride,
                          int8_t* __restrict__ codes, int64_t codes_stride,
                          float* __restrict__ scales) {
+  grid_launch_dependents();  // a product behind this may begin with its weights
   constexpr int kRows = T < 128 ? 128 / T : 1;
   const int tid = threadIdx.x % T, sub = threadIdx.x / T;
   const int64_t row = (int64_t)blockIdx.x * kRows + sub;

@@ -158,7 +158,7 @@ def test_linear_entry_refusals():
         return lib.mb_int8_linear(x, t, 33, M, b, 48, P, 4, K, None, 0, out, 0, 4, ws, nbytes, None)
 
     _refused(call(M=0), "positive")
-    _refused(call(K=131073), "too large")
+    _refused(call(K=131073), "exact")
     _refused(call(nbytes=n - 1), "workspace")
     _refused(call(ws=None), "workspace")
     _refused(call(ws=P + 8), "workspace")
