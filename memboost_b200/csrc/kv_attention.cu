@@ -9,15 +9,20 @@
 // bound by reading the codes, and the products only keep the arithmetic off
 // the fp32 units.
 //
-// No shared memory on the way in: both products' left operands come straight
-// from global memory, because the order of the inner index is free.  In
-// S^T the lane (g, j) = (lane / 4, lane % 4) holds 16 consecutive channels of
-// tokens g and g + 8 (channel 64 s + 16 j + .. in step s), and Q's registers
-// follow the same order; in O^T it holds 16 consecutive channels
-// (16 g + .., and 128 further for head_dim > 128) of tokens 2 j, 2 j + 1,
-// 2 j + 8, 2 j + 9.  Each load is 16 (8 bits) or 8 bytes (4 bits) of a row,
-// neighbours within a row.  Between the products the probabilities change
-// from S^T's layout to the right operand's by a transposing move.
+// Codes and scales reach a warp through a ring of its own in shared memory,
+// 16 tokens a stage, filled by TMA: a 16-row box of each code array (rows of
+// one page and head are contiguous) and a bulk copy of each scale array, all
+// issued by one lane and awaited on one mbarrier.  With a stage of 4.2 KB
+// (8 bits, head_dim 128), three stages and 16 warps an SM has up to 200 KB on
+// the way; held in registers instead, two thirds of a stage a warp were.
+//
+// Both products' left operands are read as they lie, because the order of the
+// inner index is free: in S^T lane (g, j) = (lane / 4, lane % 4) takes 16 bytes
+// of the rows of tokens g and g + 8, in O^T 16 channels of the four tokens of
+// its columns; Q's registers follow the keys' channel order.  The boxes' swizzle,
+// the 16-byte chunks 2 j + step and the tokens' order (token_of) keep these
+// reads free of bank conflicts.  Between the products the probabilities
+// change from S^T's layout to the right operand's by a transposing move.
 //
 // 8-bit codes become exact fp16 integers (1024 + 128 + code by a byte
 // permute, minus 1152); the key's scale multiplies the score and the value's
@@ -37,8 +42,10 @@
 // the CTAs' timing.
 #include <algorithm>
 #include <cmath>
+#include <cstring>
 
 #include "mb_cache.cuh"
+#include "mb_tma.cuh"
 
 namespace mb {
 namespace {
@@ -87,11 +94,6 @@ struct Query {
   bool bf16, vec;
 };
 
-__device__ __forceinline__ float query_at(const Query& q, int64_t i) {
-  return q.bf16 ? __bfloat162float(static_cast<const __nv_bfloat16*>(q.data)[i])
-                : __half2float(static_cast<const __half*>(q.data)[i]);
-}
-
 __device__ __forceinline__ void store_out(void* out, bool bf16, int64_t i, float y) {
   if (bf16)
     static_cast<__nv_bfloat16*>(out)[i] = __float2bfloat16_rn(y);
@@ -99,236 +101,181 @@ __device__ __forceinline__ void store_out(void* out, bool bf16, int64_t i, float
     static_cast<__half*>(out)[i] = __float2half_rn(y);
 }
 
-// One lane's part of 16 tokens' keys and values.  kSteps: 64-channel steps.
-template <int BITS, int kSteps>
-struct Tokens {
-  static constexpr int kWords = BITS == 8 ? 4 : 2;        // of 16 channels
-  static constexpr int kPasses = (kSteps + 1) / 2;        // 128-channel passes over V
-  uint32_t k[2][kSteps][kWords];                          // tokens g, g + 8
-  uint32_t v[4][kPasses][kWords];                         // tokens 2j, 2j + 1, 2j + 8, 2j + 9
-  float k_scale[2], v_scale[2];                           // 8 bits: tokens g, g + 8
-  uint32_t k_group[BITS == 4 ? 2 : 1][BITS == 4 ? kSteps : 1];   // 4 bits: (s, m)
-  uint32_t v_group[BITS == 4 ? 4 : 1][BITS == 4 ? kPasses : 1];
-
-  __device__ __forceinline__ static void load_words(uint32_t (&w)[kWords], const uint8_t* p) {
-    if constexpr (BITS == 8) {
-      const uint4 u = *reinterpret_cast<const uint4*>(p);
-      w[0] = u.x; w[1] = u.y; w[2] = u.z; w[3] = u.w;
-    } else {
-      const uint2 u = *reinterpret_cast<const uint2*>(p);
-      w[0] = u.x; w[1] = u.y;
-    }
+// How rows of a head_dim in (64 (kQuarters - 1), 64 kQuarters] lie in a stage.
+template <int BITS, int kQuarters>
+struct Layout {
+  static constexpr int kRow = kQuarters >= 3 ? (BITS == 8 ? 256 : 128) : kQuarters * 8 * BITS;
+  static constexpr int kBoxRow = kRow < 128 ? kRow : 128;  // bytes of a row in one box
+  static constexpr int kBoxes = kRow / kBoxRow;
+  static constexpr int kBox = kBlock * kBoxRow;
+  static constexpr int kCodes = kBlock * kRow;             // of keys, or of values
+  static constexpr int kSwizzle = kBoxRow == 128 ? 0x70 : kBoxRow == 64 ? 0x30 : 0x10;
+  // bytes of 16 tokens' scales, and what a stage keeps for them
+  __host__ __device__ static constexpr uint32_t scale_bytes(uint32_t dim) {
+    return kBlock * (BITS == 8 ? 4 : dim / kGroup4 * 4);
   }
+  static constexpr int kScales = kBlock * (BITS == 8 ? 4 : 2 * kQuarters * 4);
+  static constexpr int kStage = 2 * (kCodes + kScales);
 
-  // Tokens row .. row + 15; those from `seen` on get scales (4 bits: scale
-  // and minimum) of 0: what a place behind the sequence's end holds is not
-  // used.  The codes there lie in the same page.
-  __device__ __forceinline__ void load_keys(const CacheView& c, int64_t row, int seen, int g,
-                                            int j) {
-    const uint32_t bytes = c.dim * BITS / 8;
-#pragma unroll
-    for (int r = 0; r < 2; ++r) {
-      const int64_t at = row + g + 8 * r;
-#pragma unroll
-      for (int s = 0; s < kSteps; ++s) {
-        const uint32_t piece = 4 * s + j;
-        if (piece * 16 < c.dim)
-          load_words(k[r][s], c.codes[0] + at * bytes + piece * (2 * BITS));
-        if constexpr (BITS == 4) {
-          k_group[r][s] = 0;
-          if (piece * 16 < c.dim && g + 8 * r < seen)
-            k_group[r][s] =
-                reinterpret_cast<const uint32_t*>(c.scales[0])[at * (c.dim / kGroup4) + piece / 2];
-        }
-      }
-      if constexpr (BITS == 8)
-        k_scale[r] = g + 8 * r < seen ? reinterpret_cast<const float*>(c.scales[0])[at] : 0.0f;
-    }
+  // S^T: steps of 4 lanes x kKeyWords words; O^T: passes of 8 lanes x 16 channels
+  static constexpr int kKeyWords = BITS == 4 && kQuarters == 1 ? 2 : 4;
+  static constexpr int kSteps = kRow / (16 * kKeyWords);
+  static constexpr int kProducts = kSteps * kKeyWords * (BITS == 8 ? 1 : 2);  // of S^T
+  static constexpr int kPasses = (kQuarters + 1) / 2;
+
+  // Place in a stage's keys (or values) of a byte of a row.
+  __device__ __forceinline__ static uint32_t at(uint32_t row, uint32_t byte) {
+    const uint32_t o = row * kBoxRow + byte % kBoxRow;
+    return byte / kBoxRow * kBox + (o ^ ((o >> 3) & kSwizzle));
   }
-
-  __device__ __forceinline__ void load_values(const CacheView& c, int64_t row, int seen, int g,
-                                              int j) {
-    const uint32_t bytes = c.dim * BITS / 8;
-#pragma unroll
-    for (int r = 0; r < 4; ++r) {
-      const int t = 2 * j + (r & 1) + 8 * (r >> 1);
-      const int64_t at = row + t;
-#pragma unroll
-      for (int p = 0; p < kPasses; ++p) {
-        const uint32_t piece = g + 8 * p;
-        if (piece * 16 < c.dim)
-          load_words(v[r][p], c.codes[1] + at * bytes + piece * (2 * BITS));
-        if constexpr (BITS == 4) {
-          v_group[r][p] = 0;
-          if (piece * 16 < c.dim && t < seen)
-            v_group[r][p] =
-                reinterpret_cast<const uint32_t*>(c.scales[1])[at * (c.dim / kGroup4) + piece / 2];
-        }
-      }
-    }
-    if constexpr (BITS == 8) {
-#pragma unroll
-      for (int r = 0; r < 2; ++r)
-        v_scale[r] =
-            g + 8 * r < seen ? reinterpret_cast<const float*>(c.scales[1])[row + g + 8 * r] : 0.0f;
-    }
-  }
-
-  // Nothing to see: values that contribute nothing, whatever the codes.
-  __device__ __forceinline__ void clear() {
-#pragma unroll
-    for (int r = 0; r < 2; ++r) {
-      k_scale[r] = v_scale[r] = 0.0f;
-      if constexpr (BITS == 4)
-#pragma unroll
-        for (int s = 0; s < kSteps; ++s) k_group[r][s] = 0;
-    }
-    if constexpr (BITS == 4)
-#pragma unroll
-      for (int r = 0; r < 4; ++r)
-#pragma unroll
-        for (int p = 0; p < kPasses; ++p) v_group[r][p] = 0;
-  }
-
-  // S^T += K Q^T
-  template <int kTiles>
-  __device__ __forceinline__ void scores(float (&s)[kTiles][4],
-                                         const uint32_t (&q)[kTiles][kSteps][4][2]) const {
-#pragma unroll
-    for (int st = 0; st < kSteps; ++st) {
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        uint32_t a[2][2];
-#pragma unroll
-        for (int r = 0; r < 2; ++r) {
-          if constexpr (BITS == 8) {
-            const uint32_t w = k[r][st][i] ^ 0x80808080u;
-            a[r][0] = code8_pair(w, 0x4140);
-            a[r][1] = code8_pair(w, 0x4342);
-          } else {
-            const __half2 gm = bits_h2(k_group[r][st]);
-            const uint32_t w = k[r][st][i / 2] >> (8 * (i & 1));
-            a[r][0] = code4_pair<false>(w, __low2half2(gm), __high2half2(gm));
-            a[r][1] = code4_pair<true>(w, __low2half2(gm), __high2half2(gm));
-          }
-        }
-#pragma unroll
-        for (int n = 0; n < kTiles; ++n)
-          mma_f16(s[n], a[0][0], a[1][0], a[0][1], a[1][1], q[n][st][i][0], q[n][st][i][1]);
-      }
-    }
-  }
-
-  // O^T += V^T P^T; o[n][p][m]: channels 16 (g + 8 p) + 2 m, + 1 of heads 2 j, 2 j + 1
-  template <int kTiles>
-  __device__ __forceinline__ void outputs(float (&o)[kTiles][kPasses][8][4],
-                                          const uint32_t (&pt)[kTiles][2]) const {
-#pragma unroll
-    for (int p = 0; p < kPasses; ++p) {
-#pragma unroll
-      for (int i = 0; i < kWords; ++i) {
-        if constexpr (BITS == 8) {
-          const uint32_t w0 = v[0][p][i] ^ 0x80808080u, w1 = v[1][p][i] ^ 0x80808080u;
-          const uint32_t w2 = v[2][p][i] ^ 0x80808080u, w3 = v[3][p][i] ^ 0x80808080u;
-#pragma unroll
-          for (int h = 0; h < 2; ++h) {  // channels 4 i + 2 h, + 1
-            const uint32_t x = __byte_perm(w0, w1, h ? 0x7362 : 0x5140);
-            const uint32_t y = __byte_perm(w2, w3, h ? 0x7362 : 0x5140);
-            const uint32_t a0 = code8_pair(x, 0x4140), a1 = code8_pair(x, 0x4342);
-            const uint32_t a2 = code8_pair(y, 0x4140), a3 = code8_pair(y, 0x4342);
-#pragma unroll
-            for (int n = 0; n < kTiles; ++n)
-              mma_f16(o[n][p][2 * i + h], a0, a1, a2, a3, pt[n][0], pt[n][1]);
-          }
-        } else {
-          const uint32_t g01[2] = {v_group[0][p], v_group[1][p]};
-          const uint32_t g23[2] = {v_group[2][p], v_group[3][p]};
-          const __half2 s01 = bits_h2(__byte_perm(g01[0], g01[1], 0x5410));
-          const __half2 m01 = bits_h2(__byte_perm(g01[0], g01[1], 0x7632));
-          const __half2 s23 = bits_h2(__byte_perm(g23[0], g23[1], 0x5410));
-          const __half2 m23 = bits_h2(__byte_perm(g23[0], g23[1], 0x7632));
-#pragma unroll
-          for (int h = 0; h < 4; ++h) {  // channels 8 i + 2 h, + 1
-            const uint32_t sel = h < 2 ? 0x5410 : 0x7632;
-            const uint32_t x = __byte_perm(v[0][p][i], v[1][p][i], sel) >> (8 * (h & 1));
-            const uint32_t y = __byte_perm(v[2][p][i], v[3][p][i], sel) >> (8 * (h & 1));
-            const uint32_t a0 = code4_pair<false>(x, s01, m01), a1 = code4_pair<true>(x, s01, m01);
-            const uint32_t a2 = code4_pair<false>(y, s23, m23), a3 = code4_pair<true>(y, s23, m23);
-#pragma unroll
-            for (int n = 0; n < kTiles; ++n)
-              mma_f16(o[n][p][4 * i + h], a0, a1, a2, a3, pt[n][0], pt[n][1]);
-          }
-        }
-      }
-    }
+  // First byte of lane j's part of a key's row in a step.
+  __device__ __forceinline__ static uint32_t key_byte(int step, int j) {
+    if constexpr (kKeyWords == 2) return 8 * j;
+    if constexpr (kSteps == 1) return 16 * j;
+    return 128 * (step / 2) + 16 * (2 * j + step % 2);
   }
 };
+
+// Token (of 16) at row g of S^T and column k = g of O^T's inner index: pairs
+// change places in every other pair of pairs, which spreads a warp's reads of
+// the values over the banks.
+__device__ __forceinline__ int token_of(int k) { return k ^ ((k >> 1) & 1); }
 
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kRaise = 8.0f;  // how far a score may exceed the maximum in use
 
+__device__ __forceinline__ float exp2_fast(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+// Bulk copy of n bytes (a multiple of 16, both sides 16-byte aligned).
+__device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t n, uint64_t* bar) {
+  asm volatile(
+      "cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::
+          "r"(smem_u32(dst)),
+      "l"(src), "r"(n), "r"(smem_u32(bar))
+      : "memory");
+}
+
+// A warp's walk over its blocks' places in the pages.
+struct Walk {
+  uint32_t page, place;  // of the next block
+  __device__ __forceinline__ void start(uint32_t t, uint32_t page_size) {
+    page = t / page_size;
+    place = t - page * page_size;
+  }
+  __device__ __forceinline__ void advance(uint32_t pages, uint32_t rest, uint32_t page_size) {
+    page += pages;
+    place += rest;
+    if (place >= page_size) place -= page_size, ++page;
+  }
+};
+
+struct Lengths {
+  const int32_t* data;
+  int64_t most;  // tokens the table can name
+  __device__ __forceinline__ int64_t of(int64_t b) const {
+    return max64(0, min64(data[b], most));
+  }
+};
+
 // Grid: (chunks, kv heads x head blocks, batch).  parts: per (sequence, head,
 // chunk) head_dim outputs, then all (maximum, sum) pairs; null with one chunk.
-template <int BITS, int kSteps, int kTiles>
+template <int BITS, int kQuarters, int kTiles, int kStages>
 __global__ void __launch_bounds__(32 * kWarps)
-    cache_attention_kernel(CacheView c, Query q, uint32_t heads, uint32_t head_blocks,
-                           const int32_t* __restrict__ table, int64_t table_stride,
-                           int64_t most, const int32_t* __restrict__ lengths, float scale,
-                           uint32_t chunk, float* __restrict__ parts, void* __restrict__ out) {
+    cache_attention_kernel(const __grid_constant__ CUtensorMap k_map,
+                           const __grid_constant__ CUtensorMap v_map, CacheView c, Query q,
+                           uint32_t heads, uint32_t head_blocks, const int32_t* __restrict__ table,
+                           int64_t table_stride, Lengths lengths, float scale, uint32_t chunk,
+                           float* __restrict__ parts, void* __restrict__ out) {
+  using L = Layout<BITS, kQuarters>;
   constexpr int kHeads = 8 * kTiles;
-  using Piece = Tokens<BITS, kSteps>;
+  extern __shared__ uint8_t raw[];
+  uint8_t* shared = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(raw) + 1023) &
+                                               ~(uintptr_t)1023);
   __shared__ float sm[kWarps][kHeads], sl[kWarps][kHeads];
-  extern __shared__ float so[];  // [kWarps][kHeads][dim]
+  __shared__ uint64_t bars[kWarps][kStages];
   const uint32_t group = heads / c.heads;
   const uint32_t kvh = blockIdx.y / head_blocks, h0 = (blockIdx.y % head_blocks) * kHeads;
   const int64_t b = blockIdx.z;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, j = lane & 3;
-  const int64_t len = max64(0, min64(lengths[b], most));
+  const int64_t len = lengths.of(b);
   const int64_t t0 = (int64_t)blockIdx.x * chunk;
   if (t0 >= len && blockIdx.x > 0) return;  // the join reads no such part
   const int here = (int)min64(chunk, len - t0);
   const int blocks = (here + kBlock - 1) / kBlock;
   const int32_t* pages = table + b * table_stride;
 
-  // first row of a block, or -1 if its page lies outside the cache
-  const auto row_of = [&](int block) -> int64_t {
-    const uint32_t t = (uint32_t)t0 + (uint32_t)block * kBlock;
-    const uint32_t p = t / c.page_size;
-    const int64_t page = pages[p];
-    if (page < 0 || page >= c.pages) return -1;
-    return (page * c.heads + kvh) * c.page_size + (t - p * c.page_size);
-  };
-
-  Piece tok = {};
-  int64_t row = -1;
-  int seen = 0;
-  if (warp < blocks) {
-    row = row_of(warp);
-    seen = row < 0 ? 0 : min(kBlock, here - warp * kBlock);
-    if (row >= 0) {
-      tok.load_keys(c, row, seen, g, j);
-      tok.load_values(c, row, seen, g, j);
-    }
+  uint8_t* codes = shared + warp * kStages * 2 * L::kCodes;  // per stage: keys, values
+  uint8_t* scales = shared + kWarps * kStages * 2 * L::kCodes + warp * kStages * 2 * L::kScales;
+  uint64_t* bar = bars[warp];
+  const uint32_t scale_bytes = L::scale_bytes(c.dim);
+  if (lane == 0) {
+    for (int s = 0; s < kStages; ++s) mbar_init(&bar[s], 1);
+    fence_mbar_init();
   }
+  __syncwarp();
+
+  // The next block to fetch: its number, and its page, read one fetch ahead.
+  constexpr uint32_t kStride = kWarps * kBlock;
+  const uint32_t stride_pages = kStride / c.page_size, stride_rest = kStride % c.page_size;
+  Walk walk;
+  walk.start((uint32_t)t0 + warp * kBlock, c.page_size);
+  int fetch = warp;
+  int32_t page = fetch < blocks ? pages[walk.page] : 0;
+  // Fetches the next block whose page exists into a stage; the number of its
+  // tokens that the sequence has, or 0 if there is none.
+  const auto fetch_into = [&](int s) -> int {
+    while (fetch < blocks) {
+      const int32_t p = page;
+      const uint32_t place = walk.place;
+      const int seen = min(kBlock, here - fetch * kBlock);
+      fetch += kWarps;
+      walk.advance(stride_pages, stride_rest, c.page_size);
+      if (fetch < blocks) page = pages[walk.page];
+      if (p < 0 || p >= c.pages) continue;
+      if (lane == 0) {
+        const int64_t row = ((int64_t)p * c.heads + kvh) * c.page_size + place;
+        uint8_t* at = codes + s * 2 * L::kCodes;
+        uint8_t* sc = scales + s * 2 * L::kScales;
+        mbar_arrive_expect_tx(&bar[s], 2 * (L::kCodes + scale_bytes));
+#pragma unroll
+        for (int x = 0; x < L::kBoxes; ++x) {
+          tma_load_2d(at + x * L::kBox, &k_map, &bar[s], x * L::kBoxRow, (int)row);
+          tma_load_2d(at + L::kCodes + x * L::kBox, &v_map, &bar[s], x * L::kBoxRow, (int)row);
+        }
+        const int64_t first = row * (scale_bytes / kBlock);
+        bulk_load(sc, c.scales[0] + first, scale_bytes, &bar[s]);
+        bulk_load(sc + L::kScales, c.scales[1] + first, scale_bytes, &bar[s]);
+      }
+      return seen;
+    }
+    return 0;
+  };
+  int seen[kStages];  // of the stages in order, the next to use first
+#pragma unroll
+  for (int s = 0; s < kStages; ++s) seen[s] = fetch_into(s);
 
   // Q in the order of the keys' registers, below 1 by a power of two a head
-  uint32_t qf[kTiles][kSteps][4][2];
+  uint32_t qf[kTiles][L::kProducts][2];
   float factor[kTiles][2];  // of heads 2 j, 2 j + 1: scale log2(e) and that power
 #pragma unroll
   for (int n = 0; n < kTiles; ++n) {
     const uint32_t h = h0 + 8 * n + g;
     const bool live = h < group;
     const int64_t at = b * q.batch_stride + (int64_t)(kvh * group + (live ? h : 0)) * q.head_stride;
-    float x[kSteps][16];
+    constexpr int kPer = L::kKeyWords * 32 / BITS;  // channels of a lane in a step
+    float x[L::kSteps][kPer];
     uint32_t top = 0;
 #pragma unroll
-    for (int s = 0; s < kSteps; ++s) {
-      const uint32_t ch = 64 * s + 16 * j;
-      const bool in = live && ch < c.dim;
+    for (int s = 0; s < L::kSteps; ++s) {
+      const uint32_t ch = L::key_byte(s, j) * 8 / BITS;
 #pragma unroll
-      for (int e = 0; e < 2; ++e) {
+      for (int e = 0; e < kPer / 8; ++e) {
         float y[8] = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
-        if (in) {
+        if (live && ch + 8 * e < c.dim) {
           if (q.bf16)
             load8(static_cast<const __nv_bfloat16*>(q.data) + at + ch + 8 * e, q.vec, 8, y);
           else
@@ -347,48 +294,111 @@ __global__ void __launch_bounds__(32 * kWarps)
     const float down = plain ? 1.0f : __uint_as_float((253u - min(ex, 252u)) << 23);
     const float up = plain ? 1.0f : __uint_as_float((1u + min(ex, 252u)) << 23);
 #pragma unroll
-    for (int s = 0; s < kSteps; ++s)
+    for (int s = 0; s < L::kSteps; ++s)
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
+      for (int i = 0; i < L::kProducts / L::kSteps; ++i) {
         // channels of the products' registers: code8_pair and code4_pair
         const int c0 = BITS == 8 ? 4 * i : 8 * (i / 2) + 2 * (i & 1);
         const int d = BITS == 8 ? 1 : 4, e = BITS == 8 ? 2 : 1;
-        qf[n][s][i][0] =
-            h2_bits(__floats2half2_rn(x[s][c0] * down, x[s][c0 + d] * down));
-        qf[n][s][i][1] =
-            h2_bits(__floats2half2_rn(x[s][c0 + e] * down, x[s][c0 + e + d] * down));
+        uint32_t(&f)[2] = qf[n][s * (L::kProducts / L::kSteps) + i];
+        f[0] = h2_bits(__floats2half2_rn(x[s][c0] * down, x[s][c0 + d] * down));
+        f[1] = h2_bits(__floats2half2_rn(x[s][c0 + e] * down, x[s][c0 + e + d] * down));
       }
 #pragma unroll
     for (int r = 0; r < 2; ++r)
       factor[n][r] = __shfl_sync(0xffffffffu, up, 4 * (2 * j + r)) * (scale * kLog2e);
   }
 
-  float o[kTiles][Piece::kPasses][8][4] = {};
+  // o[n][p][i]: channels 16 (g + 8 p) + 2 i, + 1 of heads 2 j, 2 j + 1
+  float o[kTiles][L::kPasses][8][4] = {};
   float m[kTiles][2], l[kTiles][2] = {};
 #pragma unroll
   for (int n = 0; n < kTiles; ++n) m[n][0] = m[n][1] = -INFINITY;
   uint32_t v_exp = 1;  // exponent of the power of two the value scales are taken by
+  const int row0 = token_of(g);        // and row0 + 8: the tokens of S^T's rows
+  const int column0 = token_of(2 * j), column1 = token_of(2 * j + 1);  // of O^T, and + 8
 
+  int stage = 0;
+  uint32_t phase = 0;
 #pragma unroll 1
-  for (int block = warp; block < blocks; block += kWarps) {
-    const int next = block + kWarps;
-    const int64_t next_row = next < blocks ? row_of(next) : -1;
-    const int next_seen = next_row < 0 ? 0 : min(kBlock, here - next * kBlock);
+  while (seen[0] > 0) {
+    if (!mbar_wait(&bar[stage], phase)) {  // ran out: NaN, once the other copies are in
+#pragma unroll
+      for (int x = 1; x < kStages; ++x)
+        if (seen[x] > 0)
+          mbar_wait(&bar[(stage + x) % kStages], phase ^ (stage + x >= kStages ? 1u : 0u));
+#pragma unroll
+      for (int n = 0; n < kTiles; ++n) l[n][0] = l[n][1] = __uint_as_float(0x7FC00000u);
+      break;
+    }
+    const uint8_t* keys = codes + stage * 2 * L::kCodes;
+    const uint8_t* values = keys + L::kCodes;
+    const uint32_t* ksc = reinterpret_cast<const uint32_t*>(scales + stage * 2 * L::kScales);
+    const uint32_t* vsc = ksc + L::kScales / 4;
+    const bool whole = seen[0] == kBlock;
 
+    // ---- S^T = K Q^T
     float s[kTiles][4] = {};
-    tok.template scores<kTiles>(s, qf);
-    const float ks[2] = {tok.k_scale[0], tok.k_scale[1]};
-    if (next_row >= 0) tok.load_keys(c, next_row, next_seen, g, j);
+#pragma unroll
+    for (int st = 0; st < L::kSteps; ++st) {
+      uint32_t w[2][4];
+      __half2 gs[2], gm[2];
+#pragma unroll
+      for (int r = 0; r < 2; ++r) {
+        const uint32_t byte = L::key_byte(st, j);
+        const uint8_t* p = keys + L::at(row0 + 8 * r, byte);
+        if constexpr (L::kKeyWords == 4) {
+          const uint4 u = *reinterpret_cast<const uint4*>(p);
+          w[r][0] = u.x; w[r][1] = u.y; w[r][2] = u.z; w[r][3] = u.w;
+        } else {
+          const uint2 u = *reinterpret_cast<const uint2*>(p);
+          w[r][0] = u.x; w[r][1] = u.y;
+        }
+        if constexpr (BITS == 4) {
+          const uint32_t of = byte / 16;  // the group; past head_dim the codes are 0
+          const __half2 sm2 =
+              bits_h2(of * kGroup4 < c.dim ? ksc[(row0 + 8 * r) * (c.dim / kGroup4) + of] : 0u);
+          gs[r] = __low2half2(sm2);
+          gm[r] = __high2half2(sm2);
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < L::kProducts / L::kSteps; ++i) {
+        uint32_t a[2][2];
+#pragma unroll
+        for (int r = 0; r < 2; ++r) {
+          if constexpr (BITS == 8) {
+            const uint32_t x = w[r][i] ^ 0x80808080u;
+            a[r][0] = code8_pair(x, 0x4140);
+            a[r][1] = code8_pair(x, 0x4342);
+          } else {
+            const uint32_t x = w[r][i / 2] >> (8 * (i & 1));
+            a[r][0] = code4_pair<false>(x, gs[r], gm[r]);
+            a[r][1] = code4_pair<true>(x, gs[r], gm[r]);
+          }
+        }
+        const int at = st * (L::kProducts / L::kSteps) + i;
+#pragma unroll
+        for (int n = 0; n < kTiles; ++n)
+          mma_f16(s[n], a[0][0], a[1][0], a[0][1], a[1][1], qf[n][at][0], qf[n][at][1]);
+      }
+    }
 
-    // scores in powers of two; the maximum in use
+    // ---- scores in powers of two; the maximum in use
+    if constexpr (BITS == 8) {
+      const float ks[2] = {__uint_as_float(ksc[row0]), __uint_as_float(ksc[row0 + 8])};
+#pragma unroll
+      for (int n = 0; n < kTiles; ++n)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) s[n][e] *= ks[e >> 1];
+    }
     bool raise = false;
 #pragma unroll
     for (int n = 0; n < kTiles; ++n)
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        float y = s[n][e] * factor[n][e & 1];
-        if constexpr (BITS == 8) y *= ks[e >> 1];
-        s[n][e] = g + 8 * (e >> 1) < seen ? y : -INFINITY;
+        s[n][e] *= factor[n][e & 1];
+        if (!whole && row0 + 8 * (e >> 1) >= seen[0]) s[n][e] = -INFINITY;
         raise |= s[n][e] > m[n][e & 1] + kRaise;
       }
     if (__any_sync(0xffffffffu, raise)) {
@@ -404,7 +414,7 @@ __global__ void __launch_bounds__(32 * kWarps)
           m[n][r] = top;
           l[n][r] *= keep;
 #pragma unroll
-          for (int p = 0; p < Piece::kPasses; ++p)
+          for (int p = 0; p < L::kPasses; ++p)
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
               o[n][p][i][r] *= keep;
@@ -415,25 +425,30 @@ __global__ void __launch_bounds__(32 * kWarps)
     float vs[2] = {1.0f, 1.0f};
     if constexpr (BITS == 8) {
       // scales relative to 2^(v_exp - 127), above every scale so far
-      const uint32_t e = max(__float_as_uint(tok.v_scale[0]), __float_as_uint(tok.v_scale[1]));
+      uint32_t e0 = vsc[row0], e1 = vsc[row0 + 8];
+      if (!whole) {  // what lies behind the sequence's end is not used
+        if (row0 >= seen[0]) e0 = 0u;
+        if (row0 + 8 >= seen[0]) e1 = 0u;
+      }
+      const uint32_t e = max(e0, e1);
       if (__any_sync(0xffffffffu, e < 0x7F800000u && (e >> 23) >= v_exp)) {
-        const uint32_t now = max(v_exp, 1u + __reduce_max_sync(0xffffffffu,
-                                                  e < 0x7F800000u ? e >> 23 : 0u));
+        const uint32_t now =
+            max(v_exp, 1u + __reduce_max_sync(0xffffffffu, e < 0x7F800000u ? e >> 23 : 0u));
         const uint32_t drop = now - v_exp;  // by 2^-drop
         const float down = drop < 127u ? __uint_as_float((127u - drop) << 23) : 0.0f;
         v_exp = now;
 #pragma unroll
         for (int n = 0; n < kTiles; ++n)
 #pragma unroll
-          for (int p = 0; p < Piece::kPasses; ++p)
+          for (int p = 0; p < L::kPasses; ++p)
 #pragma unroll
             for (int i = 0; i < 8; ++i)
 #pragma unroll
               for (int r = 0; r < 4; ++r) o[n][p][i][r] *= down;
       }
       const float by = __uint_as_float((254u - v_exp) << 23);
-      vs[0] = tok.v_scale[0] * by;
-      vs[1] = tok.v_scale[1] * by;
+      vs[0] = __uint_as_float(e0) * by;
+      vs[1] = __uint_as_float(e1) * by;
     }
     uint32_t pt[kTiles][2];
 #pragma unroll
@@ -442,22 +457,86 @@ __global__ void __launch_bounds__(32 * kWarps)
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         const float top = m[n][e & 1];
-        p[e] = exp2f(s[n][e] - (top == -INFINITY ? 0.0f : top));
+        p[e] = exp2_fast(s[n][e] - (top == -INFINITY ? 0.0f : top));
         l[n][e & 1] += p[e];
-        p[e] *= vs[e >> 1];
+        if constexpr (BITS == 8) p[e] *= vs[e >> 1];
       }
       pt[n][0] = transpose8x8(h2_bits(__floats2half2_rn(p[0], p[1])));
       pt[n][1] = transpose8x8(h2_bits(__floats2half2_rn(p[2], p[3])));
     }
-    tok.template outputs<kTiles>(o, pt);
-    if (next_row >= 0)
-      tok.load_values(c, next_row, next_seen, g, j);
-    else
-      tok.clear();
-    seen = next_seen;
+
+    // ---- O^T += V^T P^T
+#pragma unroll
+    for (int p = 0; p < L::kPasses; ++p) {
+      // past the row (64-channel rows have 4 lanes' pieces): any, not stored
+      const uint32_t byte = ((kQuarters == 1 ? g & 3 : g) + 8 * p) * 2 * BITS;
+      constexpr int kWords = BITS / 2;
+      uint32_t w[4][kWords];
+      uint32_t gr[4];
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const int t = (r & 1 ? column1 : column0) + 8 * (r >> 1);
+        const uint8_t* at = values + L::at(t, byte);
+        if constexpr (BITS == 8) {
+          const uint4 u = *reinterpret_cast<const uint4*>(at);
+          w[r][0] = u.x; w[r][1] = u.y; w[r][2] = u.z; w[r][3] = u.w;
+        } else {
+          const uint2 u = *reinterpret_cast<const uint2*>(at);
+          w[r][0] = u.x; w[r][1] = u.y;
+          const uint32_t of = byte / 16;
+          gr[r] = of * kGroup4 < c.dim ? vsc[t * (c.dim / kGroup4) + of] : 0u;
+          if (!whole && t >= seen[0]) gr[r] = 0u;
+        }
+      }
+      if constexpr (BITS == 8) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const uint32_t w0 = w[0][i] ^ 0x80808080u, w1 = w[1][i] ^ 0x80808080u;
+          const uint32_t w2 = w[2][i] ^ 0x80808080u, w3 = w[3][i] ^ 0x80808080u;
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {  // channels 4 i + 2 h, + 1
+            const uint32_t x = __byte_perm(w0, w1, h ? 0x7362 : 0x5140);
+            const uint32_t y = __byte_perm(w2, w3, h ? 0x7362 : 0x5140);
+            const uint32_t a0 = code8_pair(x, 0x4140), a1 = code8_pair(x, 0x4342);
+            const uint32_t a2 = code8_pair(y, 0x4140), a3 = code8_pair(y, 0x4342);
+#pragma unroll
+            for (int n = 0; n < kTiles; ++n)
+              mma_f16(o[n][p][2 * i + h], a0, a1, a2, a3, pt[n][0], pt[n][1]);
+          }
+        }
+      } else {
+        const __half2 s01 = bits_h2(__byte_perm(gr[0], gr[1], 0x5410));
+        const __half2 m01 = bits_h2(__byte_perm(gr[0], gr[1], 0x7632));
+        const __half2 s23 = bits_h2(__byte_perm(gr[2], gr[3], 0x5410));
+        const __half2 m23 = bits_h2(__byte_perm(gr[2], gr[3], 0x7632));
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+#pragma unroll
+          for (int h = 0; h < 4; ++h) {  // channels 8 i + 2 h, + 1
+            const uint32_t sel = h < 2 ? 0x5410 : 0x7632;
+            const uint32_t x = __byte_perm(w[0][i], w[1][i], sel) >> (8 * (h & 1));
+            const uint32_t y = __byte_perm(w[2][i], w[3][i], sel) >> (8 * (h & 1));
+            const uint32_t a0 = code4_pair<false>(x, s01, m01), a1 = code4_pair<true>(x, s01, m01);
+            const uint32_t a2 = code4_pair<false>(y, s23, m23), a3 = code4_pair<true>(y, s23, m23);
+#pragma unroll
+            for (int n = 0; n < kTiles; ++n)
+              mma_f16(o[n][p][4 * i + h], a0, a1, a2, a3, pt[n][0], pt[n][1]);
+          }
+      }
+    }
+
+    // ---- the stage is read: the next block into it
+    __syncwarp();
+    const int more = fetch_into(stage);
+#pragma unroll
+    for (int x = 0; x + 1 < kStages; ++x) seen[x] = seen[x + 1];
+    seen[kStages - 1] = more;
+    if (++stage == kStages) stage = 0, phase ^= 1u;
   }
 
-  // the warps' parts, in shared memory
+  // the warps' parts, in the rings' memory
+  __syncthreads();
+  float* so = reinterpret_cast<float*>(shared);  // [kWarps][kHeads][dim]
   const float up = BITS == 8 ? __uint_as_float(v_exp << 23) : 1.0f;
 #pragma unroll
   for (int n = 0; n < kTiles; ++n) {
@@ -468,7 +547,7 @@ __global__ void __launch_bounds__(32 * kWarps)
       const int h = 8 * n + 2 * j + r;
       if (g == 0) sm[warp][h] = m[n][r], sl[warp][h] = l[n][r];
 #pragma unroll
-      for (int p = 0; p < Piece::kPasses; ++p) {
+      for (int p = 0; p < L::kPasses; ++p) {
         const uint32_t ch = 16 * (g + 8 * p);
         if (ch < c.dim)
 #pragma unroll
@@ -507,11 +586,10 @@ __global__ void __launch_bounds__(32 * kWarps)
 // A CTA a (sequence, head): the chunks' parts in order.
 __global__ void __launch_bounds__(256)
     cache_attention_join_kernel(const float* __restrict__ parts, uint32_t chunks, uint32_t chunk,
-                                uint32_t heads, uint32_t dim, int64_t most,
-                                const int32_t* __restrict__ lengths, bool bf16,
+                                uint32_t heads, uint32_t dim, Lengths lengths, bool bf16,
                                 void* __restrict__ out) {
   const int64_t head = (int64_t)blockIdx.y * heads + blockIdx.x;
-  const int64_t len = max64(0, min64(lengths[blockIdx.y], most));
+  const int64_t len = lengths.of(blockIdx.y);
   const int n = max((int)((len + chunk - 1) / chunk), 1);
   const float2* ml = reinterpret_cast<const float2*>(
                          parts + (int64_t)gridDim.y * heads * chunks * dim) + head * chunks;
@@ -550,6 +628,68 @@ inline Split split_for(const CacheView& c, int64_t batch, int64_t heads, int64_t
   s.chunks = (uint32_t)max64(1, ceil_div(most, chunk));
   s.chunk = (uint32_t)chunk;
   return s;
+}
+
+// Rows of codes as TMA reads them: [all rows, bytes], boxes of 16 rows.
+bool rows_map(CUtensorMap* map, const void* codes, const CacheView& c, int bits, uint32_t box_row) {
+  auto enc = tensor_map_encoder();
+  if (enc == nullptr) return false;
+  std::memset(map, 0, sizeof(*map));
+  const cuuint64_t bytes = (cuuint64_t)c.dim * bits / 8;
+  const cuuint64_t dims[2] = {bytes, (cuuint64_t)(c.pages * c.heads * c.page_size)};
+  const cuuint64_t strides[1] = {bytes};
+  const cuuint32_t box[2] = {box_row, (cuuint32_t)kBlock};
+  const cuuint32_t ones[2] = {1, 1};
+  const CUtensorMapSwizzle swizzle = box_row == 128  ? CU_TENSOR_MAP_SWIZZLE_128B
+                                     : box_row == 64 ? CU_TENSOR_MAP_SWIZZLE_64B
+                                                     : CU_TENSOR_MAP_SWIZZLE_32B;
+  return enc(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(codes), dims, strides, box,
+             ones, CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle, CU_TENSOR_MAP_L2_PROMOTION_NONE,
+             CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+struct Call {
+  CacheView c;
+  Query q;
+  uint32_t heads;
+  Split split;
+  dim3 grid;
+  const int32_t* table;
+  int64_t table_stride;
+  Lengths lengths;
+  float scale;
+  float* parts;
+  void* out;
+  cudaStream_t stream;
+};
+
+template <int BITS, int kQuarters, int kTiles>
+mb_status launch(const Call& a) {
+  using L = Layout<BITS, kQuarters>;
+  constexpr int kStages = 3;
+  CUtensorMap k_map, v_map;
+  if (!rows_map(&k_map, a.c.codes[0], a.c, BITS, L::kBoxRow) ||
+      !rows_map(&v_map, a.c.codes[1], a.c, BITS, L::kBoxRow))
+    return set_error(MB_ERR_CUDA, "cuTensorMapEncodeTiled rejected the cache");
+  const size_t ring = (size_t)kWarps * kStages * L::kStage;
+  const size_t join = (size_t)kWarps * 8 * kTiles * a.c.dim * sizeof(float);
+  const size_t smem = (ring > join ? ring : join) + 1024;
+  auto* kernel = cache_attention_kernel<BITS, kQuarters, kTiles, kStages>;
+  static std::atomic<uint64_t> attr_done{0};
+  MB_CUDA_TRY(set_smem_limit_once(kernel, 160 * 1024, attr_done));
+  kernel<<<a.grid, 32 * kWarps, smem, a.stream>>>(
+      k_map, v_map, a.c, a.q, a.heads, a.split.head_blocks, a.table, a.table_stride, a.lengths,
+      a.scale, a.split.chunk, a.parts, a.out);
+  MB_LAUNCH_CHECK("cache_attention_kernel");
+  return MB_OK;
+}
+
+template <int BITS>
+mb_status dispatch(const Call& a, uint32_t tiles) {
+  if (a.c.dim <= 64) return tiles == 2 ? launch<BITS, 1, 2>(a) : launch<BITS, 1, 1>(a);
+  if (a.c.dim <= 128) return tiles == 2 ? launch<BITS, 2, 2>(a) : launch<BITS, 2, 1>(a);
+  if (a.c.dim <= 192) return launch<BITS, 3, 1>(a);
+  return launch<BITS, 4, 1>(a);
 }
 
 }  // namespace
@@ -607,31 +747,16 @@ extern "C" mb_status mb_cache_attention(const mb_kv_cache* cache, const void* q,
                      (heads == 1 || q_head_stride % 8 == 0)};
   const dim3 grid(s.chunks, (unsigned)(c.heads * s.head_blocks), (unsigned)batch);
   MB_REQUIRE(grid.y <= 65535u, "too many head blocks");
-  const size_t smem = (size_t)kWarps * 8 * tiles * c.dim * sizeof(float);
-  const auto go = [&](auto kernel) {
-    kernel<<<grid, 32 * kWarps, smem, stream>>>(c, qs, (uint32_t)heads, s.head_blocks, page_table,
-                                                table_stride, most, lengths, scale, s.chunk, parts,
-                                                out);
-  };
-  const auto steps = [&](auto bits) {
-    constexpr int B = decltype(bits)::value;
-    if (c.dim <= 64)
-      tiles == 2 ? go(cache_attention_kernel<B, 1, 2>) : go(cache_attention_kernel<B, 1, 1>);
-    else if (c.dim <= 128)
-      tiles == 2 ? go(cache_attention_kernel<B, 2, 2>) : go(cache_attention_kernel<B, 2, 1>);
-    else if (c.dim <= 192)
-      go(cache_attention_kernel<B, 3, 1>);
-    else
-      go(cache_attention_kernel<B, 4, 1>);
-  };
-  if (cache->bits == 8)
-    steps(std::integral_constant<int, 8>{});
-  else
-    steps(std::integral_constant<int, 4>{});
-  MB_LAUNCH_CHECK("cache_attention_kernel");
+  MB_REQUIRE(c.pages * c.heads * c.page_size < (int64_t(1) << 31),
+             "cache too large: pages * kv_heads * page_size must fit 31 bits");
+  const Lengths all{lengths, most};
+  const Call call{c,     qs,  (uint32_t)heads, s,     grid, page_table, table_stride,
+                  all,   scale, parts,         out,   stream};
+  const mb_status st = cache->bits == 8 ? dispatch<8>(call, tiles) : dispatch<4>(call, tiles);
+  if (st != MB_OK) return st;
   if (parts != nullptr) {
     cache_attention_join_kernel<<<dim3((unsigned)heads, (unsigned)batch), 256, 0, stream>>>(
-        parts, s.chunks, s.chunk, (uint32_t)heads, c.dim, most, lengths, type == MB_BF16, out);
+        parts, s.chunks, s.chunk, (uint32_t)heads, c.dim, all, type == MB_BF16, out);
     MB_LAUNCH_CHECK("cache_attention_join_kernel");
   }
   return MB_OK;
