@@ -9,12 +9,11 @@
 // bound by reading the codes, and the products only keep the arithmetic off
 // the fp32 units.
 //
-// Codes and scales reach a warp through a ring of its own in shared memory,
-// 16 tokens a stage, filled by TMA: a 16-row box of each code array (rows of
-// one page and head are contiguous) and a bulk copy of each scale array, all
-// issued by one lane and awaited on one mbarrier.  With a stage of 4.2 KB
-// (8 bits, head_dim 128), three stages and 16 warps an SM has up to 200 KB on
-// the way; held in registers instead, two thirds of a stage a warp were.
+// A CTA has kWarps warps that compute, 16 tokens each at a time, and one that
+// fetches: units of 16 kWarps tokens go through a ring in shared memory by TMA
+// (boxes of the code arrays as tall as the pages allow -- rows of one page and
+// head are contiguous -- and bulk copies of the scales), also across the end
+// of a sequence, while the others finish it.
 //
 // Both products' left operands are read as they lie, because the order of the
 // inner index is free: in S^T lane (g, j) = (lane / 4, lane % 4) takes 16 bytes
@@ -24,22 +23,27 @@
 // reads free of bank conflicts.  Between the products the probabilities
 // change from S^T's layout to the right operand's by a transposing move.
 //
-// 8-bit codes become exact fp16 integers (1024 + 128 + code by a byte
-// permute, minus 1152); the key's scale multiplies the score and the value's
-// the probability, relative to a power of two at or above every scale so far,
-// so that the product stays in fp16's range.  4-bit codes become
-// m + s * code in fp16, one rounding, as cache_read returns them.  The query
-// is scaled by a power of two to below 1 (a bf16 value then fits fp16);
-// probabilities are rounded to fp16 (2^-11); scores, maxima, sums and the
-// accumulators are fp32.
+// 8-bit keys enter S^T as they are: an m16n8k32 integer product with the
+// query, scaled by a power of two to below 1, in two 8-bit parts (14 bits and
+// a sign: off by at most 2^-14 of the query's largest channel; exact for
+// channels above 1/8 of it, in bf16 above 1/64).  The sums are exact.  8-bit
+// values become exact fp16 integers (1024 + 128 + code by a byte permute,
+// minus 1152); their scale multiplies the probability, relative to a power of
+// two above every scale so far, so that the product stays in fp16's range.
+// 4-bit codes become m + s * code in fp16, one rounding; the query then is
+// fp16 too.  Probabilities are rounded to fp16 (2^-11); scores, maxima, sums
+// and the outputs' accumulators are fp32.
 //
 // The running maximum is raised only when a score exceeds it by 8 (in powers
 // of two): probabilities then stay below 256 and most steps rescale nothing.
 //
-// Long sequences are split over CTAs in chunks of `chunk` tokens; each leaves
-// its maximum, sum and unnormalised output in the workspace, and a second
-// kernel joins them in the chunks' order, so the result does not depend on
-// the CTAs' timing.
+// The units of all sequences and heads are dealt out evenly to two CTAs an SM,
+// whatever the lengths: a CTA's share may begin and end inside a sequence.
+// Those parts (maximum, sum, unnormalised output) go to the workspace, two a
+// CTA at most, and a second kernel joins them in the order of the tokens, so
+// the result does not depend on the CTAs' timing.  Where the table holds few
+// tokens a sequence, a CTA takes a whole sequence's head instead and nothing
+// is joined.
 #include <algorithm>
 #include <cmath>
 #include <cstring>
@@ -50,7 +54,6 @@
 namespace mb {
 namespace {
 
-constexpr int kWarps = 4;
 constexpr int kBlock = 16;  // tokens a warp takes at a time
 
 __device__ __forceinline__ void mma_f16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2,
@@ -59,6 +62,15 @@ __device__ __forceinline__ void mma_f16(float (&c)[4], uint32_t a0, uint32_t a1,
       "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 "
       "{%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
       : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+__device__ __forceinline__ void mma_s8(int (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2,
+                                       uint32_t a3, uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 "
+      "{%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+      : "+r"(c[0]), "+r"(c[1]), "+r"(c[2]), "+r"(c[3])
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
@@ -101,32 +113,43 @@ __device__ __forceinline__ void store_out(void* out, bool bf16, int64_t i, float
     static_cast<__half*>(out)[i] = __float2half_rn(y);
 }
 
-// How rows of a head_dim in (64 (kQuarters - 1), 64 kQuarters] lie in a stage.
+// How rows of a head_dim in (64 (kQuarters - 1), 64 kQuarters] are taken.
 template <int BITS, int kQuarters>
 struct Layout {
+  static constexpr int kWarps = kQuarters <= 2 ? 8 : 4;    // that compute
+  static constexpr int kUnit = kWarps * kBlock;            // tokens a stage
+  static constexpr int kThreads = 32 * (kWarps + 1);
   static constexpr int kRow = kQuarters >= 3 ? (BITS == 8 ? 256 : 128) : kQuarters * 8 * BITS;
   static constexpr int kBoxRow = kRow < 128 ? kRow : 128;  // bytes of a row in one box
   static constexpr int kBoxes = kRow / kBoxRow;
-  static constexpr int kBox = kBlock * kBoxRow;
-  static constexpr int kCodes = kBlock * kRow;             // of keys, or of values
+  static constexpr int kColumn = kUnit * kBoxRow;          // a box column of a stage
+  static constexpr int kCodes = kUnit * kRow;              // of keys, or of values
   static constexpr int kSwizzle = kBoxRow == 128 ? 0x70 : kBoxRow == 64 ? 0x30 : 0x10;
-  // bytes of 16 tokens' scales, and what a stage keeps for them
+  // bytes of a token's scales, and what a stage keeps for them at most
   __host__ __device__ static constexpr uint32_t scale_bytes(uint32_t dim) {
-    return kBlock * (BITS == 8 ? 4 : dim / kGroup4 * 4);
+    return BITS == 8 ? 4 : dim / kGroup4 * 4;
   }
-  static constexpr int kScales = kBlock * (BITS == 8 ? 4 : 2 * kQuarters * 4);
-  static constexpr int kStage = 2 * (kCodes + kScales);
+  static constexpr int kScales = kUnit * (BITS == 8 ? 4 : 2 * kQuarters * 4);
+  // a stage: the keys' codes, the values', the keys' scales, the values'
+  static constexpr int kStage = (2 * (kCodes + kScales) + 1023) / 1024 * 1024;
+  static constexpr int kStages = kStage > 24 * 1024 ? 2 : 3;
 
   // S^T: steps of 4 lanes x kKeyWords words; O^T: passes of 8 lanes x 16 channels
   static constexpr int kKeyWords = BITS == 4 && kQuarters == 1 ? 2 : 4;
   static constexpr int kSteps = kRow / (16 * kKeyWords);
-  static constexpr int kProducts = kSteps * kKeyWords * (BITS == 8 ? 1 : 2);  // of S^T
+  static constexpr int kProducts = kSteps * (BITS == 8 ? 4 : 2 * kKeyWords);  // of S^T
   static constexpr int kPasses = (kQuarters + 1) / 2;
+
+  // The warps' outputs of 8 heads before they are joined: [warp][8][kJoinRow],
+  // channel ch at ch + 4 (ch / 32) (free of bank conflicts).
+  static constexpr int kJoinRow = 64 * kQuarters + 8 * kQuarters + 1;
+  static constexpr int kJoin = kWarps * 8 * kJoinRow * 4;
+  static constexpr int kSmem = 1024 + kStages * kStage + kJoin;
 
   // Place in a stage's keys (or values) of a byte of a row.
   __device__ __forceinline__ static uint32_t at(uint32_t row, uint32_t byte) {
     const uint32_t o = row * kBoxRow + byte % kBoxRow;
-    return byte / kBoxRow * kBox + (o ^ ((o >> 3) & kSwizzle));
+    return byte / kBoxRow * kColumn + (o ^ ((o >> 3) & kSwizzle));
   }
   // First byte of lane j's part of a key's row in a step.
   __device__ __forceinline__ static uint32_t key_byte(int step, int j) {
@@ -150,6 +173,24 @@ __device__ __forceinline__ float exp2_fast(float x) {
   return y;
 }
 
+__device__ __forceinline__ uint4 lds128(uint32_t at) {
+  uint4 v;
+  asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];"
+               : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+               : "r"(at));
+  return v;
+}
+__device__ __forceinline__ uint2 lds64(uint32_t at) {
+  uint2 v;
+  asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(at));
+  return v;
+}
+__device__ __forceinline__ uint32_t lds32(uint32_t at) {
+  uint32_t v;
+  asm volatile("ld.shared.u32 %0, [%1];" : "=r"(v) : "r"(at));
+  return v;
+}
+
 // Bulk copy of n bytes (a multiple of 16, both sides 16-byte aligned).
 __device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t n, uint64_t* bar) {
   asm volatile(
@@ -159,452 +200,722 @@ __device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t n
       : "memory");
 }
 
-// A warp's walk over its blocks' places in the pages.
-struct Walk {
-  uint32_t page, place;  // of the next block
-  __device__ __forceinline__ void start(uint32_t t, uint32_t page_size) {
-    page = t / page_size;
-    place = t - page * page_size;
-  }
-  __device__ __forceinline__ void advance(uint32_t pages, uint32_t rest, uint32_t page_size) {
-    page += pages;
-    place += rest;
-    if (place >= page_size) place -= page_size, ++page;
-  }
-};
-
 struct Lengths {
   const int32_t* data;
   int64_t most;  // tokens the table can name
-  __device__ __forceinline__ int64_t of(int64_t b) const {
-    return max64(0, min64(data[b], most));
+  uint32_t batch;
+  __device__ __forceinline__ int of(uint32_t b) const {
+    return (int)max64(0, min64(data[b], most));
   }
 };
 
-// Grid: (chunks, kv heads x head blocks, batch).  parts: per (sequence, head,
-// chunk) head_dim outputs, then all (maximum, sum) pairs; null with one chunk.
-template <int BITS, int kQuarters, int kTiles, int kStages>
-__global__ void __launch_bounds__(32 * kWarps)
+// A sequence's units of `unit` tokens, and before them one without tokens: what
+// beginning and ending a sequence's head costs.  Dealing the tokens' units
+// alone left CTAs with many short sequences behind (16 sequences of 1 .. 2048
+// tokens and 32 heads: 74 us).
+constexpr uint32_t kIdle = 1;
+__device__ __forceinline__ uint32_t units_of(int len, uint32_t unit) {
+  return kIdle + ((uint32_t)len + unit - 1) / unit;
+}
+
+// The units in order: sequences, in them rows (a key/value head's block of
+// query heads), in them tokens.  before(b): the units of a row of the
+// sequences before b.
+struct Deal {
+  unsigned long long before;  // of sequence b
+  uint32_t b, n;              // that sequence, its units
+  unsigned long long total;   // of a row of all sequences
+};
+
+// The sequence that holds unit `u(total)` of all rows, found by the whole CTA
+// of kThreads.
+template <int kThreads, typename U>
+__device__ __forceinline__ Deal find_unit(const Lengths& lengths, uint32_t unit, uint32_t rows,
+                                          U&& u) {
+  constexpr int kParts = kThreads / 32;
+  __shared__ unsigned long long sums[kParts], found_before, total;
+  __shared__ uint32_t found_b, found_n;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  unsigned long long mine = 0;
+  for (uint32_t b = threadIdx.x; b < lengths.batch; b += kThreads)
+    mine += units_of(lengths.of(b), unit);
+#pragma unroll
+  for (int d = 16; d > 0; d >>= 1) mine += __shfl_xor_sync(0xffffffffu, mine, d);
+  if (lane == 0) sums[warp] = mine;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    unsigned long long t = 0;
+    for (int w = 0; w < kParts; ++w) t += sums[w];
+    total = t;
+    found_b = lengths.batch;
+  }
+  __syncthreads();
+  const unsigned long long at = u(total);
+  unsigned long long done = 0;
+  for (uint32_t b0 = 0; b0 < lengths.batch; b0 += kThreads) {
+    const uint32_t b = b0 + threadIdx.x;
+    const uint32_t n = b < lengths.batch ? units_of(lengths.of(b), unit) : 0;
+    unsigned long long upto = n;
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+      const unsigned long long x = __shfl_up_sync(0xffffffffu, upto, d);
+      if (lane >= d) upto += x;
+    }
+    __syncthreads();  // sums of the last round are read
+    if (lane == 31) sums[warp] = upto;
+    __syncthreads();
+    unsigned long long all = 0;
+    for (int w = 0; w < kParts; ++w) {
+      if (w == warp) upto += all;
+      all += sums[w];
+    }
+    const unsigned long long before = done + upto - n;
+    if (n > 0 && at >= before * rows && at < (before + n) * rows) {
+      found_b = b;
+      found_n = n;
+      found_before = before;
+    }
+    done += all;
+  }
+  __syncthreads();
+  return Deal{found_before, found_b, found_n, total};
+}
+
+// A run of a CTA's units inside one row of one sequence.
+struct Segment {
+  uint32_t b, row, c0, c1;  // sequence, row, units c0 .. c1 - 1
+  uint32_t n;               // units of the sequence
+  int len;
+  // those with tokens
+  __device__ __forceinline__ uint32_t first() const { return max(c0, kIdle) - kIdle; }
+  __device__ __forceinline__ uint32_t last() const { return max(c1, kIdle) - kIdle; }
+};
+
+// A CTA's segments in turn.
+struct Segments {
+  const Lengths* lengths;
+  uint32_t unit, rows;
+  unsigned long long left;  // units
+  Segment s;
+
+  __device__ __forceinline__ void begin(const Lengths* all, uint32_t unit_, uint32_t rows_,
+                                        const Deal& d, unsigned long long u0,
+                                        unsigned long long u1) {
+    lengths = all;
+    unit = unit_;
+    rows = rows_;
+    left = u1 - u0;
+    if (left == 0) return;
+    const unsigned long long in = u0 - d.before * rows;
+    s.b = d.b;
+    s.n = d.n;
+    s.row = (uint32_t)(in / d.n);
+    s.c0 = (uint32_t)(in - (unsigned long long)s.row * d.n);
+    s.len = lengths->of(s.b);
+    s.c1 = (uint32_t)min((unsigned long long)s.n, s.c0 + left);
+  }
+  __device__ __forceinline__ bool more() const { return left > 0; }
+  __device__ __forceinline__ void next() {
+    left -= s.c1 - s.c0;
+    if (left == 0) return;
+    if (++s.row == rows) {
+      s.row = 0;
+      ++s.b;
+      s.len = lengths->of(s.b);
+      s.n = units_of(s.len, unit);
+    }
+    s.c0 = 0;
+    s.c1 = (uint32_t)min((unsigned long long)s.n, left);
+  }
+};
+
+// No more CTAs share the units than there are, so that none between two others
+// has nothing; first unit of CTA i's share.
+__device__ __forceinline__ unsigned long long shares_used(unsigned long long units,
+                                                          uint32_t shares) {
+  return units < shares ? units : shares;
+}
+__device__ __forceinline__ unsigned long long share_begin(unsigned long long i,
+                                                          unsigned long long units,
+                                                          unsigned long long used) {
+  return i * units / used;
+}
+
+struct Heads {
+  uint32_t all, group, blocks;  // of q; of a key/value head; blocks of a group
+};
+
+// shares: CTAs the units are dealt to (then gridDim.x = shares and `parts` has
+// two places a CTA: [8 kTiles heads][head_dim] outputs, behind all of them
+// (maximum, sum) pairs), or 0: CTA i takes row i % rows of sequence i / rows.
+template <int BITS, int kQuarters, int kTiles>
+__global__ void
+__launch_bounds__(Layout<BITS, kQuarters>::kThreads, kTiles == 1 ? 2 : 1)
     cache_attention_kernel(const __grid_constant__ CUtensorMap k_map,
-                           const __grid_constant__ CUtensorMap v_map, CacheView c, Query q,
-                           uint32_t heads, uint32_t head_blocks, const int32_t* __restrict__ table,
-                           int64_t table_stride, Lengths lengths, float scale, uint32_t chunk,
+                           const __grid_constant__ CUtensorMap v_map, CacheView c,
+                           uint32_t box_rows, Query q, Heads heads,
+                           const int32_t* __restrict__ table, int64_t table_stride,
+                           const __grid_constant__ Lengths lengths, float scale, uint32_t shares,
                            float* __restrict__ parts, void* __restrict__ out) {
+  grid_launch_dependents();
   using L = Layout<BITS, kQuarters>;
   constexpr int kHeads = 8 * kTiles;
   extern __shared__ uint8_t raw[];
-  uint8_t* shared = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(raw) + 1023) &
-                                               ~(uintptr_t)1023);
-  __shared__ float sm[kWarps][kHeads], sl[kWarps][kHeads];
-  __shared__ uint64_t bars[kWarps][kStages];
-  const uint32_t group = heads / c.heads;
-  const uint32_t kvh = blockIdx.y / head_blocks, h0 = (blockIdx.y % head_blocks) * kHeads;
-  const int64_t b = blockIdx.z;
+  uint8_t* ring = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(raw) + 1023) &
+                                             ~(uintptr_t)1023);
+  float* join = reinterpret_cast<float*>(ring + L::kStages * L::kStage);
+  __shared__ float sm[L::kWarps][8], sl[L::kWarps][8];
+  __shared__ uint64_t full[L::kStages], empty[L::kStages];
+  __shared__ int tokens[L::kStages][L::kWarps];  // of a warp's 16 that there are
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, j = lane & 3;
-  const int64_t len = lengths.of(b);
-  const int64_t t0 = (int64_t)blockIdx.x * chunk;
-  if (t0 >= len && blockIdx.x > 0) return;  // the join reads no such part
-  const int here = (int)min64(chunk, len - t0);
-  const int blocks = (here + kBlock - 1) / kBlock;
-  const int32_t* pages = table + b * table_stride;
+  const uint32_t rows = c.heads * heads.blocks;
+  const uint32_t token_scales = L::scale_bytes(c.dim);
 
-  uint8_t* codes = shared + warp * kStages * 2 * L::kCodes;  // per stage: keys, values
-  uint8_t* scales = shared + kWarps * kStages * 2 * L::kCodes + warp * kStages * 2 * L::kScales;
-  uint64_t* bar = bars[warp];
-  const uint32_t scale_bytes = L::scale_bytes(c.dim);
-  if (lane == 0) {
-    for (int s = 0; s < kStages; ++s) mbar_init(&bar[s], 1);
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < L::kStages; ++s) {
+      mbar_init(&full[s], 1);
+      mbar_init(&empty[s], L::kWarps);
+    }
     fence_mbar_init();
   }
-  __syncwarp();
+  Segments run;
+  if (shares > 0) {
+    unsigned long long u0 = 0, u1 = 0;
+    const Deal d = find_unit<L::kThreads>(
+        lengths, L::kUnit, rows, [&](unsigned long long total) {
+          const unsigned long long units = total * rows, n = shares_used(units, shares);
+          if (blockIdx.x < n) {
+            u0 = share_begin(blockIdx.x, units, n);
+            u1 = share_begin(blockIdx.x + 1, units, n);
+          }
+          return u0;
+        });
+    run.begin(&lengths, L::kUnit, rows, d, u0, u1);
+  } else {
+    const uint32_t b = blockIdx.x / rows;
+    const Deal d{0, b, units_of(lengths.of(b), L::kUnit), 0};
+    const unsigned long long u0 = (unsigned long long)(blockIdx.x - b * rows) * d.n;
+    run.begin(&lengths, L::kUnit, rows, d, u0, u0 + d.n);
+  }
+  __syncthreads();
 
-  // The next block to fetch: its number, and its page, read one fetch ahead.
-  constexpr uint32_t kStride = kWarps * kBlock;
-  const uint32_t stride_pages = kStride / c.page_size, stride_rest = kStride % c.page_size;
-  Walk walk;
-  walk.start((uint32_t)t0 + warp * kBlock, c.page_size);
-  int fetch = warp;
-  int32_t page = fetch < blocks ? pages[walk.page] : 0;
-  // Fetches the next block whose page exists into a stage; the number of its
-  // tokens that the sequence has, or 0 if there is none.
-  const auto fetch_into = [&](int s) -> int {
-    while (fetch < blocks) {
-      const int32_t p = page;
-      const uint32_t place = walk.place;
-      const int seen = min(kBlock, here - fetch * kBlock);
-      fetch += kWarps;
-      walk.advance(stride_pages, stride_rest, c.page_size);
-      if (fetch < blocks) page = pages[walk.page];
-      if (p < 0 || p >= c.pages) continue;
-      if (lane == 0) {
-        const int64_t row = ((int64_t)p * c.heads + kvh) * c.page_size + place;
-        uint8_t* at = codes + s * 2 * L::kCodes;
-        uint8_t* sc = scales + s * 2 * L::kScales;
-        mbar_arrive_expect_tx(&bar[s], 2 * (L::kCodes + scale_bytes));
-#pragma unroll
-        for (int x = 0; x < L::kBoxes; ++x) {
-          tma_load_2d(at + x * L::kBox, &k_map, &bar[s], x * L::kBoxRow, (int)row);
-          tma_load_2d(at + L::kCodes + x * L::kBox, &v_map, &bar[s], x * L::kBoxRow, (int)row);
+  if (warp == L::kWarps) {
+    // ---- the warp that fetches: lane x the x-th box of a unit
+    const uint32_t boxes = L::kUnit / box_rows, mine = lane * box_rows;
+    const bool holds = lane < (int)boxes;
+    int stage = 0, issued = 0;
+    uint32_t phase = 1;
+    bool ok = true;
+    for (; run.more() && ok; run.next()) {
+      const Segment& s = run.s;
+      const uint32_t kvh = s.row / heads.blocks;
+      const int32_t* pages = table + (int64_t)s.b * table_stride;
+      for (uint32_t u = s.first(); u < s.last(); ++u) {
+        const uint32_t t = u * L::kUnit + mine;
+        const bool in = holds && t < (uint32_t)s.len;
+        const uint32_t p = t / c.page_size;
+        const int32_t page = in ? pages[p] : -1;
+        const bool there = page >= 0 && page < c.pages;
+        if (!mbar_wait(&empty[stage], phase)) {
+          ok = false;
+          break;
         }
-        const int64_t first = row * (scale_bytes / kBlock);
-        bulk_load(sc, c.scales[0] + first, scale_bytes, &bar[s]);
-        bulk_load(sc + L::kScales, c.scales[1] + first, scale_bytes, &bar[s]);
-      }
-      return seen;
-    }
-    return 0;
-  };
-  int seen[kStages];  // of the stages in order, the next to use first
+        const uint32_t lanes = __ballot_sync(0xffffffffu, there);
+        if (holds)
+          for (uint32_t x = 0; x < box_rows / kBlock; ++x)
+            tokens[stage][lane * (box_rows / kBlock) + x] =
+                there ? min(kBlock, max(0, s.len - (int)(t + x * kBlock))) : 0;
+        __syncwarp();
+        if (lane == 0)
+          mbar_arrive_expect_tx(&full[stage],
+                                __popc(lanes) * 2 * box_rows * (L::kRow + token_scales));
+        __syncwarp();
+        if (there) {
+          const int64_t row =
+              ((int64_t)page * c.heads + kvh) * c.page_size + (t - p * c.page_size);
+          uint8_t* at = ring + stage * L::kStage + mine * L::kBoxRow;
+          uint8_t* sc = ring + stage * L::kStage + 2 * L::kCodes + mine * token_scales;
 #pragma unroll
-  for (int s = 0; s < kStages; ++s) seen[s] = fetch_into(s);
-
-  // Q in the order of the keys' registers, below 1 by a power of two a head
-  uint32_t qf[kTiles][L::kProducts][2];
-  float factor[kTiles][2];  // of heads 2 j, 2 j + 1: scale log2(e) and that power
-#pragma unroll
-  for (int n = 0; n < kTiles; ++n) {
-    const uint32_t h = h0 + 8 * n + g;
-    const bool live = h < group;
-    const int64_t at = b * q.batch_stride + (int64_t)(kvh * group + (live ? h : 0)) * q.head_stride;
-    constexpr int kPer = L::kKeyWords * 32 / BITS;  // channels of a lane in a step
-    float x[L::kSteps][kPer];
-    uint32_t top = 0;
-#pragma unroll
-    for (int s = 0; s < L::kSteps; ++s) {
-      const uint32_t ch = L::key_byte(s, j) * 8 / BITS;
-#pragma unroll
-      for (int e = 0; e < kPer / 8; ++e) {
-        float y[8] = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
-        if (live && ch + 8 * e < c.dim) {
-          if (q.bf16)
-            load8(static_cast<const __nv_bfloat16*>(q.data) + at + ch + 8 * e, q.vec, 8, y);
-          else
-            load8(static_cast<const __half*>(q.data) + at + ch + 8 * e, q.vec, 8, y);
+          for (int x = 0; x < L::kBoxes; ++x) {
+            tma_load_2d(at + x * L::kColumn, &k_map, &full[stage], x * L::kBoxRow, (int)row);
+            tma_load_2d(at + L::kCodes + x * L::kColumn, &v_map, &full[stage], x * L::kBoxRow,
+                        (int)row);
+          }
+          const int64_t first = row * token_scales;
+          bulk_load(sc, c.scales[0] + first, box_rows * token_scales, &full[stage]);
+          bulk_load(sc + L::kScales, c.scales[1] + first, box_rows * token_scales, &full[stage]);
         }
-        top = max(top, abs_bits_max(y));
-#pragma unroll
-        for (int i = 0; i < 8; ++i) x[s][8 * e + i] = y[i];
+        ++issued;
+        if (++stage == L::kStages) stage = 0, phase ^= 1u;
       }
     }
-    top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
-    top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
-    // 2^-p with 2^(p - 1) <= max < 2^p; 1 for zeros, and where the query is not finite
-    const uint32_t ex = top >> 23;
-    const bool plain = ex == 0 || ex == 255;
-    const float down = plain ? 1.0f : __uint_as_float((253u - min(ex, 252u)) << 23);
-    const float up = plain ? 1.0f : __uint_as_float((1u + min(ex, 252u)) << 23);
-#pragma unroll
-    for (int s = 0; s < L::kSteps; ++s)
-#pragma unroll
-      for (int i = 0; i < L::kProducts / L::kSteps; ++i) {
-        // channels of the products' registers: code8_pair and code4_pair
-        const int c0 = BITS == 8 ? 4 * i : 8 * (i / 2) + 2 * (i & 1);
-        const int d = BITS == 8 ? 1 : 4, e = BITS == 8 ? 2 : 1;
-        uint32_t(&f)[2] = qf[n][s * (L::kProducts / L::kSteps) + i];
-        f[0] = h2_bits(__floats2half2_rn(x[s][c0] * down, x[s][c0 + d] * down));
-        f[1] = h2_bits(__floats2half2_rn(x[s][c0 + e] * down, x[s][c0 + e + d] * down));
-      }
-#pragma unroll
-    for (int r = 0; r < 2; ++r)
-      factor[n][r] = __shfl_sync(0xffffffffu, up, 4 * (2 * j + r)) * (scale * kLog2e);
+    // a reader that gave up leaves: not before the copies are in
+    for (int x = max(0, issued - L::kStages); x < issued; ++x)
+      mbar_wait(&full[x % L::kStages], (uint32_t)((x / L::kStages) & 1));
+    return;
   }
 
-  // o[n][p][i]: channels 16 (g + 8 p) + 2 i, + 1 of heads 2 j, 2 j + 1
-  float o[kTiles][L::kPasses][8][4] = {};
-  float m[kTiles][2], l[kTiles][2] = {};
+  // ---- the warps that compute
+  // Tokens (of the warp's 16): token_of(g) and 8 further at S^T's rows,
+  // token_of(2 j), token_of(2 j + 1) and 8 further at O^T's columns.  Eight rows
+  // further on is a fixed distance: the swizzle repeats.
+  const int row0 = token_of(g), column[2] = {token_of(2 * j), token_of(2 * j + 1)};
+  const uint32_t ring0 = smem_u32(ring);
+  constexpr uint32_t kEight = 8 * L::kBoxRow;
+  uint32_t key_at[2], value_at[2];  // in a stage: steps 0 and 1 (2 and 3: a box column on)
 #pragma unroll
-  for (int n = 0; n < kTiles; ++n) m[n][0] = m[n][1] = -INFINITY;
-  uint32_t v_exp = 1;  // exponent of the power of two the value scales are taken by
-  const int row0 = token_of(g);        // and row0 + 8: the tokens of S^T's rows
-  const int column0 = token_of(2 * j), column1 = token_of(2 * j + 1);  // of O^T, and + 8
-
+  for (int x = 0; x < 2; ++x) {
+    key_at[x] = ring0 + L::at(16 * warp + row0, L::key_byte(L::kSteps > 1 ? x : 0, j));
+    // past the row (64-channel rows have 4 lanes' pieces): any, not stored
+    const uint32_t byte = (kQuarters == 1 ? g & 3 : g) * 2 * BITS;
+    value_at[x] = ring0 + L::kCodes + L::at(16 * warp + column[x], byte);
+  }
+  const uint32_t groups = c.dim / kGroup4;
+  const uint32_t key_scale = ring0 + 2 * L::kCodes + (16 * warp + row0) * token_scales;
+  const uint32_t value_scale = ring0 + 2 * L::kCodes + L::kScales + 16 * warp * token_scales;
+  uint32_t stage_at = 0;  // bytes
   int stage = 0;
   uint32_t phase = 0;
-#pragma unroll 1
-  while (seen[0] > 0) {
-    if (!mbar_wait(&bar[stage], phase)) {  // ran out: NaN, once the other copies are in
-#pragma unroll
-      for (int x = 1; x < kStages; ++x)
-        if (seen[x] > 0)
-          mbar_wait(&bar[(stage + x) % kStages], phase ^ (stage + x >= kStages ? 1u : 0u));
-#pragma unroll
-      for (int n = 0; n < kTiles; ++n) l[n][0] = l[n][1] = __uint_as_float(0x7FC00000u);
-      break;
-    }
-    const uint8_t* keys = codes + stage * 2 * L::kCodes;
-    const uint8_t* values = keys + L::kCodes;
-    const uint32_t* ksc = reinterpret_cast<const uint32_t*>(scales + stage * 2 * L::kScales);
-    const uint32_t* vsc = ksc + L::kScales / 4;
-    const bool whole = seen[0] == kBlock;
+  bool ok = true;
+  for (uint32_t place = 0; run.more(); run.next(), place = 1) {
+    const Segment& seg = run.s;
+    const uint32_t kvh = seg.row / heads.blocks, h0 = (seg.row - kvh * heads.blocks) * kHeads;
 
-    // ---- S^T = K Q^T
-    float s[kTiles][4] = {};
-#pragma unroll
-    for (int st = 0; st < L::kSteps; ++st) {
-      uint32_t w[2][4];
-      __half2 gs[2], gm[2];
-#pragma unroll
-      for (int r = 0; r < 2; ++r) {
-        const uint32_t byte = L::key_byte(st, j);
-        const uint8_t* p = keys + L::at(row0 + 8 * r, byte);
-        if constexpr (L::kKeyWords == 4) {
-          const uint4 u = *reinterpret_cast<const uint4*>(p);
-          w[r][0] = u.x; w[r][1] = u.y; w[r][2] = u.z; w[r][3] = u.w;
-        } else {
-          const uint2 u = *reinterpret_cast<const uint2*>(p);
-          w[r][0] = u.x; w[r][1] = u.y;
-        }
-        if constexpr (BITS == 4) {
-          const uint32_t of = byte / 16;  // the group; past head_dim the codes are 0
-          const __half2 sm2 =
-              bits_h2(of * kGroup4 < c.dim ? ksc[(row0 + 8 * r) * (c.dim / kGroup4) + of] : 0u);
-          gs[r] = __low2half2(sm2);
-          gm[r] = __high2half2(sm2);
-        }
-      }
-#pragma unroll
-      for (int i = 0; i < L::kProducts / L::kSteps; ++i) {
-        uint32_t a[2][2];
-#pragma unroll
-        for (int r = 0; r < 2; ++r) {
-          if constexpr (BITS == 8) {
-            const uint32_t x = w[r][i] ^ 0x80808080u;
-            a[r][0] = code8_pair(x, 0x4140);
-            a[r][1] = code8_pair(x, 0x4342);
-          } else {
-            const uint32_t x = w[r][i / 2] >> (8 * (i & 1));
-            a[r][0] = code4_pair<false>(x, gs[r], gm[r]);
-            a[r][1] = code4_pair<true>(x, gs[r], gm[r]);
-          }
-        }
-        const int at = st * (L::kProducts / L::kSteps) + i;
-#pragma unroll
-        for (int n = 0; n < kTiles; ++n)
-          mma_f16(s[n], a[0][0], a[1][0], a[0][1], a[1][1], qf[n][at][0], qf[n][at][1]);
-      }
-    }
-
-    // ---- scores in powers of two; the maximum in use
-    if constexpr (BITS == 8) {
-      const float ks[2] = {__uint_as_float(ksc[row0]), __uint_as_float(ksc[row0 + 8])};
-#pragma unroll
-      for (int n = 0; n < kTiles; ++n)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) s[n][e] *= ks[e >> 1];
-    }
-    bool raise = false;
-#pragma unroll
-    for (int n = 0; n < kTiles; ++n)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        s[n][e] *= factor[n][e & 1];
-        if (!whole && row0 + 8 * (e >> 1) >= seen[0]) s[n][e] = -INFINITY;
-        raise |= s[n][e] > m[n][e & 1] + kRaise;
-      }
-    if (__any_sync(0xffffffffu, raise)) {
-#pragma unroll
-      for (int n = 0; n < kTiles; ++n)
-#pragma unroll
-        for (int r = 0; r < 2; ++r) {
-          float top = fmaxf(s[n][r], s[n][r + 2]);
-#pragma unroll
-          for (int d = 4; d < 32; d <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
-          top = fmaxf(top, m[n][r]);
-          const float keep = top == m[n][r] ? 1.0f : exp2f(m[n][r] - top);
-          m[n][r] = top;
-          l[n][r] *= keep;
-#pragma unroll
-          for (int p = 0; p < L::kPasses; ++p)
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-              o[n][p][i][r] *= keep;
-              o[n][p][i][r + 2] *= keep;
-            }
-        }
-    }
-    float vs[2] = {1.0f, 1.0f};
-    if constexpr (BITS == 8) {
-      // scales relative to 2^(v_exp - 127), above every scale so far
-      uint32_t e0 = vsc[row0], e1 = vsc[row0 + 8];
-      if (!whole) {  // what lies behind the sequence's end is not used
-        if (row0 >= seen[0]) e0 = 0u;
-        if (row0 + 8 >= seen[0]) e1 = 0u;
-      }
-      const uint32_t e = max(e0, e1);
-      if (__any_sync(0xffffffffu, e < 0x7F800000u && (e >> 23) >= v_exp)) {
-        const uint32_t now =
-            max(v_exp, 1u + __reduce_max_sync(0xffffffffu, e < 0x7F800000u ? e >> 23 : 0u));
-        const uint32_t drop = now - v_exp;  // by 2^-drop
-        const float down = drop < 127u ? __uint_as_float((127u - drop) << 23) : 0.0f;
-        v_exp = now;
-#pragma unroll
-        for (int n = 0; n < kTiles; ++n)
-#pragma unroll
-          for (int p = 0; p < L::kPasses; ++p)
-#pragma unroll
-            for (int i = 0; i < 8; ++i)
-#pragma unroll
-              for (int r = 0; r < 4; ++r) o[n][p][i][r] *= down;
-      }
-      const float by = __uint_as_float((254u - v_exp) << 23);
-      vs[0] = __uint_as_float(e0) * by;
-      vs[1] = __uint_as_float(e1) * by;
-    }
-    uint32_t pt[kTiles][2];
+    // Q in the order of the keys' registers, below 1 by a power of two a head
+    uint32_t qf[kTiles][L::kProducts][2];  // 8 bits: a pair of products, the upper and lower part
+    float factor[kTiles][2];  // of heads 2 j, 2 j + 1: scale log2(e) and that power
 #pragma unroll
     for (int n = 0; n < kTiles; ++n) {
-      float p[4];
+      const uint32_t h = h0 + 8 * n + g;
+      const bool live = h < heads.group;
+      const int64_t at = (int64_t)seg.b * q.batch_stride +
+                         (int64_t)(kvh * heads.group + (live ? h : 0)) * q.head_stride;
+      constexpr int kPer = L::kKeyWords * 32 / BITS;  // channels of a lane in a step
+      float x[L::kSteps][kPer];
+      uint32_t top = 0;
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const float top = m[n][e & 1];
-        p[e] = exp2_fast(s[n][e] - (top == -INFINITY ? 0.0f : top));
-        l[n][e & 1] += p[e];
-        if constexpr (BITS == 8) p[e] *= vs[e >> 1];
+      for (int s = 0; s < L::kSteps; ++s) {
+        const uint32_t ch = L::key_byte(s, j) * 8 / BITS;
+#pragma unroll
+        for (int e = 0; e < kPer / 8; ++e) {
+          float y[8] = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
+          if (live && ch + 8 * e < c.dim) {
+            if (q.bf16)
+              load8(static_cast<const __nv_bfloat16*>(q.data) + at + ch + 8 * e, q.vec, 8, y);
+            else
+              load8(static_cast<const __half*>(q.data) + at + ch + 8 * e, q.vec, 8, y);
+          }
+          top = max(top, abs_bits_max(y));
+#pragma unroll
+          for (int i = 0; i < 8; ++i) x[s][8 * e + i] = y[i];
+        }
       }
-      pt[n][0] = transpose8x8(h2_bits(__floats2half2_rn(p[0], p[1])));
-      pt[n][1] = transpose8x8(h2_bits(__floats2half2_rn(p[2], p[3])));
-    }
-
-    // ---- O^T += V^T P^T
+      top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
+      top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
+      // 2^-p with 2^(p - 1) <= max < 2^p; 1 for zeros, NaN where the query is not finite
+      const uint32_t ex = top >> 23;
+      const bool plain = ex == 0;
+      const float down = plain ? 1.0f : __uint_as_float((253u - min(ex, 252u)) << 23);
+      float up = plain ? 1.0f : __uint_as_float((1u + min(ex, 252u)) << 23);
+      if (ex == 255) up = __uint_as_float(0x7FC00000u);
 #pragma unroll
-    for (int p = 0; p < L::kPasses; ++p) {
-      // past the row (64-channel rows have 4 lanes' pieces): any, not stored
-      const uint32_t byte = ((kQuarters == 1 ? g & 3 : g) + 8 * p) * 2 * BITS;
-      constexpr int kWords = BITS / 2;
-      uint32_t w[4][kWords];
-      uint32_t gr[4];
-#pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        const int t = (r & 1 ? column1 : column0) + 8 * (r >> 1);
-        const uint8_t* at = values + L::at(t, byte);
+      for (int s = 0; s < L::kSteps; ++s) {
         if constexpr (BITS == 8) {
-          const uint4 u = *reinterpret_cast<const uint4*>(at);
-          w[r][0] = u.x; w[r][1] = u.y; w[r][2] = u.z; w[r][3] = u.w;
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            // q 2^14 = 256 upper + lower, both signed bytes
+            uint32_t hi = 0, lo = 0;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const int v = __float2int_rn(x[s][4 * i + e] * down * 16384.0f);
+              const int u = (v + 128) >> 8;
+              hi |= (uint32_t)(u & 0xFF) << (8 * e);
+              lo |= (uint32_t)((v - 256 * u) & 0xFF) << (8 * e);
+            }
+            qf[n][4 * s + i / 2 * 2][i & 1] = hi;
+            qf[n][4 * s + i / 2 * 2 + 1][i & 1] = lo;
+          }
         } else {
-          const uint2 u = *reinterpret_cast<const uint2*>(at);
-          w[r][0] = u.x; w[r][1] = u.y;
-          const uint32_t of = byte / 16;
-          gr[r] = of * kGroup4 < c.dim ? vsc[t * (c.dim / kGroup4) + of] : 0u;
-          if (!whole && t >= seen[0]) gr[r] = 0u;
-        }
-      }
-      if constexpr (BITS == 8) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const uint32_t w0 = w[0][i] ^ 0x80808080u, w1 = w[1][i] ^ 0x80808080u;
-          const uint32_t w2 = w[2][i] ^ 0x80808080u, w3 = w[3][i] ^ 0x80808080u;
-#pragma unroll
-          for (int h = 0; h < 2; ++h) {  // channels 4 i + 2 h, + 1
-            const uint32_t x = __byte_perm(w0, w1, h ? 0x7362 : 0x5140);
-            const uint32_t y = __byte_perm(w2, w3, h ? 0x7362 : 0x5140);
-            const uint32_t a0 = code8_pair(x, 0x4140), a1 = code8_pair(x, 0x4342);
-            const uint32_t a2 = code8_pair(y, 0x4140), a3 = code8_pair(y, 0x4342);
-#pragma unroll
-            for (int n = 0; n < kTiles; ++n)
-              mma_f16(o[n][p][2 * i + h], a0, a1, a2, a3, pt[n][0], pt[n][1]);
+          for (int i = 0; i < 2 * L::kKeyWords; ++i) {
+            const int c0 = 8 * (i / 2) + 2 * (i & 1);  // code4_pair's channels
+            uint32_t(&f)[2] = qf[n][s * 2 * L::kKeyWords + i];
+            f[0] = h2_bits(__floats2half2_rn(x[s][c0] * down, x[s][c0 + 4] * down));
+            f[1] = h2_bits(__floats2half2_rn(x[s][c0 + 1] * down, x[s][c0 + 5] * down));
           }
         }
-      } else {
-        const __half2 s01 = bits_h2(__byte_perm(gr[0], gr[1], 0x5410));
-        const __half2 m01 = bits_h2(__byte_perm(gr[0], gr[1], 0x7632));
-        const __half2 s23 = bits_h2(__byte_perm(gr[2], gr[3], 0x5410));
-        const __half2 m23 = bits_h2(__byte_perm(gr[2], gr[3], 0x7632));
+      }
 #pragma unroll
-        for (int i = 0; i < 2; ++i)
+      for (int r = 0; r < 2; ++r)
+        factor[n][r] = __shfl_sync(0xffffffffu, up, 4 * (2 * j + r)) * (scale * kLog2e) *
+                       (BITS == 8 ? 0x1p-14f : 1.0f);
+    }
+
+    // o[n][p][i]: channels 16 (g + 8 p) + 2 i, + 1 of heads 2 j, 2 j + 1
+    float o[kTiles][L::kPasses][8][4] = {};
+    float m[kTiles][2], l[kTiles][2] = {};
 #pragma unroll
-          for (int h = 0; h < 4; ++h) {  // channels 8 i + 2 h, + 1
-            const uint32_t sel = h < 2 ? 0x5410 : 0x7632;
-            const uint32_t x = __byte_perm(w[0][i], w[1][i], sel) >> (8 * (h & 1));
-            const uint32_t y = __byte_perm(w[2][i], w[3][i], sel) >> (8 * (h & 1));
-            const uint32_t a0 = code4_pair<false>(x, s01, m01), a1 = code4_pair<true>(x, s01, m01);
-            const uint32_t a2 = code4_pair<false>(y, s23, m23), a3 = code4_pair<true>(y, s23, m23);
+    for (int n = 0; n < kTiles; ++n) m[n][0] = m[n][1] = -INFINITY;
+    uint32_t v_exp = 1;  // exponent of the power of two the value scales are taken by
+
+#pragma unroll 1
+    for (uint32_t u = seg.first(); u < seg.last(); ++u) {
+      if (!ok || !mbar_wait(&full[stage], phase)) {  // ran out: NaN from here on
+        ok = false;
+        break;
+      }
+      const int seen = tokens[stage][warp];
+      const bool whole = seen == kBlock;
+
+      if (seen > 0) {
+        // ---- S^T = K Q^T
+        float s[kTiles][4] = {};
+        if constexpr (BITS == 8) {
+          int hi[kTiles][4] = {}, lo[kTiles][4] = {};
+#pragma unroll
+          for (int st = 0; st < L::kSteps; ++st) {
+            uint4 w[2];
+#pragma unroll
+            for (int r = 0; r < 2; ++r)
+              w[r] = lds128(key_at[st % 2] + stage_at + st / 2 * L::kColumn + r * kEight);
+#pragma unroll
+            for (int n = 0; n < kTiles; ++n) {
+              const uint32_t(*f)[2] = &qf[n][4 * st];
+              mma_s8(hi[n], w[0].x, w[1].x, w[0].y, w[1].y, f[0][0], f[0][1]);
+              mma_s8(lo[n], w[0].x, w[1].x, w[0].y, w[1].y, f[1][0], f[1][1]);
+              mma_s8(hi[n], w[0].z, w[1].z, w[0].w, w[1].w, f[2][0], f[2][1]);
+              mma_s8(lo[n], w[0].z, w[1].z, w[0].w, w[1].w, f[3][0], f[3][1]);
+            }
+          }
+          const float ks[2] = {__uint_as_float(lds32(key_scale + stage_at)),
+                               __uint_as_float(lds32(key_scale + stage_at + 32))};
+#pragma unroll
+          for (int n = 0; n < kTiles; ++n)
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              s[n][e] = (float)(hi[n][e] * 256 + lo[n][e]) * ks[e >> 1];
+        } else {
+#pragma unroll
+          for (int st = 0; st < L::kSteps; ++st) {
+            uint32_t w[2][4];
+            __half2 gs[2], gm[2];
+#pragma unroll
+            for (int r = 0; r < 2; ++r) {
+              // 128-channel steps of rows in one box: 16-byte chunks 2 j and 2 j + 1
+              const uint32_t at = key_at[st] + stage_at + r * kEight;
+              if constexpr (L::kKeyWords == 4) {
+                const uint4 v = lds128(at);
+                w[r][0] = v.x; w[r][1] = v.y; w[r][2] = v.z; w[r][3] = v.w;
+              } else {
+                const uint2 v = lds64(at);
+                w[r][0] = v.x; w[r][1] = v.y;
+              }
+              const uint32_t of = L::key_byte(st, j) / 16;  // past head_dim the codes are 0
+              const __half2 pair = bits_h2(
+                  of < groups ? lds32(key_scale + stage_at + (8 * r * groups + of) * 4) : 0u);
+              gs[r] = __low2half2(pair);
+              gm[r] = __high2half2(pair);
+            }
+#pragma unroll
+            for (int i = 0; i < 2 * L::kKeyWords; ++i) {
+              uint32_t a[2][2];
+#pragma unroll
+              for (int r = 0; r < 2; ++r) {
+                const uint32_t x = w[r][i / 2] >> (8 * (i & 1));
+                a[r][0] = code4_pair<false>(x, gs[r], gm[r]);
+                a[r][1] = code4_pair<true>(x, gs[r], gm[r]);
+              }
+#pragma unroll
+              for (int n = 0; n < kTiles; ++n) {
+                const uint32_t(&f)[2] = qf[n][st * 2 * L::kKeyWords + i];
+                mma_f16(s[n], a[0][0], a[1][0], a[0][1], a[1][1], f[0], f[1]);
+              }
+            }
+          }
+        }
+
+        // ---- scores in powers of two; the maximum in use
+        bool raise = false;
+#pragma unroll
+        for (int n = 0; n < kTiles; ++n)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            s[n][e] *= factor[n][e & 1];
+            if (!whole && row0 + 8 * (e >> 1) >= seen) s[n][e] = -INFINITY;
+            raise |= s[n][e] > m[n][e & 1] + kRaise;
+          }
+        if (__any_sync(0xffffffffu, raise)) {
+#pragma unroll
+          for (int n = 0; n < kTiles; ++n)
+#pragma unroll
+            for (int r = 0; r < 2; ++r) {
+              float top = fmaxf(s[n][r], s[n][r + 2]);
+#pragma unroll
+              for (int d = 4; d < 32; d <<= 1)
+                top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
+              top = fmaxf(top, m[n][r]);
+              const float keep = top == m[n][r] ? 1.0f : exp2_fast(m[n][r] - top);
+              m[n][r] = top;
+              l[n][r] *= keep;
+#pragma unroll
+              for (int p = 0; p < L::kPasses; ++p)
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                  o[n][p][i][r] *= keep;
+                  o[n][p][i][r + 2] *= keep;
+                }
+            }
+        }
+        float vs[2] = {1.0f, 1.0f};
+        if constexpr (BITS == 8) {
+          // scales relative to 2^(v_exp - 127), above every scale so far
+          uint32_t e0 = lds32(key_scale + stage_at + L::kScales);
+          uint32_t e1 = lds32(key_scale + stage_at + L::kScales + 32);
+          if (!whole) {  // what lies behind the sequence's end is not used
+            if (row0 >= seen) e0 = 0u;
+            if (row0 + 8 >= seen) e1 = 0u;
+          }
+          const uint32_t e = max(e0, e1);
+          if (__any_sync(0xffffffffu, e < 0x7F800000u && (e >> 23) >= v_exp)) {
+            const uint32_t now =
+                max(v_exp, 1u + __reduce_max_sync(0xffffffffu, e < 0x7F800000u ? e >> 23 : 0u));
+            const uint32_t drop = now - v_exp;  // by 2^-drop
+            const float down = drop < 127u ? __uint_as_float((127u - drop) << 23) : 0.0f;
+            v_exp = now;
 #pragma unroll
             for (int n = 0; n < kTiles; ++n)
-              mma_f16(o[n][p][4 * i + h], a0, a1, a2, a3, pt[n][0], pt[n][1]);
+#pragma unroll
+              for (int p = 0; p < L::kPasses; ++p)
+#pragma unroll
+                for (int i = 0; i < 8; ++i)
+#pragma unroll
+                  for (int r = 0; r < 4; ++r) o[n][p][i][r] *= down;
           }
+          const float by = __uint_as_float((254u - v_exp) << 23);
+          vs[0] = __uint_as_float(e0) * by;
+          vs[1] = __uint_as_float(e1) * by;
+        }
+        uint32_t pt[kTiles][2];
+#pragma unroll
+        for (int n = 0; n < kTiles; ++n) {
+          float p[4];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            // no maximum yet (every score -infinity): 0 stands in, p = 0
+            const float top = m[n][e & 1] == -INFINITY ? 0.0f : m[n][e & 1];
+            p[e] = exp2_fast(s[n][e] - top);
+            l[n][e & 1] += p[e];
+            if constexpr (BITS == 8) p[e] *= vs[e >> 1];
+          }
+          pt[n][0] = transpose8x8(h2_bits(__floats2half2_rn(p[0], p[1])));
+          pt[n][1] = transpose8x8(h2_bits(__floats2half2_rn(p[2], p[3])));
+        }
+
+        // ---- O^T += V^T P^T
+#pragma unroll
+        for (int p = 0; p < L::kPasses; ++p) {
+          constexpr int kWords = BITS / 2;
+          uint32_t w[4][kWords];
+          uint32_t gr[4];
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            if constexpr (BITS == 8) {
+              const uint4 v =
+                  lds128(value_at[r & 1] + stage_at + p * L::kColumn + (r >> 1) * kEight);
+              w[r][0] = v.x; w[r][1] = v.y; w[r][2] = v.z; w[r][3] = v.w;
+            } else {
+              // the second pass is the row's other half: chunks 4 .. 7
+              const uint2 v = lds64((value_at[r & 1] ^ (p * 64)) + stage_at + (r >> 1) * kEight);
+              w[r][0] = v.x; w[r][1] = v.y;
+              const uint32_t of = (g + 8 * p) / 2;
+              const int t = column[r & 1] + 8 * (r >> 1);
+              gr[r] = of < groups ? lds32(value_scale + stage_at + (t * groups + of) * 4) : 0u;
+              if (!whole && t >= seen) gr[r] = 0u;
+            }
+          }
+          if constexpr (BITS == 8) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              const uint32_t w0 = w[0][i] ^ 0x80808080u, w1 = w[1][i] ^ 0x80808080u;
+              const uint32_t w2 = w[2][i] ^ 0x80808080u, w3 = w[3][i] ^ 0x80808080u;
+#pragma unroll
+              for (int h = 0; h < 2; ++h) {  // channels 4 i + 2 h, + 1
+                const uint32_t x = __byte_perm(w0, w1, h ? 0x7362 : 0x5140);
+                const uint32_t y = __byte_perm(w2, w3, h ? 0x7362 : 0x5140);
+                const uint32_t a0 = code8_pair(x, 0x4140), a1 = code8_pair(x, 0x4342);
+                const uint32_t a2 = code8_pair(y, 0x4140), a3 = code8_pair(y, 0x4342);
+#pragma unroll
+                for (int n = 0; n < kTiles; ++n)
+                  mma_f16(o[n][p][2 * i + h], a0, a1, a2, a3, pt[n][0], pt[n][1]);
+              }
+            }
+          } else {
+            const __half2 s01 = bits_h2(__byte_perm(gr[0], gr[1], 0x5410));
+            const __half2 m01 = bits_h2(__byte_perm(gr[0], gr[1], 0x7632));
+            const __half2 s23 = bits_h2(__byte_perm(gr[2], gr[3], 0x5410));
+            const __half2 m23 = bits_h2(__byte_perm(gr[2], gr[3], 0x7632));
+#pragma unroll
+            for (int i = 0; i < 2; ++i)
+#pragma unroll
+              for (int h = 0; h < 4; ++h) {  // channels 8 i + 2 h, + 1
+                const uint32_t sel = h < 2 ? 0x5410 : 0x7632;
+                const uint32_t x = __byte_perm(w[0][i], w[1][i], sel) >> (8 * (h & 1));
+                const uint32_t y = __byte_perm(w[2][i], w[3][i], sel) >> (8 * (h & 1));
+                const uint32_t a0 = code4_pair<false>(x, s01, m01);
+                const uint32_t a1 = code4_pair<true>(x, s01, m01);
+                const uint32_t a2 = code4_pair<false>(y, s23, m23);
+                const uint32_t a3 = code4_pair<true>(y, s23, m23);
+#pragma unroll
+                for (int n = 0; n < kTiles; ++n)
+                  mma_f16(o[n][p][4 * i + h], a0, a1, a2, a3, pt[n][0], pt[n][1]);
+              }
+          }
+        }
       }
+
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&empty[stage]);
+      stage_at += L::kStage;
+      if (++stage == L::kStages) stage = 0, stage_at = 0, phase ^= 1u;
     }
 
-    // ---- the stage is read: the next block into it
-    __syncwarp();
-    const int more = fetch_into(stage);
+    // ---- the warps' parts joined, 8 heads at a time
+    const float up = BITS == 8 ? __uint_as_float(v_exp << 23) : 1.0f;
+    const bool part = seg.c1 - seg.c0 != seg.n;
+    const uint32_t slot = 2 * blockIdx.x + place;
 #pragma unroll
-    for (int x = 0; x + 1 < kStages; ++x) seen[x] = seen[x + 1];
-    seen[kStages - 1] = more;
-    if (++stage == kStages) stage = 0, phase ^= 1u;
-  }
-
-  // the warps' parts, in the rings' memory
-  __syncthreads();
-  float* so = reinterpret_cast<float*>(shared);  // [kWarps][kHeads][dim]
-  const float up = BITS == 8 ? __uint_as_float(v_exp << 23) : 1.0f;
+    for (int n = 0; n < kTiles; ++n) {
+      const uint32_t first = h0 + 8 * n;
+      const uint32_t here = first < heads.group ? min(8u, heads.group - first) : 0u;
+      if (here == 0) break;
 #pragma unroll
-  for (int n = 0; n < kTiles; ++n) {
+      for (int r = 0; r < 2; ++r) {
+        float sum = ok ? l[n][r] : __uint_as_float(0x7FC00000u);
 #pragma unroll
-    for (int r = 0; r < 2; ++r) {
+        for (int d = 4; d < 32; d <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
+        const uint32_t h = 2 * j + r;
+        if (g == 0) sm[warp][h] = m[n][r], sl[warp][h] = sum;
+        if (h < here) {
+          float* to = join + (warp * 8 + j + 4 * r) * L::kJoinRow;
 #pragma unroll
-      for (int d = 4; d < 32; d <<= 1) l[n][r] += __shfl_xor_sync(0xffffffffu, l[n][r], d);
-      const int h = 8 * n + 2 * j + r;
-      if (g == 0) sm[warp][h] = m[n][r], sl[warp][h] = l[n][r];
+          for (int p = 0; p < L::kPasses; ++p) {
+            const uint32_t ch = 16 * (g + 8 * p);
+            if (ch < 64 * kQuarters)
 #pragma unroll
-      for (int p = 0; p < L::kPasses; ++p) {
-        const uint32_t ch = 16 * (g + 8 * p);
-        if (ch < c.dim)
-#pragma unroll
-          for (int i = 0; i < 8; ++i)
-            *reinterpret_cast<float2*>(&so[(warp * kHeads + h) * c.dim + ch + 2 * i]) =
-                make_float2(o[n][p][i][r] * up, o[n][p][i][r + 2] * up);
+              for (int i = 0; i < 8; ++i) {
+                to[ch + ch / 32 * 4 + 2 * i] = o[n][p][i][r] * up;
+                to[ch + ch / 32 * 4 + 2 * i + 1] = o[n][p][i][r + 2] * up;
+              }
+          }
+        }
       }
-    }
-  }
-  __syncthreads();
-  const int64_t rows = (int64_t)gridDim.z * heads * gridDim.x;  // parts
-  for (uint32_t i = threadIdx.x; i < kHeads * c.dim; i += 32 * kWarps) {
-    const uint32_t h = i / c.dim, ch = i - h * c.dim;
-    if (h0 + h >= group) break;
-    float top = -INFINITY, sum = 0.0f, y = 0.0f;
+      asm volatile("bar.sync 1, %0;" ::"n"(32 * L::kWarps) : "memory");
+      for (uint32_t i = threadIdx.x; i < here * c.dim; i += 32 * L::kWarps) {
+        const uint32_t h = i / c.dim, ch = i - h * c.dim;
+        const float* from = join + ((h >> 1) + 4 * (h & 1)) * L::kJoinRow + ch + ch / 32 * 4;
+        float top = -INFINITY, sum = 0.0f, y = 0.0f;
 #pragma unroll
-    for (int w = 0; w < kWarps; ++w) top = fmaxf(top, sm[w][h]);
+        for (int w = 0; w < L::kWarps; ++w) top = fmaxf(top, sm[w][h]);
 #pragma unroll
-    for (int w = 0; w < kWarps; ++w) {
-      const float f = sm[w][h] == -INFINITY ? 0.0f : exp2f(sm[w][h] - top);
-      sum = fmaf(sl[w][h], f, sum);
-      y = fmaf(so[(w * kHeads + h) * c.dim + ch], f, y);
-    }
-    const int64_t head = b * heads + kvh * group + h0 + h;
-    if (parts == nullptr) {
-      store_out(out, q.bf16, head * c.dim + ch, sum == 0.0f ? 0.0f : y / sum);
-    } else {
-      const int64_t part = head * gridDim.x + blockIdx.x;
-      parts[part * c.dim + ch] = y;
-      if (ch == 0)
-        reinterpret_cast<float2*>(parts + rows * c.dim)[part] = make_float2(top, sum);
+        for (int w = 0; w < L::kWarps; ++w) {
+          const float f = sm[w][h] == -INFINITY ? 0.0f : exp2_fast(sm[w][h] - top);
+          sum = fmaf(sl[w][h], f, sum);
+          y = fmaf(from[w * 8 * L::kJoinRow], f, y);
+        }
+        if (part) {
+          const uint32_t at = slot * kHeads + 8 * n + h;
+          parts[(uint64_t)at * c.dim + ch] = y;
+          if (ch == 0)
+            reinterpret_cast<float2*>(parts + (uint64_t)2 * shares * kHeads * c.dim)[at] =
+                make_float2(top, sum);
+        } else {
+          const uint64_t head = (uint64_t)seg.b * heads.all + kvh * heads.group + first + h;
+          store_out(out, q.bf16, head * c.dim + ch, sum == 0.0f ? 0.0f : y / sum);
+        }
+      }
+      asm volatile("bar.sync 1, %0;" ::"n"(32 * L::kWarps) : "memory");
     }
   }
 }
 
-// A CTA a (sequence, head): the chunks' parts in order.
-__global__ void __launch_bounds__(256)
-    cache_attention_join_kernel(const float* __restrict__ parts, uint32_t chunks, uint32_t chunk,
-                                uint32_t heads, uint32_t dim, Lengths lengths, bool bf16,
+// A CTA a row of a sequence: where its units went to several CTAs, their parts
+// in the order of the tokens.
+constexpr int kJoinThreads = 256;
+__global__ void __launch_bounds__(kJoinThreads)
+    cache_attention_join_kernel(const float* __restrict__ parts, uint32_t shares, uint32_t unit,
+                                uint32_t part_heads, uint32_t kv_heads, Heads heads, uint32_t dim,
+                                const __grid_constant__ Lengths lengths, bool bf16,
                                 void* __restrict__ out) {
-  const int64_t head = (int64_t)blockIdx.y * heads + blockIdx.x;
-  const int64_t len = lengths.of(blockIdx.y);
-  const int n = max((int)((len + chunk - 1) / chunk), 1);
-  const float2* ml = reinterpret_cast<const float2*>(
-                         parts + (int64_t)gridDim.y * heads * chunks * dim) + head * chunks;
-  const float* o = parts + head * chunks * dim;
-  float top = -INFINITY;
-  for (int i = 0; i < n; ++i) top = fmaxf(top, ml[i].x);
-  for (uint32_t ch = threadIdx.x; ch < dim; ch += 256) {
-    float sum = 0.0f, y = 0.0f;
-    for (int i = 0; i < n; ++i) {
-      const float2 a = ml[i];
-      const float f = a.x == -INFINITY ? 0.0f : exp2f(a.x - top);
+  const uint32_t rows = kv_heads * heads.blocks;
+  const uint32_t b = blockIdx.x / rows, row = blockIdx.x - b * rows;
+  const uint32_t n = units_of(lengths.of(b), unit);
+  // units of a row before this sequence, and of all
+  unsigned long long before = 0, total = 0;
+  __shared__ unsigned long long sums[2][kJoinThreads / 32];
+  extern __shared__ float weight[];  // [part][head], then a sum a head
+  for (uint32_t i = threadIdx.x; i < lengths.batch; i += kJoinThreads) {
+    const uint32_t x = units_of(lengths.of(i), unit);
+    total += x;
+    if (i < b) before += x;
+  }
+#pragma unroll
+  for (int d = 16; d > 0; d >>= 1) {
+    before += __shfl_xor_sync(0xffffffffu, before, d);
+    total += __shfl_xor_sync(0xffffffffu, total, d);
+  }
+  const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if (lane == 0) sums[0][warp] = before, sums[1][warp] = total;
+  __syncthreads();
+  before = total = 0;
+  for (int w = 0; w < kJoinThreads / 32; ++w) before += sums[0][w], total += sums[1][w];
+  const unsigned long long units = total * rows, used = shares_used(units, shares);
+  const unsigned long long s0 = before * rows + (unsigned long long)row * n, s1 = s0 + n - 1;
+  // the CTAs that hold the first and the last unit
+  const uint32_t i0 = (uint32_t)(((s0 + 1) * used - 1) / units);
+  const uint32_t i1 = (uint32_t)(((s1 + 1) * used - 1) / units);
+  if (i0 == i1) return;  // one CTA took the row and wrote its output
+  const uint32_t kvh = row / heads.blocks, h0 = (row - kvh * heads.blocks) * part_heads;
+  const uint32_t here = min(part_heads, heads.group - h0), many = i1 - i0 + 1;
+  // a CTA's first part, or its second where it begins before this row
+  const uint32_t second = share_begin(i0, units, used) < s0 ? 1u : 0u;
+  const auto slot = [&](uint32_t i) { return (2 * (i0 + i) + (i == 0 ? second : 0u)) * part_heads; };
+  grid_dependency_wait();
+  const float2* ml =
+      reinterpret_cast<const float2*>(parts + (uint64_t)2 * shares * part_heads * dim);
+  for (uint32_t h = warp; h < here; h += kJoinThreads / 32) {
+    float top = -INFINITY, sum = 0.0f;
+    for (uint32_t i = lane; i < many; i += 32) top = fmaxf(top, ml[slot(i) + h].x);
+    top = warp_max(top);
+    for (uint32_t i = lane; i < many; i += 32) {
+      const float2 a = ml[slot(i) + h];
+      const float f = a.x == -INFINITY ? 0.0f : exp2_fast(a.x - top);
+      weight[i * part_heads + h] = f;
       sum = fmaf(a.y, f, sum);
-      y = fmaf(o[(int64_t)i * dim + ch], f, y);
     }
-    store_out(out, bf16, head * dim + ch, sum == 0.0f ? 0.0f : y / sum);
+#pragma unroll
+    for (int d = 16; d > 0; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
+    if (lane == 0) weight[many * part_heads + h] = sum;
+  }
+  __syncthreads();
+  for (uint32_t x = threadIdx.x; x < here * dim / 4; x += kJoinThreads) {
+    const uint32_t h = 4 * x / dim, ch = 4 * x - h * dim;
+    float4 y = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll 4
+    for (uint32_t i = 0; i < many; ++i) {
+      const float4 v =
+          *reinterpret_cast<const float4*>(parts + (uint64_t)(slot(i) + h) * dim + ch);
+      const float f = weight[i * part_heads + h];
+      y.x = fmaf(v.x, f, y.x);
+      y.y = fmaf(v.y, f, y.y);
+      y.z = fmaf(v.z, f, y.z);
+      y.w = fmaf(v.w, f, y.w);
+    }
+    const float sum = weight[many * part_heads + h];
+    const uint64_t at = ((uint64_t)b * heads.all + kvh * heads.group + h0 + h) * dim + ch;
+    store_out(out, bf16, at, sum == 0.0f ? 0.0f : y.x / sum);
+    store_out(out, bf16, at + 1, sum == 0.0f ? 0.0f : y.y / sum);
+    store_out(out, bf16, at + 2, sum == 0.0f ? 0.0f : y.z / sum);
+    store_out(out, bf16, at + 3, sum == 0.0f ? 0.0f : y.w / sum);
   }
 }
 
@@ -612,33 +923,23 @@ __global__ void __launch_bounds__(256)
 // else head blocks of 8 that read the codes again.
 inline uint32_t head_tiles(uint32_t group, uint32_t dim) { return group > 8 && dim <= 128 ? 2 : 1; }
 
-struct Split {
-  uint32_t head_blocks, chunk, chunks;
-};
+// Sequences of tables this narrow are taken whole.
+constexpr int64_t kWholeTokens = 512;
+constexpr int64_t kMostCtas = 2 * 148;  // two an SM
 
-// Chunks: enough CTAs for a few rounds of the GPU's resident ones, none
-// shorter than 256 tokens.
-inline Split split_for(const CacheView& c, int64_t batch, int64_t heads, int64_t most) {
-  Split s;
-  const uint32_t group = (uint32_t)(heads / c.heads);
-  s.head_blocks = (uint32_t)ceil_div(group, 8 * head_tiles(group, c.dim));
-  const int64_t rows = batch * c.heads * s.head_blocks;
-  const int64_t want = max64(1, ceil_div(148 * 4 * 2, rows));
-  const int64_t chunk = max64(256, ceil_div(ceil_div(most, want), 64) * 64);
-  s.chunks = (uint32_t)max64(1, ceil_div(most, chunk));
-  s.chunk = (uint32_t)chunk;
-  return s;
-}
+// CTAs that share the units, 0: one a sequence and row of heads.
+inline int64_t shares_for(int64_t most) { return most <= kWholeTokens ? 0 : kMostCtas; }
 
-// Rows of codes as TMA reads them: [all rows, bytes], boxes of 16 rows.
-bool rows_map(CUtensorMap* map, const void* codes, const CacheView& c, int bits, uint32_t box_row) {
+// Rows of codes as TMA reads them: [all rows, bytes].
+bool rows_map(CUtensorMap* map, const void* codes, const CacheView& c, int bits, uint32_t box_row,
+              uint32_t box_rows) {
   auto enc = tensor_map_encoder();
   if (enc == nullptr) return false;
   std::memset(map, 0, sizeof(*map));
   const cuuint64_t bytes = (cuuint64_t)c.dim * bits / 8;
   const cuuint64_t dims[2] = {bytes, (cuuint64_t)(c.pages * c.heads * c.page_size)};
   const cuuint64_t strides[1] = {bytes};
-  const cuuint32_t box[2] = {box_row, (cuuint32_t)kBlock};
+  const cuuint32_t box[2] = {box_row, box_rows};
   const cuuint32_t ones[2] = {1, 1};
   const CUtensorMapSwizzle swizzle = box_row == 128  ? CU_TENSOR_MAP_SWIZZLE_128B
                                      : box_row == 64 ? CU_TENSOR_MAP_SWIZZLE_64B
@@ -651,13 +952,12 @@ bool rows_map(CUtensorMap* map, const void* codes, const CacheView& c, int bits,
 struct Call {
   CacheView c;
   Query q;
-  uint32_t heads;
-  Split split;
-  dim3 grid;
+  Heads heads;
   const int32_t* table;
   int64_t table_stride;
   Lengths lengths;
   float scale;
+  uint32_t shares;
   float* parts;
   void* out;
   cudaStream_t stream;
@@ -666,21 +966,38 @@ struct Call {
 template <int BITS, int kQuarters, int kTiles>
 mb_status launch(const Call& a) {
   using L = Layout<BITS, kQuarters>;
-  constexpr int kStages = 3;
+  // boxes as tall as units and pages allow
+  uint32_t box_rows = L::kUnit;
+  while (a.c.page_size % box_rows != 0) box_rows /= 2;
   CUtensorMap k_map, v_map;
-  if (!rows_map(&k_map, a.c.codes[0], a.c, BITS, L::kBoxRow) ||
-      !rows_map(&v_map, a.c.codes[1], a.c, BITS, L::kBoxRow))
+  if (!rows_map(&k_map, a.c.codes[0], a.c, BITS, L::kBoxRow, box_rows) ||
+      !rows_map(&v_map, a.c.codes[1], a.c, BITS, L::kBoxRow, box_rows))
     return set_error(MB_ERR_CUDA, "cuTensorMapEncodeTiled rejected the cache");
-  const size_t ring = (size_t)kWarps * kStages * L::kStage;
-  const size_t join = (size_t)kWarps * 8 * kTiles * a.c.dim * sizeof(float);
-  const size_t smem = (ring > join ? ring : join) + 1024;
-  auto* kernel = cache_attention_kernel<BITS, kQuarters, kTiles, kStages>;
+  auto* kernel = cache_attention_kernel<BITS, kQuarters, kTiles>;
   static std::atomic<uint64_t> attr_done{0};
-  MB_CUDA_TRY(set_smem_limit_once(kernel, 160 * 1024, attr_done));
-  kernel<<<a.grid, 32 * kWarps, smem, a.stream>>>(
-      k_map, v_map, a.c, a.q, a.heads, a.split.head_blocks, a.table, a.table_stride, a.lengths,
-      a.scale, a.split.chunk, a.parts, a.out);
+  MB_CUDA_TRY(set_smem_limit_once(kernel, L::kSmem, attr_done));
+  const uint32_t rows = a.c.heads * a.heads.blocks;
+  const unsigned grid = a.shares > 0 ? a.shares : a.lengths.batch * rows;
+  kernel<<<grid, L::kThreads, L::kSmem, a.stream>>>(k_map, v_map, a.c, box_rows, a.q, a.heads,
+                                                    a.table, a.table_stride, a.lengths, a.scale,
+                                                    a.shares, a.parts, a.out);
   MB_LAUNCH_CHECK("cache_attention_kernel");
+  if (a.shares > 0) {
+    // set up while the attention runs
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(a.lengths.batch * rows);
+    cfg.blockDim = dim3(kJoinThreads);
+    cfg.dynamicSmemBytes = (a.shares + 1) * 8 * kTiles * sizeof(float);
+    cfg.stream = a.stream;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    MB_CUDA_TRY(cudaLaunchKernelEx(&cfg, cache_attention_join_kernel, (const float*)a.parts,
+                                   a.shares, (uint32_t)L::kUnit, (uint32_t)(8 * kTiles), a.c.heads,
+                                   a.heads, a.c.dim, a.lengths, a.q.bf16, a.out));
+  }
   return MB_OK;
 }
 
@@ -702,10 +1019,10 @@ extern "C" size_t mb_cache_attention_workspace_size(const mb_kv_cache* cache, in
   if (cache == nullptr || cache->kv_heads <= 0 || cache->page_size <= 0 || batch <= 0 ||
       heads < cache->kv_heads || table_width <= 0)
     return 0;
-  const CacheView c = cache_view(cache);
-  const Split s = split_for(c, batch, heads, table_width * c.page_size);
-  if (s.chunks == 1) return 0;
-  return (size_t)(batch * heads) * s.chunks * (c.dim + 2) * sizeof(float);
+  const int64_t shares = shares_for(table_width * cache->page_size);
+  const uint32_t tiles =
+      head_tiles((uint32_t)(heads / cache->kv_heads), (uint32_t)cache->head_dim);
+  return (size_t)(2 * shares * 8 * tiles) * (size_t)(cache->head_dim + 2) * sizeof(float);
 }
 
 extern "C" mb_status mb_cache_attention(const mb_kv_cache* cache, const void* q,
@@ -724,40 +1041,34 @@ extern "C" mb_status mb_cache_attention(const mb_kv_cache* cache, const void* q,
   MB_REQUIRE(heads > 0 && heads % cache->kv_heads == 0 && heads <= 65535,
              "heads must be a multiple of kv_heads up to 65535");
   MB_REQUIRE(table_width >= 0, "table_width must not be negative");
-  MB_REQUIRE(table_width <= ((int64_t(1) << 31) - 1) / cache->page_size,
+  MB_REQUIRE(table_width <= ((int64_t(1) << 31) - 1024) / cache->page_size,
              "table_width too large: positions must fit 31 bits");
   MB_REQUIRE(std::isfinite(scale), "scale must be finite");
   MB_REQUIRE(aligned(q, 2) && aligned(out, 2) && aligned(page_table, 4) && aligned(lengths, 4),
              "misaligned q, out, page_table or lengths");
-  cudaStream_t stream = reinterpret_cast<cudaStream_t>(stream_);
   const CacheView c = cache_view(cache);
-  const int64_t most = table_width * c.page_size;
-  const uint32_t group = (uint32_t)(heads / c.heads), tiles = head_tiles(group, c.dim);
-  const Split s = split_for(c, batch, heads, most);
-  const size_t need = mb_cache_attention_workspace_size(cache, batch, heads, table_width);
-  float* parts = nullptr;
-  if (need > 0) {
-    if (workspace == nullptr || workspace_bytes < need || !aligned(workspace, 8))
-      return set_error(MB_ERR_WORKSPACE,
-                       "cache_attention workspace missing, misaligned or too small");
-    parts = static_cast<float*>(workspace);
-  }
-  const Query qs{q, q_batch_stride, q_head_stride, type == MB_BF16,
-                 aligned(q, 16) && (batch == 1 || q_batch_stride % 8 == 0) &&
-                     (heads == 1 || q_head_stride % 8 == 0)};
-  const dim3 grid(s.chunks, (unsigned)(c.heads * s.head_blocks), (unsigned)batch);
-  MB_REQUIRE(grid.y <= 65535u, "too many head blocks");
   MB_REQUIRE(c.pages * c.heads * c.page_size < (int64_t(1) << 31),
              "cache too large: pages * kv_heads * page_size must fit 31 bits");
-  const Lengths all{lengths, most};
-  const Call call{c,     qs,  (uint32_t)heads, s,     grid, page_table, table_stride,
-                  all,   scale, parts,         out,   stream};
-  const mb_status st = cache->bits == 8 ? dispatch<8>(call, tiles) : dispatch<4>(call, tiles);
-  if (st != MB_OK) return st;
-  if (parts != nullptr) {
-    cache_attention_join_kernel<<<dim3((unsigned)heads, (unsigned)batch), 256, 0, stream>>>(
-        parts, s.chunks, s.chunk, (uint32_t)heads, c.dim, all, type == MB_BF16, out);
-    MB_LAUNCH_CHECK("cache_attention_join_kernel");
-  }
-  return MB_OK;
+  const int64_t most = table_width * c.page_size;
+  const uint32_t group = (uint32_t)(heads / c.heads), tiles = head_tiles(group, c.dim);
+  const Heads hs{(uint32_t)heads, group, (uint32_t)ceil_div(group, 8 * tiles)};
+  MB_REQUIRE(batch * c.heads * hs.blocks < (int64_t(1) << 31), "too many sequences and heads");
+  const size_t need = mb_cache_attention_workspace_size(cache, batch, heads, table_width);
+  if (need > 0 && (workspace == nullptr || workspace_bytes < need || !aligned(workspace, 16)))
+    return set_error(MB_ERR_WORKSPACE,
+                     "cache_attention workspace missing, misaligned or too small");
+  const Call call{c,
+                  Query{q, q_batch_stride, q_head_stride, type == MB_BF16,
+                        aligned(q, 16) && (batch == 1 || q_batch_stride % 8 == 0) &&
+                            (heads == 1 || q_head_stride % 8 == 0)},
+                  hs,
+                  page_table,
+                  table_stride,
+                  Lengths{lengths, most, (uint32_t)batch},
+                  scale,
+                  (uint32_t)shares_for(most),
+                  static_cast<float*>(workspace),
+                  out,
+                  reinterpret_cast<cudaStream_t>(stream_)};
+  return cache->bits == 8 ? dispatch<8>(call, tiles) : dispatch<4>(call, tiles);
 }

@@ -106,14 +106,15 @@ class Cache:
 
 
 def attention(q, cache, table, lengths, scale):
-    """64-bit out [batch, heads, dim] and, for an error bound, three arrays
+    """64-bit out [batch, heads, dim] and, for an error bound, four arrays
     [batch, heads, ...]: sum_t p |v| (per channel), the largest
-    sum_i |scale q_i k_i| of a token, and max |v| times the token count."""
+    sum_i |scale q_i k_i| of a token, max |v| times the token count, and the
+    largest scale max |q| sum_i |k_i| of a token."""
     q = np.asarray(q, np.float64)
     B, H, D = q.shape
     heads = cache.codes[0].shape[1]
     out, weight = np.zeros((B, H, D)), np.zeros((B, H, D))
-    reach, spread = np.zeros((B, H, 1)), np.zeros((B, H, 1))
+    reach, spread, coarse = (np.zeros((B, H, 1)) for _ in range(3))
     for b in range(B):
         for h in range(heads):
             k, v = (cache.tokens(w, table[b], int(lengths[b]), h) for w in (0, 1))
@@ -126,4 +127,5 @@ def attention(q, cache, table, lengths, scale):
                 out[b, j], weight[b, j] = p @ v, p @ np.abs(v)
                 reach[b, j] = (np.abs(k) @ np.abs(q[b, j])).max() * abs(scale)
                 spread[b, j] = np.abs(v).max() * len(k)
-    return out, weight, reach, spread
+                coarse[b, j] = np.abs(k).sum(-1).max() * np.abs(q[b, j]).max() * abs(scale)
+    return out, weight, reach, spread, coarse

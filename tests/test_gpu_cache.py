@@ -184,17 +184,21 @@ def _filled(pages, page, heads, dim, bits, dtype=torch.float16, seed=0):
 def _check_attention(got, q, cache, table, lengths, scale):
     """The kernel may round, each to fp16 at half a step (u = 2^-11): a 4-bit
     key and value as they are read, the probabilities (and with 8 bits their
-    product with the value's scale), and a query relative to its largest
-    channel; sums, maximum and exponentials are fp32.  A score s is then off by
+    product with the value's scale); sums, maximum and exponentials are fp32.
+    A query is rounded to fp16 relative to its largest channel, or with 8-bit
+    keys to 2^-14 of it.  A score s is then off by
     d <= (2 u + 2^-20) sum |scale q k| + 2^-18 (1 + |s|) (u for the key and u
     for the query; fp32 sums of at most 256 products, the exponent's scaling
-    and exp2 with it), which changes p by a factor within e^(2d); p, v and
-    p times the scale add 3 u.  Probabilities below fp16's normal numbers are
-    off by at most 2^-24 of the largest value each."""
-    want, weight, reach, spread = serving.attention(_np(q), serving.Cache(cache), table, lengths,
-                                                    scale)
+    and exp2 with it), with 8 bits also by 2^-14 scale max |q| sum |k|, which
+    changes p by a factor within e^(2d); p, v and p times the scale add 3 u.
+    Probabilities below fp16's normal numbers are off by at most 2^-24 of the
+    largest value each."""
+    want, weight, reach, spread, coarse = serving.attention(
+        _np(q), serving.Cache(cache), table, lengths, scale)
     u = 2.0 ** -11
     d = (2 * u + 2.0 ** -20) * reach + 2.0 ** -18 * (1 + reach)
+    if cache.bits == 8:
+        d = d + 2.0 ** -14 * coarse
     f = torch.finfo(got.dtype)
     work = weight * (np.exp(2 * d) * (1 + 3 * u) * (1 + 2.0 ** -16) - 1) + 2.0 ** -24 * spread
     tol = work + (f.eps / 2) * (np.abs(want) + work) + f.tiny * f.eps / 2
