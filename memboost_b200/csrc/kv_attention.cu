@@ -91,10 +91,17 @@ __device__ __forceinline__ uint32_t code8_pair(uint32_t biased, uint32_t select)
   return h2_bits(__hsub2(bits_h2(h), bits_h2(0x64806480u)));
 }
 
-// Nibbles 0 and 4 (or, `high`, 1 and 5) of w to m + s * code.
+// (x & mask) | bits in one instruction
+__device__ __forceinline__ uint32_t and_or(uint32_t x, uint32_t mask, uint32_t bits) {
+  uint32_t d;
+  asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(d) : "r"(x), "r"(mask), "r"(bits));
+  return d;
+}
+
+// Nibbles 0 and 4 (or, kHigh, 1 and 5) of w to m + s * code.
 template <bool kHigh>
 __device__ __forceinline__ uint32_t code4_pair(uint32_t w, __half2 s, __half2 m) {
-  const uint32_t h = (w & (kHigh ? 0x00F000F0u : 0x000F000Fu)) | 0x64006400u;
+  const uint32_t h = and_or(w, kHigh ? 0x00F000F0u : 0x000F000Fu, 0x64006400u);
   const __half2 c = kHigh ? __hfma2(bits_h2(h), bits_h2(0x2C002C00u), bits_h2(0xD400D400u))
                           : __hsub2(bits_h2(h), bits_h2(0x64006400u));  // (h - 1024) / 16
   return h2_bits(__hfma2(c, s, m));
@@ -165,6 +172,7 @@ struct Layout {
 __device__ __forceinline__ int token_of(int k) { return k ^ ((k >> 1) & 1); }
 
 constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kLowest = -0x1.fffffep127f;  // a maximum of nothing
 constexpr float kRaise = 8.0f;  // how far a score may exceed the maximum in use
 
 __device__ __forceinline__ float exp2_fast(float x) {
@@ -470,9 +478,12 @@ __launch_bounds__(Layout<BITS, kQuarters>::kThreads, kTiles == 1 ? 2 : 1)
     const uint32_t byte = (kQuarters == 1 ? g & 3 : g) * 2 * BITS;
     value_at[x] = ring0 + L::kCodes + L::at(16 * warp + column[x], byte);
   }
-  const uint32_t groups = c.dim / kGroup4;
+  const int last_group = (int)c.dim / kGroup4 - 1;
+  const uint32_t eight_scales = 8 * token_scales;
   const uint32_t key_scale = ring0 + 2 * L::kCodes + (16 * warp + row0) * token_scales;
-  const uint32_t value_scale = ring0 + 2 * L::kCodes + L::kScales + 16 * warp * token_scales;
+  const uint32_t value_scale[2] = {
+      ring0 + 2 * L::kCodes + L::kScales + (16 * warp + column[0]) * token_scales,
+      ring0 + 2 * L::kCodes + L::kScales + (16 * warp + column[1]) * token_scales};
   uint32_t stage_at = 0;  // bytes
   int stage = 0;
   uint32_t phase = 0;
@@ -555,7 +566,7 @@ __launch_bounds__(Layout<BITS, kQuarters>::kThreads, kTiles == 1 ? 2 : 1)
     float o[kTiles][L::kPasses][8][4] = {};
     float m[kTiles][2], l[kTiles][2] = {};
 #pragma unroll
-    for (int n = 0; n < kTiles; ++n) m[n][0] = m[n][1] = -INFINITY;
+    for (int n = 0; n < kTiles; ++n) m[n][0] = m[n][1] = kLowest;
     uint32_t v_exp = 1;  // exponent of the power of two the value scales are taken by
 
 #pragma unroll 1
@@ -610,9 +621,10 @@ __launch_bounds__(Layout<BITS, kQuarters>::kThreads, kTiles == 1 ? 2 : 1)
                 const uint2 v = lds64(at);
                 w[r][0] = v.x; w[r][1] = v.y;
               }
-              const uint32_t of = L::key_byte(st, j) / 16;  // past head_dim the codes are 0
-              const __half2 pair = bits_h2(
-                  of < groups ? lds32(key_scale + stage_at + (8 * r * groups + of) * 4) : 0u);
+              // past head_dim the query is 0 (any group's scale will do)
+              const __half2 pair =
+                  bits_h2(lds32(key_scale + stage_at + r * eight_scales +
+                                4 * min((int)L::key_byte(st, j) / 16, last_group)));
               gs[r] = __low2half2(pair);
               gm[r] = __high2half2(pair);
             }
@@ -641,9 +653,18 @@ __launch_bounds__(Layout<BITS, kQuarters>::kThreads, kTiles == 1 ? 2 : 1)
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
             s[n][e] *= factor[n][e & 1];
-            if (!whole && row0 + 8 * (e >> 1) >= seen) s[n][e] = -INFINITY;
-            raise |= s[n][e] > m[n][e & 1] + kRaise;
           }
+        if (!whole) {
+#pragma unroll
+          for (int n = 0; n < kTiles; ++n)
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              if (row0 + 8 * (e >> 1) >= seen) s[n][e] = -INFINITY;
+        }
+#pragma unroll
+        for (int n = 0; n < kTiles; ++n)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) raise |= s[n][e] > m[n][e & 1] + kRaise;
         if (__any_sync(0xffffffffu, raise)) {
 #pragma unroll
           for (int n = 0; n < kTiles; ++n)
@@ -654,7 +675,7 @@ __launch_bounds__(Layout<BITS, kQuarters>::kThreads, kTiles == 1 ? 2 : 1)
               for (int d = 4; d < 32; d <<= 1)
                 top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
               top = fmaxf(top, m[n][r]);
-              const float keep = top == m[n][r] ? 1.0f : exp2_fast(m[n][r] - top);
+              const float keep = exp2_fast(m[n][r] - top);
               m[n][r] = top;
               l[n][r] *= keep;
 #pragma unroll
@@ -701,9 +722,7 @@ __launch_bounds__(Layout<BITS, kQuarters>::kThreads, kTiles == 1 ? 2 : 1)
           float p[4];
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
-            // no maximum yet (every score -infinity): 0 stands in, p = 0
-            const float top = m[n][e & 1] == -INFINITY ? 0.0f : m[n][e & 1];
-            p[e] = exp2_fast(s[n][e] - top);
+            p[e] = exp2_fast(s[n][e] - m[n][e & 1]);
             l[n][e & 1] += p[e];
             if constexpr (BITS == 8) p[e] *= vs[e >> 1];
           }
@@ -727,10 +746,15 @@ __launch_bounds__(Layout<BITS, kQuarters>::kThreads, kTiles == 1 ? 2 : 1)
               // the second pass is the row's other half: chunks 4 .. 7
               const uint2 v = lds64((value_at[r & 1] ^ (p * 64)) + stage_at + (r >> 1) * kEight);
               w[r][0] = v.x; w[r][1] = v.y;
-              const uint32_t of = (g + 8 * p) / 2;
-              const int t = column[r & 1] + 8 * (r >> 1);
-              gr[r] = of < groups ? lds32(value_scale + stage_at + (t * groups + of) * 4) : 0u;
-              if (!whole && t >= seen) gr[r] = 0u;
+              gr[r] = lds32(value_scale[r & 1] + stage_at + 4 * min((g + 8 * p) / 2, last_group) +
+                            (r >> 1) * eight_scales);
+            }
+          }
+          if constexpr (BITS == 4) {
+            if (!whole) {
+#pragma unroll
+              for (int r = 0; r < 4; ++r)
+                if (column[r & 1] + 8 * (r >> 1) >= seen) gr[r] = 0u;
             }
           }
           if constexpr (BITS == 8) {
@@ -813,12 +837,12 @@ __launch_bounds__(Layout<BITS, kQuarters>::kThreads, kTiles == 1 ? 2 : 1)
       for (uint32_t i = threadIdx.x; i < here * c.dim; i += 32 * L::kWarps) {
         const uint32_t h = i / c.dim, ch = i - h * c.dim;
         const float* from = join + ((h >> 1) + 4 * (h & 1)) * L::kJoinRow + ch + ch / 32 * 4;
-        float top = -INFINITY, sum = 0.0f, y = 0.0f;
+        float top = kLowest, sum = 0.0f, y = 0.0f;
 #pragma unroll
         for (int w = 0; w < L::kWarps; ++w) top = fmaxf(top, sm[w][h]);
 #pragma unroll
         for (int w = 0; w < L::kWarps; ++w) {
-          const float f = sm[w][h] == -INFINITY ? 0.0f : exp2_fast(sm[w][h] - top);
+          const float f = exp2_fast(sm[w][h] - top);
           sum = fmaf(sl[w][h], f, sum);
           y = fmaf(from[w * 8 * L::kJoinRow], f, y);
         }
@@ -883,12 +907,12 @@ __global__ void __launch_bounds__(kJoinThreads)
   const float2* ml =
       reinterpret_cast<const float2*>(parts + (uint64_t)2 * shares * part_heads * dim);
   for (uint32_t h = warp; h < here; h += kJoinThreads / 32) {
-    float top = -INFINITY, sum = 0.0f;
+    float top = kLowest, sum = 0.0f;
     for (uint32_t i = lane; i < many; i += 32) top = fmaxf(top, ml[slot(i) + h].x);
     top = warp_max(top);
     for (uint32_t i = lane; i < many; i += 32) {
       const float2 a = ml[slot(i) + h];
-      const float f = a.x == -INFINITY ? 0.0f : exp2_fast(a.x - top);
+      const float f = exp2_fast(a.x - top);
       weight[i * part_heads + h] = f;
       sum = fmaf(a.y, f, sum);
     }
