@@ -37,7 +37,7 @@
 // The running maximum is raised only when a score exceeds it by 8 (in powers
 // of two): probabilities then stay below 256 and most steps rescale nothing.
 //
-// The units of all sequences and heads are dealt out evenly to two CTAs an SM,
+// The units of all sequences and heads are dealt out evenly to three CTAs an SM,
 // whatever the lengths: a CTA's share may begin and end inside a sequence.
 // Those parts (maximum, sum, unnormalised output) go to the workspace, two a
 // CTA at most, and a second kernel joins them in the order of the tokens, so
@@ -58,7 +58,7 @@ constexpr int kBlock = 16;  // tokens a warp takes at a time
 
 __device__ __forceinline__ void mma_f16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2,
                                         uint32_t a3, uint32_t b0, uint32_t b1) {
-  asm volatile(
+  asm(
       "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 "
       "{%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
       : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
@@ -67,7 +67,7 @@ __device__ __forceinline__ void mma_f16(float (&c)[4], uint32_t a0, uint32_t a1,
 
 __device__ __forceinline__ void mma_s8(int (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2,
                                        uint32_t a3, uint32_t b0, uint32_t b1) {
-  asm volatile(
+  asm(
       "mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 "
       "{%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
       : "+r"(c[0]), "+r"(c[1]), "+r"(c[2]), "+r"(c[3])
@@ -123,7 +123,7 @@ __device__ __forceinline__ void store_out(void* out, bool bf16, int64_t i, float
 // How rows of a head_dim in (64 (kQuarters - 1), 64 kQuarters] are taken.
 template <int BITS, int kQuarters>
 struct Layout {
-  static constexpr int kWarps = kQuarters <= 2 ? 8 : 4;    // that compute
+  static constexpr int kWarps = 4;                         // that compute
   static constexpr int kUnit = kWarps * kBlock;            // tokens a stage
   static constexpr int kThreads = 32 * (kWarps + 1);
   static constexpr int kRow = kQuarters >= 3 ? (BITS == 8 ? 256 : 128) : kQuarters * 8 * BITS;
@@ -139,7 +139,7 @@ struct Layout {
   static constexpr int kScales = kUnit * (BITS == 8 ? 4 : 2 * kQuarters * 4);
   // a stage: the keys' codes, the values', the keys' scales, the values'
   static constexpr int kStage = (2 * (kCodes + kScales) + 1023) / 1024 * 1024;
-  static constexpr int kStages = kStage > 24 * 1024 ? 2 : 3;
+  static constexpr int kStages = kQuarters > 2 ? 2 : BITS == 8 ? 3 : 5;
 
   // S^T: steps of 4 lanes x kKeyWords words; O^T: passes of 8 lanes x 16 channels
   static constexpr int kKeyWords = BITS == 4 && kQuarters == 1 ? 2 : 4;
@@ -221,7 +221,7 @@ struct Lengths {
 // beginning and ending a sequence's head costs.  Dealing the tokens' units
 // alone left CTAs with many short sequences behind (16 sequences of 1 .. 2048
 // tokens and 32 heads: 74 us).
-constexpr uint32_t kIdle = 1;
+constexpr uint32_t kIdle = 2;
 __device__ __forceinline__ uint32_t units_of(int len, uint32_t unit) {
   return kIdle + ((uint32_t)len + unit - 1) / unit;
 }
@@ -358,7 +358,7 @@ struct Heads {
 // (maximum, sum) pairs), or 0: CTA i takes row i % rows of sequence i / rows.
 template <int BITS, int kQuarters, int kTiles>
 __global__ void
-__launch_bounds__(Layout<BITS, kQuarters>::kThreads, kTiles == 1 ? 2 : 1)
+__launch_bounds__(Layout<BITS, kQuarters>::kThreads, kQuarters > 2 ? 2 : kTiles == 1 ? 3 : 2)
     cache_attention_kernel(const __grid_constant__ CUtensorMap k_map,
                            const __grid_constant__ CUtensorMap v_map, CacheView c,
                            uint32_t box_rows, Query q, Heads heads,
@@ -414,15 +414,26 @@ __launch_bounds__(Layout<BITS, kQuarters>::kThreads, kTiles == 1 ? 2 : 1)
     int stage = 0, issued = 0;
     uint32_t phase = 1;
     bool ok = true;
-    for (; run.more() && ok; run.next()) {
-      const Segment& s = run.s;
+    // the page of this lane's box of a unit, read a unit ahead
+    const auto page_of = [&](const Segment& s, uint32_t u) -> int32_t {
+      const uint32_t t = u * L::kUnit + mine;
+      return holds && t < (uint32_t)s.len
+                 ? table[(int64_t)s.b * table_stride + t / c.page_size]
+                 : -1;
+    };
+    int32_t next_page = run.more() && run.s.first() < run.s.last() ? page_of(run.s, run.s.first()) : -1;
+    while (run.more() && ok) {
+      const Segment s = run.s;
       const uint32_t kvh = s.row / heads.blocks;
-      const int32_t* pages = table + (int64_t)s.b * table_stride;
+      run.next();
       for (uint32_t u = s.first(); u < s.last(); ++u) {
         const uint32_t t = u * L::kUnit + mine;
-        const bool in = holds && t < (uint32_t)s.len;
         const uint32_t p = t / c.page_size;
-        const int32_t page = in ? pages[p] : -1;
+        const int32_t page = next_page;
+        if (u + 1 < s.last())
+          next_page = page_of(s, u + 1);
+        else
+          next_page = run.more() && run.s.first() < run.s.last() ? page_of(run.s, run.s.first()) : -1;
         const bool there = page >= 0 && page < c.pages;
         if (!mbar_wait(&empty[stage], phase)) {
           ok = false;
@@ -579,23 +590,45 @@ __launch_bounds__(Layout<BITS, kQuarters>::kThreads, kTiles == 1 ? 2 : 1)
       const bool whole = seen == kBlock;
 
       if (seen > 0) {
+        // the values of a pass: those of the first are on the way during S^T
+        constexpr int kWords = BITS / 2;
+        uint32_t w[4][kWords];
+        uint32_t gr[4];
+        const auto load_values = [&](int p) {
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            if constexpr (BITS == 8) {
+              const uint4 v =
+                  lds128(value_at[r & 1] + stage_at + p * L::kColumn + (r >> 1) * kEight);
+              w[r][0] = v.x; w[r][1] = v.y; w[r][2] = v.z; w[r][3] = v.w;
+            } else {
+              // the second pass is the row's other half: chunks 4 .. 7
+              const uint2 v = lds64((value_at[r & 1] ^ (p * 64)) + stage_at + (r >> 1) * kEight);
+              w[r][0] = v.x; w[r][1] = v.y;
+              gr[r] = lds32(value_scale[r & 1] + stage_at + 4 * min((g + 8 * p) / 2, last_group) +
+                            (r >> 1) * eight_scales);
+            }
+          }
+        };
+        if constexpr (BITS == 4) load_values(0);
+
         // ---- S^T = K Q^T
         float s[kTiles][4] = {};
         if constexpr (BITS == 8) {
           int hi[kTiles][4] = {}, lo[kTiles][4] = {};
 #pragma unroll
           for (int st = 0; st < L::kSteps; ++st) {
-            uint4 w[2];
+            uint4 kw[2];
 #pragma unroll
             for (int r = 0; r < 2; ++r)
-              w[r] = lds128(key_at[st % 2] + stage_at + st / 2 * L::kColumn + r * kEight);
+              kw[r] = lds128(key_at[st % 2] + stage_at + st / 2 * L::kColumn + r * kEight);
 #pragma unroll
             for (int n = 0; n < kTiles; ++n) {
               const uint32_t(*f)[2] = &qf[n][4 * st];
-              mma_s8(hi[n], w[0].x, w[1].x, w[0].y, w[1].y, f[0][0], f[0][1]);
-              mma_s8(lo[n], w[0].x, w[1].x, w[0].y, w[1].y, f[1][0], f[1][1]);
-              mma_s8(hi[n], w[0].z, w[1].z, w[0].w, w[1].w, f[2][0], f[2][1]);
-              mma_s8(lo[n], w[0].z, w[1].z, w[0].w, w[1].w, f[3][0], f[3][1]);
+              mma_s8(hi[n], kw[0].x, kw[1].x, kw[0].y, kw[1].y, f[0][0], f[0][1]);
+              mma_s8(lo[n], kw[0].x, kw[1].x, kw[0].y, kw[1].y, f[1][0], f[1][1]);
+              mma_s8(hi[n], kw[0].z, kw[1].z, kw[0].w, kw[1].w, f[2][0], f[2][1]);
+              mma_s8(lo[n], kw[0].z, kw[1].z, kw[0].w, kw[1].w, f[3][0], f[3][1]);
             }
           }
           const float ks[2] = {__uint_as_float(lds32(key_scale + stage_at)),
@@ -606,9 +639,10 @@ __launch_bounds__(Layout<BITS, kQuarters>::kThreads, kTiles == 1 ? 2 : 1)
             for (int e = 0; e < 4; ++e)
               s[n][e] = (float)(hi[n][e] * 256 + lo[n][e]) * ks[e >> 1];
         } else {
+          float s2[kTiles][4] = {};  // every other product: a shorter chain
 #pragma unroll
           for (int st = 0; st < L::kSteps; ++st) {
-            uint32_t w[2][4];
+            uint32_t kw[2][4];
             __half2 gs[2], gm[2];
 #pragma unroll
             for (int r = 0; r < 2; ++r) {
@@ -616,10 +650,10 @@ __launch_bounds__(Layout<BITS, kQuarters>::kThreads, kTiles == 1 ? 2 : 1)
               const uint32_t at = key_at[st] + stage_at + r * kEight;
               if constexpr (L::kKeyWords == 4) {
                 const uint4 v = lds128(at);
-                w[r][0] = v.x; w[r][1] = v.y; w[r][2] = v.z; w[r][3] = v.w;
+                kw[r][0] = v.x; kw[r][1] = v.y; kw[r][2] = v.z; kw[r][3] = v.w;
               } else {
                 const uint2 v = lds64(at);
-                w[r][0] = v.x; w[r][1] = v.y;
+                kw[r][0] = v.x; kw[r][1] = v.y;
               }
               // past head_dim the query is 0 (any group's scale will do)
               const __half2 pair =
@@ -633,17 +667,21 @@ __launch_bounds__(Layout<BITS, kQuarters>::kThreads, kTiles == 1 ? 2 : 1)
               uint32_t a[2][2];
 #pragma unroll
               for (int r = 0; r < 2; ++r) {
-                const uint32_t x = w[r][i / 2] >> (8 * (i & 1));
+                const uint32_t x = kw[r][i / 2] >> (8 * (i & 1));
                 a[r][0] = code4_pair<false>(x, gs[r], gm[r]);
                 a[r][1] = code4_pair<true>(x, gs[r], gm[r]);
               }
 #pragma unroll
               for (int n = 0; n < kTiles; ++n) {
                 const uint32_t(&f)[2] = qf[n][st * 2 * L::kKeyWords + i];
-                mma_f16(s[n], a[0][0], a[1][0], a[0][1], a[1][1], f[0], f[1]);
+                mma_f16(i & 1 ? s2[n] : s[n], a[0][0], a[1][0], a[0][1], a[1][1], f[0], f[1]);
               }
             }
           }
+#pragma unroll
+          for (int n = 0; n < kTiles; ++n)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) s[n][e] += s2[n][e];
         }
 
         // ---- scores in powers of two; the maximum in use
@@ -733,23 +771,7 @@ __launch_bounds__(Layout<BITS, kQuarters>::kThreads, kTiles == 1 ? 2 : 1)
         // ---- O^T += V^T P^T
 #pragma unroll
         for (int p = 0; p < L::kPasses; ++p) {
-          constexpr int kWords = BITS / 2;
-          uint32_t w[4][kWords];
-          uint32_t gr[4];
-#pragma unroll
-          for (int r = 0; r < 4; ++r) {
-            if constexpr (BITS == 8) {
-              const uint4 v =
-                  lds128(value_at[r & 1] + stage_at + p * L::kColumn + (r >> 1) * kEight);
-              w[r][0] = v.x; w[r][1] = v.y; w[r][2] = v.z; w[r][3] = v.w;
-            } else {
-              // the second pass is the row's other half: chunks 4 .. 7
-              const uint2 v = lds64((value_at[r & 1] ^ (p * 64)) + stage_at + (r >> 1) * kEight);
-              w[r][0] = v.x; w[r][1] = v.y;
-              gr[r] = lds32(value_scale[r & 1] + stage_at + 4 * min((g + 8 * p) / 2, last_group) +
-                            (r >> 1) * eight_scales);
-            }
-          }
+          if (BITS == 8 || p > 0) load_values(p);
           if constexpr (BITS == 4) {
             if (!whole) {
 #pragma unroll
@@ -812,6 +834,8 @@ __launch_bounds__(Layout<BITS, kQuarters>::kThreads, kTiles == 1 ? 2 : 1)
       const uint32_t first = h0 + 8 * n;
       const uint32_t here = first < heads.group ? min(8u, heads.group - first) : 0u;
       if (here == 0) break;
+      // the outputs joined before are read
+      asm volatile("bar.sync 1, %0;" ::"n"(32 * L::kWarps) : "memory");
 #pragma unroll
       for (int r = 0; r < 2; ++r) {
         float sum = ok ? l[n][r] : __uint_as_float(0x7FC00000u);
@@ -834,30 +858,38 @@ __launch_bounds__(Layout<BITS, kQuarters>::kThreads, kTiles == 1 ? 2 : 1)
         }
       }
       asm volatile("bar.sync 1, %0;" ::"n"(32 * L::kWarps) : "memory");
-      for (uint32_t i = threadIdx.x; i < here * c.dim; i += 32 * L::kWarps) {
-        const uint32_t h = i / c.dim, ch = i - h * c.dim;
-        const float* from = join + ((h >> 1) + 4 * (h & 1)) * L::kJoinRow + ch + ch / 32 * 4;
-        float top = kLowest, sum = 0.0f, y = 0.0f;
+      // a warp a head; with fewer heads several, taking turns at 32 channels
+      const uint32_t turns = max(1u, (uint32_t)L::kWarps / here);
+      for (uint32_t x = warp; x < here * turns; x += L::kWarps) {
+        const uint32_t h = x % here;
+        const float* from = join + ((h >> 1) + 4 * (h & 1)) * L::kJoinRow;
+        float top = kLowest, sum = 0.0f, f[L::kWarps];
 #pragma unroll
-        for (int w = 0; w < L::kWarps; ++w) top = fmaxf(top, sm[w][h]);
+        for (int w = 0; w < L::kWarps; ++w) f[w] = sm[w][h];
+#pragma unroll
+        for (int w = 0; w < L::kWarps; ++w) top = fmaxf(top, f[w]);
 #pragma unroll
         for (int w = 0; w < L::kWarps; ++w) {
-          const float f = exp2_fast(sm[w][h] - top);
-          sum = fmaf(sl[w][h], f, sum);
-          y = fmaf(from[w * 8 * L::kJoinRow], f, y);
+          f[w] = exp2_fast(f[w] - top);
+          sum = fmaf(sl[w][h], f[w], sum);
         }
-        if (part) {
-          const uint32_t at = slot * kHeads + 8 * n + h;
-          parts[(uint64_t)at * c.dim + ch] = y;
-          if (ch == 0)
-            reinterpret_cast<float2*>(parts + (uint64_t)2 * shares * kHeads * c.dim)[at] =
-                make_float2(top, sum);
-        } else {
-          const uint64_t head = (uint64_t)seg.b * heads.all + kvh * heads.group + first + h;
-          store_out(out, q.bf16, head * c.dim + ch, sum == 0.0f ? 0.0f : y / sum);
+        const uint32_t at = slot * kHeads + 8 * n + h;
+        const uint64_t head = (uint64_t)seg.b * heads.all + kvh * heads.group + first + h;
+        const float by = sum == 0.0f ? 0.0f : 1.0f / sum;
+        for (uint32_t ch = x / here * 32 + lane; ch < c.dim; ch += turns * 32) {
+          float y = 0.0f;
+#pragma unroll
+          for (int w = 0; w < L::kWarps; ++w)
+            y = fmaf(from[w * 8 * L::kJoinRow + ch + ch / 32 * 4], f[w], y);
+          if (part)
+            parts[(uint64_t)at * c.dim + ch] = y;
+          else
+            store_out(out, q.bf16, head * c.dim + ch, y * by);
         }
+        if (part && x < here && lane == 0)
+          reinterpret_cast<float2*>(parts + (uint64_t)2 * shares * kHeads * c.dim)[at] =
+              make_float2(top, sum);
       }
-      asm volatile("bar.sync 1, %0;" ::"n"(32 * L::kWarps) : "memory");
     }
   }
 }
@@ -949,7 +981,7 @@ inline uint32_t head_tiles(uint32_t group, uint32_t dim) { return group > 8 && d
 
 // Sequences of tables this narrow are taken whole.
 constexpr int64_t kWholeTokens = 512;
-constexpr int64_t kMostCtas = 2 * 148;  // two an SM
+constexpr int64_t kMostCtas = 3 * 148;
 
 // CTAs that share the units, 0: one a sequence and row of heads.
 inline int64_t shares_for(int64_t most) { return most <= kWholeTokens ? 0 : kMostCtas; }

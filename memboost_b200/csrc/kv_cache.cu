@@ -1,11 +1,12 @@
 // Keys and values quantised to 8 or 4 bits as they are written into a paged
 // cache, and read back (no counterpart in the reference).
 //
-// A row (one token's head of k or v) is taken by the 2 .. 32 lanes that hold
-// its channels, eight a lane: a 16-byte load, the maximum (8 bits: of the
-// row) or minimum and maximum (4 bits: of 32 channels, four lanes) by
-// shuffles, and one 8- or 4-byte store.  Bound by memory: 2 bytes in and 1 or
-// 0.63 out a value.
+// A CTA takes a few tokens: first the row of each in the cache (and, writing,
+// whether a later token has the same slot), then the tokens' heads.  A head's
+// row is taken by the 2 .. 32 lanes that hold its channels, eight a lane: a
+// 16-byte load, the maximum (8 bits: of the row) or minimum and maximum (4
+// bits: of 32 channels, four lanes) by shuffles, and one 8- or 4-byte store.
+// Bound by memory: 2 bytes in and 1 or 0.63 out a value.
 #include <algorithm>
 
 #include "mb_cache.cuh"
@@ -13,9 +14,13 @@
 namespace mb {
 namespace {
 
-// Up to so many tokens, a row looks through the later tokens' slots itself
-// for its own; above, a table says which token a slot belongs to.
-constexpr int64_t kScanTokens = 512;
+// Up to so many tokens, a CTA looks through the later tokens' slots itself for
+// those of its own (2048 tokens: one launch of 6 us instead of three that take
+// 18); above, where that reads too much, a table says which token a slot
+// belongs to.
+constexpr int64_t kScanTokens = 8192;
+constexpr uint32_t kThreads = 256;
+constexpr uint32_t kMostTokens = 8;  // of a CTA
 
 __host__ __device__ inline uint32_t claim_hash(uint32_t slot, uint32_t mask) {
   return (slot * 2654435761u >> 7) & mask;
@@ -30,10 +35,10 @@ inline uint32_t claim_entries(int64_t tokens) {
 // Entry: slot + 1 in the upper half, the largest token with that slot in the
 // lower.  The table has at least two entries a token, so a free one is found
 // within its length.
-__global__ void __launch_bounds__(256)
+__global__ void __launch_bounds__(kThreads)
     cache_claim_kernel(const int64_t* __restrict__ slots, uint32_t tokens, int64_t n_slots,
                        unsigned long long* __restrict__ table, uint32_t mask) {
-  const uint32_t t = blockIdx.x * 256u + threadIdx.x;
+  const uint32_t t = blockIdx.x * kThreads + threadIdx.x;
   if (t >= tokens) return;
   const int64_t slot = slots[t];
   if (slot < 0 || slot >= n_slots) return;
@@ -63,110 +68,141 @@ struct KvSource {
   bool vec[2];
 };
 
-// `width` lanes a row (a power of two, at least dim / 8).
+// How the work is cut: `tokens` a CTA; a token has 2 heads rows of `width` lanes
+// (a power of two, at least dim / 8); a CTA's lanes are dealt to gridDim.y CTAs.
+struct Cut {
+  uint32_t tokens, width, heads;
+};
+struct Place {
+  uint32_t token, which, head, lane;
+};
+__device__ __forceinline__ Place place_of(uint32_t x, const Cut& cut) {
+  Place p;
+  p.lane = x & (cut.width - 1);
+  const uint32_t row = x / cut.width;  // a power of two
+  p.token = row / (2 * cut.heads);
+  const uint32_t in = row - p.token * 2 * cut.heads;
+  p.which = in >= cut.heads;
+  p.head = in - (p.which ? cut.heads : 0u);
+  return p;
+}
+
+// First row (head 0) of a slot, -1 outside the cache.
+__device__ __forceinline__ int64_t first_row(const CacheView& c, int64_t slot) {
+  return slot >= 0 && slot < cache_slots(c) ? cache_row(c, (uint32_t)slot, 0) : -1;
+}
+
 template <typename X, int BITS>
-__global__ void __launch_bounds__(256)
+__global__ void __launch_bounds__(kThreads)
     cache_write_kernel(CacheView c, KvSource src, const int64_t* __restrict__ slots,
-                       uint32_t tokens, uint32_t width, const unsigned long long* __restrict__ table,
+                       uint32_t tokens, Cut cut, const unsigned long long* __restrict__ table,
                        uint32_t mask) {
-  const uint32_t per = 256u / width;
-  const uint32_t lane = threadIdx.x & (width - 1);
-  const uint64_t r = (uint64_t)blockIdx.x * per + threadIdx.x / width;
-  const uint32_t rows_per_token = 2 * c.heads;
-  const uint64_t t64 = r / rows_per_token;
-  const bool live = t64 < tokens;
-  const uint32_t t = live ? (uint32_t)t64 : 0u;
-  const uint32_t in = (uint32_t)(r - t64 * rows_per_token);
-  const uint32_t which = in >= c.heads, head = in - (which ? c.heads : 0u);
-  const int64_t slot = slots[t];
-  bool mine = live && slot >= 0 && slot < cache_slots(c);
-  const bool holds = lane * 8 < c.dim;
-  float v[8] = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
-  if (mine && holds)
-    load8(static_cast<const X*>(which ? src.data[1] : src.data[0]) +
-              t * (which ? src.token_stride[1] : src.token_stride[0]) +
-              head * (which ? src.head_stride[1] : src.head_stride[0]) + 8 * lane,
-          which ? src.vec[1] : src.vec[0], 8, v);
-  // the last token with this slot is the one that is kept
-  if (table != nullptr) {
-    if (mine) mine = claimed(table, mask, (uint32_t)slot, t);
-  } else {
-    bool later = false;
-    if (mine)
-      for (uint32_t o = t + 1 + lane; o < tokens; o += width) later |= slots[o] == slot;
-    for (uint32_t o = width / 2; o > 0; o >>= 1)
-      later |= __shfl_xor_sync(0xffffffffu, (int)later, o) != 0;
-    mine = mine && !later;
+  __shared__ int64_t rows[kMostTokens], mine[kMostTokens];
+  const uint32_t t0 = blockIdx.x * cut.tokens, here = min(cut.tokens, tokens - t0);
+  if (threadIdx.x < here) {
+    const int64_t slot = slots[t0 + threadIdx.x];
+    int64_t row = first_row(c, slot);
+    if (table != nullptr && row >= 0 && !claimed(table, mask, (uint32_t)slot, t0 + threadIdx.x))
+      row = -1;
+    rows[threadIdx.x] = row;
+    mine[threadIdx.x] = slot;
   }
-  const int64_t row = mine ? cache_row(c, (uint32_t)slot, head) : 0;
-  uint8_t* codes = which ? c.codes[1] : c.codes[0];
-  uint8_t* scales = which ? c.scales[1] : c.scales[0];
-  if constexpr (BITS == 8) {
-    uint32_t m = abs_bits_max(v);
-    for (uint32_t o = width / 2; o > 0; o >>= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
-    if (!mine || !holds) return;
-    const RowScale s = row_scale(m);
-    *reinterpret_cast<uint2*>(codes + row * c.dim + 8 * lane) = codes8(v, s);
-    if (lane == 0) reinterpret_cast<float*>(scales)[row] = s.scale;
-  } else {
-    // fminf and fmaxf pass over a NaN: carry it by a sum of its own
-    float lo = v[0], hi = v[0], bad = 0.0f;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      lo = fminf(lo, v[i]);
-      hi = fmaxf(hi, v[i]);
-      bad += v[i] * 0.0f;
+  __syncthreads();
+  if (table == nullptr) {  // the last token with a slot is the one that is kept
+    for (uint32_t o = t0 + 1 + threadIdx.x; o < tokens; o += kThreads) {
+      const int64_t slot = slots[o];
+      for (uint32_t k = 0; k < here; ++k)
+        if (slot == mine[k] && o > t0 + k) rows[k] = -1;
     }
+    __syncthreads();
+  }
+  const uint32_t lanes = here * 2 * cut.heads * cut.width;
+  for (uint32_t x0 = blockIdx.y * kThreads; x0 < lanes; x0 += gridDim.y * kThreads) {
+    const uint32_t x = x0 + threadIdx.x;
+    const Place p = place_of(x, cut);
+    const int64_t first = x < lanes ? rows[p.token] : -1;
+    const bool holds = first >= 0 && 8 * p.lane < c.dim;
+    float v[8] = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
+    if (holds)
+      load8(static_cast<const X*>(p.which ? src.data[1] : src.data[0]) +
+                (t0 + p.token) * (p.which ? src.token_stride[1] : src.token_stride[0]) +
+                p.head * (p.which ? src.head_stride[1] : src.head_stride[0]) + 8 * p.lane,
+            p.which ? src.vec[1] : src.vec[0], 8, v);
+    const int64_t row = first + (int64_t)p.head * c.page_size;
+    uint8_t* codes = p.which ? c.codes[1] : c.codes[0];
+    uint8_t* scales = p.which ? c.scales[1] : c.scales[0];
+    if constexpr (BITS == 8) {
+      uint32_t m = abs_bits_max(v);
+      for (uint32_t o = cut.width / 2; o > 0; o >>= 1)
+        m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
+      if (!holds) continue;
+      const RowScale s = row_scale(m);
+      *reinterpret_cast<uint2*>(codes + row * c.dim + 8 * p.lane) = codes8(v, s);
+      if (p.lane == 0) reinterpret_cast<float*>(scales)[row] = s.scale;
+    } else {
+      // fminf and fmaxf pass over a NaN: carry it by a sum of its own
+      float lo = v[0], hi = v[0], bad = 0.0f;
 #pragma unroll
-    for (int o = 1; o < 4; o <<= 1) {
-      lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, o));
-      hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, o));
-      bad += __shfl_xor_sync(0xffffffffu, bad, o);
+      for (int i = 0; i < 8; ++i) {
+        lo = fminf(lo, v[i]);
+        hi = fmaxf(hi, v[i]);
+        bad = fmaf(v[i], 0.0f, bad);
+      }
+#pragma unroll
+      for (int o = 1; o < 4; o <<= 1) {
+        lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, o));
+        hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, o));
+        bad += __shfl_xor_sync(0xffffffffu, bad, o);
+      }
+      if (!holds) continue;
+      const GroupScale g = group_scale(lo + bad, hi + bad);
+      *reinterpret_cast<uint32_t*>(codes + row * (c.dim / 2) + 4 * p.lane) = codes4(v, g);
+      if (p.lane % 4 == 0)
+        reinterpret_cast<__half2*>(scales)[row * (c.dim / kGroup4) + p.lane / 4] =
+            __halves2half2(g.scale, g.low);
     }
-    if (!mine || !holds) return;
-    const GroupScale g = group_scale(lo + bad, hi + bad);
-    *reinterpret_cast<uint32_t*>(codes + row * (c.dim / 2) + 4 * lane) = codes4(v, g);
-    if (lane % 4 == 0)
-      reinterpret_cast<__half2*>(scales)[row * (c.dim / kGroup4) + lane / 4] =
-          __halves2half2(g.scale, g.low);
   }
 }
 
 template <typename Y, int BITS>
-__global__ void __launch_bounds__(256)
-    cache_read_kernel(CacheView c, const int64_t* __restrict__ slots, uint32_t tokens,
-                      uint32_t width, Y* __restrict__ k_out, Y* __restrict__ v_out) {
-  const uint32_t per = 256u / width;
-  const uint32_t lane = threadIdx.x & (width - 1);
-  const uint64_t r = (uint64_t)blockIdx.x * per + threadIdx.x / width;
-  const uint32_t rows_per_token = 2 * c.heads;
-  const uint64_t t = r / rows_per_token;
-  if (t >= tokens || lane * 8 >= c.dim) return;
-  const uint32_t in = (uint32_t)(r - t * rows_per_token);
-  const uint32_t which = in >= c.heads, head = in - (which ? c.heads : 0u);
-  const int64_t slot = slots[t];
-  float v[8] = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
-  if (slot >= 0 && slot < cache_slots(c)) {
-    const int64_t row = cache_row(c, (uint32_t)slot, head);
-    const uint8_t* codes = which ? c.codes[1] : c.codes[0];
-    const uint8_t* scales = which ? c.scales[1] : c.scales[0];
-    if constexpr (BITS == 8) {
-      const uint2 q = *reinterpret_cast<const uint2*>(codes + row * c.dim + 8 * lane);
-      const float s = reinterpret_cast<const float*>(scales)[row];
+__global__ void __launch_bounds__(kThreads)
+    cache_read_kernel(CacheView c, const int64_t* __restrict__ slots, uint32_t tokens, Cut cut,
+                      Y* __restrict__ k_out, Y* __restrict__ v_out) {
+  __shared__ int64_t rows[kMostTokens];
+  const uint32_t t0 = blockIdx.x * cut.tokens, here = min(cut.tokens, tokens - t0);
+  if (threadIdx.x < here) rows[threadIdx.x] = first_row(c, slots[t0 + threadIdx.x]);
+  __syncthreads();
+  const uint32_t lanes = here * 2 * cut.heads * cut.width;
+#pragma unroll 4
+  for (uint32_t x = blockIdx.y * kThreads + threadIdx.x; x < lanes; x += gridDim.y * kThreads) {
+    const Place p = place_of(x, cut);
+    if (8 * p.lane >= c.dim) continue;
+    const int64_t first = rows[p.token], row = first + (int64_t)p.head * c.page_size;
+    float v[8] = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
+    if (first >= 0) {
+      const uint8_t* codes = p.which ? c.codes[1] : c.codes[0];
+      const uint8_t* scales = p.which ? c.scales[1] : c.scales[0];
+      if constexpr (BITS == 8) {
+        const uint2 q = *reinterpret_cast<const uint2*>(codes + row * c.dim + 8 * p.lane);
+        const float s = reinterpret_cast<const float*>(scales)[row];
 #pragma unroll
-      for (int i = 0; i < 8; ++i)
-        v[i] = __fmul_rn((float)(int)(int8_t)((i < 4 ? q.x : q.y) >> (8 * (i & 3))), s);
-    } else {
-      const uint32_t q = *reinterpret_cast<const uint32_t*>(codes + row * (c.dim / 2) + 4 * lane);
-      const __half2 g =
-          reinterpret_cast<const __half2*>(scales)[row * (c.dim / kGroup4) + lane / 4];
-      const float s = __low2float(g), m = __high2float(g);
-      // s * code is exact in fp32: 11 + 4 bits
+        for (int i = 0; i < 8; ++i)
+          v[i] = __fmul_rn((float)(int)(int8_t)((i < 4 ? q.x : q.y) >> (8 * (i & 3))), s);
+      } else {
+        const uint32_t q =
+            *reinterpret_cast<const uint32_t*>(codes + row * (c.dim / 2) + 4 * p.lane);
+        const __half2 g =
+            reinterpret_cast<const __half2*>(scales)[row * (c.dim / kGroup4) + p.lane / 4];
+        const float s = __low2float(g), m = __high2float(g);
+        // s * code is exact in fp32: 11 + 4 bits
 #pragma unroll
-      for (int i = 0; i < 8; ++i) v[i] = fmaf(s, (float)((q >> (4 * i)) & 15u), m);
+        for (int i = 0; i < 8; ++i) v[i] = fmaf(s, (float)((q >> (4 * i)) & 15u), m);
+      }
     }
+    store8((p.which ? v_out : k_out) + ((int64_t)(t0 + p.token) * c.heads + p.head) * c.dim +
+               8 * p.lane,
+           true, 8, v);
   }
-  store8((which ? v_out : k_out) + (t * c.heads + head) * c.dim + 8 * lane, true, 8, v);
 }
 
 inline uint32_t row_width(uint32_t dim) {
@@ -175,37 +211,54 @@ inline uint32_t row_width(uint32_t dim) {
   return w;
 }
 
+// As many tokens a CTA as keep its lanes busy 8 times over; fewer, and a
+// token's heads over several CTAs, where there are not enough for the GPU.
+struct Launch {
+  Cut cut;
+  dim3 grid;
+};
+inline Launch launch_for(const CacheView& c, uint32_t tokens) {
+  Launch l;
+  l.cut.width = row_width(c.dim);
+  l.cut.heads = c.heads;
+  const uint32_t lanes = 2 * c.heads * l.cut.width;  // of a token
+  uint32_t n = std::max(1u, 8 * kThreads / lanes);
+  n = std::min(n, std::max(1u, tokens / (4 * 148)));
+  l.cut.tokens = std::min(n, kMostTokens);
+  l.grid.x = (unsigned)ceil_div(tokens, l.cut.tokens);
+  const uint32_t turns = (uint32_t)ceil_div((int64_t)l.cut.tokens * lanes, kThreads);
+  l.grid.y = std::min(std::min(turns, 65535u), std::max(1u, 4 * 148 / l.grid.x));
+  return l;
+}
+
 template <typename X>
 void launch_write(const CacheView& c, int bits, const KvSource& src, const int64_t* slots,
                   uint32_t tokens, const unsigned long long* table, uint32_t mask,
                   cudaStream_t stream) {
-  const uint32_t width = row_width(c.dim);
-  const unsigned grid = (unsigned)ceil_div((int64_t)tokens * 2 * c.heads, 256 / width);
+  const Launch l = launch_for(c, tokens);
   if (bits == 8)
-    cache_write_kernel<X, 8><<<grid, 256, 0, stream>>>(c, src, slots, tokens, width, table, mask);
+    cache_write_kernel<X, 8>
+        <<<l.grid, kThreads, 0, stream>>>(c, src, slots, tokens, l.cut, table, mask);
   else
-    cache_write_kernel<X, 4><<<grid, 256, 0, stream>>>(c, src, slots, tokens, width, table, mask);
+    cache_write_kernel<X, 4>
+        <<<l.grid, kThreads, 0, stream>>>(c, src, slots, tokens, l.cut, table, mask);
 }
 
 template <typename Y>
 void launch_read(const CacheView& c, int bits, const int64_t* slots, uint32_t tokens, void* k,
                  void* v, cudaStream_t stream) {
-  const uint32_t width = row_width(c.dim);
-  const unsigned grid = (unsigned)ceil_div((int64_t)tokens * 2 * c.heads, 256 / width);
+  const Launch l = launch_for(c, tokens);
   if (bits == 8)
-    cache_read_kernel<Y, 8><<<grid, 256, 0, stream>>>(c, slots, tokens, width,
-                                                      static_cast<Y*>(k), static_cast<Y*>(v));
+    cache_read_kernel<Y, 8><<<l.grid, kThreads, 0, stream>>>(
+        c, slots, tokens, l.cut, static_cast<Y*>(k), static_cast<Y*>(v));
   else
-    cache_read_kernel<Y, 4><<<grid, 256, 0, stream>>>(c, slots, tokens, width,
-                                                      static_cast<Y*>(k), static_cast<Y*>(v));
+    cache_read_kernel<Y, 4><<<l.grid, kThreads, 0, stream>>>(
+        c, slots, tokens, l.cut, static_cast<Y*>(k), static_cast<Y*>(v));
 }
 
-mb_status check_tokens(const mb_kv_cache* c, int64_t tokens) {
+mb_status check_tokens(int64_t tokens) {
   MB_REQUIRE(tokens > 0, "tokens must be positive");
-  MB_REQUIRE(tokens < (int64_t(1) << 30) &&
-                 tokens * 2 * c->kv_heads / (256 / row_width((uint32_t)c->head_dim)) <
-                     (int64_t(1) << 31) - 1,
-             "too many tokens");
+  MB_REQUIRE(tokens < (int64_t(1) << 30), "too many tokens");
   return MB_OK;
 }
 
@@ -229,7 +282,7 @@ extern "C" mb_status mb_cache_write(const mb_kv_cache* cache, const void* k,
   MB_REQUIRE(k && v && slots, "cache_write pointers must not be null");
   MB_REQUIRE(type == MB_FP16 || type == MB_BF16, "k and v must be fp16 or bf16");
   MB_REQUIRE(aligned(k, 2) && aligned(v, 2) && aligned(slots, 8), "misaligned k, v or slots");
-  if (const mb_status st = check_tokens(cache, tokens); st != MB_OK) return st;
+  if (const mb_status st = check_tokens(tokens); st != MB_OK) return st;
   cudaStream_t stream = reinterpret_cast<cudaStream_t>(stream_);
   const CacheView c = cache_view(cache);
   const auto vec = [&](const void* p, int64_t ts, int64_t hs) {
@@ -249,7 +302,7 @@ extern "C" mb_status mb_cache_write(const mb_kv_cache* cache, const void* k,
     table = static_cast<unsigned long long*>(workspace);
     mask = claim_entries(tokens) - 1;
     MB_CUDA_TRY(cudaMemsetAsync(table, 0, need, stream));
-    cache_claim_kernel<<<(unsigned)ceil_div(tokens, 256), 256, 0, stream>>>(
+    cache_claim_kernel<<<(unsigned)ceil_div(tokens, kThreads), kThreads, 0, stream>>>(
         slots, (uint32_t)tokens, cache_slots(c), table, mask);
     MB_LAUNCH_CHECK("cache_claim_kernel");
   }
@@ -270,7 +323,7 @@ extern "C" mb_status mb_cache_read(const mb_kv_cache* cache, const int64_t* slot
   MB_REQUIRE(dtype_known(out_type), "unknown type of the outputs");
   MB_REQUIRE(aligned(k_out, 16) && aligned(v_out, 16) && aligned(slots, 8),
              "outputs must be 16-byte aligned");
-  if (const mb_status st = check_tokens(cache, tokens); st != MB_OK) return st;
+  if (const mb_status st = check_tokens(tokens); st != MB_OK) return st;
   cudaStream_t stream = reinterpret_cast<cudaStream_t>(stream_);
   const CacheView c = cache_view(cache);
   if (out_type == MB_FP16)

@@ -236,11 +236,16 @@ struct GroupScale {
 __device__ __forceinline__ GroupScale group_scale(float lo, float hi) {
   GroupScale g;
   g.low = __float2half_rn(lo);
-  g.scale = __float2half_rn(__double2float_rn(((double)hi - (double)lo) / 15.0));
+  // where the difference is exact in fp32 so is the division's rounding: d / 15
+  // is never within 2^-53 of the middle between two fp32 numbers
+  const float d = hi - lo;
+  float s = __fdiv_rn(d, 15.0f);
+  if ((hi - d) - lo != 0.0f) s = __double2float_rn(((double)hi - (double)lo) / 15.0);
+  g.scale = __float2half_rn(s);
   if (!isfinite(__half2float(g.low)) || !isfinite(__half2float(g.scale))) {
     g.low = g.scale = __ushort_as_half(0x7E00);
   }
-  const float s = __half2float(g.scale);
+  s = __half2float(g.scale);
   g.inv = s > 0.0f ? __fdiv_rn(1.0f, s) : 0.0f;
   return g;
 }

@@ -194,9 +194,9 @@ def test_cache_entry_refusals():
     _refused(w(r, P, 128, 64, P, 128, 64, 2, 1, P, None, 0, None), "fp16 or bf16")
     _refused(w(r, P, 128, 64, P, 128, 64, 0, 0, P, None, 0, None), "positive")
     _refused(w(r, P, 128, 64, P, 128, 64, 0, 1 << 40, P, None, 0, None), "too many tokens")
-    _refused(w(r, P, 128, 64, P, 128, 64, 0, 5000, P, None, 0, None), "workspace")
-    n = C._lib.mb_cache_write_workspace_size(5000)
-    _refused(w(r, P, 128, 64, P, 128, 64, 0, 5000, P, P, n - 1, None), "workspace")
+    _refused(w(r, P, 128, 64, P, 128, 64, 0, 50000, P, None, 0, None), "workspace")
+    n = C._lib.mb_cache_write_workspace_size(50000)
+    _refused(w(r, P, 128, 64, P, 128, 64, 0, 50000, P, P, n - 1, None), "workspace")
     _refused(rd(r, P, 1, P + 2, P, 0, None), "aligned")
     _refused(rd(r, P, 1, P, P, 9, None), "unknown type")
     _refused(at(r, P, 128, 64, 2, 1, 2, P, 1, 1, P, 1.0, P, None, 0, None), "fp16 or bf16")
