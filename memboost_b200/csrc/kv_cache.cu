@@ -15,12 +15,12 @@ namespace mb {
 namespace {
 
 // Up to so many tokens, a CTA looks through the later tokens' slots itself for
-// those of its own (2048 tokens: one launch of 6 us instead of three that take
-// 18); above, where that reads too much, a table says which token a slot
-// belongs to.
-constexpr int64_t kScanTokens = 8192;
+// those of its own; above, where that reads too much, a table says which token
+// a slot belongs to (two launches more).
+constexpr int64_t kScanTokens = 4096;
 constexpr uint32_t kThreads = 256;
-constexpr uint32_t kMostTokens = 8;  // of a CTA
+constexpr uint32_t kMostTokens = 4;  // of a CTA
+constexpr uint32_t kTurns = 4;       // of a CTA over its tokens' lanes
 
 __host__ __device__ inline uint32_t claim_hash(uint32_t slot, uint32_t mask) {
   return (slot * 2654435761u >> 7) & mask;
@@ -65,26 +65,33 @@ __device__ __forceinline__ bool claimed(const unsigned long long* __restrict__ t
 struct KvSource {
   const void* data[2];
   int64_t token_stride[2], head_stride[2];
-  bool vec[2];
+  bool vec;
 };
 
-// How the work is cut: `tokens` a CTA; a token has 2 heads rows of `width` lanes
-// (a power of two, at least dim / 8); a CTA's lanes are dealt to gridDim.y CTAs.
+// How the work is cut: `tokens` a CTA; a token has 2 heads rows of 2^shift
+// lanes (at least dim / 8); a CTA's lanes are dealt to gridDim.y CTAs.
 struct Cut {
-  uint32_t tokens, width, heads;
+  uint32_t tokens, shift, heads;  // lanes a row: 2^shift
+  uint32_t inverse;               // 2^32 / (2 heads), up: divides what is below 2^16
 };
 struct Place {
   uint32_t token, which, head, lane;
 };
 __device__ __forceinline__ Place place_of(uint32_t x, const Cut& cut) {
   Place p;
-  p.lane = x & (cut.width - 1);
-  const uint32_t row = x / cut.width;  // a power of two
-  p.token = row / (2 * cut.heads);
+  const uint32_t row = x >> cut.shift;
+  p.lane = x - (row << cut.shift);
+  p.token = __umulhi(row, cut.inverse);
   const uint32_t in = row - p.token * 2 * cut.heads;
   p.which = in >= cut.heads;
   p.head = in - (p.which ? cut.heads : 0u);
   return p;
+}
+
+// A slot in 32 bits (those of a cache fit), others as one that no cache has.
+constexpr uint32_t kNoKey = 0xFFFFFFFFu;
+__device__ __forceinline__ uint32_t key_of(int64_t slot) {
+  return (uint64_t)slot >> 32 == 0 ? (uint32_t)slot : kNoKey;
 }
 
 // First row (head 0) of a slot, -1 outside the cache.
@@ -92,48 +99,66 @@ __device__ __forceinline__ int64_t first_row(const CacheView& c, int64_t slot) {
   return slot >= 0 && slot < cache_slots(c) ? cache_row(c, (uint32_t)slot, 0) : -1;
 }
 
-template <typename X, int BITS>
+// kVec: 16-byte loads.
+template <typename X, int BITS, bool kVec>
 __global__ void __launch_bounds__(kThreads)
     cache_write_kernel(CacheView c, KvSource src, const int64_t* __restrict__ slots,
                        uint32_t tokens, Cut cut, const unsigned long long* __restrict__ table,
                        uint32_t mask) {
-  __shared__ int64_t rows[kMostTokens], mine[kMostTokens];
+  __shared__ int64_t rows[kMostTokens];
+  __shared__ uint32_t mine[kMostTokens];
   const uint32_t t0 = blockIdx.x * cut.tokens, here = min(cut.tokens, tokens - t0);
+  const uint32_t lanes = (here * 2 * cut.heads) << cut.shift;
+  // the values are on the way while the slots are looked at
+  Raw8<X> raw[kTurns];
+#pragma unroll
+  for (uint32_t i = 0; i < kTurns; ++i) {
+    const uint32_t x = (blockIdx.y + i * gridDim.y) * kThreads + threadIdx.x;
+    const Place p = place_of(x, cut);
+    if (x < lanes && 8 * p.lane < c.dim)
+      raw[i].load(static_cast<const X*>(p.which ? src.data[1] : src.data[0]) +
+                      (t0 + p.token) * (p.which ? src.token_stride[1] : src.token_stride[0]) +
+                      p.head * (p.which ? src.head_stride[1] : src.head_stride[0]) + 8 * p.lane,
+                  kVec, 8);
+  }
   if (threadIdx.x < here) {
     const int64_t slot = slots[t0 + threadIdx.x];
     int64_t row = first_row(c, slot);
     if (table != nullptr && row >= 0 && !claimed(table, mask, (uint32_t)slot, t0 + threadIdx.x))
       row = -1;
     rows[threadIdx.x] = row;
-    mine[threadIdx.x] = slot;
+    mine[threadIdx.x] = key_of(slot);
   }
   __syncthreads();
   if (table == nullptr) {  // the last token with a slot is the one that is kept
+    uint32_t own[kMostTokens];
+#pragma unroll
+    for (uint32_t k = 0; k < kMostTokens; ++k) own[k] = k < here ? mine[k] : kNoKey;
+#pragma unroll 4
     for (uint32_t o = t0 + 1 + threadIdx.x; o < tokens; o += kThreads) {
-      const int64_t slot = slots[o];
-      for (uint32_t k = 0; k < here; ++k)
-        if (slot == mine[k] && o > t0 + k) rows[k] = -1;
+      const uint32_t key = key_of(slots[o]);
+      if (key == kNoKey) continue;
+#pragma unroll
+      for (uint32_t k = 0; k < kMostTokens; ++k)
+        if (key == own[k] && o > t0 + k) rows[k] = -1;
     }
     __syncthreads();
   }
-  const uint32_t lanes = here * 2 * cut.heads * cut.width;
-  for (uint32_t x0 = blockIdx.y * kThreads; x0 < lanes; x0 += gridDim.y * kThreads) {
-    const uint32_t x = x0 + threadIdx.x;
+#pragma unroll
+  for (uint32_t i = 0; i < kTurns; ++i) {
+    const uint32_t x = (blockIdx.y + i * gridDim.y) * kThreads + threadIdx.x;
+    if (x - threadIdx.x >= lanes) break;  // the whole CTA
     const Place p = place_of(x, cut);
     const int64_t first = x < lanes ? rows[p.token] : -1;
     const bool holds = first >= 0 && 8 * p.lane < c.dim;
     float v[8] = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
-    if (holds)
-      load8(static_cast<const X*>(p.which ? src.data[1] : src.data[0]) +
-                (t0 + p.token) * (p.which ? src.token_stride[1] : src.token_stride[0]) +
-                p.head * (p.which ? src.head_stride[1] : src.head_stride[0]) + 8 * p.lane,
-            p.which ? src.vec[1] : src.vec[0], 8, v);
+    if (holds) raw[i].floats(v);
     const int64_t row = first + (int64_t)p.head * c.page_size;
     uint8_t* codes = p.which ? c.codes[1] : c.codes[0];
     uint8_t* scales = p.which ? c.scales[1] : c.scales[0];
     if constexpr (BITS == 8) {
       uint32_t m = abs_bits_max(v);
-      for (uint32_t o = cut.width / 2; o > 0; o >>= 1)
+      for (uint32_t o = 1u << cut.shift >> 1; o > 0; o >>= 1)
         m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
       if (!holds) continue;
       const RowScale s = row_scale(m);
@@ -172,32 +197,50 @@ __global__ void __launch_bounds__(kThreads)
   const uint32_t t0 = blockIdx.x * cut.tokens, here = min(cut.tokens, tokens - t0);
   if (threadIdx.x < here) rows[threadIdx.x] = first_row(c, slots[t0 + threadIdx.x]);
   __syncthreads();
-  const uint32_t lanes = here * 2 * cut.heads * cut.width;
-#pragma unroll 4
-  for (uint32_t x = blockIdx.y * kThreads + threadIdx.x; x < lanes; x += gridDim.y * kThreads) {
+  const uint32_t lanes = (here * 2 * cut.heads) << cut.shift;
+  // eight codes and their scale (4 bits: and minimum) of each turn, then the values
+  uint2 q[kTurns];
+  uint32_t scale[kTurns];
+#pragma unroll
+  for (uint32_t i = 0; i < kTurns; ++i) {
+    const uint32_t x = (blockIdx.y + i * gridDim.y) * kThreads + threadIdx.x;
     const Place p = place_of(x, cut);
-    if (8 * p.lane >= c.dim) continue;
-    const int64_t first = rows[p.token], row = first + (int64_t)p.head * c.page_size;
-    float v[8] = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
-    if (first >= 0) {
-      const uint8_t* codes = p.which ? c.codes[1] : c.codes[0];
-      const uint8_t* scales = p.which ? c.scales[1] : c.scales[0];
-      if constexpr (BITS == 8) {
-        const uint2 q = *reinterpret_cast<const uint2*>(codes + row * c.dim + 8 * p.lane);
-        const float s = reinterpret_cast<const float*>(scales)[row];
+    q[i] = make_uint2(0u, 0u);
+    scale[i] = 0u;
+    if (x >= lanes || 8 * p.lane >= c.dim || rows[p.token] < 0) continue;
+    const int64_t row = rows[p.token] + (int64_t)p.head * c.page_size;
+    const uint8_t* codes = p.which ? c.codes[1] : c.codes[0];
+    const uint32_t* scales =
+        reinterpret_cast<const uint32_t*>(p.which ? c.scales[1] : c.scales[0]);
+    if constexpr (BITS == 8) {
+      q[i] = *reinterpret_cast<const uint2*>(codes + row * c.dim + 8 * p.lane);
+      scale[i] = scales[row];
+    } else {
+      q[i].x = *reinterpret_cast<const uint32_t*>(codes + row * (c.dim / 2) + 4 * p.lane);
+      scale[i] = scales[row * (c.dim / kGroup4) + p.lane / 4];
+    }
+  }
 #pragma unroll
-        for (int i = 0; i < 8; ++i)
-          v[i] = __fmul_rn((float)(int)(int8_t)((i < 4 ? q.x : q.y) >> (8 * (i & 3))), s);
-      } else {
-        const uint32_t q =
-            *reinterpret_cast<const uint32_t*>(codes + row * (c.dim / 2) + 4 * p.lane);
-        const __half2 g =
-            reinterpret_cast<const __half2*>(scales)[row * (c.dim / kGroup4) + p.lane / 4];
-        const float s = __low2float(g), m = __high2float(g);
-        // s * code is exact in fp32: 11 + 4 bits
+  for (uint32_t i = 0; i < kTurns; ++i) {
+    const uint32_t x = (blockIdx.y + i * gridDim.y) * kThreads + threadIdx.x;
+    const Place p = place_of(x, cut);
+    if (x >= lanes || 8 * p.lane >= c.dim) continue;
+    float v[8];
+    if constexpr (BITS == 8) {
+      const float s = __uint_as_float(scale[i]);
+      // 2^23 + 128 + code from the code's byte, less 2^23 + 128
+      const uint32_t w[2] = {q[i].x ^ 0x80808080u, q[i].y ^ 0x80808080u};
 #pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] = fmaf(s, (float)((q >> (4 * i)) & 15u), m);
-      }
+      for (int e = 0; e < 8; ++e)
+        v[e] = __fmul_rn(
+            __uint_as_float(__byte_perm(w[e / 4], 0x4B000000u, 0x7440 + (e & 3))) - 8388736.0f, s);
+    } else {
+      const __half2 g = *reinterpret_cast<const __half2*>(&scale[i]);
+      const float s = __low2float(g), m = __high2float(g);
+      // s * code is exact in fp32: 11 + 4 bits; the code from 2^23 + code
+#pragma unroll
+      for (int e = 0; e < 8; ++e)
+        v[e] = fmaf(s, __uint_as_float(((q[i].x >> (4 * e)) & 15u) | 0x4B000000u) - 8388608.0f, m);
     }
     store8((p.which ? v_out : k_out) + ((int64_t)(t0 + p.token) * c.heads + p.head) * c.dim +
                8 * p.lane,
@@ -205,29 +248,31 @@ __global__ void __launch_bounds__(kThreads)
   }
 }
 
-inline uint32_t row_width(uint32_t dim) {
-  uint32_t w = 4;
-  while (w * 8 < dim) w *= 2;
+inline uint32_t row_shift(uint32_t dim) {
+  uint32_t w = 2;
+  while (8u << w < dim) ++w;
   return w;
 }
 
-// As many tokens a CTA as keep its lanes busy 8 times over; fewer, and a
-// token's heads over several CTAs, where there are not enough for the GPU.
+// As many tokens a CTA as fill its turns; fewer, and a token's heads over
+// several CTAs, where there are not enough for the GPU or a token has more.
 struct Launch {
   Cut cut;
   dim3 grid;
 };
 inline Launch launch_for(const CacheView& c, uint32_t tokens) {
   Launch l;
-  l.cut.width = row_width(c.dim);
+  l.cut.shift = row_shift(c.dim);
   l.cut.heads = c.heads;
-  const uint32_t lanes = 2 * c.heads * l.cut.width;  // of a token
-  uint32_t n = std::max(1u, 8 * kThreads / lanes);
+  l.cut.inverse = (uint32_t)((((uint64_t)1 << 32) + 2 * c.heads - 1) / (2 * c.heads));
+  const uint32_t lanes = 2 * c.heads << l.cut.shift;  // of a token
+  uint32_t n = std::max(1u, kTurns * kThreads / lanes);
   n = std::min(n, std::max(1u, tokens / (4 * 148)));
   l.cut.tokens = std::min(n, kMostTokens);
   l.grid.x = (unsigned)ceil_div(tokens, l.cut.tokens);
   const uint32_t turns = (uint32_t)ceil_div((int64_t)l.cut.tokens * lanes, kThreads);
-  l.grid.y = std::min(std::min(turns, 65535u), std::max(1u, 4 * 148 / l.grid.x));
+  l.grid.y = std::max((turns + kTurns - 1) / kTurns,
+                      std::min(turns, std::max(1u, 4 * 148 / l.grid.x)));
   return l;
 }
 
@@ -236,12 +281,13 @@ void launch_write(const CacheView& c, int bits, const KvSource& src, const int64
                   uint32_t tokens, const unsigned long long* table, uint32_t mask,
                   cudaStream_t stream) {
   const Launch l = launch_for(c, tokens);
+  const auto go = [&](auto kernel) {
+    kernel<<<l.grid, kThreads, 0, stream>>>(c, src, slots, tokens, l.cut, table, mask);
+  };
   if (bits == 8)
-    cache_write_kernel<X, 8>
-        <<<l.grid, kThreads, 0, stream>>>(c, src, slots, tokens, l.cut, table, mask);
+    src.vec ? go(cache_write_kernel<X, 8, true>) : go(cache_write_kernel<X, 8, false>);
   else
-    cache_write_kernel<X, 4>
-        <<<l.grid, kThreads, 0, stream>>>(c, src, slots, tokens, l.cut, table, mask);
+    src.vec ? go(cache_write_kernel<X, 4, true>) : go(cache_write_kernel<X, 4, false>);
 }
 
 template <typename Y>
@@ -291,8 +337,8 @@ extern "C" mb_status mb_cache_write(const mb_kv_cache* cache, const void* k,
   const KvSource src{{k, v},
                      {k_token_stride, v_token_stride},
                      {k_head_stride, v_head_stride},
-                     {vec(k, k_token_stride, k_head_stride),
-                      vec(v, v_token_stride, v_head_stride)}};
+                     vec(k, k_token_stride, k_head_stride) &&
+                         vec(v, v_token_stride, v_head_stride)};
   unsigned long long* table = nullptr;
   uint32_t mask = 0;
   if (tokens > kScanTokens) {

@@ -50,7 +50,7 @@ inline mb_status check_cache(const mb_kv_cache* c) {
                  c->head_dim % (c->bits == 8 ? 16 : kGroup4) == 0,
              c->bits == 8 ? "head_dim must be a multiple of 16 up to 256"
                           : "head_dim must be a multiple of 32 up to 256");
-  MB_REQUIRE(c->kv_heads <= 65535, "too many kv_heads");
+  MB_REQUIRE(c->kv_heads <= 4096, "too many kv_heads");
   MB_REQUIRE(c->pages <= (int64_t(1) << 31) - 1 &&
                  c->pages * c->page_size <= (int64_t(1) << 32) - 2,
              "too many slots");

@@ -252,27 +252,40 @@ __device__ __forceinline__ GroupScale group_scale(float lo, float hi) {
 
 // 4-bit codes of eight values of a group, (x - minimum) / scale to the
 // nearest, ties to even, in [0, 15]; value i at bits [4 i, 4 i + 4).  As
-// codes8: fp32 decides (error below 16 * 2^-22) unless a border is near.
+// codes8: fp32 decides (error below 16 * 2^-22) unless a border is near.  Then
+// x - minimum is taken with its rounding error e; t * scale (4 + 11 bits) is
+// exact, and so, where a border is near, are the remainder and its distance
+// from scale / 2, to which e is added: the sign is that of the exact distance.
 __device__ __forceinline__ uint32_t codes4(const float (&x)[8], GroupScale g) {
-  const float low = __half2float(g.low);
-  uint32_t c = 0;
+  const float low = __half2float(g.low), scale = __half2float(g.scale);
+  uint32_t y[8];
   float far = 0.0f;
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
     const float q = fminf(fmaxf((x[i] - low) * g.inv, 0.0f), 15.0f);
     const float m = q + kRoundMagic;
     far = fmaxf(far, fabsf(q - (m - kRoundMagic)));
-    c |= (__float_as_uint(m) & 0xFu) << (4 * i);
+    y[i] = __float_as_uint(m);
   }
   if (far > kRoundSafe) {
-    c = 0;
+    const float half = 0.5f * scale;
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-      double q = rint(((double)x[i] - (double)low) / (double)__half2float(g.scale));
-      q = fmin(fmax(q, 0.0), 15.0);
-      c |= (uint32_t)(int)q << (4 * i);
+      const float z = x[i] - low;
+      const float q = fminf(fmaxf(z * g.inv, 0.0f), 15.0f);
+      const float t = __uint_as_float(y[i]) - kRoundMagic;
+      if (fabsf(q - t) <= kRoundSafe) continue;
+      // z + e = x - low exactly
+      const float back = z + low;
+      const float e = (x[i] - back) + ((back - z) - low);
+      const float rest = fmaf(-t, scale, z);
+      const float over = (fabsf(rest) - half) + (rest > 0.0f ? e : -e);
+      if (over > 0.0f || (over == 0.0f && (y[i] & 1u))) y[i] += rest > 0.0f ? 1u : ~0u;
     }
   }
+  uint32_t c = 0;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) c |= (y[i] & 0xFu) << (4 * i);
   return c;
 }
 
