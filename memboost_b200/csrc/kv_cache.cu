@@ -10,14 +10,17 @@
 #include <algorithm>
 
 #include "mb_cache.cuh"
+#include "mb_tma.cuh"
 
 namespace mb {
 namespace {
 
-// Up to so many tokens, a CTA looks through the later tokens' slots itself for
-// those of its own; above, where that reads too much, a table says which token
-// a slot belongs to (two launches more).
-constexpr int64_t kScanTokens = 4096;
+// Which token of a slot is kept: up to kOwnTokens tokens, each writing CTA looks
+// through the later tokens' slots itself; up to kScanTokens a kernel before
+// does so for 32 tokens a CTA; above, where that reads too much, a table says
+// which token a slot belongs to (two launches more).  The kernels leave each
+// token's first row in the workspace.
+constexpr int64_t kOwnTokens = 256, kScanTokens = 16384;
 constexpr uint32_t kThreads = 256;
 constexpr uint32_t kMostTokens = 4;  // of a CTA
 constexpr uint32_t kTurns = 4;       // of a CTA over its tokens' lanes
@@ -99,12 +102,51 @@ __device__ __forceinline__ int64_t first_row(const CacheView& c, int64_t slot) {
   return slot >= 0 && slot < cache_slots(c) ? cache_row(c, (uint32_t)slot, 0) : -1;
 }
 
+// Every token's first row, -1 where it is not written.  table: from
+// cache_claim_kernel, or null: later tokens are looked through, most of them
+// only against a bit that says whether one of the CTA's slots has their hash.
+constexpr uint32_t kScanOwn = 32, kScanBits = 2048;
+__global__ void __launch_bounds__(kThreads)
+    cache_rows_kernel(CacheView c, const int64_t* __restrict__ slots, uint32_t tokens,
+                      const unsigned long long* __restrict__ table, uint32_t mask,
+                      int64_t* __restrict__ rows) {
+  grid_launch_dependents();
+  if (table != nullptr) {
+    const uint32_t t = blockIdx.x * kThreads + threadIdx.x;
+    if (t >= tokens) return;
+    const int64_t slot = slots[t], row = first_row(c, slot);
+    rows[t] = row >= 0 && claimed(table, mask, (uint32_t)slot, t) ? row : -1;
+    return;
+  }
+  __shared__ uint32_t bits[kScanBits / 32], own[kScanOwn];
+  __shared__ int64_t first[kScanOwn];
+  const uint32_t t0 = blockIdx.x * kScanOwn, here = min(kScanOwn, tokens - t0);
+  if (threadIdx.x < kScanBits / 32) bits[threadIdx.x] = 0;
+  __syncthreads();
+  if (threadIdx.x < here) {
+    const int64_t slot = slots[t0 + threadIdx.x];
+    const uint32_t key = key_of(slot);
+    own[threadIdx.x] = key;
+    first[threadIdx.x] = first_row(c, slot);
+    if (key != kNoKey) atomicOr(&bits[key % kScanBits / 32], 1u << key % 32);
+  }
+  __syncthreads();
+#pragma unroll 8
+  for (uint32_t o = t0 + 1 + threadIdx.x; o < tokens; o += kThreads) {
+    const uint32_t key = key_of(slots[o]);
+    if (key == kNoKey || (bits[key % kScanBits / 32] >> key % 32 & 1u) == 0) continue;
+    for (uint32_t k = 0; k < here; ++k)
+      if (key == own[k] && o > t0 + k) first[k] = -1;
+  }
+  __syncthreads();
+  if (threadIdx.x < here) rows[t0 + threadIdx.x] = first[threadIdx.x];
+}
+
 // kVec: 16-byte loads.
 template <typename X, int BITS, bool kVec>
 __global__ void __launch_bounds__(kThreads)
     cache_write_kernel(CacheView c, KvSource src, const int64_t* __restrict__ slots,
-                       uint32_t tokens, Cut cut, const unsigned long long* __restrict__ table,
-                       uint32_t mask) {
+                       uint32_t tokens, Cut cut, const int64_t* __restrict__ first_rows) {
   __shared__ int64_t rows[kMostTokens];
   __shared__ uint32_t mine[kMostTokens];
   const uint32_t t0 = blockIdx.x * cut.tokens, here = min(cut.tokens, tokens - t0);
@@ -121,26 +163,21 @@ __global__ void __launch_bounds__(kThreads)
                       p.head * (p.which ? src.head_stride[1] : src.head_stride[0]) + 8 * p.lane,
                   kVec, 8);
   }
-  if (threadIdx.x < here) {
-    const int64_t slot = slots[t0 + threadIdx.x];
-    int64_t row = first_row(c, slot);
-    if (table != nullptr && row >= 0 && !claimed(table, mask, (uint32_t)slot, t0 + threadIdx.x))
-      row = -1;
-    rows[threadIdx.x] = row;
-    mine[threadIdx.x] = key_of(slot);
-  }
-  __syncthreads();
-  if (table == nullptr) {  // the last token with a slot is the one that is kept
-    uint32_t own[kMostTokens];
-#pragma unroll
-    for (uint32_t k = 0; k < kMostTokens; ++k) own[k] = k < here ? mine[k] : kNoKey;
-#pragma unroll 4
+  if (first_rows != nullptr) {
+    grid_dependency_wait();
+    if (threadIdx.x < here) rows[threadIdx.x] = first_rows[t0 + threadIdx.x];
+    __syncthreads();
+  } else {  // the last token with a slot is the one that is kept
+    if (threadIdx.x < here) {
+      const int64_t slot = slots[t0 + threadIdx.x];
+      rows[threadIdx.x] = first_row(c, slot);
+      mine[threadIdx.x] = key_of(slot);
+    }
+    __syncthreads();
     for (uint32_t o = t0 + 1 + threadIdx.x; o < tokens; o += kThreads) {
       const uint32_t key = key_of(slots[o]);
-      if (key == kNoKey) continue;
-#pragma unroll
-      for (uint32_t k = 0; k < kMostTokens; ++k)
-        if (key == own[k] && o > t0 + k) rows[k] = -1;
+      for (uint32_t k = 0; k < here; ++k)
+        if (key != kNoKey && key == mine[k] && o > t0 + k) rows[k] = -1;
     }
     __syncthreads();
   }
@@ -277,17 +314,27 @@ inline Launch launch_for(const CacheView& c, uint32_t tokens) {
 }
 
 template <typename X>
-void launch_write(const CacheView& c, int bits, const KvSource& src, const int64_t* slots,
-                  uint32_t tokens, const unsigned long long* table, uint32_t mask,
-                  cudaStream_t stream) {
+mb_status launch_write(const CacheView& c, int bits, const KvSource& src, const int64_t* slots,
+                       uint32_t tokens, const int64_t* rows, cudaStream_t stream) {
   const Launch l = launch_for(c, tokens);
+  // behind the kernel of the rows: the values are loaded meanwhile
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = l.grid;
+  cfg.blockDim = dim3(kThreads);
+  cfg.stream = stream;
+  cfg.attrs = attr;
+  cfg.numAttrs = rows != nullptr ? 1 : 0;
   const auto go = [&](auto kernel) {
-    kernel<<<l.grid, kThreads, 0, stream>>>(c, src, slots, tokens, l.cut, table, mask);
+    return cudaLaunchKernelEx(&cfg, kernel, c, src, slots, tokens, l.cut, rows);
   };
   if (bits == 8)
-    src.vec ? go(cache_write_kernel<X, 8, true>) : go(cache_write_kernel<X, 8, false>);
+    MB_CUDA_TRY(src.vec ? go(cache_write_kernel<X, 8, true>) : go(cache_write_kernel<X, 8, false>));
   else
-    src.vec ? go(cache_write_kernel<X, 4, true>) : go(cache_write_kernel<X, 4, false>);
+    MB_CUDA_TRY(src.vec ? go(cache_write_kernel<X, 4, true>) : go(cache_write_kernel<X, 4, false>));
+  return MB_OK;
 }
 
 template <typename Y>
@@ -314,8 +361,8 @@ mb_status check_tokens(int64_t tokens) {
 using namespace mb;
 
 extern "C" size_t mb_cache_write_workspace_size(int64_t tokens) {
-  if (tokens <= kScanTokens || tokens >= (int64_t(1) << 30)) return 0;
-  return (size_t)claim_entries(tokens) * 8;
+  if (tokens <= kOwnTokens || tokens >= (int64_t(1) << 30)) return 0;
+  return (size_t)tokens * 8 + (tokens > kScanTokens ? (size_t)claim_entries(tokens) * 8 : 0);
 }
 
 extern "C" mb_status mb_cache_write(const mb_kv_cache* cache, const void* k,
@@ -339,25 +386,31 @@ extern "C" mb_status mb_cache_write(const mb_kv_cache* cache, const void* k,
                      {k_head_stride, v_head_stride},
                      vec(k, k_token_stride, k_head_stride) &&
                          vec(v, v_token_stride, v_head_stride)};
-  unsigned long long* table = nullptr;
-  uint32_t mask = 0;
-  if (tokens > kScanTokens) {
-    const size_t need = mb_cache_write_workspace_size(tokens);
-    if (workspace == nullptr || workspace_bytes < need || !aligned(workspace, 8))
+  int64_t* rows = nullptr;
+  if (tokens > kOwnTokens) {
+    if (workspace == nullptr || workspace_bytes < mb_cache_write_workspace_size(tokens) ||
+        !aligned(workspace, 8))
       return set_error(MB_ERR_WORKSPACE, "cache_write workspace missing, misaligned or too small");
-    table = static_cast<unsigned long long*>(workspace);
-    mask = claim_entries(tokens) - 1;
-    MB_CUDA_TRY(cudaMemsetAsync(table, 0, need, stream));
-    cache_claim_kernel<<<(unsigned)ceil_div(tokens, kThreads), kThreads, 0, stream>>>(
-        slots, (uint32_t)tokens, cache_slots(c), table, mask);
-    MB_LAUNCH_CHECK("cache_claim_kernel");
+    rows = static_cast<int64_t*>(workspace);
+    unsigned long long* table = nullptr;
+    uint32_t mask = 0;
+    unsigned grid = (unsigned)ceil_div(tokens, kScanOwn);
+    if (tokens > kScanTokens) {
+      table = reinterpret_cast<unsigned long long*>(rows + tokens);
+      mask = claim_entries(tokens) - 1;
+      MB_CUDA_TRY(cudaMemsetAsync(table, 0, ((size_t)mask + 1) * 8, stream));
+      grid = (unsigned)ceil_div(tokens, kThreads);
+      cache_claim_kernel<<<grid, kThreads, 0, stream>>>(slots, (uint32_t)tokens, cache_slots(c),
+                                                        table, mask);
+      MB_LAUNCH_CHECK("cache_claim_kernel");
+    }
+    cache_rows_kernel<<<grid, kThreads, 0, stream>>>(c, slots, (uint32_t)tokens, table, mask, rows);
+    MB_LAUNCH_CHECK("cache_rows_kernel");
   }
-  if (type == MB_FP16)
-    launch_write<__half>(c, cache->bits, src, slots, (uint32_t)tokens, table, mask, stream);
-  else
-    launch_write<__nv_bfloat16>(c, cache->bits, src, slots, (uint32_t)tokens, table, mask, stream);
-  MB_LAUNCH_CHECK("cache_write_kernel");
-  return MB_OK;
+  return type == MB_FP16 ? launch_write<__half>(c, cache->bits, src, slots, (uint32_t)tokens, rows,
+                                                stream)
+                         : launch_write<__nv_bfloat16>(c, cache->bits, src, slots,
+                                                       (uint32_t)tokens, rows, stream);
 }
 
 extern "C" mb_status mb_cache_read(const mb_kv_cache* cache, const int64_t* slots, int64_t tokens,
