@@ -14,6 +14,7 @@
 // Few tiles (few tokens): K is split over the CTAs of a cluster, which add
 // their int32 parts through distributed shared memory -- whole numbers, so
 // the result does not depend on the split.
+#include <algorithm>
 #include <cstring>
 
 #include "mb_codes.cuh"
@@ -28,16 +29,17 @@ constexpr int kWeightBytes = kChannels * kStepK;
 constexpr int kThreads = 192;             // warps 0-3 drain, 4 loads, 5 multiplies
 
 // Shared memory of a tile of kN tokens: a ring of stages (128 bytes of K of
-// both operands), whose memory the int32 parts of a split reuse ([kN tokens]
-// [128 channels]).
+// both operands), whose memory the int32 parts of a split reuse (128
+// channels by kN tokens and padding).
 template <int kN>
 struct Shape {
   static constexpr int kStage = kWeightBytes + kN * kStepK;
   static constexpr uint32_t kTmem = kN < 32 ? 32 : kN;
   static constexpr int smem(int stages) { return stages * kStage + 1024; }
-  static constexpr int kLeast = (kN * kChannels * 4 + kStage - 1) / kStage;  // stages
+  static constexpr int kLeast = ((kN + 4) * kChannels * 4 + kStage - 1) / kStage;  // stages
 };
 constexpr int kMaxStages = 12;
+constexpr uint32_t kMostParts = 8;  // of K: a portable cluster
 constexpr int kMostSmem = 227 * 1024 - 2048;  // a CTA's, less what is declared statically
 constexpr int kSms = 148;
 
@@ -106,9 +108,17 @@ __device__ __forceinline__ uint32_t cluster_address(uint32_t saddr, uint32_t ran
   asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(d) : "r"(saddr), "r"(rank));
   return d;
 }
-__device__ __forceinline__ int load_cluster(uint32_t saddr) {
-  int v;
-  asm volatile("ld.shared::cluster.s32 %0, [%1];" : "=r"(v) : "r"(saddr) : "memory");
+__device__ __forceinline__ uint32_t load_cluster(uint32_t saddr) {
+  uint32_t v;
+  asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v) : "r"(saddr) : "memory");
+  return v;
+}
+__device__ __forceinline__ int4 load_cluster4(uint32_t saddr) {
+  int4 v;
+  asm volatile("ld.shared::cluster.v4.s32 {%0, %1, %2, %3}, [%4];"
+               : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+               : "r"(saddr)
+               : "memory");
   return v;
 }
 
@@ -274,27 +284,42 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
     }
   } else {
-    int* own = reinterpret_cast<int*>(ring);  // [token][channel]
+    // a channel's sums in a row; the rows' length keeps 16-byte accesses of
+    // neighbouring channels apart
+    constexpr int kRow = kN + 4;
+    int* own = reinterpret_cast<int*>(ring) + (32 * (warp & 3) + lane) * kRow;
     if (warp < 4) {
 #pragma unroll 1
       for (int c = 0; c < columns; c += 16) {
         uint32_t v[16];
         tmem_ld16(lanes + c, v);
 #pragma unroll
-        for (int i = 0; i < 16; ++i) own[(c + i) * kChannels + 32 * warp + lane] = (int)v[i];
+        for (int i = 0; i < 16; i += 4)
+          *reinterpret_cast<int4*>(own + c + i) =
+              make_int4((int)v[i], (int)v[i + 1], (int)v[i + 2], (int)v[i + 3]);
       }
     }
     cluster_sync();
     const uint32_t base = smem_u32(own), fail = smem_u32(&failed);
     for (uint32_t r = 0; r < parts; ++r)
       if (load_cluster(cluster_address(fail, r)) != 0) sb = __uint_as_float(0x7FC00000u);
-    // this CTA's share of the tile's tokens, a channel a thread
+    // this CTA's share of the tile's tokens, four at a time, a channel a thread
     if (live) {
-      for (int c = (int)part; c < columns; c += (int)parts) {
-        int sum = 0;
-        for (uint32_t r = 0; r < parts; ++r)
-          sum += load_cluster(cluster_address(base + (c * kChannels + 32 * warp + lane) * 4, r));
-        o[c * e.out_stride] = from_float<Y>(scaled(sum, a_scale[c], sb, bias));
+      for (int c = 4 * (int)part; c < columns; c += 4 * (int)parts) {
+        int4 v[kMostParts];
+#pragma unroll
+        for (uint32_t r = 0; r < kMostParts; ++r)
+          if (r < parts) v[r] = load_cluster4(cluster_address(base + 4 * c, r));
+        int4 sum = make_int4(0, 0, 0, 0);
+#pragma unroll
+        for (uint32_t r = 0; r < kMostParts; ++r)
+          if (r < parts) sum.x += v[r].x, sum.y += v[r].y, sum.z += v[r].z, sum.w += v[r].w;
+        const float4 sa = *reinterpret_cast<const float4*>(a_scale + c);
+        Y* to = o + c * e.out_stride;
+        to[0] = from_float<Y>(scaled(sum.x, sa.x, sb, bias));
+        if (c + 1 < columns) to[e.out_stride] = from_float<Y>(scaled(sum.y, sa.y, sb, bias));
+        if (c + 2 < columns) to[2 * e.out_stride] = from_float<Y>(scaled(sum.z, sa.z, sb, bias));
+        if (c + 3 < columns) to[3 * e.out_stride] = from_float<Y>(scaled(sum.w, sa.w, sb, bias));
       }
     }
     cluster_sync();  // no CTA leaves while another reads its part
@@ -584,13 +609,19 @@ mb_status launch_pairs(const Product& p) {
 template <int kN, typename Y>
 mb_status split_tiles(const Product& p) {
   using S = Shape<kN>;
-  // K parts: until the tiles fill the SMs, each part at least two steps
   const int64_t tiles = ceil_div(p.N, kChannels) * ceil_div(p.M, kN);
   const int64_t steps = ceil_div(p.K, kStepK);
-  int parts = 1;
-  while (parts < 8 && tiles * parts * 2 <= kSms && steps >= 4 * parts) parts *= 2;
-  int stages = kN == 256 ? 4 : kN == 128 ? 6 : 5;
-  return launch_tiles<kN, Y>(p, parts, stages);
+  // K parts: as many as give two CTAs an SM work (one, where their stages are
+  // too large for two), each at least four steps
+  constexpr int kHalf = (kMostSmem - 2048) / 2;
+  constexpr bool kTwo = S::smem(std::max(4, S::kLeast)) <= kHalf;
+  int64_t parts = min64(kMostParts, min64((kTwo ? 2 : 1) * kSms / tiles, steps / 4));
+  if (parts < 2) parts = 1;
+  // as deep a ring as fits, but not deeper than a part has steps
+  int stages = ((kTwo && tiles * parts > kSms ? kHalf : kMostSmem) - 1024) / S::kStage;
+  stages = (int)min64(std::min(stages, kMaxStages), ceil_div(steps, parts));
+  if (parts > 1) stages = std::max(stages, S::kLeast);
+  return launch_tiles<kN, Y>(p, (int)parts, stages);
 }
 
 template <typename Y>

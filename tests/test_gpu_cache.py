@@ -63,7 +63,7 @@ def test_write_and_read(bits, dim, dtype):
             _check_values(got[w], mirror.read(w, ask.tolist()))
 
 
-@pytest.mark.parametrize("tokens", [1, 40, 256, 257, 3001, 16384, 16385])
+@pytest.mark.parametrize("tokens", [1, 40, 2048, 2049, 16384, 16385])
 @pytest.mark.parametrize("bits", [8, 4])
 def test_write_same_slot_and_outside(tokens, bits):
     """The last token of a slot stays, whatever their number; slots outside
