@@ -43,6 +43,10 @@ constexpr uint32_t kMostParts = 8;  // of K: a portable cluster
 constexpr int kMostSmem = 227 * 1024 - 2048;  // a CTA's, less what is declared statically
 constexpr int kSms = 148;
 
+__device__ __forceinline__ void prefetch_map(const CUtensorMap* map) {
+  asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(map)) : "memory");
+}
+
 // Shared-memory descriptor of a K-major operand written by TMA with the
 // 128-byte swizzle: rows of 128 bytes, 8-row atoms of 1024 bytes.
 __device__ __forceinline__ uint64_t umma_desc_k_sw128(uint32_t saddr) {
@@ -189,7 +193,14 @@ __global__ void __launch_bounds__(kThreads, 1)
   const int k0 = (int)((int64_t)all * part / parts), k1 = (int)((int64_t)all * (part + 1) / parts);
   const int steps = k1 - k0;
 
-  if (threadIdx.x == 0) {
+  const auto weights_of = [&](int i, int s) {
+    mbar_arrive_expect_tx(&full[s], S::kStage);
+    tma_load_2d(ring + s * S::kStage, &weights, &full[s], (k0 + i) * kStepK, (int)n0);
+  };
+  int first = 0;  // steps whose weights are on the way
+  if (warp == 4 && lane == 0) {
+    prefetch_map(&weights);
+    prefetch_map(&tokens);
     for (int s = 0; s < stages; ++s) {
       mbar_init(&full[s], 1);
       mbar_init(&empty[s], 1);
@@ -197,6 +208,9 @@ __global__ void __launch_bounds__(kThreads, 1)
     mbar_init(&done, 1);
     failed = 0;
     fence_mbar_init();
+    // the weights wait neither for this CTA's other warps nor for the kernel
+    // that quantises the tokens
+    for (; first < steps && first < stages; ++first) weights_of(first, first);
   }
   if (warp == 0) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(
@@ -210,17 +224,11 @@ __global__ void __launch_bounds__(kThreads, 1)
   const uint32_t tmem = tmem_slot;
 
   if (warp == 4 && lane == 0) {
-    const auto weights_of = [&](int i, int s) {
-      mbar_arrive_expect_tx(&full[s], S::kStage);
-      tma_load_2d(ring + s * S::kStage, &weights, &full[s], (k0 + i) * kStepK, (int)n0);
-    };
     const auto tokens_of = [&](int i, int s) {
       tma_load_2d(ring + s * S::kStage + kWeightBytes, &tokens, &full[s], (k0 + i) * kStepK,
                   (int)m0);
     };
-    // the weights do not wait for the kernel that quantises the tokens
-    int i = 0;
-    for (; i < steps && i < stages; ++i) weights_of(i, i);
+    int i = first;
     grid_dependency_wait();
     for (int f = 0; f < i; ++f) tokens_of(f, f);
     int s = i == stages ? 0 : i;
@@ -257,6 +265,10 @@ __global__ void __launch_bounds__(kThreads, 1)
     umma_commit(&done);
   }
   __syncwarp();
+  const int64_t n = n0 + 32 * warp + lane;  // warps 0-3: this thread's channel
+  const bool live = warp < 4 && n < N;
+  float sb = live ? e.b_scales[n] : 0.0f;
+  const float bias = live ? bias_at(e, n) : 0.0f;
   grid_dependency_wait();
   if (warp < 4)
     for (int i = threadIdx.x; i < kN; i += 128) a_scale[i] = m0 + i < M ? e.a_scales[m0 + i] : 0.0f;
@@ -264,12 +276,8 @@ __global__ void __launch_bounds__(kThreads, 1)
   asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
   __syncthreads();  // `failed` is final; the ring is free
 
-  const int64_t n = n0 + 32 * warp + lane;  // warps 0-3: this thread's channel
-  const bool live = warp < 4 && n < N;
   const uint32_t lanes = tmem + ((uint32_t)(32 * (warp & 3)) << 16);
   const int columns = (int)min64(kN, M - m0);
-  float sb = live ? e.b_scales[n] : 0.0f;
-  const float bias = live ? bias_at(e, n) : 0.0f;
   Y* o = static_cast<Y*>(e.out) + m0 * e.out_stride + n;
   if (parts == 1) {
     if (failed) sb = __uint_as_float(0x7FC00000u);
@@ -413,6 +421,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
   const int steps = (int)ceil_div(K, kStepK);
 
   if (threadIdx.x == 0) {
+    prefetch_map(&weights);
+    prefetch_map(&tokens);
     for (int s = 0; s < kPairStages; ++s) {
       mbar_init(&full[s], 1);
       mbar_init(&empty[s], 1);
@@ -612,10 +622,12 @@ mb_status split_tiles(const Product& p) {
   const int64_t tiles = ceil_div(p.N, kChannels) * ceil_div(p.M, kN);
   const int64_t steps = ceil_div(p.K, kStepK);
   // K parts: as many as give two CTAs an SM work (one, where their stages are
-  // too large for two), each at least four steps
+  // too large for two), each at least eight steps: joining costs about 2 us (one
+  // token, 4096 x 4096: 13.8 us with 1 part, 10.7 with 2, 8.3 with 4, 9.0 with 8;
+  // 16 tokens, 4096 x 11008: 30.5, 21.1, 15.2 and 13.9)
   constexpr int kHalf = (kMostSmem - 2048) / 2;
   constexpr bool kTwo = S::smem(std::max(4, S::kLeast)) <= kHalf;
-  int64_t parts = min64(kMostParts, min64((kTwo ? 2 : 1) * kSms / tiles, steps / 4));
+  int64_t parts = min64(kMostParts, min64((kTwo ? 2 : 1) * kSms / tiles, steps / 8));
   if (parts < 2) parts = 1;
   // as deep a ring as fits, but not deeper than a part has steps
   int stages = ((kTwo && tiles * parts > kSms ? kHalf : kMostSmem) - 1024) / S::kStage;
