@@ -616,36 +616,66 @@ mb_status launch_pairs(const Product& p) {
   return MB_OK;
 }
 
+// Tokens a tile and K parts of a product too small for the pairs: the least of
+// an estimate, in us, of what a CTA streams (75 GB a second of operands an SM,
+// 9 TB of all from L2), what draining a tile costs (0.01 a token) and what
+// joining parts costs (1, and their sums at 15 GB a second).  Measured against
+// it, whole calls: 64 x 4096 x 4096: 64 tokens in 4 parts 11.9 us, in 1 14.3;
+// 256 x 4096 x 4096: 64 tokens in 1 part 15.0, 256 tokens in 4 20.4; 300 x 300
+// x 300: 32 tokens 4.9, 256 tokens 8.1; 1000 x 1000 x 1000: 64 tokens 7.9, 256
+// tokens 10.8; 1 x 4096 x 4096: 4 parts 8.3, 1 part 13.8.
+struct Tiling {
+  int tokens, parts;
+};
+inline Tiling tiling_for(int64_t M, int64_t N, int64_t K) {
+  const int64_t steps = ceil_div(K, kStepK), channel_tiles = ceil_div(N, kChannels);
+  Tiling best{16, 1};
+  double least = 0.0;
+  for (int tokens = 16; tokens <= 256; tokens *= 2) {
+    if (tokens > 16 && tokens >= 2 * M) break;
+    const int64_t tiles = channel_tiles * ceil_div(M, tokens);
+    for (int parts = 1; parts <= (int)kMostParts && parts <= steps; ++parts) {
+      const int64_t ctas = tiles * parts, rounds = ceil_div(ctas, kSms);
+      if (parts > 1 && ctas > 2 * kSms) break;
+      const double bytes = (double)ceil_div(steps, parts) * (kWeightBytes + tokens * kStepK);
+      const double stream =
+          std::max((double)rounds * bytes / 75e3, (double)ctas * bytes / 9e6);
+      const double join = parts > 1 ? 1.0 + tokens * kChannels * 4 / 15e3 : 0.0;
+      const double cost = stream + join + 0.01 * tokens * (double)rounds;
+      if (least == 0.0 || cost < least) least = cost, best = Tiling{tokens, parts};
+    }
+  }
+  return best;
+}
+
 template <int kN, typename Y>
-mb_status split_tiles(const Product& p) {
+mb_status split_tiles(const Product& p, int parts) {
   using S = Shape<kN>;
-  const int64_t tiles = ceil_div(p.N, kChannels) * ceil_div(p.M, kN);
-  const int64_t steps = ceil_div(p.K, kStepK);
-  // K parts: as many as give two CTAs an SM work (one, where their stages are
-  // too large for two), each at least eight steps: joining costs about 2 us (one
-  // token, 4096 x 4096: 13.8 us with 1 part, 10.7 with 2, 8.3 with 4, 9.0 with 8;
-  // 16 tokens, 4096 x 11008: 30.5, 21.1, 15.2 and 13.9)
+  const int64_t ctas = ceil_div(p.N, kChannels) * ceil_div(p.M, kN) * parts;
+  // as deep a ring as fits (with two CTAs an SM where there are that many and
+  // four stages fit), but not deeper than a part has steps
   constexpr int kHalf = (kMostSmem - 2048) / 2;
   constexpr bool kTwo = S::smem(std::max(4, S::kLeast)) <= kHalf;
-  int64_t parts = min64(kMostParts, min64((kTwo ? 2 : 1) * kSms / tiles, steps / 8));
-  if (parts < 2) parts = 1;
-  // as deep a ring as fits, but not deeper than a part has steps
-  int stages = ((kTwo && tiles * parts > kSms ? kHalf : kMostSmem) - 1024) / S::kStage;
-  stages = (int)min64(std::min(stages, kMaxStages), ceil_div(steps, parts));
+  int stages = ((kTwo && ctas > kSms ? kHalf : kMostSmem) - 1024) / S::kStage;
+  stages = (int)min64(std::min(stages, kMaxStages), ceil_div(ceil_div(p.K, kStepK), parts));
   if (parts > 1) stages = std::max(stages, S::kLeast);
-  return launch_tiles<kN, Y>(p, (int)parts, stages);
+  return launch_tiles<kN, Y>(p, parts, stages);
 }
 
 template <typename Y>
 mb_status dispatch(const Product& p) {
-  // pairs where their tiles give every pair of SMs work
+  // pairs where their tiles give every pair of SMs work (1500 x 4096 x 4096:
+  // 30.4 us either way; 1024: 19.2 with pairs, 18.1 without)
   if (ceil_div(p.N, 2 * kChannels) * ceil_div(p.M, kPairTokens) >= kSms / 2)
     return launch_pairs<Y>(p);
-  if (p.M <= 16) return split_tiles<16, Y>(p);
-  if (p.M <= 32) return split_tiles<32, Y>(p);
-  if (p.M <= 64) return split_tiles<64, Y>(p);
-  if (p.M <= 128) return split_tiles<128, Y>(p);
-  return split_tiles<256, Y>(p);
+  const Tiling t = tiling_for(p.M, p.N, p.K);
+  switch (t.tokens) {
+    case 16: return split_tiles<16, Y>(p, t.parts);
+    case 32: return split_tiles<32, Y>(p, t.parts);
+    case 64: return split_tiles<64, Y>(p, t.parts);
+    case 128: return split_tiles<128, Y>(p, t.parts);
+    default: return split_tiles<256, Y>(p, t.parts);
+  }
 }
 
 mb_status multiply(const int8_t* a_codes, int64_t a_stride, const float* a_scales, int64_t M,
