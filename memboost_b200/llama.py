@@ -11,6 +11,10 @@ forwards its own) and each layer's GPTQ runs with the tokens and weight rows
 split (gptq.quantize_layer_distributed): the layers stay sequential (layer
 l + 1's inputs need layer l quantized), the work inside each layer is spread.
 
+``CachedDecoder`` serves such layers: their projections in 8 bits
+(gptq.Int8Linear) and the keys and values of each layer in a quantised paged
+cache, prompts in chunks and then single tokens.
+
 No checkpoint or tokenizer exists here: layer weights are seeded N(0, 0.02^2)
 draws of the Llama shapes and the calibration hidden states seeded Gaussian
 embeddings.  The block's math is the architecture's (RMSNorm, rotary
@@ -26,7 +30,8 @@ import torch
 import torch.nn.functional as F
 
 from . import gptq
-from .ops import dequantize
+from .formats import QuantizedCache
+from .ops import cache_attention, cache_read, cache_write, dequantize
 
 
 @dataclass
@@ -90,31 +95,83 @@ def rope_tables(head_dim: int, seq_len: int, theta: float, device):
     return ang.cos(), ang.sin()
 
 
-def _rotate(x: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor) -> torch.Tensor:
+def _rotate(x: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor,
+            positions: torch.Tensor | None = None) -> torch.Tensor:
     T, half = x.shape[2], x.shape[-1] // 2
-    c, s = cos[:T][None, None], sin[:T][None, None]
+    if positions is None:
+        c, s = cos[:T][None, None], sin[:T][None, None]
+    else:  # [batch, T]
+        c, s = cos[positions][:, None], sin[positions][:, None]
     a, b = x[..., :half], x[..., half:]
     return torch.cat([a * c - b * s, b * c + a * s], dim=-1).to(x.dtype)
 
 
+@dataclass
+class CacheStep:
+    """Where the tokens of one forward pass go in a layer's cache, and what
+    they attend to.
+
+      positions   int64 [batch, T]         places of the tokens in their sequences
+      slots       int64 [batch * T]        of the cache; outside it for padding
+      page_table  int32 [batch, pages]
+      lengths     int32 [batch]            tokens of the sequences, these included
+      context     int64 [batch * tokens] or None: slots of the places 0 .. of
+                  every sequence that a chunk behind others attends to"""
+    cache: QuantizedCache
+    positions: torch.Tensor
+    slots: torch.Tensor
+    page_table: torch.Tensor
+    lengths: torch.Tensor
+    context: torch.Tensor | None = None
+
+
+def _cached_attention(cfg: LlamaConfig, q, k, v, step: CacheStep) -> torch.Tensor:
+    """Attention output [batch, T, heads * head_dim] of q, k, v [batch, T, heads,
+    head_dim], k and v stored in the cache first.  A single token attends to
+    the cache as it is held; the first chunk of a prompt to itself; a later
+    one to what the cache holds, read back."""
+    B, T, H, hd = q.shape
+    scale = 1.0 / math.sqrt(hd)
+    cache_write(step.cache, k.flatten(0, 1), v.flatten(0, 1), step.slots)
+    if T == 1:
+        y = cache_attention(q[:, 0], step.cache, step.page_table, step.lengths, scale)
+        return y.view(B, 1, H * hd)
+    mask = None
+    if step.context is not None:
+        k, v = (t.unflatten(0, (B, -1)) for t in cache_read(step.cache, step.context, q.dtype))
+        places = torch.arange(k.shape[1], device=q.device)
+        mask = (places <= step.positions[:, :, None])[:, None]
+    rep = H // k.shape[2]
+    q, k, v = (t.transpose(1, 2) for t in (q, k, v))
+    if rep > 1:
+        k, v = k.repeat_interleave(rep, dim=1), v.repeat_interleave(rep, dim=1)
+    y = F.scaled_dot_product_attention(q, k, v, attn_mask=mask, is_causal=mask is None, scale=scale)
+    return y.transpose(1, 2).reshape(B, T, -1)
+
+
 def block_forward(cfg: LlamaConfig, x: torch.Tensor, linear: dict, cos, sin,
-                  capture: dict | None = None) -> torch.Tensor:
+                  capture: dict | None = None, cache: CacheStep | None = None) -> torch.Tensor:
     """One decoder block.  ``linear``: projection name -> callable(x) -> x W^T.
     ``capture`` receives the four projection inputs whose Hessians GPTQ needs
     ("attn": q/k/v input, "o": o_proj input, "mlp": gate/up input, "down":
-    down_proj input)."""
+    down_proj input).  With ``cache`` keys and values are stored in a
+    quantised cache and attended to there."""
     B, T, _ = x.shape
     hd = cfg.n_embd // cfg.n_head
     a_in = rms_norm(x, cfg.rms_norm_eps)
     q = linear["self_attn.q_proj"](a_in).view(B, T, cfg.n_head, hd).transpose(1, 2)
     k = linear["self_attn.k_proj"](a_in).view(B, T, cfg.n_kv_heads, hd).transpose(1, 2)
     v = linear["self_attn.v_proj"](a_in).view(B, T, cfg.n_kv_heads, hd).transpose(1, 2)
-    q, k = _rotate(q, cos, sin), _rotate(k, cos, sin)
-    rep = cfg.n_head // cfg.n_kv_heads
-    if rep > 1:
-        k, v = k.repeat_interleave(rep, dim=1), v.repeat_interleave(rep, dim=1)
-    y = F.scaled_dot_product_attention(q, k, v, is_causal=T > 1, scale=1.0 / math.sqrt(hd))
-    o_in = y.transpose(1, 2).reshape(B, T, -1)
+    at = None if cache is None else cache.positions
+    q, k = _rotate(q, cos, sin, at), _rotate(k, cos, sin, at)
+    if cache is not None:
+        o_in = _cached_attention(cfg, *(t.transpose(1, 2) for t in (q, k, v)), cache)
+    else:
+        rep = cfg.n_head // cfg.n_kv_heads
+        if rep > 1:
+            k, v = k.repeat_interleave(rep, dim=1), v.repeat_interleave(rep, dim=1)
+        y = F.scaled_dot_product_attention(q, k, v, is_causal=T > 1, scale=1.0 / math.sqrt(hd))
+        o_in = y.transpose(1, 2).reshape(B, T, -1)
     x = x + linear["self_attn.o_proj"](o_in)
     m_in = rms_norm(x, cfg.rms_norm_eps)
     d_in = F.silu(linear["mlp.gate_proj"](m_in)) * linear["mlp.up_proj"](m_in)
@@ -133,6 +190,74 @@ def _fp16_linears(w: dict) -> dict:
 def _quantized_linears(q: dict) -> dict:
     deq = {k: dequantize(qt) for k, qt in q.items()}
     return {k: (lambda x, W=W: F.linear(x.to(torch.float16), W)) for k, W in deq.items()}
+
+
+class CachedDecoder:
+    """Decoder layers with projections in 8 bits and a quantised key/value
+    cache, for up to ``max_tokens`` tokens of ``batch`` sequences.
+
+    ``layers``: name -> QuantizedTensor as quantize_llama_synthetic returns
+    them ("layers.<l>.<projection>").  Calls take hidden states [batch, T,
+    n_embd] -- a prompt, chunks of it, then single tokens -- and return the last
+    layer's.  The sequences' lengths stay on the device: a single token's
+    call does not wait for it."""
+
+    def __init__(self, cfg: LlamaConfig, layers: dict, batch: int, max_tokens: int,
+                 page_size: int = 64, bits: int = 8, n_layers: int | None = None):
+        n_layers = cfg.n_layer if n_layers is None else n_layers
+        hd = cfg.n_embd // cfg.n_head
+        self.cfg, self.batch = cfg, batch
+        self.linears = [{name: gptq.Int8Linear.from_quantized(layers[f"layers.{i}.{name}"])
+                         for name in PROJECTIONS} for i in range(n_layers)]
+        device = self.linears[0][PROJECTIONS[0]].weight.device
+        pages = (max_tokens + page_size - 1) // page_size
+        self.max_tokens = pages * page_size
+        self.caches = [QuantizedCache.allocate(batch * pages, page_size, cfg.n_kv_heads, hd, bits,
+                                               device) for _ in range(n_layers)]
+        self.page_table = torch.arange(batch * pages, dtype=torch.int32,
+                                       device=device).view(batch, pages)
+        self.lengths = torch.zeros(batch, dtype=torch.int32, device=device)
+        self.cos, self.sin = rope_tables(hd, self.max_tokens, cfg.rope_theta, device)
+        self.used = 0  # tokens of the longest sequence
+
+    def slots(self, positions: torch.Tensor) -> torch.Tensor:
+        """Slots of places [batch, n] of the sequences."""
+        page = self.caches[0].page_size
+        pages = torch.gather(self.page_table.long(), 1, positions // page)
+        return pages * page + positions % page
+
+    @torch.no_grad()
+    def __call__(self, x: torch.Tensor, tokens: torch.Tensor | None = None,
+                 capture: list | None = None) -> torch.Tensor:
+        """``tokens`` (int32 [batch], default T): how many of the T places of
+        each sequence are tokens; the others are padding, which is not stored.
+        ``capture``: a dict a layer, as block_forward's."""
+        if x.dim() != 3 or x.shape[0] != self.batch or x.shape[2] != self.cfg.n_embd:
+            raise RuntimeError(f"x must be [{self.batch}, T, {self.cfg.n_embd}]")
+        T = x.shape[1]
+        if T == 0 or self.used + T > self.max_tokens:
+            raise RuntimeError(f"{T} tokens do not fit behind {self.used} of {self.max_tokens}")
+        step = torch.arange(T, device=x.device)
+        positions = self.lengths.long()[:, None] + step
+        slots = self.slots(positions)
+        if tokens is None:
+            lengths = self.lengths + T
+        else:
+            lengths = self.lengths + tokens
+            slots = torch.where(step < tokens[:, None], slots, -1)
+        context = None
+        if T > 1 and self.used > 0:
+            places = torch.arange(self.used + T, device=x.device).expand(self.batch, -1)
+            context = self.slots(places).flatten()
+        slots = slots.flatten()
+        for i, (linear, cache) in enumerate(zip(self.linears, self.caches)):
+            x = block_forward(self.cfg, x, linear, self.cos, self.sin,
+                              capture=None if capture is None else capture[i],
+                              cache=CacheStep(cache, positions, slots, self.page_table, lengths,
+                                              context))
+        self.lengths = lengths
+        self.used += T
+        return x
 
 
 def quantize_llama_synthetic(cfg: LlamaConfig, n_samples: int = 128, seq_len: int = 2048,
