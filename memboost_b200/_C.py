@@ -805,6 +805,7 @@ _DTYPES = {torch.float16: 0, torch.bfloat16: 1, torch.float32: 2}
 _DTYPES_16 = {torch.float16: 0, torch.bfloat16: 1}
 _SAME_DEVICE = contextlib.nullcontext()
 _raw_stream = torch._C._cuda_getCurrentRawStream  # torch.cuda.current_stream's handle
+_empty = torch.empty_strided  # the quickest way to a new tensor of a given layout
 
 
 def _on(index: int):
@@ -867,10 +868,8 @@ def quantize_int8(x: torch.Tensor):
     with _on(dev.index):
         x, rows, K, stride = _rows_of(x)
         pitch = (K + 15) // 16 * 16
-        codes = torch.empty((rows, pitch), dtype=torch.int8, device=dev)
-        if pitch != K:
-            codes = codes[:, :K]
-        scales = torch.empty((rows,), dtype=torch.float32, device=dev)
+        codes = _empty((rows, K), (pitch, 1), dtype=torch.int8, device=dev)
+        scales = _empty((rows,), (1,), dtype=torch.float32, device=dev)
         if rows > 0:
             _check(_lib.mb_int8_quantize(x.data_ptr(), code, rows, K, stride, codes.data_ptr(),
                                          pitch, scales.data_ptr(), _raw_stream(dev.index)))
@@ -885,7 +884,7 @@ def dequantize_int8(codes: torch.Tensor, scales: torch.Tensor, dtype: torch.dtyp
     dev = codes.device
     with _on(dev.index):
         if out is None:
-            out = torch.empty((rows, K), dtype=dtype, device=dev)
+            out = _empty((rows, K), (K, 1), dtype=dtype, device=dev)
         elif out.dtype != dtype or out.shape != codes.shape or out.device != dev \
                 or not out.is_contiguous():
             raise RuntimeError("out must be a contiguous [rows, K] tensor of dtype on the device "
@@ -924,14 +923,16 @@ def int8_matmul(x, w_codes: torch.Tensor, w_scales: torch.Tensor,
         bias_code = _dtype(bias.dtype, "bias")
         if bias.dim() != 1 or bias.shape[0] != N or bias.get_device() != dev.index:
             raise RuntimeError(f"bias must be [{N}] on the device of w")
-    shape = xs.shape[:-1] + (N,)
-    if out is not None and (out.dtype != out_dtype or out.shape != shape or out.device != dev
-                            or not out.is_contiguous()):
+    if out is not None and (out.dtype != out_dtype or out.shape != xs.shape[:-1] + (N,)
+                            or out.device != dev or not out.is_contiguous()):
         raise RuntimeError("out must be a contiguous tensor of x's leading dimensions and N "
                            "columns, of out_dtype, on the device of w")
     with _on(dev.index):
         if out is None:
-            out = torch.empty(shape, dtype=out_dtype, device=dev)
+            if xs.dim() == 2:
+                out = _empty((xs.shape[0], N), (N, 1), dtype=out_dtype, device=dev)
+            else:
+                out = torch.empty(xs.shape[:-1] + (N,), dtype=out_dtype, device=dev)
         if out.numel() == 0:
             return out
         if bias is not None:
@@ -946,7 +947,7 @@ def int8_matmul(x, w_codes: torch.Tensor, w_scales: torch.Tensor,
         else:
             x, M, _, x_stride = _rows_of(x)
             n = M * ((K + 15) // 16 * 16 + 4)  # mb_int8_linear_workspace_size
-            ws = torch.empty((n,), dtype=torch.uint8, device=dev)
+            ws = w_codes.new_empty(n)
             _check(_lib.mb_int8_linear(x.data_ptr(), x_code, x_stride, M, w_codes.data_ptr(),
                                        w_stride, w_scales.data_ptr(), N, K, bias_ptr, bias_code,
                                        out.data_ptr(), out_code, N, ws.data_ptr(), n,
@@ -1034,7 +1035,7 @@ def cache_write(cache, k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor) ->
             v = v.contiguous()
             vs = v.stride()
         n = _lib.mb_cache_write_workspace_size(tokens)
-        ws = torch.empty((n,), dtype=torch.uint8, device=dev) if n else None
+        ws = cache.k_codes.new_empty(n) if n else None
         _check(_lib.mb_cache_write(ctypes.byref(c), k.data_ptr(), ks[0], ks[1], v.data_ptr(),
                                    vs[0], vs[1], code, tokens, slots.data_ptr(),
                                    ws.data_ptr() if n else None, n, _raw_stream(dev.index)))
@@ -1047,9 +1048,9 @@ def cache_read(cache, slots: torch.Tensor, dtype: torch.dtype):
     slots = _slots(slots, dev.index)
     tokens = slots.shape[0]
     with _on(dev.index):
-        shape = (tokens, c.kv_heads, c.head_dim)
-        k = torch.empty(shape, dtype=dtype, device=dev)
-        v = torch.empty(shape, dtype=dtype, device=dev)
+        H, D = c.kv_heads, c.head_dim
+        k = _empty((tokens, H, D), (H * D, D, 1), dtype=dtype, device=dev)
+        v = torch.empty_like(k)
         if tokens > 0:
             _check(_lib.mb_cache_read(ctypes.byref(c), slots.data_ptr(), tokens, k.data_ptr(),
                                       v.data_ptr(), code, _raw_stream(dev.index)))
@@ -1078,7 +1079,7 @@ def cache_attention(q: torch.Tensor, cache, page_table: torch.Tensor, lengths: t
         raise RuntimeError("out must be a contiguous tensor of q's shape, dtype and device")
     with _on(dev.index):
         if out is None:
-            out = torch.empty(shape, dtype=q.dtype, device=dev)
+            out = torch.empty_like(q, memory_format=torch.contiguous_format)
         if batch == 0:
             return out
         qs = q.stride()
@@ -1094,7 +1095,7 @@ def cache_attention(q: torch.Tensor, cache, page_table: torch.Tensor, lengths: t
             lengths = lengths.contiguous()
         cache_ref = ctypes.byref(c)
         n = _lib.mb_cache_attention_workspace_size(cache_ref, batch, heads, width)
-        ws = torch.empty((n,), dtype=torch.uint8, device=dev) if n else None
+        ws = cache.k_codes.new_empty(n) if n else None
         _check(_lib.mb_cache_attention(cache_ref, q.data_ptr(), qs[0], qs[1], code, batch, heads,
                                        page_table.data_ptr(), table_stride, width,
                                        lengths.data_ptr(), scale, out.data_ptr(),

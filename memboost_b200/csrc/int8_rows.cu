@@ -99,7 +99,14 @@ __global__ void __launch_bounds__(kDecodeThreads)
     if (i >= total) break;
     row[h] = i / pieces;
     c0[h] = 8 * (i - row[h] * pieces);
-    q[h] = *reinterpret_cast<const uint2*>(codes + row[h] * codes_stride + c0[h]);
+    const int8_t* from = codes + row[h] * codes_stride + c0[h];
+    if (c0[h] + 8 <= K) {
+      q[h] = *reinterpret_cast<const uint2*>(from);
+    } else {  // nothing behind a row's end is read
+      q[h] = make_uint2(0u, 0u);
+      for (int e = 0; e < (int)(K - c0[h]); ++e)
+        (e < 4 ? q[h].x : q[h].y) |= (uint32_t)(uint8_t)from[e] << (8 * (e & 3));
+    }
     s[h] = scales[row[h]];
   }
 #pragma unroll
