@@ -31,8 +31,9 @@
 // minus 1152); their scale multiplies the probability, relative to a power of
 // two above every scale so far, so that the product stays in fp16's range.
 // 4-bit codes become m + s * code in fp16, one rounding; the query then is
-// fp16 too.  Probabilities are rounded to fp16 (2^-11); scores, maxima, sums
-// and the outputs' accumulators are fp32.
+// fp16 too.  Probabilities are rounded to fp16 (2^-11), and for an fp16 output,
+// whose own rounding is no larger, what that drops is multiplied too; scores,
+// maxima, sums and the outputs' accumulators are fp32.
 //
 // The running maximum is raised only when a score exceeds it by 8 (in powers
 // of two): probabilities then stay below 256 and most steps rescale nothing.
@@ -499,6 +500,7 @@ __launch_bounds__(Layout<BITS, kQuarters>::kThreads, kQuarters > 2 ? 2 : kTiles 
   int stage = 0;
   uint32_t phase = 0;
   bool ok = true;
+  const bool fine = !q.bf16;  // an fp16 output: what fp16 drops of the probabilities too
   for (uint32_t place = 0; run.more(); run.next(), place = 1) {
     const Segment& seg = run.s;
     const uint32_t kvh = seg.row / heads.blocks, h0 = (seg.row - kvh * heads.blocks) * kHeads;
@@ -754,7 +756,7 @@ __launch_bounds__(Layout<BITS, kQuarters>::kThreads, kQuarters > 2 ? 2 : kTiles 
           vs[0] = __uint_as_float(e0) * by;
           vs[1] = __uint_as_float(e1) * by;
         }
-        uint32_t pt[kTiles][2];
+        uint32_t pt[kTiles][2], low[kTiles][2] = {};
 #pragma unroll
         for (int n = 0; n < kTiles; ++n) {
           float p[4];
@@ -764,8 +766,16 @@ __launch_bounds__(Layout<BITS, kQuarters>::kThreads, kQuarters > 2 ? 2 : kTiles 
             l[n][e & 1] += p[e];
             if constexpr (BITS == 8) p[e] *= vs[e >> 1];
           }
-          pt[n][0] = transpose8x8(h2_bits(__floats2half2_rn(p[0], p[1])));
-          pt[n][1] = transpose8x8(h2_bits(__floats2half2_rn(p[2], p[3])));
+#pragma unroll
+          for (int r = 0; r < 2; ++r) {
+            const __half2 high = __floats2half2_rn(p[2 * r], p[2 * r + 1]);
+            pt[n][r] = transpose8x8(h2_bits(high));
+            if (fine) {
+              const float2 back = __half22float2(high);
+              low[n][r] = transpose8x8(
+                  h2_bits(__floats2half2_rn(p[2 * r] - back.x, p[2 * r + 1] - back.y)));
+            }
+          }
         }
 
         // ---- O^T += V^T P^T
@@ -791,8 +801,10 @@ __launch_bounds__(Layout<BITS, kQuarters>::kThreads, kQuarters > 2 ? 2 : kTiles 
                 const uint32_t a0 = code8_pair(x, 0x4140), a1 = code8_pair(x, 0x4342);
                 const uint32_t a2 = code8_pair(y, 0x4140), a3 = code8_pair(y, 0x4342);
 #pragma unroll
-                for (int n = 0; n < kTiles; ++n)
+                for (int n = 0; n < kTiles; ++n) {
                   mma_f16(o[n][p][2 * i + h], a0, a1, a2, a3, pt[n][0], pt[n][1]);
+                  if (fine) mma_f16(o[n][p][2 * i + h], a0, a1, a2, a3, low[n][0], low[n][1]);
+                }
               }
             }
           } else {
@@ -812,8 +824,10 @@ __launch_bounds__(Layout<BITS, kQuarters>::kThreads, kQuarters > 2 ? 2 : kTiles 
                 const uint32_t a2 = code4_pair<false>(y, s23, m23);
                 const uint32_t a3 = code4_pair<true>(y, s23, m23);
 #pragma unroll
-                for (int n = 0; n < kTiles; ++n)
+                for (int n = 0; n < kTiles; ++n) {
                   mma_f16(o[n][p][4 * i + h], a0, a1, a2, a3, pt[n][0], pt[n][1]);
+                  if (fine) mma_f16(o[n][p][4 * i + h], a0, a1, a2, a3, low[n][0], low[n][1]);
+                }
               }
           }
         }
