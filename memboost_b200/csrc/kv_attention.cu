@@ -141,6 +141,10 @@ struct Layout {
   // a stage: the keys' codes, the values', the keys' scales, the values'
   static constexpr int kStage = (2 * (kCodes + kScales) + 1023) / 1024 * 1024;
   static constexpr int kStages = kQuarters > 2 ? 2 : BITS == 8 ? 3 : 5;
+  // CTAs an SM: what registers and shared memory leave room for
+  __host__ __device__ static constexpr int ctas(int tiles) {
+    return kQuarters > 2 || tiles == 2 ? 2 : 3;
+  }
 
   // S^T: steps of 4 lanes x kKeyWords words; O^T: passes of 8 lanes x 16 channels
   static constexpr int kKeyWords = BITS == 4 && kQuarters == 1 ? 2 : 4;
@@ -359,7 +363,7 @@ struct Heads {
 // (maximum, sum) pairs), or 0: CTA i takes row i % rows of sequence i / rows.
 template <int BITS, int kQuarters, int kTiles>
 __global__ void
-__launch_bounds__(Layout<BITS, kQuarters>::kThreads, kQuarters > 2 ? 2 : kTiles == 1 ? 3 : 2)
+__launch_bounds__(Layout<BITS, kQuarters>::kThreads, (Layout<BITS, kQuarters>::ctas(kTiles)))
     cache_attention_kernel(const __grid_constant__ CUtensorMap k_map,
                            const __grid_constant__ CUtensorMap v_map, CacheView c,
                            uint32_t box_rows, Query q, Heads heads,
@@ -1023,21 +1027,34 @@ __global__ void __launch_bounds__(32 * kJoinWarps)
   for (int w = 0; w < kJoinWarps; ++w) top = fmaxf(top, tops[w]);
   float sum = 0.0f;
   float4 y[2] = {make_float4(0.0f, 0.0f, 0.0f, 0.0f), make_float4(0.0f, 0.0f, 0.0f, 0.0f)};
-#pragma unroll 8
-  for (uint32_t i = r.i0 + warp; i <= r.i1; i += kJoinWarps) {
-    const uint32_t at = r.slot(i, a.part_heads) + h;
-    const float2 m = ml[at];
-    const float f = exp2_fast(m.x - top);
-    sum = fmaf(m.y, f, sum);
+  constexpr int kAtOnce = 8;  // parts a warp has on the way
+  for (uint32_t i = r.i0 + warp; i <= r.i1; i += kAtOnce * kJoinWarps) {
+    float2 m[kAtOnce];
+    float4 v[kAtOnce][2];
 #pragma unroll
-    for (int x = 0; x < 2; ++x) {
-      const uint32_t ch = 4 * (lane + 32 * x);
-      if (ch >= a.dim) break;
-      const float4 v = *reinterpret_cast<const float4*>(a.parts + (uint64_t)at * a.dim + ch);
-      y[x].x = fmaf(v.x, f, y[x].x);
-      y[x].y = fmaf(v.y, f, y[x].y);
-      y[x].z = fmaf(v.z, f, y[x].z);
-      y[x].w = fmaf(v.w, f, y[x].w);
+    for (int e = 0; e < kAtOnce; ++e) {
+      const uint32_t from = i + e * kJoinWarps;
+      const uint32_t at = r.slot(min(from, r.i1), a.part_heads) + h;
+      m[e] = ml[at];
+#pragma unroll
+      for (int x = 0; x < 2; ++x)
+        v[e][x] = 4 * (lane + 32 * x) < a.dim
+                      ? *reinterpret_cast<const float4*>(a.parts + (uint64_t)at * a.dim +
+                                                         4 * (lane + 32 * x))
+                      : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    }
+#pragma unroll
+    for (int e = 0; e < kAtOnce; ++e) {
+      if (i + e * kJoinWarps > r.i1) break;
+      const float f = exp2_fast(m[e].x - top);
+      sum = fmaf(m[e].y, f, sum);
+#pragma unroll
+      for (int x = 0; x < 2; ++x) {
+        y[x].x = fmaf(v[e][x].x, f, y[x].x);
+        y[x].y = fmaf(v[e][x].y, f, y[x].y);
+        y[x].z = fmaf(v[e][x].z, f, y[x].z);
+        y[x].w = fmaf(v[e][x].w, f, y[x].w);
+      }
     }
   }
 #pragma unroll
@@ -1058,12 +1075,10 @@ __global__ void __launch_bounds__(32 * kJoinWarps)
 // else head blocks of 8 that read the codes again.
 inline uint32_t head_tiles(uint32_t group, uint32_t dim) { return group > 8 && dim <= 128 ? 2 : 1; }
 
-// Sequences of tables this narrow are taken whole.
+// Sequences of tables this narrow are taken whole, a CTA a row: nothing to join.
 constexpr int64_t kWholeTokens = 512;
-constexpr int64_t kMostCtas = 3 * 148;
-
-// CTAs that share the units, 0: one a sequence and row of heads.
-inline int64_t shares_for(int64_t most) { return most <= kWholeTokens ? 0 : kMostCtas; }
+constexpr int64_t kMostShares = 3 * 148;  // Layout::ctas an SM at most
+inline bool whole(int64_t most) { return most <= kWholeTokens; }
 
 // Rows of codes as TMA reads them: [all rows, bytes].
 bool rows_map(CUtensorMap* map, const void* codes, const CacheView& c, int bits, uint32_t box_row,
@@ -1092,8 +1107,7 @@ struct Call {
   int64_t table_stride;
   Lengths lengths;
   float scale;
-  uint32_t shares;
-  float* parts;
+  float* parts;  // null: sequences are taken whole
   void* out;
   cudaStream_t stream;
 };
@@ -1112,12 +1126,13 @@ mb_status launch(const Call& a) {
   static std::atomic<uint64_t> attr_done{0};
   MB_CUDA_TRY(set_smem_limit_once(kernel, L::kSmem, attr_done));
   const uint32_t rows = a.c.heads * a.heads.blocks;
-  const unsigned grid = a.shares > 0 ? a.shares : a.lengths.batch * rows;
+  const uint32_t shares = a.parts == nullptr ? 0 : 148 * L::ctas(kTiles);
+  const unsigned grid = shares > 0 ? shares : a.lengths.batch * rows;
   kernel<<<grid, L::kThreads, L::kSmem, a.stream>>>(k_map, v_map, a.c, box_rows, a.q, a.heads,
                                                     a.table, a.table_stride, a.lengths, a.scale,
-                                                    a.shares, a.parts, a.out);
+                                                    shares, a.parts, a.out);
   MB_LAUNCH_CHECK("cache_attention_kernel");
-  if (a.shares > 0) {
+  if (shares > 0) {
     // set up while the attention runs
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -1128,12 +1143,12 @@ mb_status launch(const Call& a) {
     cfg.stream = a.stream;
     cfg.attrs = attr;
     cfg.numAttrs = 1;
-    const Join join{a.parts,       a.shares,  (uint32_t)L::kUnit, (uint32_t)(8 * kTiles),
+    const Join join{a.parts,       shares,    (uint32_t)L::kUnit, (uint32_t)(8 * kTiles),
                     a.c.heads,     a.heads,   a.c.dim,            a.lengths,
                     a.q.bf16,      a.out};
     // Parts a row of eight and more: 1 x 100000 tokens of one key/value head 38 us
     // with the heads' kernel, 75 with the rows'; 48 x 8192 of eight 96 and 87.
-    if (a.shares >= 8 * cfg.gridDim.x) {
+    if (shares >= 8 * cfg.gridDim.x) {
       cfg.gridDim.y = std::min<uint32_t>(8 * kTiles, a.heads.group);
       MB_CUDA_TRY(cudaLaunchKernelEx(&cfg, cache_attention_join_heads_kernel, join));
     } else {
@@ -1161,10 +1176,10 @@ extern "C" size_t mb_cache_attention_workspace_size(const mb_kv_cache* cache, in
   if (cache == nullptr || cache->kv_heads <= 0 || cache->page_size <= 0 || batch <= 0 ||
       heads < cache->kv_heads || table_width <= 0)
     return 0;
-  const int64_t shares = shares_for(table_width * cache->page_size);
+  if (whole(table_width * cache->page_size)) return 0;
   const uint32_t tiles =
       head_tiles((uint32_t)(heads / cache->kv_heads), (uint32_t)cache->head_dim);
-  return (size_t)(2 * shares * 8 * tiles) * (size_t)(cache->head_dim + 2) * sizeof(float);
+  return (size_t)(2 * kMostShares * 8 * tiles) * (size_t)(cache->head_dim + 2) * sizeof(float);
 }
 
 extern "C" mb_status mb_cache_attention(const mb_kv_cache* cache, const void* q,
@@ -1208,8 +1223,7 @@ extern "C" mb_status mb_cache_attention(const mb_kv_cache* cache, const void* q,
                   table_stride,
                   Lengths{lengths, most, (uint32_t)batch},
                   scale,
-                  (uint32_t)shares_for(most),
-                  static_cast<float*>(workspace),
+                  need > 0 ? static_cast<float*>(workspace) : nullptr,
                   out,
                   reinterpret_cast<cudaStream_t>(stream_)};
   return cache->bits == 8 ? dispatch<8>(call, tiles) : dispatch<4>(call, tiles);
