@@ -411,7 +411,8 @@ mb_status mb_int8_dequantize(const int8_t* codes, int64_t codes_stride, const fl
 /* out[m, n] = a_scales[m] * b_scales[n] * sum_k a_codes[m, k] b_codes[n, k]
  *             + bias[n]
  * (bias may be NULL): a = the tokens, b = the weights (an output channel a
- * row).  The sum is a whole number and exact; it is rounded to fp32,
+ * row).  The sum is a whole number and exact (codes made by
+ * others stay within [-127, 127] too); it is rounded to fp32,
  * multiplied by the two scales and added to the bias in fp32, and rounded
  * once more to out_type.  If a wait inside the kernel ran out (2 s), the
  * outputs it concerns are NaN. */
@@ -488,7 +489,10 @@ size_t mb_cache_attention_workspace_size(const mb_kv_cache* cache, int64_t batch
  * elements (channels contiguous), out contiguous, both of `type` (fp16 or
  * bf16).  A length beyond the table counts as the table's, tokens of a page
  * outside [0, pages) are left out, and a sequence with no token gives 0.
- * scale is finite. */
+ * scale is finite; pages * kv_heads * page_size is below 2^31.  A query, key or
+ * value that is not finite gives outputs that are NaN.  If a wait inside the
+ * kernel ran out (2 s), the outputs it concerns are NaN.  workspace: 16-byte
+ * aligned. */
 mb_status mb_cache_attention(const mb_kv_cache* cache, const void* q, int64_t q_batch_stride,
                              int64_t q_head_stride, mb_dtype type, int64_t batch, int64_t heads,
                              const int32_t* page_table, int64_t table_stride,

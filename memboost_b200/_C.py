@@ -835,7 +835,7 @@ def _rows_of(x: torch.Tensor):
         if x.dim() == 2 and x.shape[0] > 1 and x.stride(0) >= K:
             return x, x.shape[0], K, x.stride(0)
         x = x.contiguous()  # rows that overlap, as an expanded tensor's
-    return x, (x.numel() // K if K > 0 else 0), K, K
+    return x, (x.numel() // K if K > 0 else x.shape[:-1].numel()), K, K
 
 
 def _int8_operand(codes: torch.Tensor, scales: torch.Tensor, name: str):
@@ -870,7 +870,9 @@ def quantize_int8(x: torch.Tensor):
         pitch = (K + 15) // 16 * 16
         codes = _empty((rows, K), (pitch, 1), dtype=torch.int8, device=dev)
         scales = _empty((rows,), (1,), dtype=torch.float32, device=dev)
-        if rows > 0:
+        if K == 0:
+            scales.zero_()
+        elif rows > 0:
             _check(_lib.mb_int8_quantize(x.data_ptr(), code, rows, K, stride, codes.data_ptr(),
                                          pitch, scales.data_ptr(), _raw_stream(dev.index)))
     return codes, scales

@@ -38,8 +38,8 @@
 // The running maximum is raised only when a score exceeds it by 8 (in powers
 // of two): probabilities then stay below 256 and most steps rescale nothing.
 //
-// The units of all sequences and heads are dealt out evenly to three CTAs an SM,
-// whatever the lengths: a CTA's share may begin and end inside a sequence.
+// The units of all sequences and heads are dealt out evenly to the resident
+// CTAs (two or three an SM), whatever the lengths: a CTA's share may begin and end inside a sequence.
 // Those parts (maximum, sum, unnormalised output) go to the workspace, two a
 // CTA at most, and a second kernel joins them in the order of the tokens, so
 // the result does not depend on the CTAs' timing.  Where the table holds few
@@ -224,8 +224,9 @@ struct Lengths {
 
 // A sequence's units of `unit` tokens, and before them one without tokens: what
 // beginning and ending a sequence's head costs.  Dealing the tokens' units
-// alone left CTAs with many short sequences behind (16 sequences of 1 .. 2048
-// tokens and 32 heads: 74 us).
+// alone leaves CTAs with many short sequences behind (16 sequences of 1 .. 2048
+// tokens and 32 heads, two CTAs of eight warps an SM: 74 us, with one such unit
+// 52, with two 44, with three 45).
 constexpr uint32_t kIdle = 2;
 __device__ __forceinline__ uint32_t units_of(int len, uint32_t unit) {
   return kIdle + ((uint32_t)len + unit - 1) / unit;
@@ -426,7 +427,10 @@ __launch_bounds__(Layout<BITS, kQuarters>::kThreads, (Layout<BITS, kQuarters>::c
                  ? table[(int64_t)s.b * table_stride + t / c.page_size]
                  : -1;
     };
-    int32_t next_page = run.more() && run.s.first() < run.s.last() ? page_of(run.s, run.s.first()) : -1;
+    const auto first_page = [&]() -> int32_t {
+      return run.more() && run.s.first() < run.s.last() ? page_of(run.s, run.s.first()) : -1;
+    };
+    int32_t next_page = first_page();
     while (run.more() && ok) {
       const Segment s = run.s;
       const uint32_t kvh = s.row / heads.blocks;
@@ -435,10 +439,7 @@ __launch_bounds__(Layout<BITS, kQuarters>::kThreads, (Layout<BITS, kQuarters>::c
         const uint32_t t = u * L::kUnit + mine;
         const uint32_t p = t / c.page_size;
         const int32_t page = next_page;
-        if (u + 1 < s.last())
-          next_page = page_of(s, u + 1);
-        else
-          next_page = run.more() && run.s.first() < run.s.last() ? page_of(run.s, run.s.first()) : -1;
+        next_page = u + 1 < s.last() ? page_of(s, u + 1) : first_page();
         const bool there = page >= 0 && page < c.pages;
         if (!mbar_wait(&empty[stage], phase)) {
           ok = false;
@@ -540,12 +541,12 @@ __launch_bounds__(Layout<BITS, kQuarters>::kThreads, (Layout<BITS, kQuarters>::c
       }
       top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
       top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
-      // 2^-p with 2^(p - 1) <= max < 2^p; 1 for zeros, NaN where the query is not finite
-      const uint32_t ex = top >> 23;
-      const bool plain = ex == 0;
-      const float down = plain ? 1.0f : __uint_as_float((253u - min(ex, 252u)) << 23);
-      float up = plain ? 1.0f : __uint_as_float((1u + min(ex, 252u)) << 23);
-      if (ex == 255) up = __uint_as_float(0x7FC00000u);
+      // down = 2^-p with 2^(p - 1) <= max < 2^p (subnormal for the largest two
+      // exponents), up = 2^(p - 8); a query below 2^-118 is taken relative to
+      // that; NaN where it is not finite
+      const uint32_t ex = min(max(top >> 23, 8u), 254u);
+      const float down = __uint_as_float(ex <= 252 ? (253 - ex) << 23 : 0x00800000u >> (ex - 252));
+      const float up = __uint_as_float(top >= 0x7F800000u ? 0x7FC00000u : (ex - 7) << 23);
 #pragma unroll
       for (int s = 0; s < L::kSteps; ++s) {
         if constexpr (BITS == 8) {
@@ -576,7 +577,7 @@ __launch_bounds__(Layout<BITS, kQuarters>::kThreads, (Layout<BITS, kQuarters>::c
 #pragma unroll
       for (int r = 0; r < 2; ++r)
         factor[n][r] = __shfl_sync(0xffffffffu, up, 4 * (2 * j + r)) * (scale * kLog2e) *
-                       (BITS == 8 ? 0x1p-14f : 1.0f);
+                       (BITS == 8 ? 0x1p-6f : 0x1p8f);
     }
 
     // o[n][p][i]: channels 16 (g + 8 p) + 2 i, + 1 of heads 2 j, 2 j + 1

@@ -307,6 +307,30 @@ def test_attention_extreme_sizes_of_values():
             _check_attention(got, q, cache, table.numpy(), n.tolist(), scale)
 
 
+def test_attention_queries_at_the_ends_of_bf16():
+    """Queries up to the largest bf16 numbers and down to the smallest, with a
+    scale that makes scores of ordinary size; one that is not finite."""
+    for bits in (8, 4):
+        cache = _filled(4, 16, 1, 64, bits, seed=9)
+        table = torch.arange(4, dtype=torch.int32).unsqueeze(0).repeat(6, 1)
+        g = torch.Generator().manual_seed(4)
+        base = torch.randn((6, 2, 64), generator=g)
+        n = torch.full((6,), 60, dtype=torch.int32)
+        for exponent in (127, 126, 125, 100, -100, -115, -125, -132):
+            q = (base / base.abs().amax(-1, keepdim=True) * 1.9).double() * 2.0 ** exponent
+            q = q.bfloat16().cuda()
+            scale = float(np.float32(2.0 ** min(-exponent, 127)))
+            got = mb.cache_attention(q, cache, table.cuda(), n.cuda(), scale=scale)
+            if exponent >= -118:  # below, the query's rounding is not relative to itself
+                _check_attention(got, q, cache, table.numpy(), n.tolist(), scale)
+            assert torch.isfinite(got).all()
+        q[1, 1, 5], q[2, 0, 7] = float("nan"), float("inf")
+        got = mb.cache_attention(q, cache, table.cuda(), n.cuda())
+        bad = torch.zeros_like(got, dtype=torch.bool)
+        bad[1, 1], bad[2, 0] = True, True
+        assert torch.equal(torch.isnan(got), bad)
+
+
 def test_attention_values_that_are_all_zero():
     for bits in (8, 4):
         cache = mb.QuantizedCache.allocate(4, 16, 1, 64, bits=bits)

@@ -99,6 +99,8 @@ def test_rows_strides(dtype):
 def test_rows_empty_and_out():
     assert mb.quantize_int8(torch.zeros((0, 40), dtype=torch.float16, device="cuda")).shape \
         == (0, 40)
+    t = mb.quantize_int8(torch.zeros((3, 2, 0), dtype=torch.float16, device="cuda"))
+    assert t.shape == (6, 0) and (t.scales == 0).all()
     t = mb.quantize_int8(_x(5, 40, torch.float16).cuda())
     out = torch.full((7, 40), 9.0, dtype=torch.float16, device="cuda")
     assert mb.dequantize_int8(t, torch.float16, out=out[1:6]).data_ptr() == out[1].data_ptr()
