@@ -16,7 +16,8 @@ namespace mb {
 namespace {
 
 // T threads a row, kPieces pieces of 8 values a thread kept in registers;
-// CTAs of max(T, 128) threads.  kWhole: rows of whole 8-value pieces that begin on 16-byte boundaries.
+// CTAs of max(T, 128) threads.  kWhole: rows of whole 8-value pieces that begin
+// on 16-byte boundaries.
 template <typename X, int T, int kPieces, bool kWhole>
 __global__ void __launch_bounds__(T < 128 ? 128 : T)
     int8_quantize_kernel(const X* __restrict__ x, int64_t rows, int64_t K, int64_t x_stride,
@@ -26,34 +27,48 @@ __global__ void __launch_bounds__(T < 128 ? 128 : T)
   constexpr int kRows = T < 128 ? 128 / T : 1;
   const int tid = threadIdx.x % T, sub = threadIdx.x / T;
   const int64_t row = (int64_t)blockIdx.x * kRows + sub;
-  if (T == 32 && row >= rows) return;  // a warp without a row
   const X* xr = x + row * x_stride;
   const int k = row < rows ? (int)K : 0, n8 = (k + 7) / 8;
 
+  // x as a whole, which a row that begins anywhere may read from
+  const uintptr_t begin = reinterpret_cast<uintptr_t>(x);
+  const uintptr_t end = begin + ((rows - 1) * x_stride + K) * (int64_t)sizeof(X);
+  const auto fetch = [&](Raw8<X>& to, int c) {
+    if constexpr (kWhole || sizeof(X) == 4)
+      to.load(xr + 8 * c, kWhole, k - 8 * c);
+    else
+      to.load_any(xr + 8 * c, k - 8 * c, begin, end);
+  };
   Raw8<X> v[kPieces];
   uint32_t m = 0;
 #pragma unroll
   for (int j = 0; j < kPieces; ++j) {
     const int c = tid + j * T;
-    if (c < n8) v[j].load(xr + 8 * c, kWhole, kWhole ? 8 : k - 8 * c);
+    if (c < n8) fetch(v[j], c);
   }
 #pragma unroll
   for (int j = 0; j < kPieces; ++j)
     if (tid + j * T < n8) m = v[j].abs_max(m);
   for (int c = tid + kPieces * T; c < n8; c += T) {
     Raw8<X> u;
-    u.load(xr + 8 * c, kWhole, kWhole ? 8 : k - 8 * c);
+    fetch(u, c);
     m = u.abs_max(m);
   }
-  m = __reduce_max_sync(0xffffffffu, Raw8<X>::abs_max_bits(m));
+  m = Raw8<X>::abs_max_bits(m);
+  if constexpr (T < 32) {
+#pragma unroll
+    for (int o = 1; o < T; o <<= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
+  } else {
+    m = __reduce_max_sync(0xffffffffu, m);
+  }
   if constexpr (T > 32) {
     __shared__ uint32_t part[kRows][T / 32];
     if ((threadIdx.x & 31) == 0) part[sub][tid / 32] = m;
     __syncthreads();
 #pragma unroll
     for (int w = 0; w < T / 32; ++w) m = max(m, part[sub][w]);
-    if (row >= rows) return;
   }
+  if (row >= rows) return;
   const RowScale r = row_scale(m);
   if (tid == 0) scales[row] = r.scale;
   int8_t* cr = codes + row * codes_stride;
@@ -75,7 +90,7 @@ __global__ void __launch_bounds__(T < 128 ? 128 : T)
   }
   for (int c = tid + kPieces * T; c < n8; c += T) {
     Raw8<X> u;
-    u.load(xr + 8 * c, kWhole, kWhole ? 8 : k - 8 * c);
+    fetch(u, c);
     put(c, u);
   }
 }
@@ -88,7 +103,7 @@ template <typename Y>
 __global__ void __launch_bounds__(kDecodeThreads)
     int8_dequantize_kernel(const int8_t* __restrict__ codes, int64_t codes_stride,
                            const float* __restrict__ scales, uint32_t pieces, uint32_t total,
-                           int64_t K, Y* __restrict__ out, int64_t out_stride, bool out_vec) {
+                           Y* __restrict__ out, int64_t out_stride) {
   const uint32_t i0 = blockIdx.x * kDecodePieces + threadIdx.x;
   uint2 q[2];
   float s[2];
@@ -99,14 +114,7 @@ __global__ void __launch_bounds__(kDecodeThreads)
     if (i >= total) break;
     row[h] = i / pieces;
     c0[h] = 8 * (i - row[h] * pieces);
-    const int8_t* from = codes + row[h] * codes_stride + c0[h];
-    if (c0[h] + 8 <= K) {
-      q[h] = *reinterpret_cast<const uint2*>(from);
-    } else {  // nothing behind a row's end is read
-      q[h] = make_uint2(0u, 0u);
-      for (int e = 0; e < (int)(K - c0[h]); ++e)
-        (e < 4 ? q[h].x : q[h].y) |= (uint32_t)(uint8_t)from[e] << (8 * (e & 3));
-    }
+    q[h] = *reinterpret_cast<const uint2*>(codes + row[h] * codes_stride + c0[h]);
     s[h] = scales[row[h]];
   }
 #pragma unroll
@@ -116,8 +124,32 @@ __global__ void __launch_bounds__(kDecodeThreads)
 #pragma unroll
     for (int e = 0; e < 8; ++e)
       v[e] = __fmul_rn((float)(int)(int8_t)((e < 4 ? q[h].x : q[h].y) >> (8 * (e & 3))), s[h]);
-    store8(out + row[h] * out_stride + c0[h], out_vec, (int)min64(8, K - c0[h]), v);
+    store8(out + row[h] * out_stride + c0[h], true, 8, v);
   }
+}
+
+// Rows whose outputs begin anywhere, or that end inside a piece: a warp takes
+// 256 values of a row, neighbouring lanes neighbouring values.
+constexpr int kDecodeValues = 8;
+template <typename Y>
+__global__ void __launch_bounds__(kDecodeThreads)
+    int8_dequantize_any_kernel(const int8_t* __restrict__ codes, int64_t codes_stride,
+                               const float* __restrict__ scales, uint32_t K, uint32_t pieces,
+                               uint32_t total, Y* __restrict__ out, int64_t out_stride) {
+  const uint32_t i = (blockIdx.x * kDecodeThreads + threadIdx.x) / 32;
+  if (i >= total) return;
+  const uint32_t row = i / pieces;
+  const uint32_t c0 = (i - row * pieces) * (32 * kDecodeValues) + threadIdx.x % 32;
+  const int8_t* from = codes + row * codes_stride + c0;
+  Y* to = out + row * out_stride + c0;
+  const float s = scales[row];
+  int8_t q[kDecodeValues];
+#pragma unroll
+  for (int e = 0; e < kDecodeValues; ++e)
+    if (c0 + 32 * e < K) q[e] = from[32 * e];
+#pragma unroll
+  for (int e = 0; e < kDecodeValues; ++e)
+    if (c0 + 32 * e < K) to[32 * e] = from_float<Y>(__fmul_rn((float)(int)q[e], s));
 }
 
 template <typename X, int T, int kPieces>
@@ -149,12 +181,14 @@ void dispatch_quantize(const void* x, int64_t rows, int64_t K, int64_t x_stride,
   // the GPU up to 256, which shorten the call (8 x 4096: 1.6 us against 4.3
   // with 32, 8192 x 4096: 18.4 us with 128, 23.4 with 256, 28.9 with 32).
   const int64_t n8 = ceil_div(K, 8);
-  int threads = 32;
+  int threads = n8 <= 32 ? 8 : 32;
   while (threads < 1024 && ceil_div(n8, threads) > 6) threads *= 2;
   if (rows < 4 * 148)
     while (threads < 256 && n8 > threads) threads *= 2;
   const int64_t pieces = ceil_div(n8, threads);
   switch (threads) {
+    case 8: return kept(integral_constant<int, 8>{}, pieces);
+    case 16: return kept(integral_constant<int, 16>{}, pieces);
     case 32: return kept(integral_constant<int, 32>{}, pieces);
     case 64: return kept(integral_constant<int, 64>{}, pieces);
     case 128: return kept(integral_constant<int, 128>{}, pieces);
@@ -216,20 +250,25 @@ extern "C" mb_status mb_int8_dequantize(const int8_t* codes, int64_t codes_strid
   MB_REQUIRE(aligned(out, dtype_size(out_type)) && aligned(scales, 4), "misaligned out or scales");
   cudaStream_t stream = reinterpret_cast<cudaStream_t>(stream_);
   const size_t size = dtype_size(out_type);
-  const bool vec = aligned(out, 16) && (rows == 1 || out_stride * size % 16 == 0);
-  const int64_t pieces = ceil_div(K, 8);
-  // a launch counts its 8-code pieces in 32 bits
-  const int64_t most = std::max<int64_t>(1, (int64_t(1) << 31) / pieces);
+  const bool whole =
+      K % 8 == 0 && aligned(out, 16) && (rows == 1 || out_stride * size % 16 == 0);
+  // a launch counts its pieces (8 values, or a warp's 256) in 32 bits, threads in 31
+  const int64_t per_row = whole ? K / 8 : ceil_div(K, 32 * kDecodeValues);
+  const int64_t most = std::max<int64_t>(1, (int64_t(1) << 30) / per_row);
   for (int64_t r0 = 0; r0 < rows; r0 += most) {
     const int64_t n = min64(most, rows - r0);
-    const uint32_t total = (uint32_t)(n * pieces);
-    const unsigned grid = (unsigned)ceil_div(total, kDecodePieces);
+    const uint32_t total = (uint32_t)(n * per_row);
     const int8_t* c = codes + r0 * codes_stride;
     uint8_t* o = static_cast<uint8_t*>(out) + (size_t)(r0 * out_stride) * size;
     const auto go = [&](auto* typed) {
-      int8_dequantize_kernel<<<grid, kDecodeThreads, 0, stream>>>(c, codes_stride, scales + r0,
-                                                       (uint32_t)pieces, total, K, typed,
-                                                       out_stride, vec);
+      if (whole)
+        int8_dequantize_kernel<<<(unsigned)ceil_div(total, kDecodePieces), kDecodeThreads, 0,
+                                 stream>>>(c, codes_stride, scales + r0, (uint32_t)per_row, total,
+                                           typed, out_stride);
+      else
+        int8_dequantize_any_kernel<<<(unsigned)ceil_div((int64_t)total * 32, kDecodeThreads),
+                                     kDecodeThreads, 0, stream>>>(
+            c, codes_stride, scales + r0, (uint32_t)K, (uint32_t)per_row, total, typed, out_stride);
     };
     if (out_type == MB_FP16)
       go(reinterpret_cast<__half*>(o));

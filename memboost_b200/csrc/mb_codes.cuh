@@ -107,6 +107,40 @@ struct Raw8 {
     }
   }
 
+  // load of a 16-bit type from any address, by the 16-byte blocks that hold the
+  // values where those lie inside [begin, end), else one by one.
+  __device__ __forceinline__ void load_any(const T* __restrict__ p, int n, uintptr_t begin,
+                                           uintptr_t end) {
+    static_assert(sizeof(T) == 2, "16-bit types");
+    n = min(n, 8);
+    const uintptr_t at = reinterpret_cast<uintptr_t>(p), low = at & ~(uintptr_t)15;
+    const uint32_t skip = (uint32_t)(at - low);  // bytes of the first block before the values
+    const bool two = skip + 2 * n > 16;
+    if (low < begin || low + (two ? 32 : 16) > end) {
+      load(p, false, n);
+      return;
+    }
+    const uint4 a = reinterpret_cast<const uint4*>(low)[0];
+    uint4 b = make_uint4(0u, 0u, 0u, 0u);
+    if (two) b = reinterpret_cast<const uint4*>(low)[1];
+    uint32_t x[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+    if (skip & 8) {
+#pragma unroll
+      for (int i = 0; i < 6; ++i) x[i] = x[i + 2];
+    }
+    if (skip & 4) {
+#pragma unroll
+      for (int i = 0; i < 5; ++i) x[i] = x[i + 1];
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      w[i] = skip & 2 ? __funnelshift_r(x[i], x[i + 1], 16) : x[i];
+      // past n: 0
+      if (2 * i >= n) w[i] = 0u;
+      if (2 * i + 1 == n) w[i] &= 0xFFFFu;
+    }
+  }
+
   __device__ __forceinline__ void floats(float (&v)[8]) const {
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
