@@ -204,6 +204,10 @@ __device__ __forceinline__ uint32_t lds32(uint32_t at) {
   return v;
 }
 
+__device__ __forceinline__ void prefetch_l1(const void* p) {
+  asm volatile("prefetch.global.L1 [%0];" ::"l"(p));
+}
+
 // Bulk copy of n bytes (a multiple of 16, both sides 16-byte aligned).
 __device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t n, uint64_t* bar) {
   asm volatile(
@@ -216,21 +220,21 @@ __device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t n
 struct Lengths {
   const int32_t* data;
   int64_t most;  // tokens the table can name
-  uint32_t batch;
+  uint32_t batch, unit, idle;
   __device__ __forceinline__ int of(uint32_t b) const {
     return (int)max64(0, min64(data[b], most));
   }
+  // Units of `unit` tokens, and before them `idle` without tokens: what
+  // beginning and ending a sequence's head costs.
+  __device__ __forceinline__ uint32_t units(int len) const {
+    return idle + ((uint32_t)len + unit - 1) / unit;
+  }
 };
 
-// A sequence's units of `unit` tokens, and before them one without tokens: what
-// beginning and ending a sequence's head costs.  Dealing the tokens' units
-// alone leaves CTAs with many short sequences behind (16 sequences of 1 .. 2048
-// tokens and 32 heads, two CTAs of eight warps an SM: 74 us, with one such unit
-// 52, with two 44, with three 45).
-constexpr uint32_t kIdle = 2;
-__device__ __forceinline__ uint32_t units_of(int len, uint32_t unit) {
-  return kIdle + ((uint32_t)len + unit - 1) / unit;
-}
+// Dealing the tokens' units alone leaves CTAs with many short sequences behind.
+// 16 sequences of 1 .. 2048 tokens, a head a group: 38 us with two idle units, 41
+// with four; 48 of 1 .. 8192, eight heads a group: 88 with two, 81 with four.
+inline uint32_t idle_units(uint32_t group) { return 2 + std::min(group, 16u) / 4; }
 
 // The units in order: sequences, in them rows (a key/value head's block of
 // query heads), in them tokens.  before(b): the units of a row of the
@@ -244,15 +248,14 @@ struct Deal {
 // The sequence that holds unit `u(total)` of all rows, found by the whole CTA
 // of kThreads.
 template <int kThreads, typename U>
-__device__ __forceinline__ Deal find_unit(const Lengths& lengths, uint32_t unit, uint32_t rows,
-                                          U&& u) {
+__device__ __forceinline__ Deal find_unit(const Lengths& lengths, uint32_t rows, U&& u) {
   constexpr int kParts = kThreads / 32;
   __shared__ unsigned long long sums[kParts], found_before, total;
   __shared__ uint32_t found_b, found_n;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   unsigned long long mine = 0;
   for (uint32_t b = threadIdx.x; b < lengths.batch; b += kThreads)
-    mine += units_of(lengths.of(b), unit);
+    mine += lengths.units(lengths.of(b));
 #pragma unroll
   for (int d = 16; d > 0; d >>= 1) mine += __shfl_xor_sync(0xffffffffu, mine, d);
   if (lane == 0) sums[warp] = mine;
@@ -268,7 +271,7 @@ __device__ __forceinline__ Deal find_unit(const Lengths& lengths, uint32_t unit,
   unsigned long long done = 0;
   for (uint32_t b0 = 0; b0 < lengths.batch; b0 += kThreads) {
     const uint32_t b = b0 + threadIdx.x;
-    const uint32_t n = b < lengths.batch ? units_of(lengths.of(b), unit) : 0;
+    const uint32_t n = b < lengths.batch ? lengths.units(lengths.of(b)) : 0;
     unsigned long long upto = n;
 #pragma unroll
     for (int d = 1; d < 32; d <<= 1) {
@@ -299,25 +302,25 @@ __device__ __forceinline__ Deal find_unit(const Lengths& lengths, uint32_t unit,
 struct Segment {
   uint32_t b, row, c0, c1;  // sequence, row, units c0 .. c1 - 1
   uint32_t n;               // units of the sequence
+  uint32_t idle;
   int len;
   // those with tokens
-  __device__ __forceinline__ uint32_t first() const { return max(c0, kIdle) - kIdle; }
-  __device__ __forceinline__ uint32_t last() const { return max(c1, kIdle) - kIdle; }
+  __device__ __forceinline__ uint32_t first() const { return max(c0, idle) - idle; }
+  __device__ __forceinline__ uint32_t last() const { return max(c1, idle) - idle; }
 };
 
 // A CTA's segments in turn.
 struct Segments {
   const Lengths* lengths;
-  uint32_t unit, rows;
+  uint32_t rows;
   unsigned long long left;  // units
   Segment s;
 
-  __device__ __forceinline__ void begin(const Lengths* all, uint32_t unit_, uint32_t rows_,
-                                        const Deal& d, unsigned long long u0,
-                                        unsigned long long u1) {
+  __device__ __forceinline__ void begin(const Lengths* all, uint32_t rows_, const Deal& d,
+                                        unsigned long long u0, unsigned long long u1) {
     lengths = all;
-    unit = unit_;
     rows = rows_;
+    s.idle = all->idle;
     left = u1 - u0;
     if (left == 0) return;
     const unsigned long long in = u0 - d.before * rows;
@@ -336,7 +339,7 @@ struct Segments {
       s.row = 0;
       ++s.b;
       s.len = lengths->of(s.b);
-      s.n = units_of(s.len, unit);
+      s.n = lengths->units(s.len);
     }
     s.c0 = 0;
     s.c1 = (uint32_t)min((unsigned long long)s.n, left);
@@ -396,7 +399,7 @@ __launch_bounds__(Layout<BITS, kQuarters>::kThreads, (Layout<BITS, kQuarters>::c
   if (shares > 0) {
     unsigned long long u0 = 0, u1 = 0;
     const Deal d = find_unit<L::kThreads>(
-        lengths, L::kUnit, rows, [&](unsigned long long total) {
+        lengths, rows, [&](unsigned long long total) {
           const unsigned long long units = total * rows, n = shares_used(units, shares);
           if (blockIdx.x < n) {
             u0 = share_begin(blockIdx.x, units, n);
@@ -404,12 +407,12 @@ __launch_bounds__(Layout<BITS, kQuarters>::kThreads, (Layout<BITS, kQuarters>::c
           }
           return u0;
         });
-    run.begin(&lengths, L::kUnit, rows, d, u0, u1);
+    run.begin(&lengths, rows, d, u0, u1);
   } else {
     const uint32_t b = blockIdx.x / rows;
-    const Deal d{0, b, units_of(lengths.of(b), L::kUnit), 0};
+    const Deal d{0, b, lengths.units(lengths.of(b)), 0};
     const unsigned long long u0 = (unsigned long long)(blockIdx.x - b * rows) * d.n;
-    run.begin(&lengths, L::kUnit, rows, d, u0, u0 + d.n);
+    run.begin(&lengths, rows, d, u0, u0 + d.n);
   }
   __syncthreads();
 
@@ -435,6 +438,16 @@ __launch_bounds__(Layout<BITS, kQuarters>::kThreads, (Layout<BITS, kQuarters>::c
       const Segment s = run.s;
       const uint32_t kvh = s.row / heads.blocks;
       run.next();
+      if (run.more()) {  // the next row's query, which the other warps want at its begin
+        const uint32_t next = run.s.row / heads.blocks, lines = (2 * c.dim + 127) / 128;
+        const uint32_t from = (run.s.row - next * heads.blocks) * kHeads;
+        for (uint32_t x = lane; x < kHeads * lines; x += 32)
+          if (from + x / lines < heads.group)
+            prefetch_l1(static_cast<const uint8_t*>(q.data) +
+                        2 * ((int64_t)run.s.b * q.batch_stride +
+                             (int64_t)(next * heads.group + from + x / lines) * q.head_stride) +
+                        128 * (x % lines));
+      }
       for (uint32_t u = s.first(); u < s.last(); ++u) {
         const uint32_t t = u * L::kUnit + mine;
         const uint32_t p = t / c.page_size;
@@ -918,7 +931,7 @@ __launch_bounds__(Layout<BITS, kQuarters>::kThreads, (Layout<BITS, kQuarters>::c
 constexpr int kJoinWarps = 8;
 struct Join {
   const float* parts;
-  uint32_t shares, unit, part_heads, kv_heads;
+  uint32_t shares, part_heads, kv_heads;
   Heads heads;
   uint32_t dim;
   Lengths lengths;
@@ -944,7 +957,7 @@ __device__ __forceinline__ Row find_row(const Join& a) {
   // units of a row before this sequence, and of all
   unsigned long long before = 0, total = 0;
   for (uint32_t i = threadIdx.x; i < a.lengths.batch; i += 32 * kJoinWarps) {
-    const uint32_t x = units_of(a.lengths.of(i), a.unit);
+    const uint32_t x = a.lengths.units(a.lengths.of(i));
     total += x;
     if (i < r.b) before += x;
   }
@@ -959,7 +972,7 @@ __device__ __forceinline__ Row find_row(const Join& a) {
   before = total = 0;
 #pragma unroll
   for (int w = 0; w < kJoinWarps; ++w) before += counts[0][w], total += counts[1][w];
-  const uint32_t n = units_of(a.lengths.of(r.b), a.unit);
+  const uint32_t n = a.lengths.units(a.lengths.of(r.b));
   const unsigned long long units = total * rows, used = shares_used(units, a.shares);
   const unsigned long long s0 = before * rows + (unsigned long long)row * n, s1 = s0 + n - 1;
   r.i0 = (uint32_t)(((s0 + 1) * used - 1) / units);
@@ -1127,10 +1140,13 @@ mb_status launch(const Call& a) {
   static std::atomic<uint64_t> attr_done{0};
   MB_CUDA_TRY(set_smem_limit_once(kernel, L::kSmem, attr_done));
   const uint32_t rows = a.c.heads * a.heads.blocks;
+  Lengths lengths = a.lengths;
+  lengths.unit = L::kUnit;
+  lengths.idle = idle_units(a.heads.group);
   const uint32_t shares = a.parts == nullptr ? 0 : 148 * L::ctas(kTiles);
   const unsigned grid = shares > 0 ? shares : a.lengths.batch * rows;
   kernel<<<grid, L::kThreads, L::kSmem, a.stream>>>(k_map, v_map, a.c, box_rows, a.q, a.heads,
-                                                    a.table, a.table_stride, a.lengths, a.scale,
+                                                    a.table, a.table_stride, lengths, a.scale,
                                                     shares, a.parts, a.out);
   MB_LAUNCH_CHECK("cache_attention_kernel");
   if (shares > 0) {
@@ -1144,9 +1160,8 @@ mb_status launch(const Call& a) {
     cfg.stream = a.stream;
     cfg.attrs = attr;
     cfg.numAttrs = 1;
-    const Join join{a.parts,       shares,    (uint32_t)L::kUnit, (uint32_t)(8 * kTiles),
-                    a.c.heads,     a.heads,   a.c.dim,            a.lengths,
-                    a.q.bf16,      a.out};
+    const Join join{a.parts, shares,  (uint32_t)(8 * kTiles), a.c.heads, a.heads,
+                    a.c.dim, lengths, a.q.bf16,               a.out};
     // Parts a row of eight and more: 1 x 100000 tokens of one key/value head 38 us
     // with the heads' kernel, 75 with the rows'; 48 x 8192 of eight 96 and 87.
     if (shares >= 8 * cfg.gridDim.x) {
@@ -1222,7 +1237,7 @@ extern "C" mb_status mb_cache_attention(const mb_kv_cache* cache, const void* q,
                   hs,
                   page_table,
                   table_stride,
-                  Lengths{lengths, most, (uint32_t)batch},
+                  Lengths{lengths, most, (uint32_t)batch, 0, 0},  // units: launch
                   scale,
                   need > 0 ? static_cast<float*>(workspace) : nullptr,
                   out,
