@@ -6,7 +6,10 @@
 // row is taken by the 2 .. 32 lanes that hold its channels, eight a lane: a
 // 16-byte load, the maximum (8 bits: of the row) or minimum and maximum (4
 // bits: of 32 channels, four lanes) by shuffles, and one 8- or 4-byte store.
-// Bound by memory: 2 bytes in and 1 or 0.63 out a value.
+// Bound by memory: 2 bytes in and 1 or 0.63 out a value; at usual sizes by the
+// chain of loads (slot, row, codes) and the launches: 2048 tokens of 8 heads of
+// 128 channels written in 11.7 us, 8000 read in 12.9 (4 bits), where their bytes
+// alone take 1.7 and 6.7.
 #include <algorithm>
 
 #include "mb_cache.cuh"
