@@ -213,6 +213,7 @@ extern "C" mb_status mb_int8_quantize(const void* x, mb_dtype x_type, int64_t ro
   MB_REQUIRE(rows < (int64_t(1) << 31), "too many rows");
   MB_REQUIRE(K < (int64_t(1) << 31) - 8192, "K too large");
   MB_REQUIRE(rows == 1 || codes_stride >= K, "codes_stride must be at least K");
+  MB_REQUIRE(rows == 1 || x_stride >= 0, "x_stride must not be negative");
   MB_REQUIRE(aligned(codes, 16) && codes_stride % 16 == 0,
              "codes must begin on 16-byte boundaries");
   MB_REQUIRE(aligned(x, dtype_size(x_type)) && aligned(scales, 4), "misaligned x or scales");

@@ -230,13 +230,20 @@ class CachedDecoder:
     def __call__(self, x: torch.Tensor, tokens: torch.Tensor | None = None,
                  capture: list | None = None) -> torch.Tensor:
         """``tokens`` (int32 [batch], default T): how many of the T places of
-        each sequence are tokens; the others are padding, which is not stored.
+        each sequence are tokens (0 .. T, others count as the nearer of these);
+        the others are padding, which is not stored.
         ``capture``: a dict a layer, as block_forward's."""
         if x.dim() != 3 or x.shape[0] != self.batch or x.shape[2] != self.cfg.n_embd:
             raise RuntimeError(f"x must be [{self.batch}, T, {self.cfg.n_embd}]")
         T = x.shape[1]
         if T == 0 or self.used + T > self.max_tokens:
             raise RuntimeError(f"{T} tokens do not fit behind {self.used} of {self.max_tokens}")
+        if tokens is not None:
+            if tokens.shape != self.lengths.shape or tokens.dtype != torch.int32 \
+                    or tokens.device != self.lengths.device:
+                raise RuntimeError(f"tokens must be int32 [{self.batch}] on the device of the "
+                                   "caches")
+            tokens = tokens.clamp(0, T)  # places index tables behind a length
         step = torch.arange(T, device=x.device)
         positions = self.lengths.long()[:, None] + step
         slots = self.slots(positions)

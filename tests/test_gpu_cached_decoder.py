@@ -115,3 +115,19 @@ def test_decoder_refusals():
     dec(torch.zeros((2, 32, 256), dtype=torch.float16, device="cuda"))
     with pytest.raises(RuntimeError, match="do not fit"):
         dec(torch.zeros((2, 1, 256), dtype=torch.float16, device="cuda"))
+
+
+def test_counts_of_tokens_outside_the_chunk():
+    """Counts beyond the chunk count as the whole of it, negative ones as none,
+    so a sequence's end stays within its pages; other types are refused."""
+    dec = llama.CachedDecoder(CFG, _layers(CFG), batch=3, max_tokens=16, page_size=16, n_layers=1)
+    for bad in (torch.tensor([1, 1, 1]).cuda(), torch.ones(2, dtype=torch.int32).cuda(),
+                torch.ones(3, dtype=torch.int32)):
+        with pytest.raises(RuntimeError, match="tokens must be int32"):
+            dec(torch.zeros((3, 4, 256), dtype=torch.float16, device="cuda"), bad)
+    x = torch.randn((3, 4, 256), generator=torch.Generator().manual_seed(0)).half().cuda()
+    dec(x, torch.tensor([2, 4, 0], dtype=torch.int32).cuda())
+    dec(x, torch.tensor([5, 2 ** 31 - 1, -3], dtype=torch.int32).cuda())
+    assert dec.lengths.tolist() == [6, 8, 0]
+    y = dec(x[:, :1])
+    assert dec.lengths.tolist() == [7, 9, 1] and torch.isfinite(y).all()

@@ -115,7 +115,7 @@ def _refused(status, words):
     (dict(x=None), "null"), (dict(t=3), "unknown type"), (dict(rows=0), "positive"),
     (dict(K=-1), "positive"), (dict(cs=31), "codes_stride must be at least"),
     (dict(cs=40), "16-byte"), (dict(codes=P + 8), "16-byte"), (dict(x=P + 1), "misaligned"),
-    (dict(rows=1 << 31), "too many rows"),
+    (dict(rows=1 << 31), "too many rows"), (dict(xs=-32), "x_stride must not be negative"),
 ])
 def test_quantize_entry_refusals(change, words):
     a = dict(x=P, t=0, rows=2, K=32, xs=32, codes=P, cs=32, scales=P)
