@@ -26,6 +26,8 @@ if not os.path.exists(_LIB_PATH):
 
 _lib = ctypes.CDLL(_LIB_PATH)
 
+from . import _calls  # noqa: E402  (csrc/calls.cpp, built beside the library)
+
 _P = ctypes.c_void_p
 _I64 = ctypes.c_int64
 _lib.mb_last_error.restype = ctypes.c_char_p
@@ -797,9 +799,10 @@ class QuantizeBatch:
 # ---- 8-bit rows and their product; quantised key/value cache ----
 #
 # A call of these takes a few microseconds on the GPU, so the host's side of it
-# is kept short: the checks are attribute comparisons whose messages are put
-# together only where one fails, pointers go to ctypes as integers, the stream
-# is read as a handle and the device is only switched where it has to be.
+# is kept short.  The usual call -- contiguous tensors of the current device,
+# outputs to be made -- goes through csrc/calls.cpp as a whole, which returns None
+# for any other; that one is checked, brought into the entries' layouts or
+# refused here.
 
 _DTYPES = {torch.float16: 0, torch.bfloat16: 1, torch.float32: 2}
 _DTYPES_16 = {torch.float16: 0, torch.bfloat16: 1}
@@ -861,6 +864,9 @@ def _int8_operand(codes: torch.Tensor, scales: torch.Tensor, name: str):
 def quantize_int8(x: torch.Tensor):
     """(codes, scales) of the rows of x ([..., K], the leading dimensions
     flattened), by ``mb_int8_quantize``."""
+    made = _calls.quantize_int8(x)
+    if made is not None:
+        return made
     code = _dtype(x.dtype, "x")
     if not x.is_cuda:
         raise RuntimeError("x must be on CUDA")
@@ -880,6 +886,10 @@ def quantize_int8(x: torch.Tensor):
 
 def dequantize_int8(codes: torch.Tensor, scales: torch.Tensor, dtype: torch.dtype,
                     out: torch.Tensor | None = None) -> torch.Tensor:
+    if out is None:
+        made = _calls.dequantize_int8(codes, scales, dtype)
+        if made is not None:
+            return made
     scales, stride = _int8_operand(codes, scales, "t")
     code = _dtype(dtype, "dtype")
     rows, K = codes.shape
@@ -902,11 +912,15 @@ def int8_matmul(x, w_codes: torch.Tensor, w_scales: torch.Tensor,
                 out: torch.Tensor | None = None) -> torch.Tensor:
     """[..., N] = x W^T + bias; x a floating tensor [..., K] (``mb_int8_linear``
     quantises its rows) or a pair (codes, scales) (``mb_int8_matmul``)."""
+    given = type(x) is tuple
+    xs = x[0] if given else x
+    if out is None:
+        made = _calls.int8_matmul(xs, x[1] if given else None, w_codes, w_scales, bias, out_dtype)
+        if made is not None:
+            return made
     w_scales, w_stride = _int8_operand(w_codes, w_scales, "w")
     N, K = w_codes.shape
     dev = w_codes.device
-    given = type(x) is tuple
-    xs = x[0] if given else x
     if xs.get_device() != dev.index:
         raise RuntimeError("x must be on the device of w")
     if xs.dim() == 0 or xs.shape[-1] != K:
@@ -1011,6 +1025,9 @@ def _slots(slots: torch.Tensor, dev: int) -> torch.Tensor:
 
 
 def cache_write(cache, k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor) -> None:
+    if _calls.cache_write(cache.k_codes, cache.v_codes, cache.k_scales, cache.v_scales, k, v,
+                          slots):
+        return
     c = _cache_struct(cache)
     dev = cache.k_codes.device
     code = _dtype(k.dtype, "k", _DTYPES_16)
@@ -1044,6 +1061,10 @@ def cache_write(cache, k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor) ->
 
 
 def cache_read(cache, slots: torch.Tensor, dtype: torch.dtype):
+    made = _calls.cache_read(cache.k_codes, cache.v_codes, cache.k_scales, cache.v_scales, slots,
+                             dtype)
+    if made is not None:
+        return made
     c = _cache_struct(cache)
     dev = cache.k_codes.device
     code = _dtype(dtype, "dtype")
@@ -1061,6 +1082,11 @@ def cache_read(cache, slots: torch.Tensor, dtype: torch.dtype):
 
 def cache_attention(q: torch.Tensor, cache, page_table: torch.Tensor, lengths: torch.Tensor,
                     scale: float, out: torch.Tensor | None = None) -> torch.Tensor:
+    if out is None:
+        made = _calls.cache_attention(cache.k_codes, cache.v_codes, cache.k_scales, cache.v_scales,
+                                      q, page_table, lengths, scale)
+        if made is not None:
+            return made
     c = _cache_struct(cache)
     dev = cache.k_codes.device
     code = _dtype(q.dtype, "q", _DTYPES_16)

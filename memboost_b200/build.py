@@ -1,10 +1,12 @@
-"""Build memboost_b200/libmemboost_b200.so from memboost_b200/csrc/*.cu.
+"""Build memboost_b200/libmemboost_b200.so from memboost_b200/csrc/*.cu, and
+memboost_b200/_calls.so from csrc/calls.cpp.
 
 Every translation unit is compiled for sm_100a only
 (-gencode arch=compute_100a,code=sm_100a) with -lineinfo, and linked into one
 shared library with a statically linked CUDA runtime.  The library exports
 exactly the C ABI declared in include/memboost_b200.h.  nvcc cross-compiles,
-so this runs on machines without a GPU.
+so this runs on machines without a GPU.  _calls.so is a CPython module over
+torch's tensors that calls the library.
 
 Usage: python memboost_b200/build.py [--force] [-v]
 (run by path: importing the package needs the library this builds)
@@ -13,10 +15,12 @@ from __future__ import annotations
 
 import concurrent.futures as cf
 import glob
+import importlib.util
 import os
 import shutil
 import subprocess
 import sys
+import sysconfig
 
 PKG = os.path.dirname(os.path.abspath(__file__))
 ROOT = os.path.dirname(PKG)
@@ -24,6 +28,7 @@ CSRC = os.path.join(PKG, "csrc")
 INCLUDE = os.path.join(ROOT, "include")
 BUILD = os.path.join(PKG, "_build")
 LIB = os.path.join(PKG, "libmemboost_b200.so")
+CALLS = os.path.join(PKG, "_calls.so")
 
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 NVCC_FLAGS = ["-O3", "-std=c++17", "-lineinfo", "-Xcompiler", "-fPIC", "-Xcompiler", "-O3",
@@ -64,6 +69,30 @@ def _compile(src: str, verbose: bool) -> str:
     return obj
 
 
+def _build_calls(verbose: bool) -> None:
+    src = os.path.join(CSRC, "calls.cpp")
+    if not _stale(CALLS, [src, __file__, os.path.join(INCLUDE, "memboost_b200.h")]):
+        return
+    torch = importlib.util.find_spec("torch").submodule_search_locations[0]
+    system = [os.path.join(torch, "include"),
+              os.path.join(torch, "include", "torch", "csrc", "api", "include"),
+              sysconfig.get_paths()["include"],
+              os.path.join(os.environ.get("CUDA_HOME", "/usr/local/cuda"), "include")]
+    tmp = CALLS + ".tmp"
+    cmd = [os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-fPIC", "-shared", "-I", INCLUDE]
+    for d in system:
+        cmd += ["-isystem", d]
+    cmd += [src, "-o", tmp, "-L", PKG, "-l:libmemboost_b200.so", "-L", os.path.join(torch, "lib"),
+            "-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch_cuda", "-ltorch_python",
+            "-Wl,-rpath,$ORIGIN"]
+    if verbose:
+        print(" ".join(cmd), flush=True)
+    r = subprocess.run(cmd, capture_output=True, text=True)
+    if r.returncode != 0:
+        raise RuntimeError(f"building {CALLS} failed:\n{r.stdout}\n{r.stderr}")
+    os.replace(tmp, CALLS)
+
+
 def build(force: bool = False, verbose: bool = False) -> str:
     os.makedirs(BUILD, exist_ok=True)
     srcs = _sources()
@@ -81,6 +110,9 @@ def build(force: bool = False, verbose: bool = False) -> str:
         if r.returncode != 0:
             raise RuntimeError(f"link failed:\n{r.stdout}\n{r.stderr}")
         os.replace(tmp, LIB)
+    if force and os.path.exists(CALLS):
+        os.remove(CALLS)
+    _build_calls(verbose)
     return LIB
 
 

@@ -435,3 +435,36 @@ def test_offsets_past_32_bits(bits):
     out = mb.cache_attention(q, cache, table, m)
     assert torch.equal(out, mb.cache_attention(q, last, table * 0, m))
     _check_attention(out, q, last, np.zeros((1, 1), np.int32), [256], 1 / 16)
+
+
+@pytest.mark.parametrize("bits", [8, 4])
+def test_every_way_into_a_cache_call_agrees(bits):
+    """Strided keys, slots, tables, lengths and queries, subclasses and given
+    outputs: what the cache holds and the attention are the same."""
+    cache, other = (mb.QuantizedCache.allocate(5, 16, 2, 64, bits=bits) for _ in range(2))
+    k, v = _kv(70, 2, 64, torch.float16, seed=3)
+    slots = torch.randperm(80, generator=torch.Generator().manual_seed(1))[:70].cuda()
+    mb.cache_write(cache, k, v, slots)
+    mb.cache_write(other, torch.stack([k, v], -1)[..., 0], torch.nn.Parameter(v),
+                   torch.stack([slots, slots], 1)[:, 0])
+    for a, b in zip((cache.k_codes, cache.v_codes, cache.k_scales, cache.v_scales),
+                    (other.k_codes, other.v_codes, other.k_scales, other.v_scales)):
+        assert torch.equal(a, b)
+    read = mb.cache_read(cache, slots)
+    again = mb.cache_read(cache, torch.stack([slots, slots], 1)[:, 0])
+    assert all(torch.equal(a, b) for a, b in zip(read, again))
+    q = torch.randn((3, 4, 64), generator=torch.Generator().manual_seed(2)).half().cuda()
+    table = torch.tensor([[0, 1, 2, 3, 4], [4, 3, 2, 1, 0], [2, 2, 2, 2, 2]], dtype=torch.int32).cuda()
+    lengths = torch.tensor([80, 33, 0], dtype=torch.int32).cuda()
+    want = mb.cache_attention(q, cache, table, lengths)
+    out = torch.empty_like(want)
+    for args in ((q, cache, table, lengths, 0.125, out),
+                 (torch.stack([q, q], -1)[..., 0], cache, table, lengths),
+                 (torch.nn.Parameter(q), cache, table, lengths),
+                 (q, cache, table.t().contiguous().t(), torch.stack([lengths, lengths], 1)[:, 0]),
+                 (q, cache, table, lengths, torch.tensor(0.125).item()),
+                 (torch.stack([q, q], 1)[:, 0], cache, table, lengths)):
+        got = mb.cache_attention(*args)
+        assert torch.equal(got, want) and not got.requires_grad
+    assert torch.equal(mb.cache_attention(q, cache, table, lengths, 0),
+                       mb.cache_attention(q, cache, table, lengths, 0.0))

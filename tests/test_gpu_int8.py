@@ -273,3 +273,52 @@ def test_int8_linear_from_a_quantized_weight():
     w8 = mb.quantize_int8(mb.dequantize(qt))
     assert torch.equal(y, mb.int8_matmul(x, w8))
     _check_product(y.view(10, 96), mb.quantize_int8(x), w8)
+
+
+class _Subclass(torch.Tensor):
+    pass
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16, torch.float32])
+def test_every_way_into_a_call_agrees(dtype):
+    """Parameters, subclasses, transposed and strided tensors, leading dimensions,
+    a stride of one row, given outputs: the same codes and products."""
+    g = torch.Generator().manual_seed(11)
+    x = torch.randn((6, 80), generator=g).to(dtype).cuda()
+    w = mb.quantize_int8(torch.randn((24, 80), generator=g).cuda())
+    bias = torch.randn(24, generator=g).cuda()
+    a = mb.quantize_int8(x)
+    want = mb.int8_matmul(x, w, bias)
+    assert want.dtype == dtype
+    wide = torch.zeros((6, 100), dtype=dtype, device="cuda")
+    wide[:, :80] = x
+    for same in (torch.nn.Parameter(x), x.as_subclass(_Subclass), x.t().contiguous().t(),
+                 wide[:, :80], x.view(2, 3, 80), x.view(1, 6, 1, 80), wide.double()[:, :80].to(dtype)):
+        b = mb.quantize_int8(same)
+        assert torch.equal(a.codes, b.codes) and torch.equal(a.scales, b.scales)
+        y = mb.int8_matmul(same, w, bias)
+        assert y.shape == same.shape[:-1] + (24,) and not y.requires_grad
+        assert torch.equal(y.reshape(6, 24), want)
+        assert torch.equal(mb.int8_matmul(same, w, torch.stack([bias, bias], 1)[:, 0]).reshape(6, 24),
+                           want)
+        out = torch.empty_like(want).view(y.shape)
+        assert mb.int8_matmul(same, w, bias, out=out) is out and torch.equal(out, y)
+    for to in (torch.float16, torch.bfloat16, torch.float32):
+        out = torch.empty((6, 80), dtype=to, device="cuda")
+        assert torch.equal(mb.dequantize_int8(a, to), mb.dequantize_int8(a, to, out=out))
+        y = mb.int8_matmul(a, w, bias, out_dtype=to)
+        assert y.dtype == to and torch.equal(y, mb.int8_matmul(x, w, bias, out_dtype=to))
+    assert mb.int8_matmul(a, w).dtype == torch.float16
+    # the rows of another scales' tensor, and one row of many
+    spread = torch.stack([a.scales, a.scales], 1)[:, 0]
+    assert torch.equal(mb.dequantize_int8(mb.Int8Tensor(a.codes, spread)), mb.dequantize_int8(a))
+    one = mb.quantize_int8(x[2:3])
+    assert torch.equal(one.codes[0], a.codes[2]) and torch.equal(one.scales, a.scales[2:3])
+    assert torch.equal(mb.int8_matmul(x[2:3], w, bias), want[2:3])
+
+
+def test_allocation_failures_are_torch_errors():
+    w = mb.quantize_int8(torch.zeros((1 << 20, 16), device="cuda"))
+    x = torch.zeros((1 << 22, 16), dtype=torch.float16, device="cuda")
+    with pytest.raises(torch.OutOfMemoryError):  # 8 TB of outputs
+        mb.int8_matmul(x, w)

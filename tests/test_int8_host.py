@@ -205,3 +205,28 @@ def test_cache_entry_refusals():
     _refused(at(r, P, 128, 64, 0, 1, 2, P, 1, -1, P, 1.0, P, None, 0, None), "table_width")
     _refused(at(r, P, 128, 64, 0, 1, 2, None, 1, 1, P, 1.0, P, None, 0, None), "null")
     _refused(at(r, P, 128, 64, 0, 1, 2, P, 1, 1, P, float("inf"), P, None, 0, None), "finite")
+
+
+def test_calls_leave_the_unusual_alone(mb):
+    """The native form of the calls takes ordinary CUDA tensors only; it
+    returns None, and does nothing, for all else."""
+    from memboost_b200 import _calls
+    x = torch.zeros(2, 16)
+    codes, scales = torch.zeros(2, 16, dtype=torch.int8), torch.zeros(2)
+    cache = mb.QuantizedCache.allocate(1, 16, 1, 64, device="cpu")
+    parts = (cache.k_codes, cache.v_codes, cache.k_scales, cache.v_scales)
+    slots = torch.zeros(1, dtype=torch.int64)
+    kv = torch.zeros(1, 1, 64, dtype=torch.float16)
+    table, lengths = torch.zeros(1, 1, dtype=torch.int32), torch.zeros(1, dtype=torch.int32)
+    for fn, args in ((_calls.quantize_int8, (x,)),
+                     (_calls.dequantize_int8, (codes, scales, torch.float16)),
+                     (_calls.int8_matmul, (x, None, codes, scales, None, None)),
+                     (_calls.int8_matmul, (codes, scales, codes, scales, None, None)),
+                     (_calls.cache_write, parts + (kv, kv, slots)),
+                     (_calls.cache_read, parts + (slots, torch.float16)),
+                     (_calls.cache_attention, parts + (kv, table, lengths, 1.0))):
+        assert fn(*args) is None
+        assert fn() is None and fn(*args[:-1]) is None and fn(*args, None) is None
+        for i in range(len(args)):
+            for other in (None, 1, "x", torch.float64, torch.zeros(0)):
+                assert fn(*args[:i], other, *args[i + 1:]) is None
