@@ -23,7 +23,10 @@ __global__ void __launch_bounds__(T < 128 ? 128 : T)
     int8_quantize_kernel(const X* __restrict__ x, int64_t rows, int64_t K, int64_t x_stride,
                          int8_t* __restrict__ codes, int64_t codes_stride,
                          float* __restrict__ scales) {
-  grid_launch_dependents();  // a product behind this may begin with its weights
+  // in this order: a product behind this may begin with its weights, which the
+  // kernel before may have written
+  grid_dependency_wait();
+  grid_launch_dependents();
   constexpr int kRows = T < 128 ? 128 / T : 1;
   const int tid = threadIdx.x % T, sub = threadIdx.x / T;
   const int64_t row = (int64_t)blockIdx.x * kRows + sub;
@@ -104,6 +107,7 @@ __global__ void __launch_bounds__(kDecodeThreads)
     int8_dequantize_kernel(const int8_t* __restrict__ codes, int64_t codes_stride,
                            const float* __restrict__ scales, uint32_t pieces, uint32_t total,
                            Y* __restrict__ out, int64_t out_stride) {
+  grid_dependency_wait();
   const uint32_t i0 = blockIdx.x * kDecodePieces + threadIdx.x;
   uint2 q[2];
   float s[2];
@@ -136,6 +140,7 @@ __global__ void __launch_bounds__(kDecodeThreads)
     int8_dequantize_any_kernel(const int8_t* __restrict__ codes, int64_t codes_stride,
                                const float* __restrict__ scales, uint32_t K, uint32_t pieces,
                                uint32_t total, Y* __restrict__ out, int64_t out_stride) {
+  grid_dependency_wait();
   const uint32_t i = (blockIdx.x * kDecodeThreads + threadIdx.x) / 32;
   if (i >= total) return;
   const uint32_t row = i / pieces;
@@ -158,8 +163,8 @@ void launch_quantize(const void* x, int64_t rows, int64_t K, int64_t x_stride, b
   constexpr int kThreads = T < 128 ? 128 : T;
   const unsigned grid = (unsigned)ceil_div(rows, kThreads / T);
   const auto go = [&](auto kernel) {
-    kernel<<<grid, kThreads, 0, stream>>>(static_cast<const X*>(x), rows, K, x_stride, codes,
-                                          codes_stride, scales);
+    launch_dependent(kernel, grid, kThreads, 0, stream, static_cast<const X*>(x), rows, K, x_stride,
+                     codes, codes_stride, scales);
   };
   whole ? go(int8_quantize_kernel<X, T, kPieces, true>)
         : go(int8_quantize_kernel<X, T, kPieces, false>);
@@ -263,13 +268,14 @@ extern "C" mb_status mb_int8_dequantize(const int8_t* codes, int64_t codes_strid
     uint8_t* o = static_cast<uint8_t*>(out) + (size_t)(r0 * out_stride) * size;
     const auto go = [&](auto* typed) {
       if (whole)
-        int8_dequantize_kernel<<<(unsigned)ceil_div(total, kDecodePieces), kDecodeThreads, 0,
-                                 stream>>>(c, codes_stride, scales + r0, (uint32_t)per_row, total,
-                                           typed, out_stride);
+        launch_dependent(int8_dequantize_kernel<std::remove_pointer_t<decltype(typed)>>,
+                         (unsigned)ceil_div(total, kDecodePieces), kDecodeThreads, 0, stream, c,
+                         codes_stride, scales + r0, (uint32_t)per_row, total, typed, out_stride);
       else
-        int8_dequantize_any_kernel<<<(unsigned)ceil_div((int64_t)total * 32, kDecodeThreads),
-                                     kDecodeThreads, 0, stream>>>(
-            c, codes_stride, scales + r0, (uint32_t)K, (uint32_t)per_row, total, typed, out_stride);
+        launch_dependent(int8_dequantize_any_kernel<std::remove_pointer_t<decltype(typed)>>,
+                         (unsigned)ceil_div((int64_t)total * 32, kDecodeThreads), kDecodeThreads, 0,
+                         stream, c, codes_stride, scales + r0, (uint32_t)K, (uint32_t)per_row,
+                         total, typed, out_stride);
     };
     if (out_type == MB_FP16)
       go(reinterpret_cast<__half*>(o));

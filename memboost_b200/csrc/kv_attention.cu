@@ -380,7 +380,6 @@ __launch_bounds__(Layout<BITS, kQuarters>::kThreads, (Layout<BITS, kQuarters>::c
                            const int32_t* __restrict__ table, int64_t table_stride,
                            const __grid_constant__ Lengths lengths, float scale, uint32_t shares,
                            float* __restrict__ parts, void* __restrict__ out) {
-  grid_launch_dependents();
   using L = Layout<BITS, kQuarters>;
   constexpr int kHeads = 8 * kTiles;
   extern __shared__ uint8_t raw[];
@@ -401,6 +400,9 @@ __launch_bounds__(Layout<BITS, kQuarters>::kThreads, (Layout<BITS, kQuarters>::c
     }
     fence_mbar_init();
   }
+  // in this order: the joining kernel reads the lengths before it waits
+  grid_dependency_wait();
+  grid_launch_dependents();
   Segments run;
   if (shares > 0) {
     unsigned long long u0 = 0, u1 = 0;
@@ -991,8 +993,8 @@ __device__ __forceinline__ Row find_row(const Join& a) {
 __global__ void __launch_bounds__(32 * kJoinWarps)
     cache_attention_join_rows_kernel(const __grid_constant__ Join a) {
   const Row r = find_row(a);
+  grid_dependency_wait();  // by CTAs without work too: their end is the call's
   if (r.i0 == r.i1) return;
-  grid_dependency_wait();
   const uint32_t here = min(a.part_heads, a.heads.group - r.h0);
   const float2* ml =
       reinterpret_cast<const float2*>(a.parts + (uint64_t)2 * a.shares * a.part_heads * a.dim);
@@ -1033,8 +1035,8 @@ __global__ void __launch_bounds__(32 * kJoinWarps)
   __shared__ __align__(16) float so[kJoinWarps][256];
   const Row r = find_row(a);
   const uint32_t h = blockIdx.y, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  if (r.i0 == r.i1 || r.h0 + h >= a.heads.group) return;
   grid_dependency_wait();
+  if (r.i0 == r.i1 || r.h0 + h >= a.heads.group) return;
   const float2* ml =
       reinterpret_cast<const float2*>(a.parts + (uint64_t)2 * a.shares * a.part_heads * a.dim);
   float top = kLowest;
@@ -1151,31 +1153,20 @@ mb_status launch(const Call& a) {
   lengths.idle = idle_units(a.heads.group);
   const uint32_t shares = a.parts == nullptr ? 0 : 148 * L::ctas(kTiles);
   const unsigned grid = shares > 0 ? shares : a.lengths.batch * rows;
-  kernel<<<grid, L::kThreads, L::kSmem, a.stream>>>(k_map, v_map, a.c, box_rows, a.q, a.heads,
-                                                    a.table, a.table_stride, lengths, a.scale,
-                                                    shares, a.parts, a.out);
-  MB_LAUNCH_CHECK("cache_attention_kernel");
+  MB_CUDA_TRY(launch_dependent(kernel, grid, L::kThreads, L::kSmem, a.stream, k_map, v_map, a.c,
+                               box_rows, a.q, a.heads, a.table, a.table_stride, lengths, a.scale,
+                               shares, a.parts, a.out));
   if (shares > 0) {
-    // set up while the attention runs
-    cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[0].val.programmaticStreamSerializationAllowed = 1;
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(a.lengths.batch * rows);
-    cfg.blockDim = dim3(32 * kJoinWarps);
-    cfg.stream = a.stream;
-    cfg.attrs = attr;
-    cfg.numAttrs = 1;
+    dim3 joins(a.lengths.batch * rows);
     const Join join{a.parts, shares,  (uint32_t)(8 * kTiles), a.c.heads, a.heads,
                     a.c.dim, lengths, a.q.bf16,               a.out};
     // Parts a row of eight and more: 1 x 100000 tokens of one key/value head 38 us
     // with the heads' kernel, 75 with the rows'; 48 x 8192 of eight 96 and 87.
-    if (shares >= 8 * cfg.gridDim.x) {
-      cfg.gridDim.y = std::min<uint32_t>(8 * kTiles, a.heads.group);
-      MB_CUDA_TRY(cudaLaunchKernelEx(&cfg, cache_attention_join_heads_kernel, join));
-    } else {
-      MB_CUDA_TRY(cudaLaunchKernelEx(&cfg, cache_attention_join_rows_kernel, join));
-    }
+    const bool by_heads = shares >= 8 * joins.x;
+    if (by_heads) joins.y = std::min<uint32_t>(8 * kTiles, a.heads.group);
+    MB_CUDA_TRY(launch_dependent(
+        by_heads ? cache_attention_join_heads_kernel : cache_attention_join_rows_kernel, joins,
+        32 * kJoinWarps, 0, a.stream, join));
   }
   return MB_OK;
 }

@@ -115,7 +115,8 @@ __global__ void __launch_bounds__(kThreads)
     cache_rows_kernel(CacheView c, const int64_t* __restrict__ slots, uint32_t tokens,
                       const unsigned long long* __restrict__ table, uint32_t mask,
                       int64_t* __restrict__ rows) {
-  grid_launch_dependents();
+  grid_dependency_wait();
+  grid_launch_dependents();  // the writing kernel begins with the values
   if (table != nullptr) {
     const uint32_t t = blockIdx.x * kThreads + threadIdx.x;
     if (t >= tokens) return;
@@ -156,6 +157,7 @@ __global__ void __launch_bounds__(kThreads)
   __shared__ uint32_t mine[kMostTokens];
   const uint32_t t0 = blockIdx.x * cut.tokens, here = min(cut.tokens, tokens - t0);
   const uint32_t lanes = (here * 2 * cut.heads) << cut.shift;
+  if (first_rows == nullptr) grid_dependency_wait();
   // the values are on the way while the slots are looked at
   Raw8<X> raw[kTurns];
 #pragma unroll
@@ -243,6 +245,7 @@ __global__ void __launch_bounds__(kThreads)
                       Y* __restrict__ k_out, Y* __restrict__ v_out) {
   __shared__ int64_t rows[kMostTokens];
   const uint32_t t0 = blockIdx.x * cut.tokens, here = min(cut.tokens, tokens - t0);
+  grid_dependency_wait();
   if (threadIdx.x < here) rows[threadIdx.x] = first_row(c, slots[t0 + threadIdx.x]);
   __syncthreads();
   const uint32_t lanes = (here * 2 * cut.heads) << cut.shift;
@@ -328,18 +331,9 @@ template <typename X>
 mb_status launch_write(const CacheView& c, int bits, const KvSource& src, const int64_t* slots,
                        uint32_t tokens, const int64_t* rows, cudaStream_t stream) {
   const Launch l = launch_for(c, tokens);
-  // behind the kernel of the rows: the values are loaded meanwhile
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = 1;
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = l.grid;
-  cfg.blockDim = dim3(kThreads);
-  cfg.stream = stream;
-  cfg.attrs = attr;
-  cfg.numAttrs = rows != nullptr ? 1 : 0;
   const auto go = [&](auto kernel) {
-    return cudaLaunchKernelEx(&cfg, kernel, c, src, slots, tokens, l.cut, rows);
+    return launch_dependent(kernel, l.grid, kThreads, 0, stream, c, src, slots, tokens, l.cut,
+                            rows);
   };
   if (bits == 8)
     MB_CUDA_TRY(src.vec ? go(cache_write_kernel<X, 8, true>) : go(cache_write_kernel<X, 8, false>));
@@ -353,11 +347,11 @@ void launch_read(const CacheView& c, int bits, const int64_t* slots, uint32_t to
                  void* v, cudaStream_t stream) {
   const Launch l = launch_for(c, tokens);
   if (bits == 8)
-    cache_read_kernel<Y, 8><<<l.grid, kThreads, 0, stream>>>(
-        c, slots, tokens, l.cut, static_cast<Y*>(k), static_cast<Y*>(v));
+    launch_dependent(cache_read_kernel<Y, 8>, l.grid, kThreads, 0, stream, c, slots, tokens, l.cut,
+                     static_cast<Y*>(k), static_cast<Y*>(v));
   else
-    cache_read_kernel<Y, 4><<<l.grid, kThreads, 0, stream>>>(
-        c, slots, tokens, l.cut, static_cast<Y*>(k), static_cast<Y*>(v));
+    launch_dependent(cache_read_kernel<Y, 4>, l.grid, kThreads, 0, stream, c, slots, tokens, l.cut,
+                     static_cast<Y*>(k), static_cast<Y*>(v));
 }
 
 mb_status check_tokens(int64_t tokens) {
@@ -415,8 +409,8 @@ extern "C" mb_status mb_cache_write(const mb_kv_cache* cache, const void* k,
                                                         table, mask);
       MB_LAUNCH_CHECK("cache_claim_kernel");
     }
-    cache_rows_kernel<<<grid, kThreads, 0, stream>>>(c, slots, (uint32_t)tokens, table, mask, rows);
-    MB_LAUNCH_CHECK("cache_rows_kernel");
+    MB_CUDA_TRY(launch_dependent(cache_rows_kernel, grid, kThreads, 0, stream, c, slots,
+                                 (uint32_t)tokens, table, mask, rows));
   }
   return type == MB_FP16 ? launch_write<__half>(c, cache->bits, src, slots, (uint32_t)tokens, rows,
                                                 stream)

@@ -11,6 +11,7 @@
 #include <cudaTypedefs.h>
 
 #include <cstdint>
+#include <utility>
 
 namespace mb {
 
@@ -176,6 +177,24 @@ __device__ __forceinline__ void grid_launch_dependents() {
 }
 
 // ---- host ----
+
+// Launches a kernel that begins with grid_dependency_wait(): it is set up on the
+// GPU while the kernel before it in the stream ends.
+template <typename... P, typename... A>
+inline cudaError_t launch_dependent(void (*kernel)(P...), dim3 grid, unsigned threads, size_t smem,
+                                    cudaStream_t stream, A&&... args) {
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = stream;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, kernel, std::forward<A>(args)...);
+}
 
 // cuTensorMapEncodeTiled from the driver, without linking libcuda.
 PFN_cuTensorMapEncodeTiled_v12000 tensor_map_encoder();
