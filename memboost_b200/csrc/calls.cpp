@@ -3,7 +3,7 @@
 //
 // Such a call takes a few microseconds on the GPU, and taking its tensors apart
 // in Python and handing them over through ctypes takes as long or longer: 8 x
-// 4096 to codes and back 19.3 us that way, 10.2 this way, the kernels 3.5.  So
+// 4096 to codes and back 19.3 us that way, 9.2 this way, the kernels 3.2.  So
 // the usual call -- ordinary tensors of one device that is the current one, laid
 // out as the C entries want them, outputs to be made -- is taken here.  For
 // everything else, a mistaken argument too, these functions do nothing and

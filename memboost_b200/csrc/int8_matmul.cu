@@ -17,9 +17,9 @@
 //
 // Few tokens are bound by reading the weights, at the rate at which one SM
 // takes operands in (75 to 90 GB/s each, launch and drain aside): 4096 x 4096 at
-// one token 8.6 us with the quantising kernel, 11008 x 4096 at 48 tokens 16.3.
+// one token 8.2 us with the quantising kernel, 11008 x 4096 at 48 tokens 16.
 // Thousands of tokens are bound by the tensor cores and, back to back, by the
-// card's power: 8192 x 11008 x 4096 takes 274 us, 2.7e15 operations a second
+// card's power: 8192 x 11008 x 4096 takes 272 us, 2.7e15 operations a second
 // (228 us without the outputs' way out; the pipe is busy for 72 % of it).
 #include <algorithm>
 #include <cstring>

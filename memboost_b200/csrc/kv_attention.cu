@@ -48,8 +48,8 @@
 //
 // Measured: 8 bits stream at 92 % of the copy rate (one sequence of 65536 tokens
 // and 32 heads: 93 us for 86 us of bytes), 4 bits are bound by the instructions
-// that make fp16 of the codes (some 430 a warp for 16 tokens of 128 channels and
-// 8 query heads: 97 us for 52).  Beside that a call costs about 8 us (launch,
+// that make fp16 of the codes (460 a warp for 16 tokens of 128 channels and up to
+// 8 query heads: 96 us for 52).  Beside that a call costs about 8 us (launch,
 // the first units, the join) and each sequence's head about 4 us of a CTA.
 #include <algorithm>
 #include <cmath>
