@@ -19,10 +19,11 @@ import torch
 
 _LIB_PATH = os.path.join(os.path.dirname(os.path.abspath(__file__)), "libmemboost_b200.so")
 
-if not os.path.exists(_LIB_PATH):
-    raise ImportError(
-        f"memboost_b200: native library {_LIB_PATH} is missing; build it with "
-        "`python memboost_b200/build.py` (there is no CPU fallback)")
+for _path in (_LIB_PATH, os.path.join(os.path.dirname(_LIB_PATH), "_calls.so")):
+    if not os.path.exists(_path):
+        raise ImportError(
+            f"memboost_b200: native library {_path} is missing; build it with "
+            "`python memboost_b200/build.py` (there is no CPU fallback)")
 
 _lib = ctypes.CDLL(_LIB_PATH)
 

@@ -211,7 +211,7 @@ constexpr float kRoundSafe = 0.49998f;
 // Codes of eight values, x / scale to the nearest integer, ties to even, of
 // the exact quotient.  The product x * inv (inv rounds once, the sum with the
 // magic number once) decides, unless one of the eight comes within 2e-5 of a
-// border (one in 6000 warps' steps or so).  Then the remainder x - t * scale
+// border (one in a hundred warps' steps or so).  Then the remainder x - t * scale
 // says for each whether t is the nearest: it is exact for |t| >= 2 (a
 // multiple of scale's last place, below 2^24 of them) and for t = 0; for
 // |t| = 1 its rounding can at most turn a remainder just above scale / 2 into
