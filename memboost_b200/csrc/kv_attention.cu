@@ -1098,9 +1098,15 @@ __global__ void __launch_bounds__(32 * kJoinWarps)
 inline uint32_t head_tiles(uint32_t group, uint32_t dim) { return group > 8 && dim <= 128 ? 2 : 1; }
 
 // Sequences of tables this narrow are taken whole, a CTA a row: nothing to join.
-constexpr int64_t kWholeTokens = 512;
+// A row costs its CTA about 1 us for 64 tokens, dealing and joining 4 us; with
+// many rows the CTAs have enough to do either way.  Whole and dealt out, 32 rows:
+// 256 tokens 7.7 and 8.9 us, 352 9.7 and 8.9, 512 12.0 and 9.3; 128 rows of 512: 12.0 and
+// 13.6; 512 rows of 512: 16.3 and 20.5.
+constexpr int64_t kWholeTokens = 320, kWholeTokensOfMany = 512, kManyRows = 64;
 constexpr int64_t kMostShares = 3 * 148;  // Layout::ctas an SM at most
-inline bool whole(int64_t most) { return most <= kWholeTokens; }
+inline bool whole(int64_t most, int64_t rows) {
+  return most <= (rows > kManyRows ? kWholeTokensOfMany : kWholeTokens);
+}
 
 // Rows of codes as TMA reads them: [all rows, bytes].
 bool rows_map(CUtensorMap* map, const void* codes, const CacheView& c, int bits, uint32_t box_row,
@@ -1189,9 +1195,10 @@ extern "C" size_t mb_cache_attention_workspace_size(const mb_kv_cache* cache, in
   if (cache == nullptr || cache->kv_heads <= 0 || cache->page_size <= 0 || batch <= 0 ||
       heads < cache->kv_heads || table_width <= 0)
     return 0;
-  if (whole(table_width * cache->page_size)) return 0;
-  const uint32_t tiles =
-      head_tiles((uint32_t)(heads / cache->kv_heads), (uint32_t)cache->head_dim);
+  const int64_t group = heads / cache->kv_heads;
+  const uint32_t tiles = head_tiles((uint32_t)group, (uint32_t)cache->head_dim);
+  const int64_t rows = batch * cache->kv_heads * ceil_div(group, 8 * tiles);
+  if (whole(table_width * cache->page_size, rows)) return 0;
   return (size_t)(2 * kMostShares * 8 * tiles) * (size_t)(cache->head_dim + 2) * sizeof(float);
 }
 
