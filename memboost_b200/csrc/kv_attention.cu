@@ -456,6 +456,9 @@ __launch_bounds__(Layout<BITS, kQuarters>::kThreads, (Layout<BITS, kQuarters>::c
                              (int64_t)(next * heads.group + from + x / lines) * q.head_stride) +
                         128 * (x % lines));
       }
+      // nothing to fetch (idle units, a sequence without tokens): the page read
+      // ahead is that of the segment behind it
+      if (s.first() >= s.last()) next_page = first_page();
       for (uint32_t u = s.first(); u < s.last(); ++u) {
         const uint32_t t = u * L::kUnit + mine;
         const uint32_t p = t / c.page_size;
