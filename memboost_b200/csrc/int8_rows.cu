@@ -141,7 +141,8 @@ __global__ void __launch_bounds__(kDecodeThreads)
                                const float* __restrict__ scales, uint32_t K, uint32_t pieces,
                                uint32_t total, Y* __restrict__ out, int64_t out_stride) {
   grid_dependency_wait();
-  const uint32_t i = (blockIdx.x * kDecodeThreads + threadIdx.x) / 32;
+  // warps counted, not threads: 32 times as many pass 32 bits
+  const uint32_t i = blockIdx.x * (kDecodeThreads / 32) + threadIdx.x / 32;
   if (i >= total) return;
   const uint32_t row = i / pieces;
   const uint32_t c0 = (i - row * pieces) * (32 * kDecodeValues) + threadIdx.x % 32;
@@ -258,7 +259,8 @@ extern "C" mb_status mb_int8_dequantize(const int8_t* codes, int64_t codes_strid
   const size_t size = dtype_size(out_type);
   const bool whole =
       K % 8 == 0 && aligned(out, 16) && (rows == 1 || out_stride * size % 16 == 0);
-  // a launch counts its pieces (8 values, or a warp's 256) in 32 bits, threads in 31
+  // a launch counts its pieces (8 values, or a warp's 256) in 32 bits; its CTAs,
+  // of 512 pieces or 8 warps, are 2^27 at most
   const int64_t per_row = whole ? K / 8 : ceil_div(K, 32 * kDecodeValues);
   const int64_t most = std::max<int64_t>(1, (int64_t(1) << 30) / per_row);
   for (int64_t r0 = 0; r0 < rows; r0 += most) {
