@@ -28,15 +28,21 @@
 // a sign: off by at most 2^-14 of the query's largest channel; exact for
 // channels above 1/8 of it, in bf16 above 1/64).  The sums are exact.  8-bit
 // values become exact fp16 integers (1024 + 128 + code by a byte permute,
-// minus 1152); their scale multiplies the probability, relative to a power of
-// two above every scale so far, so that the product stays in fp16's range.
+// minus 1152); their scale multiplies the probability.
 // 4-bit codes become m + s * code in fp16, one rounding; the query then is
-// fp16 too.  Probabilities are rounded to fp16 (2^-11), and for an fp16 output,
-// whose own rounding is no larger, what that drops is multiplied too; scores,
-// maxima, sums and the outputs' accumulators are fp32.
+// fp16 too.  Scores, maxima, sums and the outputs' accumulators are fp32.
 //
-// The running maximum is raised only when a score exceeds it by 8 (in powers
-// of two): probabilities then stay below 256 and most steps rescale nothing.
+// Weights -- probabilities, with 8 bits times the value's scale -- are rounded
+// to fp16 (2^-11), and for an fp16 output, whose own rounding is no larger,
+// what that drops is multiplied too.  They are taken relative to the largest
+// weight of the head so far, not the largest scale or score alone: a token
+// whose values are huge but whose probability is nothing does not push the
+// others out of fp16's range.  The largest lies at 2^10 when it is set and is
+// set again above 2^15, so that weights down to 2^-24 of it are normal numbers
+// and what is lost of a smaller one is below 2^-35 of it; most steps rescale
+// nothing.  With 4 bits the probabilities' own maximum serves; with 8 a factor
+// of its own (`unit`), and the maximum, which only the sum refers to then, is
+// raised when a score exceeds it by 8 (in powers of two).
 //
 // The units of all sequences and heads are dealt out evenly to the resident
 // CTAs (two or three an SM), whatever the lengths: a CTA's share may begin and end inside a sequence.
@@ -184,7 +190,13 @@ __device__ __forceinline__ int token_of(int k) { return k ^ ((k >> 1) & 1); }
 
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLowest = -0x1.fffffep127f;  // a maximum of nothing
-constexpr float kRaise = 8.0f;  // how far a score may exceed the maximum in use
+// Exponents of the largest weight: when it is set, and above which it is set again.
+constexpr int kAim = 10, kMost = 15;
+// 8 bits: how far a score may exceed the maximum that the sum refers to.
+constexpr int kRaise = 8;
+// 8 bits: the largest unit, what a head begins with.  Times a probability of up
+// to 2^8 it stays in fp32; times one of 1 and the smallest normal scale it is 2^-8.
+constexpr float kMostUnit = 0x1p118f;
 
 __device__ __forceinline__ float exp2_fast(float x) {
   float y;
@@ -605,11 +617,14 @@ __launch_bounds__(Layout<BITS, kQuarters>::kThreads, (Layout<BITS, kQuarters>::c
     }
 
     // o[n][p][i]: channels 16 (g + 8 p) + 2 i, + 1 of heads 2 j, 2 j + 1
+    // (8 bits: times unit, relative to the same maximum m as the sums l)
     float o[kTiles][L::kPasses][8][4] = {};
-    float m[kTiles][2], l[kTiles][2] = {};
+    float m[kTiles][2], l[kTiles][2] = {}, unit[kTiles][2];
 #pragma unroll
-    for (int n = 0; n < kTiles; ++n) m[n][0] = m[n][1] = kLowest;
-    uint32_t v_exp = 1;  // exponent of the power of two the value scales are taken by
+    for (int n = 0; n < kTiles; ++n) {
+      m[n][0] = m[n][1] = kLowest;
+      unit[n][0] = unit[n][1] = kMostUnit;
+    }
 
 #pragma unroll 1
     for (uint32_t u = seg.first(); u < seg.last(); ++u) {
@@ -623,7 +638,7 @@ __launch_bounds__(Layout<BITS, kQuarters>::kThreads, (Layout<BITS, kQuarters>::c
       if (seen > 0) {
         // the values of a pass: those of the first are on the way during S^T
         constexpr int kWords = BITS / 2;
-        uint32_t w[4][kWords];
+        uint32_t vw[4][kWords];
         uint32_t gr[4];
         const auto load_values = [&](int p) {
 #pragma unroll
@@ -631,11 +646,11 @@ __launch_bounds__(Layout<BITS, kQuarters>::kThreads, (Layout<BITS, kQuarters>::c
             if constexpr (BITS == 8) {
               const uint4 v =
                   lds128(value_at[r & 1] + stage_at + p * L::kColumn + (r >> 1) * kEight);
-              w[r][0] = v.x; w[r][1] = v.y; w[r][2] = v.z; w[r][3] = v.w;
+              vw[r][0] = v.x; vw[r][1] = v.y; vw[r][2] = v.z; vw[r][3] = v.w;
             } else {
               // the second pass is the row's other half: chunks 4 .. 7
               const uint2 v = lds64((value_at[r & 1] ^ (p * 64)) + stage_at + (r >> 1) * kEight);
-              w[r][0] = v.x; w[r][1] = v.y;
+              vw[r][0] = v.x; vw[r][1] = v.y;
               gr[r] = lds32(value_scale[r & 1] + stage_at + 4 * min((g + 8 * p) / 2, last_group) +
                             (r >> 1) * eight_scales);
             }
@@ -715,8 +730,7 @@ __launch_bounds__(Layout<BITS, kQuarters>::kThreads, (Layout<BITS, kQuarters>::c
             for (int e = 0; e < 4; ++e) s[n][e] += s2[n][e];
         }
 
-        // ---- scores in powers of two; the maximum in use
-        bool raise = false;
+        // ---- scores in powers of two; weights, and what they are relative to
 #pragma unroll
         for (int n = 0; n < kTiles; ++n)
 #pragma unroll
@@ -730,79 +744,98 @@ __launch_bounds__(Layout<BITS, kQuarters>::kThreads, (Layout<BITS, kQuarters>::c
             for (int e = 0; e < 4; ++e)
               if (row0 + 8 * (e >> 1) >= seen) s[n][e] = -INFINITY;
         }
+        float vs[2] = {1.0f, 1.0f};
+        if constexpr (BITS == 8) {
+          vs[0] = __uint_as_float(lds32(key_scale + stage_at + L::kScales));
+          vs[1] = __uint_as_float(lds32(key_scale + stage_at + L::kScales + 32));
+          if (!whole) {  // what lies behind the sequence's end is not used
+            if (row0 >= seen) vs[0] = 0.0f;
+            if (row0 + 8 >= seen) vs[1] = 0.0f;
+          }
+        }
+        float p[kTiles][4], w[kTiles][4];
+        const auto weigh = [&](int n, int e) {
+          p[n][e] = exp2_fast(s[n][e] - m[n][e & 1]);
+          w[n][e] = BITS == 8 ? p[n][e] * unit[n][e & 1] * vs[e >> 1] : p[n][e];
+        };
+        bool raise = false;
 #pragma unroll
         for (int n = 0; n < kTiles; ++n)
 #pragma unroll
-          for (int e = 0; e < 4; ++e) raise |= s[n][e] > m[n][e & 1] + kRaise;
+          for (int e = 0; e < 4; ++e) {
+            weigh(n, e);
+            raise |= w[n][e] > (float)(1 << kMost);
+            if constexpr (BITS == 8) raise |= p[n][e] > (float)(1 << kRaise);
+          }
         if (__any_sync(0xffffffffu, raise)) {
 #pragma unroll
-          for (int n = 0; n < kTiles; ++n)
+          for (int n = 0; n < kTiles; ++n) {
+            float f[2];
 #pragma unroll
             for (int r = 0; r < 2; ++r) {
               float top = fmaxf(s[n][r], s[n][r + 2]);
 #pragma unroll
               for (int d = 4; d < 32; d <<= 1)
                 top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
-              top = fmaxf(top, m[n][r]);
-              const float keep = exp2_fast(m[n][r] - top);
+              top = fmaxf(BITS == 8 ? top : top - kAim, m[n][r]);
+              f[r] = exp2_fast(m[n][r] - top);
+              l[n][r] *= f[r];
+              if constexpr (BITS == 8) {
+                // weights stay relative to what they were, up to the largest unit
+                const float now = unit[n][r] * exp2_fast(top - m[n][r]);
+                f[r] = now <= kMostUnit
+                           ? 1.0f
+                           : f[r] * 0x1p64f / unit[n][r] * (kMostUnit * 0x1p-64f);
+                unit[n][r] = fminf(now, kMostUnit);
+              }
               m[n][r] = top;
-              l[n][r] *= keep;
+              weigh(n, r);
+              weigh(n, r + 2);
+              if constexpr (BITS == 8) {
+                // down to 2^kAim, by the exponents of the factors: the weight may be
+                // past fp32 (a scale that is not finite has no say)
+                uint32_t e = 0;
 #pragma unroll
-              for (int p = 0; p < L::kPasses; ++p)
-#pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                  o[n][p][i][r] *= keep;
-                  o[n][p][i][r + 2] *= keep;
+                for (int t = 0; t < 2; ++t) {
+                  const uint32_t x = __float_as_uint(vs[t]) & 0x7FFFFFFFu;
+                  if (x < 0x7F800000u)
+                    e = max(e, (__float_as_uint(p[n][r + 2 * t] * unit[n][r]) >> 23) + (x >> 23));
                 }
+#pragma unroll
+                for (int d = 4; d < 32; d <<= 1) e = max(e, __shfl_xor_sync(0xffffffffu, e, d));
+                // the weight is below 2^(e - 252)
+                const uint32_t drop = e > 252 + kMost ? min(e - (252 + kAim), 252u) : 0u;
+                const float half0 = __uint_as_float((127 - drop / 2) << 23);
+                const float half1 = __uint_as_float((127 - (drop + 1) / 2) << 23);
+                f[r] = f[r] * half0 * half1;
+                unit[n][r] = unit[n][r] * half0 * half1;
+                weigh(n, r);
+                weigh(n, r + 2);
+              }
             }
-        }
-        float vs[2] = {1.0f, 1.0f};
-        if constexpr (BITS == 8) {
-          // scales relative to 2^(v_exp - 127), above every scale so far
-          uint32_t e0 = lds32(key_scale + stage_at + L::kScales);
-          uint32_t e1 = lds32(key_scale + stage_at + L::kScales + 32);
-          if (!whole) {  // what lies behind the sequence's end is not used
-            if (row0 >= seen) e0 = 0u;
-            if (row0 + 8 >= seen) e1 = 0u;
+#pragma unroll
+            for (int t = 0; t < L::kPasses; ++t)
+#pragma unroll
+              for (int i = 0; i < 8; ++i)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) o[n][t][i][e] *= f[e & 1];
           }
-          const uint32_t e = max(e0, e1);
-          if (__any_sync(0xffffffffu, e < 0x7F800000u && (e >> 23) >= v_exp)) {
-            const uint32_t now =
-                max(v_exp, 1u + __reduce_max_sync(0xffffffffu, e < 0x7F800000u ? e >> 23 : 0u));
-            const uint32_t drop = now - v_exp;  // by 2^-drop
-            const float down = drop < 127u ? __uint_as_float((127u - drop) << 23) : 0.0f;
-            v_exp = now;
-#pragma unroll
-            for (int n = 0; n < kTiles; ++n)
-#pragma unroll
-              for (int p = 0; p < L::kPasses; ++p)
-#pragma unroll
-                for (int i = 0; i < 8; ++i)
-#pragma unroll
-                  for (int r = 0; r < 4; ++r) o[n][p][i][r] *= down;
-          }
-          const float by = __uint_as_float((254u - v_exp) << 23);
-          vs[0] = __uint_as_float(e0) * by;
-          vs[1] = __uint_as_float(e1) * by;
         }
+#pragma unroll
+        for (int n = 0; n < kTiles; ++n)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) l[n][e & 1] += p[n][e];
         uint32_t pt[kTiles][2], low[kTiles][2] = {};
 #pragma unroll
         for (int n = 0; n < kTiles; ++n) {
-          float p[4];
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            p[e] = exp2_fast(s[n][e] - m[n][e & 1]);
-            l[n][e & 1] += p[e];
-            if constexpr (BITS == 8) p[e] *= vs[e >> 1];
-          }
 #pragma unroll
           for (int r = 0; r < 2; ++r) {
-            const __half2 high = __floats2half2_rn(p[2 * r], p[2 * r + 1]);
+            const __half2 high = __floats2half2_rn(w[n][2 * r], w[n][2 * r + 1]);
             pt[n][r] = transpose8x8(h2_bits(high));
             if (fine) {
               const float2 back = __half22float2(high);
               low[n][r] = transpose8x8(
-                  h2_bits(__floats2half2_rn(p[2 * r] - back.x, p[2 * r + 1] - back.y)));
+                  h2_bits(__floats2half2_rn(w[n][2 * r] - back.x, w[n][2 * r + 1] - back.y)));
             }
           }
         }
@@ -821,8 +854,8 @@ __launch_bounds__(Layout<BITS, kQuarters>::kThreads, (Layout<BITS, kQuarters>::c
           if constexpr (BITS == 8) {
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-              const uint32_t w0 = w[0][i] ^ 0x80808080u, w1 = w[1][i] ^ 0x80808080u;
-              const uint32_t w2 = w[2][i] ^ 0x80808080u, w3 = w[3][i] ^ 0x80808080u;
+              const uint32_t w0 = vw[0][i] ^ 0x80808080u, w1 = vw[1][i] ^ 0x80808080u;
+              const uint32_t w2 = vw[2][i] ^ 0x80808080u, w3 = vw[3][i] ^ 0x80808080u;
 #pragma unroll
               for (int h = 0; h < 2; ++h) {  // channels 4 i + 2 h, + 1
                 const uint32_t x = __byte_perm(w0, w1, h ? 0x7362 : 0x5140);
@@ -846,8 +879,8 @@ __launch_bounds__(Layout<BITS, kQuarters>::kThreads, (Layout<BITS, kQuarters>::c
 #pragma unroll
               for (int h = 0; h < 4; ++h) {  // channels 8 i + 2 h, + 1
                 const uint32_t sel = h < 2 ? 0x5410 : 0x7632;
-                const uint32_t x = __byte_perm(w[0][i], w[1][i], sel) >> (8 * (h & 1));
-                const uint32_t y = __byte_perm(w[2][i], w[3][i], sel) >> (8 * (h & 1));
+                const uint32_t x = __byte_perm(vw[0][i], vw[1][i], sel) >> (8 * (h & 1));
+                const uint32_t y = __byte_perm(vw[2][i], vw[3][i], sel) >> (8 * (h & 1));
                 const uint32_t a0 = code4_pair<false>(x, s01, m01);
                 const uint32_t a1 = code4_pair<true>(x, s01, m01);
                 const uint32_t a2 = code4_pair<false>(y, s23, m23);
@@ -869,7 +902,6 @@ __launch_bounds__(Layout<BITS, kQuarters>::kThreads, (Layout<BITS, kQuarters>::c
     }
 
     // ---- the warps' parts joined, 8 heads at a time
-    const float up = BITS == 8 ? __uint_as_float(v_exp << 23) : 1.0f;
     const bool part = seg.c1 - seg.c0 != seg.n;
     const uint32_t slot = 2 * blockIdx.x + place;
 #pragma unroll
@@ -882,6 +914,7 @@ __launch_bounds__(Layout<BITS, kQuarters>::kThreads, (Layout<BITS, kQuarters>::c
 #pragma unroll
       for (int r = 0; r < 2; ++r) {
         float sum = ok ? l[n][r] : __uint_as_float(0x7FC00000u);
+        const float up = BITS == 8 ? 1.0f / unit[n][r] : 1.0f;
 #pragma unroll
         for (int d = 4; d < 32; d <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
         const uint32_t h = 2 * j + r;

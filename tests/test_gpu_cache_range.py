@@ -1,0 +1,108 @@
+"""cache_attention where sizes differ widely within a sequence: scales of values
+that tokens without weight carry, one token with nearly all the weight, query
+channels far above the others, keys far from 0.
+
+The bound, against 64 bits.  A query is held to 2^-22 of its largest channel
+(8-bit keys; as it is with 4-bit ones), keys and sums as they are: a score is
+off by
+  d <= 2^-22 scale max |q| sum |k| + 2^-20 sum |scale q k| + 2^-18 (1 + sum |scale q k|)
+(fp32 sums of at most 256 products, the exponent's scaling and exp2 with it),
+which changes p by a factor within e^(2d).  Probabilities (with 8 bits: times
+the value's scale) and 4-bit values are rounded to fp16, u = 2^-11 each, the
+former above fp16's normal numbers: below them each is off by at most 2^-32 of
+the largest that the sequence has (8 bits), or 2^-32 of the largest probability
+times the largest value (4 bits)."""
+import math
+
+import numpy as np
+import pytest
+import torch
+
+import memboost_b200 as mb
+from oracle import serving
+from test_gpu_cache import _np
+
+pytestmark = pytest.mark.gpu
+
+
+def _check(got, q, cache, table, lengths, scale):
+    q, mirror = _np(q), serving.Cache(cache)
+    heads, bits = cache.kv_heads, cache.bits
+    group = q.shape[1] // heads
+    u, f = 2.0 ** -11, torch.finfo(got.dtype)
+    for b in range(q.shape[0]):
+        for h in range(heads):
+            k, v = (mirror.tokens(w, table[b], int(lengths[b]), h) for w in (0, 1))
+            big = np.abs(v).max(-1)
+            for j in range(h * group, (h + 1) * group):
+                s = (k @ q[b, j]) * scale
+                p = np.exp(s - s.max())
+                p /= p.sum()
+                want, weight = p @ v, p @ np.abs(v)
+                reach = (np.abs(k) @ np.abs(q[b, j])).max() * abs(scale)
+                d = 2.0 ** -20 * reach + 2.0 ** -18 * (1 + reach)
+                if bits == 8:
+                    d += 2.0 ** -22 * np.abs(k).sum(-1).max() * np.abs(q[b, j]).max() * abs(scale)
+                lost = 2.0 ** -32 * len(k) * ((p * big).max() if bits == 8 else p.max() * big.max())
+                work = weight * (np.exp(2 * d) * (1 + 2 * u) * (1 + 2.0 ** -16) - 1) + lost
+                tol = work + f.eps / 2 * (np.abs(want) + work) + f.tiny * f.eps / 2
+                err = np.abs(_np(got[b, j]) - want)
+                assert np.all(err <= tol), (b, j, (err / tol).max(), err.max())
+
+
+def _cache(k, v, bits, page=16):
+    """One sequence's tokens in pages 0, 1, ..., and the table."""
+    pages = -(-k.shape[0] // page)
+    cache = mb.QuantizedCache.allocate(pages, page, k.shape[1], k.shape[2], bits=bits)
+    mb.cache_write(cache, k.cuda(), v.cuda(), torch.arange(k.shape[0], device="cuda"))
+    return cache, torch.arange(pages, dtype=torch.int32).unsqueeze(0)
+
+
+def _attend(q, k, v, bits, scale):
+    cache, table = _cache(k, v, bits)
+    n = torch.tensor([k.shape[0]], dtype=torch.int32)
+    got = mb.cache_attention(q.cuda(), cache, table.cuda(), n.cuda(), scale=scale)
+    assert torch.isfinite(got).all()
+    _check(got, q, cache, table.numpy(), n.tolist(), scale)
+
+
+def _inputs(n, heads, group, dim, seed):
+    g = torch.Generator().manual_seed(seed)
+    k, v = (torch.randn((n, heads, dim), generator=g) for _ in range(2))
+    return torch.randn((1, heads * group, dim), generator=g), k, v
+
+
+LENGTHS = [40, 300, 3000]
+
+
+@pytest.mark.parametrize("dtype,size", [(torch.float16, 15000.0), (torch.bfloat16, 1e12),
+                                        (torch.bfloat16, 1e30)])
+@pytest.mark.parametrize("n", LENGTHS)
+@pytest.mark.parametrize("dim,group", [(64, 1), (128, 12), (192, 3)])
+def test_large_values_without_weight(n, dim, group, dtype, size):
+    """Tokens whose probability is 0 carry values far above the others'."""
+    q, k, v = _inputs(n, 2, group, dim, seed=n)
+    q[..., 0], k[..., 0] = 8, 0
+    some = torch.arange(n) % 7 == 3
+    k[some, :, 0] = -100  # scores about -100 and -70: no weight
+    v[some] *= size
+    v.clamp_(-torch.finfo(dtype).max, torch.finfo(dtype).max)
+    _attend(q.to(dtype), k.to(dtype), v.to(dtype), 8, 1 / math.sqrt(dim))
+
+
+@pytest.mark.parametrize("bits_ahead,bits", [(20, 8), (27, 8), (27, 4)])
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16], ids=["fp16", "bf16"])
+@pytest.mark.parametrize("n", LENGTHS)
+@pytest.mark.parametrize("dim,group", [(64, 1), (128, 12), (256, 3)])
+def test_one_token_with_nearly_all_weight(n, dim, group, dtype, bits_ahead, bits):
+    """The first token has 2^20 or 2^27 times the others' weight and values of
+    0: the output is what the others add."""
+    q, k, v = _inputs(n, 2, group, dim, seed=n)
+    scale = 1 / math.sqrt(dim)
+    q, k = q * 0.2, k * 0.5
+    q[..., 0], k[..., 0] = 8, 0
+    k[0] = 0
+    k[0, :, 0] = bits_ahead * math.log(2) / (8 * scale)
+    v = 1 + 0.1 * v
+    v[0] = 0
+    _attend(q.to(dtype), k.to(dtype), v.to(dtype), bits, scale)
