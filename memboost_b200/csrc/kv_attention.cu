@@ -235,6 +235,12 @@ __device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t n
       : "memory");
 }
 
+// mbar_wait of a whole warp: lanes may see the time run out apart, and what
+// follows needs all of them.
+__device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity) {
+  return __all_sync(0xffffffffu, mbar_wait(bar, parity));
+}
+
 struct Lengths {
   const int32_t* data;
   int64_t most;  // tokens the table can name
@@ -477,7 +483,7 @@ __launch_bounds__(Layout<BITS, kQuarters>::kThreads, (Layout<BITS, kQuarters>::c
         const int32_t page = next_page;
         next_page = u + 1 < s.last() ? page_of(s, u + 1) : first_page();
         const bool there = page >= 0 && page < c.pages;
-        if (!mbar_wait(&empty[stage], phase)) {
+        if (!warp_wait(&empty[stage], phase)) {
           ok = false;
           break;
         }
@@ -628,7 +634,7 @@ __launch_bounds__(Layout<BITS, kQuarters>::kThreads, (Layout<BITS, kQuarters>::c
 
 #pragma unroll 1
     for (uint32_t u = seg.first(); u < seg.last(); ++u) {
-      if (!ok || !mbar_wait(&full[stage], phase)) {  // ran out: NaN from here on
+      if (!ok || !warp_wait(&full[stage], phase)) {  // ran out: NaN from here on
         ok = false;
         break;
       }

@@ -322,3 +322,31 @@ def test_allocation_failures_are_torch_errors():
     x = torch.zeros((1 << 22, 16), dtype=torch.float16, device="cuda")
     with pytest.raises(torch.OutOfMemoryError):  # 8 TB of outputs
         mb.int8_matmul(x, w)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32], ids=["bf16", "fp32"])
+@pytest.mark.parametrize("M,N", [(1, 200), (40, 300), (300, 1000), (2300, 2100)])
+def test_product_of_very_large_and_very_small_tokens(M, N, dtype):
+    """Tokens next to the ends of fp32 whose products are of ordinary size: the
+    sum times the token's scale alone would be infinite, or subnormal."""
+    g = torch.Generator().manual_seed(M)
+    x = torch.randn((M, 4096), generator=g)
+    big = torch.arange(M) % 3
+    x = x * torch.tensor([4e37, 1.0, 1e-40])[big].unsqueeze(1)  # the third: subnormal scales
+    x = x.clamp(-3e38, 3e38).to(dtype).cuda()
+    for size in (1e-3, 1e-30, 1e30):
+        w = mb.quantize_int8(torch.randn((N, 4096), generator=g).cuda() * size)
+        y = mb.int8_matmul(x, w)
+        a = mb.quantize_int8(x)
+        with np.errstate(over="ignore"):
+            want, mag = serving.matmul(a.codes.cpu().numpy(), a.scales.cpu().numpy(),
+                                       w.codes.cpu().numpy(), w.scales.cpu().numpy())
+        f = torch.finfo(dtype)
+        u = 2.0 ** -24
+        work = mag * ((1 + u) ** 3 - 1) + 2.0 ** -149
+        tol = work + (f.eps / 2) * (np.abs(want) + work) + f.tiny * f.eps / 2
+        got = _np(y)
+        fits = np.abs(want) + tol <= f.max
+        assert np.all(np.abs(got - want)[fits] <= tol[fits])
+        beyond = np.abs(want) - tol > f.max * (1 + f.eps / 2)
+        assert np.all(np.isinf(got[beyond])) and not np.isnan(got).any()
