@@ -149,8 +149,18 @@ __device__ __forceinline__ float bias_at(const Epilogue& e, int64_t n) {
                                   : static_cast<const float*>(e.bias)[n];
 }
 
+// The sum times the token's scale is at most 2^31 times it: past this scale it
+// may be infinite, below the smallest normal scale lose bits, where the result
+// is an ordinary number.
+__device__ __forceinline__ bool extreme(float sa) {
+  return sa > 0x1p96f || (sa > 0.0f && sa < 0x1p-126f);
+}
 __device__ __forceinline__ float scaled(int sum, float sa, float sb, float bias) {
   return fmaf(__fmul_rn((float)sum, sa), sb, bias);
+}
+// In 64 bits, for a tile with an extreme scale.
+__device__ __noinline__ float scaled_wide(int sum, float sa, float sb, float bias) {
+  return __double2float_rn(fma((double)sum * (double)sa, (double)sb, (double)bias));
 }
 
 // A channel's (a lane's) sums with 16 tokens, `count` of which exist: sa in
@@ -158,8 +168,12 @@ __device__ __forceinline__ float scaled(int sum, float sa, float sb, float bias)
 // `stride` apart.  A warp writes 32 consecutive channels a token.
 template <typename Y>
 __device__ __forceinline__ void put16(const uint32_t (&v)[16], const float* sa, float sb,
-                                      float bias, Y* o, int64_t stride, int count) {
-  if (count >= 16) {
+                                      float bias, bool wide, Y* o, int64_t stride, int count) {
+  if (wide) {
+#pragma unroll
+    for (int i = 0; i < 16; ++i)
+      if (i < count) o[i * stride] = from_float<Y>(scaled_wide((int)v[i], sa[i], sb, bias));
+  } else if (count >= 16) {
 #pragma unroll
     for (int i = 0; i < 16; i += 4) {
       const float4 s = *reinterpret_cast<const float4*>(sa + i);
@@ -277,11 +291,16 @@ __global__ void __launch_bounds__(kThreads, 1)
   float sb = live ? e.b_scales[n] : 0.0f;
   const float bias = live ? bias_at(e, n) : 0.0f;
   grid_dependency_wait();
+  bool wide = false;
   if (warp < 4)
-    for (int i = threadIdx.x; i < kN; i += 128) a_scale[i] = m0 + i < M ? e.a_scales[m0 + i] : 0.0f;
+    for (int i = threadIdx.x; i < kN; i += 128) {
+      const float sa = m0 + i < M ? e.a_scales[m0 + i] : 0.0f;
+      a_scale[i] = sa;
+      wide |= extreme(sa);
+    }
   if (!mbar_wait(&done, 0)) atomicExch(&failed, 1u);
   asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-  __syncthreads();  // `failed` is final; the ring is free
+  wide = __syncthreads_or(wide) != 0;  // `failed` is final; the ring is free
 
   const uint32_t lanes = tmem + ((uint32_t)(32 * (warp & 3)) << 16);
   const int columns = (int)min64(kN, M - m0);
@@ -295,7 +314,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         __syncwarp();
         tmem_ld16(lanes + c, v);
         if (live)
-          put16<Y>(v, a_scale + c, sb, bias, o + c * e.out_stride, e.out_stride, columns - c);
+          put16<Y>(v, a_scale + c, sb, bias, wide, o + c * e.out_stride, e.out_stride, columns - c);
       }
     }
   } else {
@@ -331,10 +350,13 @@ __global__ void __launch_bounds__(kThreads, 1)
           if (r < parts) sum.x += v[r].x, sum.y += v[r].y, sum.z += v[r].z, sum.w += v[r].w;
         const float4 sa = *reinterpret_cast<const float4*>(a_scale + c);
         Y* to = o + c * e.out_stride;
-        to[0] = from_float<Y>(scaled(sum.x, sa.x, sb, bias));
-        if (c + 1 < columns) to[e.out_stride] = from_float<Y>(scaled(sum.y, sa.y, sb, bias));
-        if (c + 2 < columns) to[2 * e.out_stride] = from_float<Y>(scaled(sum.z, sa.z, sb, bias));
-        if (c + 3 < columns) to[3 * e.out_stride] = from_float<Y>(scaled(sum.w, sa.w, sb, bias));
+        const auto y = [&](int x, float s) {
+          return from_float<Y>(wide ? scaled_wide(x, s, sb, bias) : scaled(x, s, sb, bias));
+        };
+        to[0] = y(sum.x, sa.x);
+        if (c + 1 < columns) to[e.out_stride] = y(sum.y, sa.y);
+        if (c + 2 < columns) to[2 * e.out_stride] = y(sum.z, sa.z);
+        if (c + 3 < columns) to[3 * e.out_stride] = y(sum.w, sa.w);
       }
     }
     cluster_sync();  // no CTA leaves while another reads its part
@@ -396,6 +418,18 @@ __device__ __forceinline__ void pair_commit(uint64_t* bar) {
 __device__ __forceinline__ void arrive_cluster(uint32_t bar) {
   asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar)
                : "memory");
+}
+
+// Barrier of the four warps that drain; whether any of their threads says so.
+__device__ __forceinline__ bool drain_warps_or(bool x) {
+  uint32_t any;
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\tsetp.ne.b32 p, %1, 0;\n\t"
+      "barrier.cta.red.or.pred q, 1, 128, p;\n\tselp.u32 %0, 1, 0, q;\n\t}"
+      : "=r"(any)
+      : "r"((uint32_t)x)
+      : "memory");
+  return any != 0;
 }
 
 // Tile -> (channel tile, token tile): kPairGroup token tiles by all channel
@@ -512,10 +546,14 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
       const bool live = n < N;
       float sb = live ? e.b_scales[n] : 0.0f;
       const float bias = live ? bias_at(e, n) : 0.0f;
-      for (int i = threadIdx.x; i < kPairTokens; i += 128)
-        a_scale[buf][i] = m0 + i < M ? e.a_scales[m0 + i] : 0.0f;
+      bool wide = false;
+      for (int i = threadIdx.x; i < kPairTokens; i += 128) {
+        const float sa = m0 + i < M ? e.a_scales[m0 + i] : 0.0f;
+        a_scale[buf][i] = sa;
+        wide |= extreme(sa);
+      }
       // the four warps: the scales are there; those of two tiles ago are read
-      asm volatile("bar.sync 1, 128;" ::: "memory");
+      wide = drain_warps_or(wide);
       ok = ok && mbar_wait(&drain[buf], (uint32_t)((a / 2) & 1));
       if (!ok) sb = __uint_as_float(0x7FC00000u);
       asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
@@ -528,7 +566,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
         __syncwarp();
         tmem_ld16(at + c, v);
         if (live)
-          put16<Y>(v, a_scale[buf] + c, sb, bias, o + c * e.out_stride, e.out_stride, columns - c);
+          put16<Y>(v, a_scale[buf] + c, sb, bias, wide, o + c * e.out_stride, e.out_stride, columns - c);
       }
       asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
       __syncwarp();
