@@ -24,10 +24,11 @@
 // change from S^T's layout to the right operand's by a transposing move.
 //
 // 8-bit keys enter S^T as they are: an m16n8k32 integer product with the
-// query, scaled by a power of two to below 1, in two 8-bit parts (14 bits and
-// a sign: off by at most 2^-14 of the query's largest channel; exact for
-// channels above 1/8 of it, in bf16 above 1/64).  The sums are exact.  8-bit
-// values become exact fp16 integers (1024 + 128 + code by a byte permute,
+// query, scaled by a power of two to below 1, in three 8-bit parts (22 bits and
+// a sign: off by at most 2^-22 of the query's largest channel, exact for
+// channels above 2^-11 of it; with two parts, 14 bits, a channel far above the
+// others cost them theirs, and 16 x 2048 took 39.6 us for 41.0, 2 x 100001 65.5 for
+// 69.0).  The sums are exact.  8-bit values become exact fp16 integers (1024 + 128 + code by a byte permute,
 // minus 1152); their scale multiplies the probability.
 // 4-bit codes become m + s * code in fp16, one rounding; the query then is
 // fp16 too.  Scores, maxima, sums and the outputs' accumulators are fp32.
@@ -162,13 +163,22 @@ struct Layout {
   static constexpr int kKeyWords = BITS == 4 && kQuarters == 1 ? 2 : 4;
   static constexpr int kSteps = kRow / (16 * kKeyWords);
   static constexpr int kProducts = kSteps * (BITS == 8 ? 4 : 2 * kKeyWords);  // of S^T
+  // 8 bits: the products with the query's lower part, whose operand two CTAs an SM
+  // leave in shared memory, each lane its own (three have the registers for it)
+  static constexpr int kLow = BITS == 8 ? 2 * kSteps : 0;
+  __host__ __device__ static constexpr bool low_in_smem(int tiles) {
+    return BITS == 8 && ctas(tiles) == 2;
+  }
   static constexpr int kPasses = (kQuarters + 1) / 2;
 
   // The warps' outputs of 8 heads before they are joined: [warp][8][kJoinRow],
   // channel ch at ch + 4 (ch / 32) (free of bank conflicts).
   static constexpr int kJoinRow = 64 * kQuarters + 8 * kQuarters + 1;
   static constexpr int kJoin = kWarps * 8 * kJoinRow * 4;
-  static constexpr int kSmem = 1024 + kStages * kStage + kJoin;
+  static constexpr int kRing = kStages * kStage;
+  __host__ __device__ static constexpr int smem(int tiles) {
+    return 1024 + kRing + kJoin + (low_in_smem(tiles) ? kWarps * 32 * 8 * kLow * tiles : 0);
+  }
 
   // Place in a stage's keys (or values) of a byte of a row.
   __device__ __forceinline__ static uint32_t at(uint32_t row, uint32_t byte) {
@@ -198,6 +208,12 @@ constexpr int kRaise = 8;
 // to 2^8 it stays in fp32; times one of 1 and the smallest normal scale it is 2^-8.
 constexpr float kMostUnit = 0x1p118f;
 
+// Integer products begin at the bits of 1.5 2^23: sums of up to 2^22 (256 channels
+// of 128 times 128) then are the bits of 1.5 2^23 plus the sum, which a subtraction
+// makes an fp32 number (converting goes through the unit that exp2 needs).
+constexpr int kSumBits = 0x4B400000;
+__device__ __forceinline__ float whole_sum(int x) { return __int_as_float(x) - kRoundMagic; }
+
 __device__ __forceinline__ float exp2_fast(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
@@ -215,6 +231,9 @@ __device__ __forceinline__ uint2 lds64(uint32_t at) {
   uint2 v;
   asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(at));
   return v;
+}
+__device__ __forceinline__ void sts64(uint32_t at, uint32_t x, uint32_t y) {
+  asm volatile("st.shared.v2.u32 [%0], {%1, %2};" ::"r"(at), "r"(x), "r"(y));
 }
 __device__ __forceinline__ uint32_t lds32(uint32_t at) {
   uint32_t v;
@@ -403,7 +422,7 @@ __launch_bounds__(Layout<BITS, kQuarters>::kThreads, (Layout<BITS, kQuarters>::c
   extern __shared__ uint8_t raw[];
   uint8_t* ring = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(raw) + 1023) &
                                              ~(uintptr_t)1023);
-  float* join = reinterpret_cast<float*>(ring + L::kStages * L::kStage);
+  float* join = reinterpret_cast<float*>(ring + L::kRing);
   __shared__ float sm[L::kWarps][8], sl[L::kWarps][8];
   __shared__ uint64_t full[L::kStages], empty[L::kStages];
   __shared__ int tokens[L::kStages][L::kWarps];  // of a warp's 16 that there are
@@ -547,13 +566,18 @@ __launch_bounds__(Layout<BITS, kQuarters>::kThreads, (Layout<BITS, kQuarters>::c
   int stage = 0;
   uint32_t phase = 0;
   bool ok = true;
+  constexpr bool kLowSmem = L::low_in_smem(kTiles);
+  [[maybe_unused]] const uint32_t low_at =
+      ring0 + L::kRing + L::kJoin + 8 * (warp * 32 * L::kLow * kTiles + lane);
   const bool fine = !q.bf16;  // an fp16 output: what fp16 drops of the probabilities too
   for (uint32_t place = 0; run.more(); run.next(), place = 1) {
     const Segment& seg = run.s;
     const uint32_t kvh = seg.row / heads.blocks, h0 = (seg.row - kvh * heads.blocks) * kHeads;
 
     // Q in the order of the keys' registers, below 1 by a power of two a head
-    uint32_t qf[kTiles][L::kProducts][2];  // 8 bits: a pair of products, the upper and lower part
+    // 8 bits: pairs of products, the upper and the middle part; ql the lower
+    uint32_t qf[kTiles][L::kProducts][2];
+    [[maybe_unused]] uint32_t ql[kTiles][kLowSmem || BITS == 4 ? 1 : L::kLow][2];
     float factor[kTiles][2];  // of heads 2 j, 2 j + 1: scale log2(e) and that power
 #pragma unroll
     for (int n = 0; n < kTiles; ++n) {
@@ -592,19 +616,30 @@ __launch_bounds__(Layout<BITS, kQuarters>::kThreads, (Layout<BITS, kQuarters>::c
 #pragma unroll
       for (int s = 0; s < L::kSteps; ++s) {
         if constexpr (BITS == 8) {
+          // q 2^22 = 65536 upper + 256 middle + lower, all signed bytes: those of
+          // v = q 2^22 + 128 (256 + 1), the lower two less 128
+          uint32_t low[4];
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
-            // q 2^14 = 256 upper + lower, both signed bytes
-            uint32_t hi = 0, lo = 0;
+            uint32_t v[4];
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              const int v = __float2int_rn(x[s][4 * i + e] * down * 16384.0f);
-              const int u = (v + 128) >> 8;
-              hi |= (uint32_t)(u & 0xFF) << (8 * e);
-              lo |= (uint32_t)((v - 256 * u) & 0xFF) << (8 * e);
+            for (int e = 0; e < 4; ++e)
+              v[e] = __float_as_uint(fmaf(x[s][4 * i + e] * down, 0x1p22f, kRoundMagic)) -
+                     (uint32_t)kSumBits + 0x8080u;
+            const uint32_t a = __byte_perm(v[0], v[1], 0x5140), b = __byte_perm(v[2], v[3], 0x5140);
+            qf[n][4 * s + i / 2 * 2][i & 1] = __byte_perm(
+                __byte_perm(v[0], v[1], 0x0062), __byte_perm(v[2], v[3], 0x0062), 0x5410);
+            qf[n][4 * s + i / 2 * 2 + 1][i & 1] = __byte_perm(a, b, 0x7632) ^ 0x80808080u;
+            low[i] = __byte_perm(a, b, 0x5410) ^ 0x80808080u;
+          }
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            if constexpr (kLowSmem) {
+              sts64(low_at + 256 * (n * L::kLow + 2 * s + i), low[2 * i], low[2 * i + 1]);
+            } else {
+              ql[n][2 * s + i][0] = low[2 * i];
+              ql[n][2 * s + i][1] = low[2 * i + 1];
             }
-            qf[n][4 * s + i / 2 * 2][i & 1] = hi;
-            qf[n][4 * s + i / 2 * 2 + 1][i & 1] = lo;
           }
         } else {
 #pragma unroll
@@ -619,7 +654,7 @@ __launch_bounds__(Layout<BITS, kQuarters>::kThreads, (Layout<BITS, kQuarters>::c
 #pragma unroll
       for (int r = 0; r < 2; ++r)
         factor[n][r] = __shfl_sync(0xffffffffu, up, 4 * (2 * j + r)) * (scale * kLog2e) *
-                       (BITS == 8 ? 0x1p-6f : 0x1p8f);
+                       (BITS == 8 ? 0x1p-14f : 0x1p8f);
     }
 
     // o[n][p][i]: channels 16 (g + 8 p) + 2 i, + 1 of heads 2 j, 2 j + 1
@@ -667,7 +702,11 @@ __launch_bounds__(Layout<BITS, kQuarters>::kThreads, (Layout<BITS, kQuarters>::c
         // ---- S^T = K Q^T
         float s[kTiles][4] = {};
         if constexpr (BITS == 8) {
-          int hi[kTiles][4] = {}, lo[kTiles][4] = {};
+          int hi[kTiles][4], mid[kTiles][4], lo[kTiles][4];
+#pragma unroll
+          for (int n = 0; n < kTiles; ++n)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) hi[n][e] = mid[n][e] = lo[n][e] = kSumBits;
 #pragma unroll
           for (int st = 0; st < L::kSteps; ++st) {
             uint4 kw[2];
@@ -678,9 +717,19 @@ __launch_bounds__(Layout<BITS, kQuarters>::kThreads, (Layout<BITS, kQuarters>::c
             for (int n = 0; n < kTiles; ++n) {
               const uint32_t(*f)[2] = &qf[n][4 * st];
               mma_s8(hi[n], kw[0].x, kw[1].x, kw[0].y, kw[1].y, f[0][0], f[0][1]);
-              mma_s8(lo[n], kw[0].x, kw[1].x, kw[0].y, kw[1].y, f[1][0], f[1][1]);
+              mma_s8(mid[n], kw[0].x, kw[1].x, kw[0].y, kw[1].y, f[1][0], f[1][1]);
               mma_s8(hi[n], kw[0].z, kw[1].z, kw[0].w, kw[1].w, f[2][0], f[2][1]);
-              mma_s8(lo[n], kw[0].z, kw[1].z, kw[0].w, kw[1].w, f[3][0], f[3][1]);
+              mma_s8(mid[n], kw[0].z, kw[1].z, kw[0].w, kw[1].w, f[3][0], f[3][1]);
+              uint2 f0, f1;
+              if constexpr (kLowSmem) {
+                f0 = lds64(low_at + 256 * (n * L::kLow + 2 * st));
+                f1 = lds64(low_at + 256 * (n * L::kLow + 2 * st + 1));
+              } else {
+                f0 = make_uint2(ql[n][2 * st][0], ql[n][2 * st][1]);
+                f1 = make_uint2(ql[n][2 * st + 1][0], ql[n][2 * st + 1][1]);
+              }
+              mma_s8(lo[n], kw[0].x, kw[1].x, kw[0].y, kw[1].y, f0.x, f0.y);
+              mma_s8(lo[n], kw[0].z, kw[1].z, kw[0].w, kw[1].w, f1.x, f1.y);
             }
           }
           const float ks[2] = {__uint_as_float(lds32(key_scale + stage_at)),
@@ -689,7 +738,9 @@ __launch_bounds__(Layout<BITS, kQuarters>::kThreads, (Layout<BITS, kQuarters>::c
           for (int n = 0; n < kTiles; ++n)
 #pragma unroll
             for (int e = 0; e < 4; ++e)
-              s[n][e] = (float)(hi[n][e] * 256 + lo[n][e]) * ks[e >> 1];
+              s[n][e] = fmaf(whole_sum(hi[n][e]), 65536.0f,
+                             fmaf(whole_sum(mid[n][e]), 256.0f, whole_sum(lo[n][e]))) *
+                        ks[e >> 1];
         } else {
           float s2[kTiles][4] = {};  // every other product: a shorter chain
 #pragma unroll
@@ -1194,15 +1245,15 @@ mb_status launch(const Call& a) {
     return set_error(MB_ERR_CUDA, "cuTensorMapEncodeTiled rejected the cache");
   auto* kernel = cache_attention_kernel<BITS, kQuarters, kTiles>;
   static std::atomic<uint64_t> attr_done{0};
-  MB_CUDA_TRY(set_smem_limit_once(kernel, L::kSmem, attr_done));
+  MB_CUDA_TRY(set_smem_limit_once(kernel, L::smem(kTiles), attr_done));
   const uint32_t rows = a.c.heads * a.heads.blocks;
   Lengths lengths = a.lengths;
   lengths.unit = L::kUnit;
   lengths.idle = idle_units(a.heads.group);
   const uint32_t shares = a.parts == nullptr ? 0 : 148 * L::ctas(kTiles);
   const unsigned grid = shares > 0 ? shares : a.lengths.batch * rows;
-  MB_CUDA_TRY(launch_dependent(kernel, grid, L::kThreads, L::kSmem, a.stream, k_map, v_map, a.c,
-                               box_rows, a.q, a.heads, a.table, a.table_stride, lengths, a.scale,
+  MB_CUDA_TRY(launch_dependent(kernel, grid, L::kThreads, L::smem(kTiles), a.stream, k_map, v_map,
+                               a.c, box_rows, a.q, a.heads, a.table, a.table_stride, lengths, a.scale,
                                shares, a.parts, a.out));
   if (shares > 0) {
     dim3 joins(a.lengths.batch * rows);

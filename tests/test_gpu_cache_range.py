@@ -106,3 +106,20 @@ def test_one_token_with_nearly_all_weight(n, dim, group, dtype, bits_ahead, bits
     v = 1 + 0.1 * v
     v[0] = 0
     _attend(q.to(dtype), k.to(dtype), v.to(dtype), bits, scale)
+
+
+@pytest.mark.parametrize("bits", [8, 4])
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16], ids=["fp16", "bf16"])
+@pytest.mark.parametrize("n", [2, 5, 300, 3000])
+@pytest.mark.parametrize("dim,group", [(64, 1), (128, 12), (192, 3)])
+def test_query_channels_far_above_the_others(n, dim, group, dtype, bits):
+    """One channel of the query a thousand times the others, where the keys
+    have nothing."""
+    if bits == 4 and dim == 192:
+        dim = 160
+    q, k, v = _inputs(n, 2, group, dim, seed=n)
+    q[..., 5] = 1000
+    k[..., 5] = 0
+    if bits == 4:  # a group of its own, so that its code 0 stands for 0
+        k[..., :32] = 0
+    _attend(q.to(dtype), k.to(dtype), v.to(dtype), bits, 1 / math.sqrt(dim))
