@@ -492,7 +492,9 @@ size_t mb_cache_attention_workspace_size(const mb_kv_cache* cache, int64_t batch
  * bf16).  A length beyond the table counts as the table's, tokens of a page
  * outside [0, pages) are left out, and a sequence with no token gives 0.
  * scale is finite; pages * kv_heads * page_size is below 2^31.  A query, key or
- * value that is not finite gives outputs that are NaN.  If a wait inside the
+ * value that is not finite gives outputs that are NaN; a 4-bit cache's
+ * values (not its keys) are taken in fp16 here: beyond 65504 they count as
+ * infinite.  If a wait inside the
  * kernel ran out (2 s), the outputs it concerns are NaN.  workspace: 16-byte
  * aligned. */
 mb_status mb_cache_attention(const mb_kv_cache* cache, const void* q, int64_t q_batch_stride,

@@ -17,21 +17,30 @@
 //
 // Both products' left operands are read as they lie, because the order of the
 // inner index is free: in S^T lane (g, j) = (lane / 4, lane % 4) takes 16 bytes
-// of the rows of tokens g and g + 8, in O^T 16 channels of the four tokens of
-// its columns; Q's registers follow the keys' channel order.  The boxes' swizzle,
-// the 16-byte chunks 2 j + step and the tokens' order (token_of) keep these
-// reads free of bank conflicts.  Between the products the probabilities
-// change from S^T's layout to the right operand's by a transposing move.
+// (4 bits: 4 of each group's 16) of the rows of tokens g and g + 8, in O^T 16
+// channels of the four tokens of its columns; Q's registers follow the keys'
+// channel order.  The boxes' swizzle, the 16-byte chunks 2 j + step and the
+// tokens' order (token_of) keep these reads free of bank conflicts.  Between
+// the products the probabilities change from S^T's layout to the right
+// operand's by a transposing move.
 //
 // 8-bit keys enter S^T as they are: an m16n8k32 integer product with the
 // query, scaled by a power of two to below 1, in three 8-bit parts (22 bits and
 // a sign: off by at most 2^-22 of the query's largest channel, exact for
 // channels above 2^-11 of it; with two parts, 14 bits, a channel far above the
 // others cost them theirs, and 16 x 2048 took 39.6 us for 41.0, 2 x 100001 65.5 for
-// 69.0).  The sums are exact.  8-bit values become exact fp16 integers (1024 + 128 + code by a byte permute,
-// minus 1152); their scale multiplies the probability.
-// 4-bit codes become m + s * code in fp16, one rounding; the query then is
-// fp16 too.  Scores, maxima, sums and the outputs' accumulators are fp32.
+// 69.0).  The sums are exact.  8-bit values become exact fp16 integers (1024 +
+// 128 + code by a byte permute, minus 1152); their scale multiplies the
+// probability.
+//
+// 4-bit keys enter S^T as codes, too: their pairs under a mask are subnormal
+// fp16 numbers, code 2^-24 (the upper ones code 2^-20), and exact.  The query is
+// fp16 relative to its largest channel (up to 2^15: exact for channels above
+// 2^-25 of it); a group's sum is multiplied by its scale, and its minimum by the
+// query's sum over the group, in fp32.  4-bit values become m + s * code in fp16,
+// one rounding (2^-11 of the value; beyond 65504 infinite).
+//
+// Scores, maxima, sums and the outputs' accumulators are fp32.
 //
 // Weights -- probabilities, with 8 bits times the value's scale -- are rounded
 // to fp16 (2^-11), and for an fp16 output, whose own rounding is no larger,
@@ -159,10 +168,12 @@ struct Layout {
     return kQuarters > 2 || tiles == 2 ? 2 : 3;
   }
 
-  // S^T: steps of 4 lanes x kKeyWords words; O^T: passes of 8 lanes x 16 channels
-  static constexpr int kKeyWords = BITS == 4 && kQuarters == 1 ? 2 : 4;
-  static constexpr int kSteps = kRow / (16 * kKeyWords);
-  static constexpr int kProducts = kSteps * (BITS == 8 ? 4 : 2 * kKeyWords);  // of S^T
+  // S^T: steps of 4 lanes x 4 words, or groups of 4 lanes x a word; O^T: passes of 8
+  // lanes x 16 channels
+  static constexpr int kSteps = kRow / 64;                           // 8 bits
+  static constexpr int kGroups = kRow / 16;                          // 4 bits: of 32 channels
+  static constexpr int kProducts = BITS == 8 ? 4 * kSteps : 2 * kGroups;  // of S^T
+  static constexpr int kPieces = BITS == 8 ? 2 * kSteps : kGroups;   // a lane's, of 8 channels
   // 8 bits: the products with the query's lower part, whose operand two CTAs an SM
   // leave in shared memory, each lane its own (three have the registers for it)
   static constexpr int kLow = BITS == 8 ? 2 * kSteps : 0;
@@ -177,7 +188,10 @@ struct Layout {
   static constexpr int kJoin = kWarps * 8 * kJoinRow * 4;
   static constexpr int kRing = kStages * kStage;
   __host__ __device__ static constexpr int smem(int tiles) {
-    return 1024 + kRing + kJoin + (low_in_smem(tiles) ? kWarps * 32 * 8 * kLow * tiles : 0);
+    return 1024 + kRing + kJoin +
+           (BITS == 4            ? kWarps * kGroups * 8 * 4 * tiles
+            : low_in_smem(tiles) ? kWarps * 32 * 8 * kLow * tiles
+                                 : 0);
   }
 
   // Place in a stage's keys (or values) of a byte of a row.
@@ -185,11 +199,15 @@ struct Layout {
     const uint32_t o = row * kBoxRow + byte % kBoxRow;
     return byte / kBoxRow * kColumn + (o ^ ((o >> 3) & kSwizzle));
   }
-  // First byte of lane j's part of a key's row in a step.
+  // 8 bits: first byte of lane j's part of a key's row in a step.
   __device__ __forceinline__ static uint32_t key_byte(int step, int j) {
-    if constexpr (kKeyWords == 2) return 8 * j;
     if constexpr (kSteps == 1) return 16 * j;
     return 128 * (step / 2) + 16 * (2 * j + step % 2);
+  }
+  // First channel of lane j's piece of 8.
+  __device__ __forceinline__ static uint32_t piece_channel(int piece, int j) {
+    if constexpr (BITS == 8) return key_byte(piece / 2, j) + 8 * (piece % 2);
+    return 32 * piece + 8 * j;
   }
 };
 
@@ -231,6 +249,16 @@ __device__ __forceinline__ uint2 lds64(uint32_t at) {
   uint2 v;
   asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(at));
   return v;
+}
+// Four 8 x 16-byte matrices, a row a lane's address: lane (g, j) has bytes 4 j .. of
+// row g of each.
+__device__ __forceinline__ void ldmatrix4(uint32_t (&v)[4], uint32_t at) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];"
+               : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3])
+               : "r"(at));
+}
+__device__ __forceinline__ void sts32(uint32_t at, uint32_t x) {
+  asm volatile("st.shared.u32 [%0], %1;" ::"r"(at), "r"(x));
 }
 __device__ __forceinline__ void sts64(uint32_t at, uint32_t x, uint32_t y) {
   asm volatile("st.shared.v2.u32 [%0], {%1, %2};" ::"r"(at), "r"(x), "r"(y));
@@ -551,7 +579,10 @@ __launch_bounds__(Layout<BITS, kQuarters>::kThreads, (Layout<BITS, kQuarters>::c
   uint32_t key_at[2], value_at[2];  // in a stage: steps 0 and 1 (2 and 3: a box column on)
 #pragma unroll
   for (int x = 0; x < 2; ++x) {
-    key_at[x] = ring0 + L::at(16 * warp + row0, L::key_byte(L::kSteps > 1 ? x : 0, j));
+    // 4 bits: lane 8 i + r names row r of the i-th of four 8 x 16-byte matrices
+    key_at[x] = ring0 + (BITS == 8
+                             ? L::at(16 * warp + row0, L::key_byte(L::kSteps > 1 ? x : 0, j))
+                             : L::at(16 * warp + token_of(lane & 7) + (lane & 8), lane & 16));
     // past the row (64-channel rows have 4 lanes' pieces): any, not stored
     const uint32_t byte = (kQuarters == 1 ? g & 3 : g) * 2 * BITS;
     value_at[x] = ring0 + L::kCodes + L::at(16 * warp + column[x], byte);
@@ -569,6 +600,9 @@ __launch_bounds__(Layout<BITS, kQuarters>::kThreads, (Layout<BITS, kQuarters>::c
   constexpr bool kLowSmem = L::low_in_smem(kTiles);
   [[maybe_unused]] const uint32_t low_at =
       ring0 + L::kRing + L::kJoin + 8 * (warp * 32 * L::kLow * kTiles + lane);
+  // 4 bits: the sums of the query's groups [tile][group][8 heads], each warp its own
+  [[maybe_unused]] const uint32_t sum_at =
+      ring0 + L::kRing + L::kJoin + 32 * warp * L::kGroups * kTiles;
   const bool fine = !q.bf16;  // an fp16 output: what fp16 drops of the probabilities too
   for (uint32_t place = 0; run.more(); run.next(), place = 1) {
     const Segment& seg = run.s;
@@ -585,25 +619,18 @@ __launch_bounds__(Layout<BITS, kQuarters>::kThreads, (Layout<BITS, kQuarters>::c
       const bool live = h < heads.group;
       const int64_t at = (int64_t)seg.b * q.batch_stride +
                          (int64_t)(kvh * heads.group + (live ? h : 0)) * q.head_stride;
-      constexpr int kPer = L::kKeyWords * 32 / BITS;  // channels of a lane in a step
-      float x[L::kSteps][kPer];
+      float x[L::kPieces][8] = {};
       uint32_t top = 0;
 #pragma unroll
-      for (int s = 0; s < L::kSteps; ++s) {
-        const uint32_t ch = L::key_byte(s, j) * 8 / BITS;
-#pragma unroll
-        for (int e = 0; e < kPer / 8; ++e) {
-          float y[8] = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
-          if (live && ch + 8 * e < c.dim) {
-            if (q.bf16)
-              load8(static_cast<const __nv_bfloat16*>(q.data) + at + ch + 8 * e, q.vec, 8, y);
-            else
-              load8(static_cast<const __half*>(q.data) + at + ch + 8 * e, q.vec, 8, y);
-          }
-          top = max(top, abs_bits_max(y));
-#pragma unroll
-          for (int i = 0; i < 8; ++i) x[s][8 * e + i] = y[i];
+      for (int s = 0; s < L::kPieces; ++s) {
+        const uint32_t ch = L::piece_channel(s, j);
+        if (live && ch < c.dim) {
+          if (q.bf16)
+            load8(static_cast<const __nv_bfloat16*>(q.data) + at + ch, q.vec, 8, x[s]);
+          else
+            load8(static_cast<const __half*>(q.data) + at + ch, q.vec, 8, x[s]);
         }
+        top = max(top, abs_bits_max(x[s]));
       }
       top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
       top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
@@ -613,9 +640,9 @@ __launch_bounds__(Layout<BITS, kQuarters>::kThreads, (Layout<BITS, kQuarters>::c
       const uint32_t ex = min(max(top >> 23, 8u), 254u);
       const float down = __uint_as_float(ex <= 252 ? (253 - ex) << 23 : 0x00800000u >> (ex - 252));
       const float up = __uint_as_float(top >= 0x7F800000u ? 0x7FC00000u : (ex - 7) << 23);
+      if constexpr (BITS == 8) {
 #pragma unroll
-      for (int s = 0; s < L::kSteps; ++s) {
-        if constexpr (BITS == 8) {
+        for (int s = 0; s < L::kSteps; ++s) {
           // q 2^22 = 65536 upper + 256 middle + lower, all signed bytes: those of
           // v = q 2^22 + 128 (256 + 1), the lower two less 128
           uint32_t low[4];
@@ -624,7 +651,8 @@ __launch_bounds__(Layout<BITS, kQuarters>::kThreads, (Layout<BITS, kQuarters>::c
             uint32_t v[4];
 #pragma unroll
             for (int e = 0; e < 4; ++e)
-              v[e] = __float_as_uint(fmaf(x[s][4 * i + e] * down, 0x1p22f, kRoundMagic)) -
+              v[e] = __float_as_uint(fmaf(x[2 * s + i / 2][4 * (i & 1) + e] * down, 0x1p22f,
+                                          kRoundMagic)) -
                      (uint32_t)kSumBits + 0x8080u;
             const uint32_t a = __byte_perm(v[0], v[1], 0x5140), b = __byte_perm(v[2], v[3], 0x5140);
             qf[n][4 * s + i / 2 * 2][i & 1] = __byte_perm(
@@ -641,20 +669,34 @@ __launch_bounds__(Layout<BITS, kQuarters>::kThreads, (Layout<BITS, kQuarters>::c
               ql[n][2 * s + i][1] = low[2 * i + 1];
             }
           }
-        } else {
-#pragma unroll
-          for (int i = 0; i < 2 * L::kKeyWords; ++i) {
-            const int c0 = 8 * (i / 2) + 2 * (i & 1);  // code4_pair's channels
-            uint32_t(&f)[2] = qf[n][s * 2 * L::kKeyWords + i];
-            f[0] = h2_bits(__floats2half2_rn(x[s][c0] * down, x[s][c0 + 4] * down));
-            f[1] = h2_bits(__floats2half2_rn(x[s][c0 + 1] * down, x[s][c0 + 5] * down));
-          }
         }
+      } else {
+#pragma unroll
+        for (int s = 0; s < L::kGroups; ++s) {
+          // channels as the codes' pairs have them, to below 2^15 (2^11: codes times 16)
+          float sum = 0.0f;
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            x[s][i] *= down;
+            sum += x[s][i];
+          }
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            uint32_t(&f)[2] = qf[n][2 * s + i];
+            f[0] = h2_bits(__floats2half2_rn(x[s][2 * i] * 0x1p15f, x[s][2 * i + 4] * 0x1p15f));
+            f[1] = h2_bits(__floats2half2_rn(x[s][2 * i + 1] * 0x1p11f, x[s][2 * i + 5] * 0x1p11f));
+          }
+          sum += __shfl_xor_sync(0xffffffffu, sum, 1);
+          sum += __shfl_xor_sync(0xffffffffu, sum, 2);
+          if (j == 0)  // times 2^15, as the others, less the codes' 2^24
+            sts32(sum_at + 32 * (n * L::kGroups + s) + 4 * g, __float_as_uint(sum * 0x1p-9f));
+        }
+        __syncwarp();
       }
 #pragma unroll
       for (int r = 0; r < 2; ++r)
         factor[n][r] = __shfl_sync(0xffffffffu, up, 4 * (2 * j + r)) * (scale * kLog2e) *
-                       (BITS == 8 ? 0x1p-14f : 0x1p8f);
+                       (BITS == 8 ? 0x1p-14f : 0x1p17f);
     }
 
     // o[n][p][i]: channels 16 (g + 8 p) + 2 i, + 1 of heads 2 j, 2 j + 1
@@ -742,49 +784,50 @@ __launch_bounds__(Layout<BITS, kQuarters>::kThreads, (Layout<BITS, kQuarters>::c
                              fmaf(whole_sum(mid[n][e]), 256.0f, whole_sum(lo[n][e]))) *
                         ks[e >> 1];
         } else {
-          float s2[kTiles][4] = {};  // every other product: a shorter chain
+          // sum of q k = sum over the groups of s (sum of q code) + m (sum of q), the
+          // sums in fp32: nothing is rounded to fp16
+          uint64_t both[kTiles][2];  // heads 2 j, 2 j + 1 of a token
 #pragma unroll
-          for (int st = 0; st < L::kSteps; ++st) {
-            uint32_t kw[2][4];
-            __half2 gs[2], gm[2];
+          for (int n = 0; n < kTiles; ++n) both[n][0] = both[n][1] = 0;
 #pragma unroll
-            for (int r = 0; r < 2; ++r) {
-              // 128-channel steps of rows in one box: 16-byte chunks 2 j and 2 j + 1
-              const uint32_t at = key_at[st] + stage_at + r * kEight;
-              if constexpr (L::kKeyWords == 4) {
-                const uint4 v = lds128(at);
-                kw[r][0] = v.x; kw[r][1] = v.y; kw[r][2] = v.z; kw[r][3] = v.w;
-              } else {
-                const uint2 v = lds64(at);
-                kw[r][0] = v.x; kw[r][1] = v.y;
-              }
-              // past head_dim the query is 0 (any group's scale will do)
-              const __half2 pair =
-                  bits_h2(lds32(key_scale + stage_at + r * eight_scales +
-                                4 * min((int)L::key_byte(st, j) / 16, last_group)));
-              gs[r] = __low2half2(pair);
-              gm[r] = __high2half2(pair);
-            }
+          for (int i = 0; i < L::kGroups; i += 2) {
+            uint32_t kw[4];
+            ldmatrix4(kw, (key_at[0] ^ (16 * i)) + stage_at);
 #pragma unroll
-            for (int i = 0; i < 2 * L::kKeyWords; ++i) {
-              uint32_t a[2][2];
+            for (int h = 0; h < 2; ++h) {
+              uint64_t gs[2], gm[2];
 #pragma unroll
               for (int r = 0; r < 2; ++r) {
-                const uint32_t x = kw[r][i / 2] >> (8 * (i & 1));
-                a[r][0] = code4_pair<false>(x, gs[r], gm[r]);
-                a[r][1] = code4_pair<true>(x, gs[r], gm[r]);
+                // past head_dim the query is 0 (any group's scale will do)
+                const float2 pair = __half22float2(
+                    bits_h2(lds32(key_scale + stage_at + r * eight_scales +
+                                  4 * min(i + h, last_group))));
+                gs[r] = f2_pack(pair.x, pair.x);
+                gm[r] = f2_pack(pair.y, pair.y);
               }
+              const uint32_t w0 = kw[2 * h], w1 = kw[2 * h + 1];
 #pragma unroll
               for (int n = 0; n < kTiles; ++n) {
-                const uint32_t(&f)[2] = qf[n][st * 2 * L::kKeyWords + i];
-                mma_f16(i & 1 ? s2[n] : s[n], a[0][0], a[1][0], a[0][1], a[1][1], f[0], f[1]);
+                float sum[4] = {};
+#pragma unroll
+                for (int x = 0; x < 2; ++x) {
+                  const uint32_t(&f)[2] = qf[n][2 * (i + h) + x];
+                  mma_f16(sum, w0 >> (8 * x) & 0x000F000Fu, w1 >> (8 * x) & 0x000F000Fu,
+                          w0 >> (8 * x) & 0x00F000F0u, w1 >> (8 * x) & 0x00F000F0u, f[0], f[1]);
+                }
+                const uint2 qs = lds64(sum_at + 32 * (n * L::kGroups + i + h) + 8 * j);
+                const uint64_t q2 = f2_pack(__uint_as_float(qs.x), __uint_as_float(qs.y));
+#pragma unroll
+                for (int r = 0; r < 2; ++r)
+                  both[n][r] = f2_fma(gs[r], f2_pack(sum[2 * r], sum[2 * r + 1]),
+                                      f2_fma(gm[r], q2, both[n][r]));
               }
             }
           }
 #pragma unroll
           for (int n = 0; n < kTiles; ++n)
 #pragma unroll
-            for (int e = 0; e < 4; ++e) s[n][e] += s2[n][e];
+            for (int r = 0; r < 2; ++r) f2_unpack(both[n][r], s[n][2 * r], s[n][2 * r + 1]);
         }
 
         // ---- scores in powers of two; weights, and what they are relative to

@@ -142,8 +142,9 @@ def cache_attention(q: torch.Tensor, cache: QuantizedCache, page_table: torch.Te
     lengths[b] of the cache, token t in page page_table[b, t // page_size]
     (int32 [batch, pages]; lengths int32 [batch]).  ``scale`` defaults to
     1 / sqrt(head_dim).  The cache is read as it is held, never expanded in
-    memory.  Tokens of a page outside the cache are left out; a sequence
-    without tokens gives zeros."""
+    memory (the values of a 4-bit one in fp16: infinite beyond 65504).  Tokens
+    of a page outside the cache are left out; a sequence without tokens gives
+    zeros."""
     if scale is None:
         scale = 1.0 / math.sqrt(cache.head_dim)
     return _C.cache_attention(q, cache, page_table, lengths, scale, out)

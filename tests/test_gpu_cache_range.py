@@ -90,11 +90,12 @@ def test_large_values_without_weight(n, dim, group, dtype, size):
     _attend(q.to(dtype), k.to(dtype), v.to(dtype), 8, 1 / math.sqrt(dim))
 
 
-@pytest.mark.parametrize("bits_ahead,bits", [(20, 8), (27, 8), (27, 4)])
+@pytest.mark.parametrize("bits", [8, 4])
 @pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16], ids=["fp16", "bf16"])
 @pytest.mark.parametrize("n", LENGTHS)
+@pytest.mark.parametrize("bits_ahead", [20, 27])
 @pytest.mark.parametrize("dim,group", [(64, 1), (128, 12), (256, 3)])
-def test_one_token_with_nearly_all_weight(n, dim, group, dtype, bits_ahead, bits):
+def test_one_token_with_nearly_all_weight(n, dim, group, bits_ahead, dtype, bits):
     """The first token has 2^20 or 2^27 times the others' weight and values of
     0: the output is what the others add."""
     q, k, v = _inputs(n, 2, group, dim, seed=n)
@@ -123,3 +124,30 @@ def test_query_channels_far_above_the_others(n, dim, group, dtype, bits):
     if bits == 4:  # a group of its own, so that its code 0 stands for 0
         k[..., :32] = 0
     _attend(q.to(dtype), k.to(dtype), v.to(dtype), bits, 1 / math.sqrt(dim))
+
+
+@pytest.mark.parametrize("bits", [8, 4])
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16], ids=["fp16", "bf16"])
+@pytest.mark.parametrize("n", [2, 5, 300, 3000])
+@pytest.mark.parametrize("dim,group", [(32, 1), (96, 5), (128, 12), (256, 3)])
+def test_keys_far_from_zero(n, dim, group, dtype, bits):
+    """Each group of channels lies around 500 or -500, a few steps wide."""
+    q, k, v = _inputs(n, 2, group, dim, seed=n)
+    side = torch.where(torch.arange(dim) // 32 % 2 == 0, 500.0, -500.0)
+    _attend(q.to(dtype), (k + side).to(dtype), v.to(dtype), bits, 1 / math.sqrt(dim))
+
+
+def test_values_of_a_4_bit_cache_beyond_fp16():
+    """Read back they are finite; the attention takes them as infinite.  Keys may
+    be as large as the cache holds."""
+    q, k, v = _inputs(70, 1, 2, 64, seed=1)
+    v[33, 0, 40] = 1e5
+    cache, table = _cache(k.bfloat16(), v.bfloat16(), 4)
+    read = mb.cache_read(cache, torch.arange(70, device="cuda"), torch.float32)[1]
+    assert torch.isfinite(read).all() and read[33, 0, 40] > 65504
+    n = torch.tensor([70], dtype=torch.int32).cuda()
+    got = mb.cache_attention(q.bfloat16().cuda(), cache, table.cuda(), n)
+    where = ~torch.isfinite(got)
+    assert where[..., 40].all() and not where[..., :32].any()
+    k[..., 3] = 1e5
+    _attend((q * 1e-4).bfloat16(), k.bfloat16(), torch.ones_like(v).bfloat16(), 4, 1.0)
