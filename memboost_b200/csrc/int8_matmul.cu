@@ -710,8 +710,13 @@ mb_status split_tiles(const Product& p, int parts) {
 template <typename Y>
 mb_status dispatch(const Product& p) {
   // pairs where their tiles give every pair of SMs work (1500 x 4096 x 4096:
-  // 30.4 us either way; 1024: 19.2 with pairs, 18.1 without)
-  if (ceil_div(p.N, 2 * kChannels) * ceil_div(p.M, kPairTokens) >= kSms / 2)
+  // 30.4 us either way; 1024: 19.2 with pairs, 18.1 without), unless most of
+  // their 256 columns are empty (a wide N and few tokens, weights from HBM, with
+  // pairs and without: 28672 x 8192 1 token 66.5 and 41.6 us, 64 56.1 and 44.1, 128
+  // 58.3 and 56.1, 256 61.9 and 70.2; 32000 x 4096 43.8 and 26.6, 35.8 and 26.9, 37.1
+  // and 38.7, 37.9 and 46.0)
+  if (p.M > 64 &&
+      ceil_div(p.N, 2 * kChannels) * ceil_div(p.M, kPairTokens) >= kSms / 2)
     return launch_pairs<Y>(p);
   const Tiling t = tiling_for(p.M, p.N, p.K);
   switch (t.tokens) {

@@ -146,6 +146,20 @@ def test_product(M, N, K, dtype):
                            mb.int8_matmul(x, w, out_dtype=out))
 
 
+@pytest.mark.parametrize("M", [1, 16, 64, 65, 256])
+@pytest.mark.parametrize("N,K", [(19100, 300), (32000, 1024)])
+def test_product_few_tokens_over_many_channels(M, N, K):
+    """On either side of where the kernel changes: the sums are whole numbers,
+    so a wide product equals its parts'."""
+    x = _x(M, K, torch.bfloat16, seed=M).cuda()
+    w = mb.quantize_int8(_x(N, K, torch.float32, seed=N, spread=False).cuda() * 0.02)
+    y = mb.int8_matmul(x, w)
+    parts = [mb.Int8Tensor(w.codes[n:n + 3000], w.scales[n:n + 3000]) for n in range(0, N, 3000)]
+    assert torch.equal(y, torch.cat([mb.int8_matmul(x, p) for p in parts], 1))
+    some = slice(N - 500, N)
+    _check_product(y[:, some], mb.quantize_int8(x), mb.Int8Tensor(w.codes[some], w.scales[some]))
+
+
 @pytest.mark.parametrize("M", [1, 20, 150, 600])
 def test_product_largest_sums(M):
     """All codes +-127 over the longest K: sums next to 2^31."""
