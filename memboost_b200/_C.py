@@ -14,6 +14,7 @@ from __future__ import annotations
 import contextlib
 import ctypes
 import os
+import warnings
 
 import torch
 
@@ -27,7 +28,32 @@ for _path in (_LIB_PATH, os.path.join(os.path.dirname(_LIB_PATH), "_calls.so")):
 
 _lib = ctypes.CDLL(_LIB_PATH)
 
-from . import _calls  # noqa: E402  (csrc/calls.cpp, built beside the library)
+
+class _NoCalls:
+    """In place of csrc/calls.cpp's module: takes no call."""
+
+    def __getattr__(self, name):
+        return lambda *args: None
+
+
+def _load_calls():
+    """csrc/calls.cpp's module, built beside the library.  It belongs to one
+    torch's C++ interface; with another the calls it would take go the longer
+    way through ctypes, and everything else is as it was."""
+    try:
+        from . import _calls
+        if _calls.torch_version == str(torch.__version__):
+            return _calls
+        why = f"built for torch {_calls.torch_version}, this is {torch.__version__}"
+    except ImportError as e:
+        why = str(e)
+    warnings.warn(f"memboost_b200: _calls.so is not used ({why}): the 8-bit and cache calls take "
+                  "some 10 us longer; `python memboost_b200/build.py` builds it for this torch",
+                  RuntimeWarning, stacklevel=3)
+    return _NoCalls()
+
+
+_calls = _load_calls()
 
 _P = ctypes.c_void_p
 _I64 = ctypes.c_int64

@@ -6,7 +6,8 @@ Every translation unit is compiled for sm_100a only
 shared library with a statically linked CUDA runtime.  The library exports
 exactly the C ABI declared in include/memboost_b200.h.  nvcc cross-compiles,
 so this runs on machines without a GPU.  _calls.so is a CPython module over
-torch's tensors that calls the library.
+torch's tensors that calls the library: it belongs to the torch and Python it was
+built with, and is built again when either has changed.
 
 Usage: python memboost_b200/build.py [--force] [-v]
 (run by path: importing the package needs the library this builds)
@@ -29,6 +30,7 @@ INCLUDE = os.path.join(ROOT, "include")
 BUILD = os.path.join(PKG, "_build")
 LIB = os.path.join(PKG, "libmemboost_b200.so")
 CALLS = os.path.join(PKG, "_calls.so")
+CALLS_FOR = os.path.join(BUILD, "_calls.for")  # the torch and Python it was built with
 
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 NVCC_FLAGS = ["-O3", "-std=c++17", "-lineinfo", "-Xcompiler", "-fPIC", "-Xcompiler", "-O3",
@@ -69,17 +71,38 @@ def _compile(src: str, verbose: bool) -> str:
     return obj
 
 
-def _build_calls(verbose: bool) -> None:
+def _torch() -> tuple[str, str]:
+    """(directory, version) of the installed torch, without importing it."""
+    where = importlib.util.find_spec("torch").submodule_search_locations[0]
+    scope: dict = {}
+    with open(os.path.join(where, "version.py")) as f:
+        exec(f.read(), scope)
+    return where, str(scope["__version__"])
+
+
+def _calls_stale(made_for: str) -> bool:
     src = os.path.join(CSRC, "calls.cpp")
-    if not _stale(CALLS, [src, __file__, os.path.join(INCLUDE, "memboost_b200.h")]):
+    if _stale(CALLS, [src, __file__, os.path.join(INCLUDE, "memboost_b200.h")]):
+        return True
+    if not os.path.exists(CALLS_FOR):
+        return True
+    with open(CALLS_FOR) as f:
+        return f.read() != made_for
+
+
+def _build_calls(verbose: bool) -> None:
+    torch, version = _torch()
+    made_for = f"torch {version}, Python {sysconfig.get_python_version()}\n"
+    if not _calls_stale(made_for):
         return
-    torch = importlib.util.find_spec("torch").submodule_search_locations[0]
+    src = os.path.join(CSRC, "calls.cpp")
     system = [os.path.join(torch, "include"),
               os.path.join(torch, "include", "torch", "csrc", "api", "include"),
               sysconfig.get_paths()["include"],
               os.path.join(os.environ.get("CUDA_HOME", "/usr/local/cuda"), "include")]
     tmp = CALLS + ".tmp"
-    cmd = [os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-fPIC", "-shared", "-I", INCLUDE]
+    cmd = [os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-fPIC", "-shared", "-I", INCLUDE,
+           f'-DMB_TORCH_VERSION="{version}"']
     for d in system:
         cmd += ["-isystem", d]
     cmd += [src, "-o", tmp, "-L", PKG, "-l:libmemboost_b200.so", "-L", os.path.join(torch, "lib"),
@@ -91,6 +114,8 @@ def _build_calls(verbose: bool) -> None:
     if r.returncode != 0:
         raise RuntimeError(f"building {CALLS} failed:\n{r.stdout}\n{r.stderr}")
     os.replace(tmp, CALLS)
+    with open(CALLS_FOR, "w") as f:
+        f.write(made_for)
 
 
 def build(force: bool = False, verbose: bool = False) -> str:
