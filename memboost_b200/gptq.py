@@ -147,7 +147,9 @@ class Int8Linear(nn.Module):
     """Linear layer with its weight in 8 bits, a scale for each output
     channel, and its input quantised a token at a time: int8_matmul on the
     tensor cores instead of QuantizedLinear's fp16 product, without expanding
-    the weight in each call.  No counterpart in the reference."""
+    the weight in each call.  For serving: it has no gradient, and refuses an
+    input that wants one (QuantizedLinear passes it on).  No counterpart in
+    the reference."""
 
     def __init__(self, weight: Int8Tensor, bias: torch.Tensor | None = None):
         super().__init__()
@@ -161,6 +163,9 @@ class Int8Linear(nn.Module):
         return cls(quantize_int8(dequantize(q_weight)))
 
     def forward(self, x: torch.Tensor) -> torch.Tensor:
+        if x.requires_grad and torch.is_grad_enabled():
+            raise RuntimeError("Int8Linear has no gradient: call it under torch.no_grad() or with "
+                               "x.detach()")
         return int8_matmul(x, self.weight, bias=self.bias)
 
 

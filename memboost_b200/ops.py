@@ -96,7 +96,10 @@ def quantize_int8(x: torch.Tensor) -> Int8Tensor:
     flattened) in 8 bits: a token's activations, or an output channel's
     weights.  scale = max|row| / 127 in fp32, code = x / scale to the nearest
     integer (ties to even).  A row of zeros has scale 0; a row that holds a NaN
-    or an infinity has scale NaN, and whatever is computed from it is NaN."""
+    or an infinity has scale NaN, and whatever is computed from it is NaN.
+
+    Neither this nor the calls below have gradients: what they return never
+    requires one, whatever their inputs do."""
     return Int8Tensor(*_C.quantize_int8(x))
 
 

@@ -230,3 +230,17 @@ def test_calls_leave_the_unusual_alone(mb):
         for i in range(len(args)):
             for other in (None, 1, "x", torch.float64, torch.zeros(0)):
                 assert fn(*args[:i], other, *args[i + 1:]) is None
+
+
+def test_int8_linear_refuses_an_input_that_wants_a_gradient(mb):
+    from memboost_b200 import gptq
+    lin = gptq.Int8Linear(mb.Int8Tensor(torch.zeros(4, 16, dtype=torch.int8), torch.zeros(4)))
+    x = torch.zeros(2, 16, requires_grad=True)
+    with pytest.raises(RuntimeError, match="no gradient"):
+        lin(x)
+    with pytest.raises(RuntimeError, match="no gradient"):
+        lin(x * 2)
+    with torch.no_grad(), pytest.raises(RuntimeError, match="w.codes must be on CUDA"):
+        lin(x)
+    with pytest.raises(RuntimeError, match="w.codes must be on CUDA"):
+        lin(x.detach())
