@@ -200,7 +200,8 @@ class CachedDecoder:
     them ("layers.<l>.<projection>").  Calls take hidden states [batch, T,
     n_embd] -- a prompt, chunks of it, then single tokens -- and return the last
     layer's.  The sequences' lengths stay on the device: a single token's
-    call does not wait for it."""
+    call does not wait for it, unless the places taken so far, padding
+    included, leave no room and the lengths themselves have to be looked at."""
 
     def __init__(self, cfg: LlamaConfig, layers: dict, batch: int, max_tokens: int,
                  page_size: int = 64, bits: int = 8, n_layers: int | None = None):
@@ -218,7 +219,7 @@ class CachedDecoder:
                                        device=device).view(batch, pages)
         self.lengths = torch.zeros(batch, dtype=torch.int32, device=device)
         self.cos, self.sin = rope_tables(hd, self.max_tokens, cfg.rope_theta, device)
-        self.used = 0  # tokens of the longest sequence
+        self.used = 0  # no sequence holds more (the places of all calls, padding included)
 
     def slots(self, positions: torch.Tensor) -> torch.Tensor:
         """Slots of places [batch, n] of the sequences."""
@@ -236,25 +237,31 @@ class CachedDecoder:
         if x.dim() != 3 or x.shape[0] != self.batch or x.shape[2] != self.cfg.n_embd:
             raise RuntimeError(f"x must be [{self.batch}, T, {self.cfg.n_embd}]")
         T = x.shape[1]
-        if T == 0 or self.used + T > self.max_tokens:
-            raise RuntimeError(f"{T} tokens do not fit behind {self.used} of {self.max_tokens}")
+        if T == 0:
+            raise RuntimeError("x must hold at least one token")
         if tokens is not None:
             if tokens.shape != self.lengths.shape or tokens.dtype != torch.int32 \
                     or tokens.device != self.lengths.device:
                 raise RuntimeError(f"tokens must be int32 [{self.batch}] on the device of the "
                                    "caches")
             tokens = tokens.clamp(0, T)  # places index tables behind a length
+        lengths = self.lengths + (T if tokens is None else tokens)
+        if self.used + T > self.max_tokens:
+            self.used = int(self.lengths.max())
+            if self.used + T > self.max_tokens and int(lengths.max()) > self.max_tokens:
+                raise RuntimeError(f"{T} tokens do not fit behind {self.used} of "
+                                   f"{self.max_tokens}")
+        end = min(self.used + T, self.max_tokens)
         step = torch.arange(T, device=x.device)
         positions = self.lengths.long()[:, None] + step
+        if self.used + T > self.max_tokens:  # padding behind the last place
+            positions = positions.clamp(max=self.max_tokens - 1)
         slots = self.slots(positions)
-        if tokens is None:
-            lengths = self.lengths + T
-        else:
-            lengths = self.lengths + tokens
+        if tokens is not None:
             slots = torch.where(step < tokens[:, None], slots, -1)
         context = None
         if T > 1 and self.used > 0:
-            places = torch.arange(self.used + T, device=x.device).expand(self.batch, -1)
+            places = torch.arange(end, device=x.device).expand(self.batch, -1)
             context = self.slots(places).flatten()
         slots = slots.flatten()
         for i, (linear, cache) in enumerate(zip(self.linears, self.caches)):
@@ -263,7 +270,7 @@ class CachedDecoder:
                               cache=CacheStep(cache, positions, slots, self.page_table, lengths,
                                               context))
         self.lengths = lengths
-        self.used += T
+        self.used = end
         return x
 
 

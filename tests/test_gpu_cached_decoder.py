@@ -131,3 +131,39 @@ def test_counts_of_tokens_outside_the_chunk():
     assert dec.lengths.tolist() == [6, 8, 0]
     y = dec(x[:, :1])
     assert dec.lengths.tolist() == [7, 9, 1] and torch.isfinite(y).all()
+
+
+@pytest.mark.parametrize("max_tokens", [48, 96])
+def test_padded_chunks_fill_the_cache(max_tokens):
+    """Chunks padded for different sequences: what fits by the sequences' own
+    lengths is taken, also where the places with padding are more, and is
+    stored as with more room; one token too many is refused."""
+    layers = _layers(CFG, seed=5)
+    dec = llama.CachedDecoder(CFG, layers, batch=2, max_tokens=max_tokens, page_size=16,
+                              n_layers=1)
+    mirror = serving.Cache(dec.caches[0])
+    g = torch.Generator().manual_seed(7)
+    lengths = np.zeros(2, np.int64)
+    for T, counts in ((20, [20, 2]), (20, [0, 20]), (20, [20, 3]), (12, [1, 12]), (1, [1, 1]),
+                      (30, [6, 0]), (9, [0, 9]), (1, [0, 1])):
+        x = torch.randn((2, T, CFG.n_embd), generator=g).half().cuda()
+        cap = _Capture(CFG, dec.linears[0])
+        y = dec(x, torch.tensor(counts, dtype=torch.int32, device="cuda"), capture=[cap])
+        assert torch.isfinite(y).all()
+        positions = torch.from_numpy(lengths[:, None] + np.arange(T)).cuda()
+        _, k, v = cap.qkv(dec.cos, dec.sin, positions.clamp(max=dec.max_tokens - 1))
+        for b in range(2):
+            n = counts[b]
+            at = positions[b, :n].cpu().numpy()
+            slots = dec.page_table[b].cpu().numpy()[at // 16].astype(np.int64) * 16 + at % 16
+            mirror.write(k[b, :n].double().cpu().numpy(), v[b, :n].double().cpu().numpy(), slots)
+        _check_fields(dec.caches[0], mirror)
+        lengths += np.array(counts)
+        assert dec.lengths.tolist() == lengths.tolist()
+    assert lengths.tolist() == [48, 48]
+    if max_tokens == 48:
+        x = torch.zeros((2, 1, CFG.n_embd), dtype=torch.float16, device="cuda")
+        with pytest.raises(RuntimeError, match="1 tokens do not fit behind 48 of 48"):
+            dec(x, torch.tensor([0, 1], dtype=torch.int32, device="cuda"))
+        y = dec(x, torch.tensor([0, 0], dtype=torch.int32, device="cuda"))
+        assert torch.isfinite(y).all() and dec.lengths.tolist() == [48, 48]
