@@ -128,7 +128,7 @@ __global__ void __launch_bounds__(kDecodeThreads)
 #pragma unroll
     for (int e = 0; e < 8; ++e)
       v[e] = __fmul_rn((float)(int)(int8_t)((e < 4 ? q[h].x : q[h].y) >> (8 * (e & 3))), s[h]);
-    store8(out + row[h] * out_stride + c0[h], true, 8, v);
+    store8(out + row[h] * out_stride + c0[h], v);
   }
 }
 

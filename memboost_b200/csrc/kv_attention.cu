@@ -626,9 +626,9 @@ __launch_bounds__(Layout<BITS, kQuarters>::kThreads, (Layout<BITS, kQuarters>::c
         const uint32_t ch = L::piece_channel(s, j);
         if (live && ch < c.dim) {
           if (q.bf16)
-            load8(static_cast<const __nv_bfloat16*>(q.data) + at + ch, q.vec, 8, x[s]);
+            load8(static_cast<const __nv_bfloat16*>(q.data) + at + ch, q.vec, x[s]);
           else
-            load8(static_cast<const __half*>(q.data) + at + ch, q.vec, 8, x[s]);
+            load8(static_cast<const __half*>(q.data) + at + ch, q.vec, x[s]);
         }
         top = max(top, abs_bits_max(x[s]));
       }

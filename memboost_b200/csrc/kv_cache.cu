@@ -295,7 +295,7 @@ __global__ void __launch_bounds__(kThreads)
     }
     store8((p.which ? v_out : k_out) + ((int64_t)(t0 + p.token) * c.heads + p.head) * c.dim +
                8 * p.lane,
-           true, 8, v);
+           v);
   }
 }
 

@@ -17,8 +17,6 @@ inline bool aligned(const void* p, size_t n) { return reinterpret_cast<uintptr_t
 template <typename T>
 __device__ __forceinline__ float to_float(T x);
 template <>
-__device__ __forceinline__ float to_float<float>(float x) { return x; }
-template <>
 __device__ __forceinline__ float to_float<__half>(__half x) { return __half2float(x); }
 template <>
 __device__ __forceinline__ float to_float<__nv_bfloat16>(__nv_bfloat16 x) {
@@ -36,51 +34,39 @@ __device__ __forceinline__ __nv_bfloat16 from_float<__nv_bfloat16>(float x) {
   return __float2bfloat16_rn(x);
 }
 
-// Eight consecutive values: two 16-byte loads or stores for fp32, one for the
-// 16-bit types (`vec`: the address is 16-byte aligned and n is 8), else one by
-// one, 0 past n.
+// Eight consecutive values of a 16-bit type: one 16-byte load (`vec`: the address
+// is 16-byte aligned), else one by one.
 template <typename T>
-__device__ __forceinline__ void load8(const T* __restrict__ p, bool vec, int n, float (&v)[8]) {
-  if (vec && n >= 8) {
-    if constexpr (sizeof(T) == 4) {
-      const float4 a = reinterpret_cast<const float4*>(p)[0];
-      const float4 b = reinterpret_cast<const float4*>(p)[1];
-      v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
-      v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
-    } else {
-      const uint4 u = *reinterpret_cast<const uint4*>(p);
-      const T* e = reinterpret_cast<const T*>(&u);
+__device__ __forceinline__ void load8(const T* __restrict__ p, bool vec, float (&v)[8]) {
+  static_assert(sizeof(T) == 2, "16-bit types");
+  if (vec) {
+    const uint4 u = *reinterpret_cast<const uint4*>(p);
+    const T* e = reinterpret_cast<const T*>(&u);
 #pragma unroll
-      for (int i = 0; i < 8; ++i) v[i] = to_float<T>(e[i]);
-    }
+    for (int i = 0; i < 8; ++i) v[i] = to_float<T>(e[i]);
   } else {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = i < n ? to_float<T>(p[i]) : 0.0f;
+    for (int i = 0; i < 8; ++i) v[i] = to_float<T>(p[i]);
   }
 }
 
+// Eight consecutive values to a 16-byte aligned address.
 template <typename T>
-__device__ __forceinline__ void store8(T* __restrict__ p, bool vec, int n, const float (&v)[8]) {
-  if (vec && n >= 8) {
-    if constexpr (sizeof(T) == 4) {
-      reinterpret_cast<float4*>(p)[0] = make_float4(v[0], v[1], v[2], v[3]);
-      reinterpret_cast<float4*>(p)[1] = make_float4(v[4], v[5], v[6], v[7]);
-    } else {
-      uint4 u;
-      T* e = reinterpret_cast<T*>(&u);
-#pragma unroll
-      for (int i = 0; i < 8; ++i) e[i] = from_float<T>(v[i]);
-      *reinterpret_cast<uint4*>(p) = u;
-    }
+__device__ __forceinline__ void store8(T* __restrict__ p, const float (&v)[8]) {
+  if constexpr (sizeof(T) == 4) {
+    reinterpret_cast<float4*>(p)[0] = make_float4(v[0], v[1], v[2], v[3]);
+    reinterpret_cast<float4*>(p)[1] = make_float4(v[4], v[5], v[6], v[7]);
   } else {
+    uint4 u;
+    T* e = reinterpret_cast<T*>(&u);
 #pragma unroll
-    for (int i = 0; i < 8; ++i)
-      if (i < n) p[i] = from_float<T>(v[i]);
+    for (int i = 0; i < 8; ++i) e[i] = from_float<T>(v[i]);
+    *reinterpret_cast<uint4*>(p) = u;
   }
 }
 
-// Eight consecutive values as they are held (16 or 32 bytes), loaded as load8
-// does; 0 past n.
+// Eight consecutive values as they are held (16 or 32 bytes), by 16-byte loads
+// (`vec`: the address is 16-byte aligned) where n is 8; 0 past n.
 template <typename T>
 struct Raw8 {
   static constexpr int kWords = sizeof(T) * 2;

@@ -125,7 +125,7 @@ class CacheStep:
     context: torch.Tensor | None = None
 
 
-def _cached_attention(cfg: LlamaConfig, q, k, v, step: CacheStep) -> torch.Tensor:
+def _cached_attention(q, k, v, step: CacheStep) -> torch.Tensor:
     """Attention output [batch, T, heads * head_dim] of q, k, v [batch, T, heads,
     head_dim], k and v stored in the cache first.  A single token attends to
     the cache as it is held; the first chunk of a prompt to itself; a later
@@ -165,7 +165,7 @@ def block_forward(cfg: LlamaConfig, x: torch.Tensor, linear: dict, cos, sin,
     at = None if cache is None else cache.positions
     q, k = _rotate(q, cos, sin, at), _rotate(k, cos, sin, at)
     if cache is not None:
-        o_in = _cached_attention(cfg, *(t.transpose(1, 2) for t in (q, k, v)), cache)
+        o_in = _cached_attention(*(t.transpose(1, 2) for t in (q, k, v)), cache)
     else:
         rep = cfg.n_head // cfg.n_kv_heads
         if rep > 1:
