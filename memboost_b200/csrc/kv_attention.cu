@@ -694,9 +694,13 @@ __launch_bounds__(Layout<BITS, kQuarters>::kThreads, (Layout<BITS, kQuarters>::c
         __syncwarp();
       }
 #pragma unroll
-      for (int r = 0; r < 2; ++r)
-        factor[n][r] = __shfl_sync(0xffffffffu, up, 4 * (2 * j + r)) * (scale * kLog2e) *
-                       (BITS == 8 ? 0x1p-14f : 0x1p17f);
+      for (int r = 0; r < 2; ++r) {
+        // (finite, so that a sum of 0 stays 0; NaN stays NaN)
+        const float y = __shfl_sync(0xffffffffu, up, 4 * (2 * j + r)) *
+                        (BITS == 8 ? 0x1p-14f : 1.0f) * (scale * kLog2e) *
+                        (BITS == 8 ? 1.0f : 0x1p17f);
+        factor[n][r] = isinf(y) ? copysignf(-kLowest, y) : y;
+      }
     }
 
     // o[n][p][i]: channels 16 (g + 8 p) + 2 i, + 1 of heads 2 j, 2 j + 1

@@ -151,3 +151,15 @@ def test_values_of_a_4_bit_cache_beyond_fp16():
     assert where[..., 40].all() and not where[..., :32].any()
     k[..., 3] = 1e5
     _attend((q * 1e-4).bfloat16(), k.bfloat16(), torch.ones_like(v).bfloat16(), 4, 1.0)
+
+
+@pytest.mark.parametrize("bits", [8, 4])
+@pytest.mark.parametrize("sign", [1, -1])
+def test_queries_and_scales_near_the_end_of_fp32(sign, bits):
+    """The query times the scale alone is beyond fp32: keys that make scores of a
+    few, and keys of zero."""
+    q, k, v = _inputs(100, 1, 2, 64, seed=2)
+    q = (q / q.abs().max() * 1.9).double() * 2.0 ** 126
+    small = (k.double() * 2.0 ** -137) if bits == 8 else k.double() * 0
+    for keys in (small, k.double() * 0):
+        _attend(q.bfloat16(), keys.bfloat16(), v.bfloat16(), bits, sign * 2.0 ** 9)
