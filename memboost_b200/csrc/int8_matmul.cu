@@ -47,7 +47,15 @@ struct Shape {
 };
 constexpr int kMaxStages = 12;
 constexpr uint32_t kMostParts = 8;  // of K: a portable cluster
-constexpr int kMostSmem = 227 * 1024 - 2048;  // a CTA's, less what is declared statically
+// A CTA's shared memory, less what is declared statically.  CTAs of a cluster wait
+// for one another, and each for its TMEM columns: two clusters that share two
+// SMs, each with the columns on one that the other waits for on the second, would
+// never end.  So a CTA of a cluster takes so much shared memory that no second one
+// for whose columns there is no room comes beside it: a pair's, with all 512, all
+// of it, the others, with 256 at most, half of it at least (all would leave too few
+// places for clusters of eight: 8 x 2048 x 2048 10.9 us instead of 7.0).  Lone CTAs
+// wait for no other.
+constexpr int kMostSmem = 227 * 1024 - 2048;
 constexpr int kSms = 148;
 
 __device__ __forceinline__ void prefetch_map(const CUtensorMap* map) {
@@ -380,7 +388,9 @@ __global__ void __launch_bounds__(kThreads, 1)
 constexpr int kPairTokens = 256;                       // tokens a tile
 constexpr int kPairStage = kWeightBytes + kPairTokens / 2 * kStepK;  // of one CTA
 constexpr int kPairStages = 6;
-constexpr int kPairSmem = kPairStages * kPairStage + 1024;
+// All that a CTA can have, although its ring needs less: see kMostSmem.
+constexpr int kPairSmem = kMostSmem - 2048;
+static_assert(kPairSmem >= kPairStages * kPairStage + 1024, "the ring does not fit");
 constexpr int kPairGroup = 8;                          // token tiles taken together
 
 __host__ __device__ constexpr uint32_t pair_idesc() {
@@ -609,8 +619,7 @@ struct Product {
 };
 
 template <int kN, typename Y>
-mb_status launch_tiles(const Product& p, int parts, int stages) {
-  using S = Shape<kN>;
+mb_status launch_tiles(const Product& p, int parts, int stages, int smem) {
   static std::atomic<uint64_t> attr_done{0};
   MB_CUDA_TRY(set_smem_limit_once(int8_matmul_kernel<kN, Y>, kMostSmem, attr_done));
   CUtensorMap tokens, weights;
@@ -627,7 +636,7 @@ mb_status launch_tiles(const Product& p, int parts, int stages) {
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(ceil_div(p.N, kChannels) * parts), (unsigned)ceil_div(p.M, kN));
   cfg.blockDim = dim3(kThreads);
-  cfg.dynamicSmemBytes = (size_t)S::smem(stages);
+  cfg.dynamicSmemBytes = (size_t)smem;
   cfg.stream = p.stream;
   cfg.attrs = attr;
   cfg.numAttrs = p.chained ? 2 : 1;
@@ -704,7 +713,8 @@ mb_status split_tiles(const Product& p, int parts) {
   int stages = ((kTwo && ctas > kSms ? kHalf : kMostSmem) - 1024) / S::kStage;
   stages = (int)min64(std::min(stages, kMaxStages), ceil_div(ceil_div(p.K, kStepK), parts));
   if (parts > 1) stages = std::max(stages, S::kLeast);
-  return launch_tiles<kN, Y>(p, parts, stages);
+  return launch_tiles<kN, Y>(p, parts, stages,
+                             parts > 1 ? std::max(kHalf, S::smem(stages)) : S::smem(stages));
 }
 
 template <typename Y>

@@ -274,6 +274,32 @@ def test_two_products_at_once():
         assert all(torch.equal(y, want[i]) for y in got[i])
 
 
+def test_clusters_of_two_streams_at_once():
+    """Products on pairs of CTAs, which take all of an SM's TMEM, and small ones
+    split over clusters, side by side and starting together."""
+    wide = mb.quantize_int8(_x(2100, 300, torch.float32, seed=8, spread=False).cuda() * 0.02)
+    small = [mb.quantize_int8(_x(4096, 1024, torch.float32, seed=i, spread=False).cuda() * 0.02)
+             for i in range(2)]
+    many = _x(2300, 300, torch.bfloat16, seed=1).cuda()
+    few = [_x(m, 1024, torch.bfloat16, seed=m).cuda() for m in (1, 40)]
+    want = mb.int8_matmul(many, wide), [mb.int8_matmul(x, w) for x, w in zip(few, small)]
+    streams = [torch.cuda.Stream() for _ in range(3)]
+    for _ in range(20):
+        got, go = [], torch.cuda.Event()
+        torch.cuda._sleep(200000)  # the three start when this ends
+        go.record()
+        for s in streams:
+            s.wait_event(go)
+        for _ in range(4):
+            with torch.cuda.stream(streams[0]):
+                got.append((mb.int8_matmul(many, wide), want[0]))
+            for s, x, w, y in zip(streams[1:], few, small, want[1]):
+                with torch.cuda.stream(s):
+                    got.append((mb.int8_matmul(x, w), y))
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in got)
+
+
 def test_int8_linear_from_a_quantized_weight():
     """Int8Linear of a 2/4-bit weight: the product of its dequantised matrix
     held in 8 bits."""
