@@ -494,8 +494,8 @@ size_t mb_cache_attention_workspace_size(const mb_kv_cache* cache, int64_t batch
  * scale is finite; pages * kv_heads * page_size is below 2^31.  A query, key or
  * value that is not finite gives outputs that are NaN; a 4-bit cache's
  * values (not its keys) are taken in fp16 here: beyond 65504 they count as
- * infinite.  Sums of weights times values are fp32 before they are divided by
- * the sum of weights: 8-bit values above 2^89 (bf16) may give infinities.  If a wait inside the
+ * infinite.  Beside 8-bit values above 2^107 (bf16) tokens with less than
+ * 2^-26 of the largest weight may count for nothing.  If a wait inside the
  * kernel ran out (2 s), the outputs it concerns are NaN.  workspace: 16-byte
  * aligned. */
 mb_status mb_cache_attention(const mb_kv_cache* cache, const void* q, int64_t q_batch_stride,

@@ -36,8 +36,9 @@
 // 4-bit keys enter S^T as codes, too: their pairs under a mask are subnormal
 // fp16 numbers, code 2^-24 (the upper ones code 2^-20), and exact.  The query is
 // fp16 relative to its largest channel (up to 2^15: exact for channels above
-// 2^-25 of it); a group's sum is multiplied by its scale, and its minimum by the
-// query's sum over the group, in fp32.  4-bit values become m + s * code in fp16,
+// 2^-25 of it); a group's sum is multiplied by its scale in fp32, and the minima
+// by the queries' sums over the groups in a product of their own (fp16, 22 bits
+// of each sum in two parts).  4-bit values become m + s * code in fp16,
 // one rounding (2^-11 of the value; beyond 65504 infinite).
 //
 // Scores, maxima, sums and the outputs' accumulators are fp32.
@@ -47,26 +48,26 @@
 // what that drops is multiplied too.  They are taken relative to the largest
 // weight of the head so far, not the largest scale or score alone: a token
 // whose values are huge but whose probability is nothing does not push the
-// others out of fp16's range.  The largest lies at 2^10 when it is set and is
-// set again above 2^15, so that weights down to 2^-24 of it are normal numbers
-// and what is lost of a smaller one is below 2^-35 of it; most steps rescale
-// nothing.  With 4 bits the probabilities' own maximum serves; with 8 a factor
-// of its own (`unit`), and the maximum, which only the sum refers to then, is
-// raised when a score exceeds it by 8 (in powers of two).
+// others out of fp16's range.  The reference m of a head's exponents is set so
+// that the largest weight lies at 2^10, and again when one exceeds 2^15: weights
+// down to 2^-24 of the largest are normal numbers, what is lost of a smaller one
+// is below 2^-35 of it, and most steps rescale nothing.  The sum of probabilities
+// has the same reference; with 8 bits they reach from 2^-111 (the largest scale)
+// to 2^90 (a value of 0), which fp32 has room for.
 //
 // The units of all sequences and heads are dealt out evenly to the resident
-// CTAs (two or three an SM), whatever the lengths: a CTA's share may begin and end inside a sequence.
-// Those parts (maximum, sum, unnormalised output) go to the workspace, two a
+// CTAs (two or three an SM), whatever the lengths: a CTA's share may begin and
+// end inside a sequence, and pass sequences without tokens.  Those parts (maximum, sum, unnormalised output) go to the workspace, two a
 // CTA at most, and a second kernel joins them in the order of the tokens, so
 // the result does not depend on the CTAs' timing.  Where the table holds few
 // tokens a sequence, a CTA takes a whole sequence's head instead and nothing
 // is joined.
 //
-// Measured: 8 bits stream at 92 % of the copy rate (one sequence of 65536 tokens
-// and 32 heads: 93 us for 86 us of bytes), 4 bits are bound by the instructions
-// that make fp16 of the codes (460 a warp for 16 tokens of 128 channels and up to
-// 8 query heads: 96 us for 52).  Beside that a call costs about 8 us (launch,
-// the first units, the join) and each sequence's head about 4 us of a CTA.
+// Measured: 8 bits stream at 85 % of the copy rate (one sequence of 65536 tokens
+// and 32 heads: 101 us for 86 us of bytes; 370 instructions a warp for 16 tokens
+// of 128 channels and up to 8 query heads), 4 bits are bound by their instructions
+// (480: 101 us for 52).  Beside that a call costs about 8 us (launch, the first
+// units, the join) and each sequence's head about 4 us of a CTA.
 #include <algorithm>
 #include <cmath>
 #include <cstring>
@@ -86,6 +87,14 @@ __device__ __forceinline__ void mma_f16(float (&c)[4], uint32_t a0, uint32_t a1,
       "{%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
       : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+__device__ __forceinline__ void mma_f16_k8(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t b) {
+  asm(
+      "mma.sync.aligned.m16n8k8.row.col.f32.f16.f16.f32 "
+      "{%0, %1, %2, %3}, {%4, %5}, {%6}, {%0, %1, %2, %3};"
+      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+      : "r"(a0), "r"(a1), "r"(b));
 }
 
 __device__ __forceinline__ void mma_s8(int (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2,
@@ -172,13 +181,12 @@ struct Layout {
   // lanes x 16 channels
   static constexpr int kSteps = kRow / 64;                           // 8 bits
   static constexpr int kGroups = kRow / 16;                          // 4 bits: of 32 channels
-  static constexpr int kProducts = BITS == 8 ? 4 * kSteps : 2 * kGroups;  // of S^T
+  static constexpr int kProducts = 2 * (BITS == 8 ? kSteps : kGroups);  // of S^T, and a part
   static constexpr int kPieces = BITS == 8 ? 2 * kSteps : kGroups;   // a lane's, of 8 channels
-  // 8 bits: the products with the query's lower part, whose operand two CTAs an SM
-  // leave in shared memory, each lane its own (three have the registers for it)
-  static constexpr int kLow = BITS == 8 ? 2 * kSteps : 0;
-  __host__ __device__ static constexpr bool low_in_smem(int tiles) {
-    return BITS == 8 && ctas(tiles) == 2;
+  // 8 bits: parts of the query (of three, the lower ones) that registers have no
+  // room for and shared memory holds, each lane its own
+  __host__ __device__ static constexpr int parts_in_smem(int tiles) {
+    return BITS == 4 ? 0 : tiles == 2 ? 2 : kQuarters > 2 ? 1 : 0;
   }
   static constexpr int kPasses = (kQuarters + 1) / 2;
 
@@ -188,10 +196,7 @@ struct Layout {
   static constexpr int kJoin = kWarps * 8 * kJoinRow * 4;
   static constexpr int kRing = kStages * kStage;
   __host__ __device__ static constexpr int smem(int tiles) {
-    return 1024 + kRing + kJoin +
-           (BITS == 4            ? kWarps * kGroups * 8 * 4 * tiles
-            : low_in_smem(tiles) ? kWarps * 32 * 8 * kLow * tiles
-                                 : 0);
+    return 1024 + kRing + kJoin + kWarps * 32 * 8 * parts_in_smem(tiles) * kProducts * tiles;
   }
 
   // Place in a stage's keys (or values) of a byte of a row.
@@ -220,11 +225,10 @@ constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLowest = -0x1.fffffep127f;  // a maximum of nothing
 // Exponents of the largest weight: when it is set, and above which it is set again.
 constexpr int kAim = 10, kMost = 15;
-// 8 bits: how far a score may exceed the maximum that the sum refers to.
-constexpr int kRaise = 8;
-// 8 bits: the largest unit, what a head begins with.  Times a probability of up
-// to 2^8 it stays in fp32; times one of 1 and the smallest normal scale it is 2^-8.
-constexpr float kMostUnit = 0x1p118f;
+// 8 bits: a probability above which it is set again, and the least exponent that a
+// value's scale counts as when it is (one of 0 has no weight, but belongs to the sum).
+constexpr float kMostP = 0x1p90f;
+constexpr int kLeastScale = -70;
 
 // Integer products begin at the bits of 1.5 2^23: sums of up to 2^22 (256 channels
 // of 128 times 128) then are the bits of 1.5 2^23 plus the sum, which a subtraction
@@ -256,9 +260,6 @@ __device__ __forceinline__ void ldmatrix4(uint32_t (&v)[4], uint32_t at) {
   asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];"
                : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3])
                : "r"(at));
-}
-__device__ __forceinline__ void sts32(uint32_t at, uint32_t x) {
-  asm volatile("st.shared.u32 [%0], %1;" ::"r"(at), "r"(x));
 }
 __device__ __forceinline__ void sts64(uint32_t at, uint32_t x, uint32_t y) {
   asm volatile("st.shared.v2.u32 [%0], {%1, %2};" ::"r"(at), "r"(x), "r"(y));
@@ -303,8 +304,8 @@ struct Lengths {
 };
 
 // Dealing the tokens' units alone leaves CTAs with many short sequences behind.
-// 16 sequences of 1 .. 2048 tokens, a head a group: 38 us with two idle units, 41
-// with four; 48 of 1 .. 8192, eight heads a group: 88 with two, 81 with four.
+// 16 sequences of 1 .. 2048 tokens, a head a group: 41 us with two idle units, 44
+// with four; 48 of 1 .. 8192, eight heads a group: 91 with two, 83 with four.
 inline uint32_t idle_units(uint32_t group) { return 2 + std::min(group, 16u) / 4; }
 
 // The units in order: sequences, in them rows (a key/value head's block of
@@ -597,21 +598,22 @@ __launch_bounds__(Layout<BITS, kQuarters>::kThreads, (Layout<BITS, kQuarters>::c
   int stage = 0;
   uint32_t phase = 0;
   bool ok = true;
-  constexpr bool kLowSmem = L::low_in_smem(kTiles);
-  [[maybe_unused]] const uint32_t low_at =
-      ring0 + L::kRing + L::kJoin + 8 * (warp * 32 * L::kLow * kTiles + lane);
-  // 4 bits: the sums of the query's groups [tile][group][8 heads], each warp its own
-  [[maybe_unused]] const uint32_t sum_at =
-      ring0 + L::kRing + L::kJoin + 32 * warp * L::kGroups * kTiles;
+  constexpr int kHeld = L::parts_in_smem(kTiles);
+  // of part x (1 middle, 2 lower), tile n and product i
+  const auto held_at = [&](int x, int n, int i) {
+    return ring0 + L::kRing + L::kJoin +
+           8 * (((warp * kHeld + 2 - x) * kTiles + n) * L::kProducts + i) * 32 + 8 * lane;
+  };
   const bool fine = !q.bf16;  // an fp16 output: what fp16 drops of the probabilities too
   for (uint32_t place = 0; run.more(); run.next(), place = 1) {
     const Segment& seg = run.s;
     const uint32_t kvh = seg.row / heads.blocks, h0 = (seg.row - kvh * heads.blocks) * kHeads;
 
     // Q in the order of the keys' registers, below 1 by a power of two a head
-    // 8 bits: pairs of products, the upper and the middle part; ql the lower
-    uint32_t qf[kTiles][L::kProducts][2];
-    [[maybe_unused]] uint32_t ql[kTiles][kLowSmem || BITS == 4 ? 1 : L::kLow][2];
+    // 8 bits: qf[0] the upper part, qf[1] the middle, qf[2] the lower
+    uint32_t qf[BITS == 8 ? 3 - kHeld : 1][kTiles][L::kProducts][2];
+    // 4 bits: the query's sum over group j (and j + 4) in two parts, 22 bits
+    [[maybe_unused]] uint32_t qs[kTiles][(L::kGroups + 3) / 4];
     float factor[kTiles][2];  // of heads 2 j, 2 j + 1: scale log2(e) and that power
 #pragma unroll
     for (int n = 0; n < kTiles; ++n) {
@@ -645,7 +647,7 @@ __launch_bounds__(Layout<BITS, kQuarters>::kThreads, (Layout<BITS, kQuarters>::c
         for (int s = 0; s < L::kSteps; ++s) {
           // q 2^22 = 65536 upper + 256 middle + lower, all signed bytes: those of
           // v = q 2^22 + 128 (256 + 1), the lower two less 128
-          uint32_t low[4];
+          uint32_t part[3][4];
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
             uint32_t v[4];
@@ -655,20 +657,22 @@ __launch_bounds__(Layout<BITS, kQuarters>::kThreads, (Layout<BITS, kQuarters>::c
                                           kRoundMagic)) -
                      (uint32_t)kSumBits + 0x8080u;
             const uint32_t a = __byte_perm(v[0], v[1], 0x5140), b = __byte_perm(v[2], v[3], 0x5140);
-            qf[n][4 * s + i / 2 * 2][i & 1] = __byte_perm(
-                __byte_perm(v[0], v[1], 0x0062), __byte_perm(v[2], v[3], 0x0062), 0x5410);
-            qf[n][4 * s + i / 2 * 2 + 1][i & 1] = __byte_perm(a, b, 0x7632) ^ 0x80808080u;
-            low[i] = __byte_perm(a, b, 0x5410) ^ 0x80808080u;
+            part[0][i] = __byte_perm(__byte_perm(v[0], v[1], 0x0062),
+                                     __byte_perm(v[2], v[3], 0x0062), 0x5410);
+            part[1][i] = __byte_perm(a, b, 0x7632) ^ 0x80808080u;
+            part[2][i] = __byte_perm(a, b, 0x5410) ^ 0x80808080u;
           }
 #pragma unroll
-          for (int i = 0; i < 2; ++i) {
-            if constexpr (kLowSmem) {
-              sts64(low_at + 256 * (n * L::kLow + 2 * s + i), low[2 * i], low[2 * i + 1]);
-            } else {
-              ql[n][2 * s + i][0] = low[2 * i];
-              ql[n][2 * s + i][1] = low[2 * i + 1];
+          for (int i = 0; i < 2; ++i)
+#pragma unroll
+            for (int y = 0; y < 3; ++y) {
+              if (y < 3 - kHeld) {
+                qf[y < 3 - kHeld ? y : 0][n][2 * s + i][0] = part[y][2 * i];
+                qf[y < 3 - kHeld ? y : 0][n][2 * s + i][1] = part[y][2 * i + 1];
+              } else {
+                sts64(held_at(y, n, 2 * s + i), part[y][2 * i], part[y][2 * i + 1]);
+              }
             }
-          }
         }
       } else {
 #pragma unroll
@@ -682,16 +686,19 @@ __launch_bounds__(Layout<BITS, kQuarters>::kThreads, (Layout<BITS, kQuarters>::c
           }
 #pragma unroll
           for (int i = 0; i < 2; ++i) {
-            uint32_t(&f)[2] = qf[n][2 * s + i];
+            uint32_t(&f)[2] = qf[0][n][2 * s + i];
             f[0] = h2_bits(__floats2half2_rn(x[s][2 * i] * 0x1p15f, x[s][2 * i + 4] * 0x1p15f));
             f[1] = h2_bits(__floats2half2_rn(x[s][2 * i + 1] * 0x1p11f, x[s][2 * i + 5] * 0x1p11f));
           }
           sum += __shfl_xor_sync(0xffffffffu, sum, 1);
           sum += __shfl_xor_sync(0xffffffffu, sum, 2);
-          if (j == 0)  // times 2^15, as the others, less the codes' 2^24
-            sts32(sum_at + 32 * (n * L::kGroups + s) + 4 * g, __float_as_uint(sum * 0x1p-9f));
+          if (s % 4 == 0) qs[n][s / 4] = 0u;
+          if (j == s % 4) {
+            const __half high = __float2half_rn(sum * 0x1p9f);
+            qs[n][s / 4] = h2_bits(__halves2half2(
+                high, __float2half_rn(fmaf(sum, 0x1p9f, -__half2float(high)))));
+          }
         }
-        __syncwarp();
       }
 #pragma unroll
       for (int r = 0; r < 2; ++r) {
@@ -704,14 +711,10 @@ __launch_bounds__(Layout<BITS, kQuarters>::kThreads, (Layout<BITS, kQuarters>::c
     }
 
     // o[n][p][i]: channels 16 (g + 8 p) + 2 i, + 1 of heads 2 j, 2 j + 1
-    // (8 bits: times unit, relative to the same maximum m as the sums l)
     float o[kTiles][L::kPasses][8][4] = {};
-    float m[kTiles][2], l[kTiles][2] = {}, unit[kTiles][2];
+    float m[kTiles][2], l[kTiles][2] = {};
 #pragma unroll
-    for (int n = 0; n < kTiles; ++n) {
-      m[n][0] = m[n][1] = kLowest;
-      unit[n][0] = unit[n][1] = kMostUnit;
-    }
+    for (int n = 0; n < kTiles; ++n) m[n][0] = m[n][1] = kLowest;
 
 #pragma unroll 1
     for (uint32_t u = seg.first(); u < seg.last(); ++u) {
@@ -748,11 +751,13 @@ __launch_bounds__(Layout<BITS, kQuarters>::kThreads, (Layout<BITS, kQuarters>::c
         // ---- S^T = K Q^T
         float s[kTiles][4] = {};
         if constexpr (BITS == 8) {
-          int hi[kTiles][4], mid[kTiles][4], lo[kTiles][4];
+          int sums[3][kTiles][4];  // with the upper, middle and lower part
 #pragma unroll
-          for (int n = 0; n < kTiles; ++n)
+          for (int y = 0; y < 3; ++y)
 #pragma unroll
-            for (int e = 0; e < 4; ++e) hi[n][e] = mid[n][e] = lo[n][e] = kSumBits;
+            for (int n = 0; n < kTiles; ++n)
+#pragma unroll
+              for (int e = 0; e < 4; ++e) sums[y][n][e] = kSumBits;
 #pragma unroll
           for (int st = 0; st < L::kSteps; ++st) {
             uint4 kw[2];
@@ -761,21 +766,21 @@ __launch_bounds__(Layout<BITS, kQuarters>::kThreads, (Layout<BITS, kQuarters>::c
               kw[r] = lds128(key_at[st % 2] + stage_at + st / 2 * L::kColumn + r * kEight);
 #pragma unroll
             for (int n = 0; n < kTiles; ++n) {
-              const uint32_t(*f)[2] = &qf[n][4 * st];
-              mma_s8(hi[n], kw[0].x, kw[1].x, kw[0].y, kw[1].y, f[0][0], f[0][1]);
-              mma_s8(mid[n], kw[0].x, kw[1].x, kw[0].y, kw[1].y, f[1][0], f[1][1]);
-              mma_s8(hi[n], kw[0].z, kw[1].z, kw[0].w, kw[1].w, f[2][0], f[2][1]);
-              mma_s8(mid[n], kw[0].z, kw[1].z, kw[0].w, kw[1].w, f[3][0], f[3][1]);
-              uint2 f0, f1;
-              if constexpr (kLowSmem) {
-                f0 = lds64(low_at + 256 * (n * L::kLow + 2 * st));
-                f1 = lds64(low_at + 256 * (n * L::kLow + 2 * st + 1));
-              } else {
-                f0 = make_uint2(ql[n][2 * st][0], ql[n][2 * st][1]);
-                f1 = make_uint2(ql[n][2 * st + 1][0], ql[n][2 * st + 1][1]);
+#pragma unroll
+              for (int i = 0; i < 2; ++i) {
+                const uint32_t a0 = i ? kw[0].z : kw[0].x, a1 = i ? kw[1].z : kw[1].x;
+                const uint32_t a2 = i ? kw[0].w : kw[0].y, a3 = i ? kw[1].w : kw[1].y;
+#pragma unroll
+                for (int y = 0; y < 3; ++y) {
+                  uint2 f;
+                  if (y < 3 - kHeld)
+                    f = make_uint2(qf[y < 3 - kHeld ? y : 0][n][2 * st + i][0],
+                                   qf[y < 3 - kHeld ? y : 0][n][2 * st + i][1]);
+                  else
+                    f = lds64(held_at(y, n, 2 * st + i));
+                  mma_s8(sums[y][n], a0, a1, a2, a3, f.x, f.y);
+                }
               }
-              mma_s8(lo[n], kw[0].x, kw[1].x, kw[0].y, kw[1].y, f0.x, f0.y);
-              mma_s8(lo[n], kw[0].z, kw[1].z, kw[0].w, kw[1].w, f1.x, f1.y);
             }
           }
           const float ks[2] = {__uint_as_float(lds32(key_scale + stage_at)),
@@ -784,48 +789,66 @@ __launch_bounds__(Layout<BITS, kQuarters>::kThreads, (Layout<BITS, kQuarters>::c
           for (int n = 0; n < kTiles; ++n)
 #pragma unroll
             for (int e = 0; e < 4; ++e)
-              s[n][e] = fmaf(whole_sum(hi[n][e]), 65536.0f,
-                             fmaf(whole_sum(mid[n][e]), 256.0f, whole_sum(lo[n][e]))) *
+              s[n][e] = fmaf(whole_sum(sums[0][n][e]), 65536.0f,
+                             fmaf(whole_sum(sums[1][n][e]), 256.0f, whole_sum(sums[2][n][e]))) *
                         ks[e >> 1];
         } else {
-          // sum of q k = sum over the groups of s (sum of q code) + m (sum of q), the
-          // sums in fp32: nothing is rounded to fp16
+          // sum of q k = sum over the groups of s (sum of q code) + m (sum of q): the
+          // second is a product of its own, over groups, with both parts of a sum
           uint64_t both[kTiles][2];  // heads 2 j, 2 j + 1 of a token
+          {
+            float low[kTiles][4] = {};
 #pragma unroll
-          for (int n = 0; n < kTiles; ++n) both[n][0] = both[n][1] = 0;
+            for (int i = 0; i < L::kGroups; i += 4) {
+              uint32_t gm[2];
+#pragma unroll
+              for (int r = 0; r < 2; ++r)
+                // past head_dim the query is 0 (any group's minimum will do)
+                gm[r] = h2_bits(__high2half2(
+                    bits_h2(lds32(key_scale + stage_at + r * eight_scales +
+                                  4 * min(i + j, last_group)))));
+#pragma unroll
+              for (int n = 0; n < kTiles; ++n) mma_f16_k8(low[n], gm[0], gm[1], qs[n][i / 4]);
+            }
+            const uint64_t to = f2_pack(0x1p-18f, 0x1p-18f);  // 2^6 less the codes' 2^24
+#pragma unroll
+            for (int n = 0; n < kTiles; ++n)
+#pragma unroll
+              for (int r = 0; r < 2; ++r)
+                both[n][r] = f2_mul(f2_pack(low[n][2 * r], low[n][2 * r + 1]), to);
+          }
 #pragma unroll
           for (int i = 0; i < L::kGroups; i += 2) {
             uint32_t kw[4];
             ldmatrix4(kw, (key_at[0] ^ (16 * i)) + stage_at);
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
-              uint64_t gs[2], gm[2];
+              uint64_t gs[2];
 #pragma unroll
               for (int r = 0; r < 2; ++r) {
-                // past head_dim the query is 0 (any group's scale will do)
-                const float2 pair = __half22float2(
+                const float x = __low2float(
                     bits_h2(lds32(key_scale + stage_at + r * eight_scales +
                                   4 * min(i + h, last_group))));
-                gs[r] = f2_pack(pair.x, pair.x);
-                gm[r] = f2_pack(pair.y, pair.y);
+                gs[r] = f2_pack(x, x);
               }
               const uint32_t w0 = kw[2 * h], w1 = kw[2 * h + 1];
+              float sum[kTiles][4] = {};
 #pragma unroll
-              for (int n = 0; n < kTiles; ++n) {
-                float sum[4] = {};
+              for (int x = 0; x < 2; ++x) {
+                const uint32_t a0 = w0 >> (8 * x) & 0x000F000Fu, a1 = w1 >> (8 * x) & 0x000F000Fu;
+                const uint32_t a2 = w0 >> (8 * x) & 0x00F000F0u, a3 = w1 >> (8 * x) & 0x00F000F0u;
 #pragma unroll
-                for (int x = 0; x < 2; ++x) {
-                  const uint32_t(&f)[2] = qf[n][2 * (i + h) + x];
-                  mma_f16(sum, w0 >> (8 * x) & 0x000F000Fu, w1 >> (8 * x) & 0x000F000Fu,
-                          w0 >> (8 * x) & 0x00F000F0u, w1 >> (8 * x) & 0x00F000F0u, f[0], f[1]);
+                for (int n = 0; n < kTiles; ++n) {
+                  const uint32_t(&f)[2] = qf[0][n][2 * (i + h) + x];
+                  mma_f16(sum[n], a0, a1, a2, a3, f[0], f[1]);
                 }
-                const uint2 qs = lds64(sum_at + 32 * (n * L::kGroups + i + h) + 8 * j);
-                const uint64_t q2 = f2_pack(__uint_as_float(qs.x), __uint_as_float(qs.y));
+              }
+#pragma unroll
+              for (int n = 0; n < kTiles; ++n)
 #pragma unroll
                 for (int r = 0; r < 2; ++r)
-                  both[n][r] = f2_fma(gs[r], f2_pack(sum[2 * r], sum[2 * r + 1]),
-                                      f2_fma(gm[r], q2, both[n][r]));
-              }
+                  both[n][r] = f2_fma(gs[r], f2_pack(sum[n][2 * r], sum[n][2 * r + 1]),
+                                      both[n][r]);
             }
           }
 #pragma unroll
@@ -860,62 +883,44 @@ __launch_bounds__(Layout<BITS, kQuarters>::kThreads, (Layout<BITS, kQuarters>::c
         float p[kTiles][4], w[kTiles][4];
         const auto weigh = [&](int n, int e) {
           p[n][e] = exp2_fast(s[n][e] - m[n][e & 1]);
-          w[n][e] = BITS == 8 ? p[n][e] * unit[n][e & 1] * vs[e >> 1] : p[n][e];
+          w[n][e] = BITS == 8 ? p[n][e] * vs[e >> 1] : p[n][e];
         };
-        bool raise = false;
+        float most = 0.0f, most_p = 0.0f;  // (a NaN is in neither)
 #pragma unroll
         for (int n = 0; n < kTiles; ++n)
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
             weigh(n, e);
-            raise |= w[n][e] > (float)(1 << kMost);
-            if constexpr (BITS == 8) raise |= p[n][e] > (float)(1 << kRaise);
+            most = fmaxf(most, w[n][e]);
+            if constexpr (BITS == 8) most_p = fmaxf(most_p, p[n][e]);
           }
-        if (__any_sync(0xffffffffu, raise)) {
+        if (__any_sync(0xffffffffu, most > (float)(1 << kMost) || most_p > kMostP)) {
+          // how far below a score its weight's reference lies
+          float below[2] = {(float)kAim, (float)kAim};
+          if constexpr (BITS == 8) {
+#pragma unroll
+            for (int t = 0; t < 2; ++t) {
+              const uint32_t x = __float_as_uint(vs[t]) & 0x7FFFFFFFu;
+              // (a scale that is not finite has no say)
+              const int e = x < 0x7F800000u ? (int)(x >> 23) - 127 : kLeastScale;
+              below[t] -= (float)max(e, kLeastScale);
+            }
+          }
 #pragma unroll
           for (int n = 0; n < kTiles; ++n) {
             float f[2];
 #pragma unroll
             for (int r = 0; r < 2; ++r) {
-              float top = fmaxf(s[n][r], s[n][r + 2]);
+              float top = fmaxf(s[n][r] - below[0], s[n][r + 2] - below[1]);
 #pragma unroll
               for (int d = 4; d < 32; d <<= 1)
                 top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
-              top = fmaxf(BITS == 8 ? top : top - kAim, m[n][r]);
+              top = fmaxf(top, m[n][r]);
               f[r] = exp2_fast(m[n][r] - top);
               l[n][r] *= f[r];
-              if constexpr (BITS == 8) {
-                // weights stay relative to what they were, up to the largest unit
-                const float now = unit[n][r] * exp2_fast(top - m[n][r]);
-                f[r] = now <= kMostUnit
-                           ? 1.0f
-                           : f[r] * 0x1p64f / unit[n][r] * (kMostUnit * 0x1p-64f);
-                unit[n][r] = fminf(now, kMostUnit);
-              }
               m[n][r] = top;
               weigh(n, r);
               weigh(n, r + 2);
-              if constexpr (BITS == 8) {
-                // down to 2^kAim, by the exponents of the factors: the weight may be
-                // past fp32 (a scale that is not finite has no say)
-                uint32_t e = 0;
-#pragma unroll
-                for (int t = 0; t < 2; ++t) {
-                  const uint32_t x = __float_as_uint(vs[t]) & 0x7FFFFFFFu;
-                  if (x < 0x7F800000u)
-                    e = max(e, (__float_as_uint(p[n][r + 2 * t] * unit[n][r]) >> 23) + (x >> 23));
-                }
-#pragma unroll
-                for (int d = 4; d < 32; d <<= 1) e = max(e, __shfl_xor_sync(0xffffffffu, e, d));
-                // the weight is below 2^(e - 252)
-                const uint32_t drop = e > 252 + kMost ? min(e - (252 + kAim), 252u) : 0u;
-                const float half0 = __uint_as_float((127 - drop / 2) << 23);
-                const float half1 = __uint_as_float((127 - (drop + 1) / 2) << 23);
-                f[r] = f[r] * half0 * half1;
-                unit[n][r] = unit[n][r] * half0 * half1;
-                weigh(n, r);
-                weigh(n, r + 2);
-              }
             }
 #pragma unroll
             for (int t = 0; t < L::kPasses; ++t)
@@ -1018,7 +1023,6 @@ __launch_bounds__(Layout<BITS, kQuarters>::kThreads, (Layout<BITS, kQuarters>::c
 #pragma unroll
       for (int r = 0; r < 2; ++r) {
         float sum = ok ? l[n][r] : __uint_as_float(0x7FC00000u);
-        const float up = BITS == 8 ? 1.0f / unit[n][r] : 1.0f;
 #pragma unroll
         for (int d = 4; d < 32; d <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
         const uint32_t h = 2 * j + r;
@@ -1031,8 +1035,8 @@ __launch_bounds__(Layout<BITS, kQuarters>::kThreads, (Layout<BITS, kQuarters>::c
             if (ch < 64 * kQuarters)
 #pragma unroll
               for (int i = 0; i < 8; ++i) {
-                to[ch + ch / 32 * 4 + 2 * i] = o[n][p][i][r] * up;
-                to[ch + ch / 32 * 4 + 2 * i + 1] = o[n][p][i][r + 2] * up;
+                to[ch + ch / 32 * 4 + 2 * i] = o[n][p][i][r];
+                to[ch + ch / 32 * 4 + 2 * i + 1] = o[n][p][i][r + 2];
               }
           }
         }
@@ -1240,8 +1244,8 @@ inline uint32_t head_tiles(uint32_t group, uint32_t dim) { return group > 8 && d
 // Sequences of tables this narrow are taken whole, a CTA a row: nothing to join.
 // A row costs its CTA about 1 us for 64 tokens, dealing and joining 4 us; with
 // many rows the CTAs have enough to do either way.  Whole and dealt out, 32 rows:
-// 256 tokens 7.7 and 8.9 us, 352 9.7 and 8.9, 512 12.0 and 9.3; 128 rows of 512: 12.0 and
-// 13.6; 512 rows of 512: 16.3 and 20.5.
+// 256 tokens 7.7 and 9.2 us, 352 9.3 and 9.8, 512 11.0 and 9.8; 128 rows of 512:
+// 11.1 and 13.8; 512 rows of 512: 20.7 and 25.3.
 constexpr int64_t kWholeTokens = 320, kWholeTokensOfMany = 512, kManyRows = 64;
 constexpr int64_t kMostShares = 3 * 148;  // Layout::ctas an SM at most
 inline bool whole(int64_t most, int64_t rows) {
@@ -1306,8 +1310,8 @@ mb_status launch(const Call& a) {
     dim3 joins(a.lengths.batch * rows);
     const Join join{a.parts, shares,  (uint32_t)(8 * kTiles), a.c.heads, a.heads,
                     a.c.dim, lengths, a.q.bf16,               a.out};
-    // Parts a row of eight and more: 1 x 100000 tokens of one key/value head 38 us
-    // with the heads' kernel, 75 with the rows'; 48 x 8192 of eight 96 and 87.
+    // Parts a row of eight and more: 1 x 100000 tokens of one key/value head 27 us
+    // with the heads' kernel, 117 with the rows'; 48 x 8192 of eight 105 and 82.
     const bool by_heads = shares >= 8 * joins.x;
     if (by_heads) joins.y = std::min<uint32_t>(8 * kTiles, a.heads.group);
     MB_CUDA_TRY(launch_dependent(

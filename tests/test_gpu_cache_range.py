@@ -163,3 +163,11 @@ def test_queries_and_scales_near_the_end_of_fp32(sign, bits):
     small = (k.double() * 2.0 ** -137) if bits == 8 else k.double() * 0
     for keys in (small, k.double() * 0):
         _attend(q.bfloat16(), keys.bfloat16(), v.bfloat16(), bits, sign * 2.0 ** 9)
+
+
+@pytest.mark.parametrize("n", [40, 3000])
+def test_values_near_the_end_of_bf16(n):
+    """Outputs of a size next to fp32's largest are not infinite on their way."""
+    q, k, v = _inputs(n, 2, 12, 128, seed=n + 1)
+    for size in (2.0 ** 105, 2.0 ** 124, 2.0 ** -66):
+        _attend(q.bfloat16(), k.bfloat16(), (v.clamp(-3, 3) * size).bfloat16(), 8, 128 ** -0.5)
