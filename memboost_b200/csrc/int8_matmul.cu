@@ -15,12 +15,14 @@
 // their int32 parts through distributed shared memory -- whole numbers, so
 // the result does not depend on the split.
 //
-// Few tokens are bound by reading the weights, at the rate at which one SM
-// takes operands in (75 to 90 GB/s each, launch and drain aside): 4096 x 4096 at
-// one token 8.2 us with the quantising kernel, 11008 x 4096 at 48 tokens 16.
-// Thousands of tokens are bound by the tensor cores and, back to back, by the
-// card's power: 8192 x 11008 x 4096 takes 272 us, 2.7e15 operations a second
-// (228 us without the outputs' way out; the pipe is busy for 72 % of it).
+// One token is bound by what comes one after another: 4096 x 4096 takes 8.2 us, 2
+// of them the quantising launch, the others set-up, the weights (131 KB for each
+// of 128 CTAs, 1.5 to 1.8 us at the 75 to 90 GB/s that one SM takes in), the join
+// over the cluster and the drain.  11008 x 4096 at 48 tokens takes 15.6 us, bound by
+// that intake: 790 KB for each of the 86 SMs that have a tile.  Thousands of
+// tokens are bound by the tensor cores and, back to back, by the card's power: 8192
+// x 11008 x 4096 takes 277 us in a replayed graph, 2.7e15 operations a second, 322 us
+// a call, 2.3e15 (the pipe is busy for 71 % of a launch alone).
 #include <algorithm>
 #include <cstring>
 

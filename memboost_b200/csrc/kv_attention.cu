@@ -28,8 +28,8 @@
 // query, scaled by a power of two to below 1, in three 8-bit parts (22 bits and
 // a sign: off by at most 2^-22 of the query's largest channel, exact for
 // channels above 2^-11 of it; with two parts, 14 bits, a channel far above the
-// others cost them theirs, and 16 x 2048 took 39.6 us for 41.0, 2 x 100001 65.5 for
-// 69.0).  The sums are exact.  8-bit values become exact fp16 integers (1024 +
+// others cost them theirs, and 16 x 2048 took 2 % less time, 2 x 100001 4 %).
+// The sums are exact.  8-bit values become exact fp16 integers (1024 +
 // 128 + code by a byte permute, minus 1152); their scale multiplies the
 // probability.
 //
@@ -63,10 +63,10 @@
 // tokens a sequence, a CTA takes a whole sequence's head instead and nothing
 // is joined.
 //
-// Measured: 8 bits stream at 85 % of the copy rate (one sequence of 65536 tokens
-// and 32 heads: 101 us for 86 us of bytes; 370 instructions a warp for 16 tokens
+// Measured: 8 bits stream at 88 % of the copy rate (one sequence of 65536 tokens
+// and 32 heads: 97 us for 86 us of bytes; 360 instructions a warp for 16 tokens
 // of 128 channels and up to 8 query heads), 4 bits are bound by their instructions
-// (480: 101 us for 52).  Beside that a call costs about 8 us (launch, the first
+// (470: 98 us for 52).  Beside that a call costs about 8 us (launch, the first
 // units, the join) and each sequence's head about 4 us of a CTA.
 #include <algorithm>
 #include <cmath>
@@ -304,8 +304,8 @@ struct Lengths {
 };
 
 // Dealing the tokens' units alone leaves CTAs with many short sequences behind.
-// 16 sequences of 1 .. 2048 tokens, a head a group: 41 us with two idle units, 44
-// with four; 48 of 1 .. 8192, eight heads a group: 91 with two, 83 with four.
+// 16 sequences of 1 .. 2048 tokens, a head a group: 40 us with two idle units, 43
+// with four; 48 of 1 .. 8192, eight heads a group: 89 with two, 81 with four.
 inline uint32_t idle_units(uint32_t group) { return 2 + std::min(group, 16u) / 4; }
 
 // The units in order: sequences, in them rows (a key/value head's block of
@@ -1244,8 +1244,8 @@ inline uint32_t head_tiles(uint32_t group, uint32_t dim) { return group > 8 && d
 // Sequences of tables this narrow are taken whole, a CTA a row: nothing to join.
 // A row costs its CTA about 1 us for 64 tokens, dealing and joining 4 us; with
 // many rows the CTAs have enough to do either way.  Whole and dealt out, 32 rows:
-// 256 tokens 7.7 and 9.2 us, 352 9.3 and 9.8, 512 11.0 and 9.8; 128 rows of 512:
-// 11.1 and 13.8; 512 rows of 512: 20.7 and 25.3.
+// 256 tokens 7.0 and 8.4 us, 352 8.7 and 9.1, 512 10.4 and 9.1; 128 rows of 512:
+// 10.6 and 12.8; 512 rows of 512: 19.3 and 23.4.
 constexpr int64_t kWholeTokens = 320, kWholeTokensOfMany = 512, kManyRows = 64;
 constexpr int64_t kMostShares = 3 * 148;  // Layout::ctas an SM at most
 inline bool whole(int64_t most, int64_t rows) {
@@ -1310,8 +1310,8 @@ mb_status launch(const Call& a) {
     dim3 joins(a.lengths.batch * rows);
     const Join join{a.parts, shares,  (uint32_t)(8 * kTiles), a.c.heads, a.heads,
                     a.c.dim, lengths, a.q.bf16,               a.out};
-    // Parts a row of eight and more: 1 x 100000 tokens of one key/value head 27 us
-    // with the heads' kernel, 117 with the rows'; 48 x 8192 of eight 105 and 82.
+    // Parts a row of eight and more: 1 x 100000 tokens of one key/value head 26 us
+    // with the heads' kernel, 114 with the rows'; 48 x 8192 of eight 103 and 80.
     const bool by_heads = shares >= 8 * joins.x;
     if (by_heads) joins.y = std::min<uint32_t>(8 * kTiles, a.heads.group);
     MB_CUDA_TRY(launch_dependent(

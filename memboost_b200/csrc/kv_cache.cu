@@ -7,9 +7,10 @@
 // 16-byte load, the maximum (8 bits: of the row) or minimum and maximum (4
 // bits: of 32 channels, four lanes) by shuffles, and one 8- or 4-byte store.
 // Bound by memory: 2 bytes in and 1 or 0.63 out a value; at usual sizes by the
-// chain of loads (slot, row, codes) and the launches: 2048 tokens of 8 heads of
-// 128 channels written in 11.7 us, 8000 read in 12.9 (4 bits), where their bytes
-// alone take 1.7 and 6.7.
+// chain of loads (slot, row, codes), by the slots that each writing CTA looks
+// through, and by the launches: 2048 tokens of 8 heads of 128 channels written and
+// 8000 read (4 bits) in 20.9 us as two calls in turn, where their bytes take 1.7 and
+// 6.7 (under ncu, with cold caches, 11.7 and 12.9).
 #include <algorithm>
 
 #include "mb_cache.cuh"
