@@ -53,3 +53,25 @@ def test_sequences_without_tokens(batch, longest, heads, group, dim, bits, where
     got = mb.cache_attention(q, cache, table.cuda(), n.cuda())
     _check_attention(got, q, cache, table.numpy(), lengths, 1 / math.sqrt(dim))
     assert all((got[b] == 0).all() for b in range(batch) if lengths[b] <= 0)
+
+
+@pytest.mark.parametrize("bits", [8, 4])
+def test_replayed_with_other_sequences_empty(bits):
+    """A captured call takes the lengths as they are when it is replayed."""
+    batch, longest, heads, dim, page = 16, 2048, 32, 64, 64
+    cache = _filled(40, page, heads, dim, bits, seed=bits)
+    g = torch.Generator().manual_seed(bits)
+    table = torch.randint(0, 40, (batch, longest // page), generator=g, dtype=torch.int32)
+    q = torch.randn((batch, heads, dim), generator=g).half().cuda()
+    table_, n = table.cuda(), torch.full((batch,), longest, dtype=torch.int32, device="cuda")
+    mb.cache_attention(q, cache, table_, n)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = mb.cache_attention(q, cache, table_, n)
+    for where in WHERE.values():
+        lengths = _lengths(batch, longest, where)
+        n.copy_(torch.tensor(lengths, dtype=torch.int32))
+        graph.replay()
+        torch.cuda.synchronize()
+        _check_attention(got, q, cache, table.numpy(), lengths, 1 / math.sqrt(dim))
