@@ -413,10 +413,9 @@ mb_status mb_int8_dequantize(const int8_t* codes, int64_t codes_stride, const fl
  * (bias may be NULL): a = the tokens, b = the weights (an output channel a
  * row).  The sum is a whole number and exact (codes made by
  * others stay within [-127, 127] too); it is rounded to fp32,
- * multiplied by the two scales and added to the bias in fp32 (in 64 bits next
- * to a token whose scale is above 2^96 or subnormal: a product of two of them
- * may be beyond fp32 where all three are not), and rounded once more to
- * out_type.  If a wait inside the kernel ran out (2 s), the
+ * multiplied by the two scales and added to the bias in fp32 (in 64 bits for a
+ * token whose scale is above 2^96 or subnormal: a product of two of them may be
+ * beyond fp32 where all three are not), and rounded once more to out_type.  If a wait inside the kernel ran out (2 s), the
  * outputs it concerns are NaN. */
 mb_status mb_int8_matmul(const int8_t* a_codes, int64_t a_stride, const float* a_scales, int64_t M,
                          const int8_t* b_codes, int64_t b_stride, const float* b_scales, int64_t N,

@@ -168,9 +168,11 @@ __device__ __forceinline__ bool extreme(float sa) {
 __device__ __forceinline__ float scaled(int sum, float sa, float sb, float bias) {
   return fmaf(__fmul_rn((float)sum, sa), sb, bias);
 }
-// In 64 bits, for a tile with an extreme scale.
-__device__ __noinline__ float scaled_wide(int sum, float sa, float sb, float bias) {
-  return __double2float_rn(fma((double)sum * (double)sa, (double)sb, (double)bias));
+// In 64 bits where the token's scale is extreme: of a tile that has such a token
+// (the others' results do not depend on it).
+__device__ __noinline__ float scaled_any(int sum, float sa, float sb, float bias) {
+  return extreme(sa) ? __double2float_rn(fma((double)sum * (double)sa, (double)sb, (double)bias))
+                     : scaled(sum, sa, sb, bias);
 }
 
 // A channel's (a lane's) sums with 16 tokens, `count` of which exist: sa in
@@ -182,7 +184,7 @@ __device__ __forceinline__ void put16(const uint32_t (&v)[16], const float* sa, 
   if (wide) {
 #pragma unroll
     for (int i = 0; i < 16; ++i)
-      if (i < count) o[i * stride] = from_float<Y>(scaled_wide((int)v[i], sa[i], sb, bias));
+      if (i < count) o[i * stride] = from_float<Y>(scaled_any((int)v[i], sa[i], sb, bias));
   } else if (count >= 16) {
 #pragma unroll
     for (int i = 0; i < 16; i += 4) {
@@ -324,7 +326,8 @@ __global__ void __launch_bounds__(kThreads, 1)
         __syncwarp();
         tmem_ld16(lanes + c, v);
         if (live)
-          put16<Y>(v, a_scale + c, sb, bias, wide, o + c * e.out_stride, e.out_stride, columns - c);
+          put16<Y>(v, a_scale + c, sb, bias, wide, o + c * e.out_stride, e.out_stride,
+                   columns - c);
       }
     }
   } else {
@@ -361,7 +364,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         const float4 sa = *reinterpret_cast<const float4*>(a_scale + c);
         Y* to = o + c * e.out_stride;
         const auto y = [&](int x, float s) {
-          return from_float<Y>(wide ? scaled_wide(x, s, sb, bias) : scaled(x, s, sb, bias));
+          return from_float<Y>(wide ? scaled_any(x, s, sb, bias) : scaled(x, s, sb, bias));
         };
         to[0] = y(sum.x, sa.x);
         if (c + 1 < columns) to[e.out_stride] = y(sum.y, sa.y);
@@ -578,7 +581,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
         __syncwarp();
         tmem_ld16(at + c, v);
         if (live)
-          put16<Y>(v, a_scale[buf] + c, sb, bias, wide, o + c * e.out_stride, e.out_stride, columns - c);
+          put16<Y>(v, a_scale[buf] + c, sb, bias, wide, o + c * e.out_stride, e.out_stride,
+                   columns - c);
       }
       asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
       __syncwarp();

@@ -390,3 +390,6 @@ def test_product_of_very_large_and_very_small_tokens(M, N, dtype):
         assert np.all(np.abs(got - want)[fits] <= tol[fits])
         beyond = np.abs(want) - tol > f.max * (1 + f.eps / 2)
         assert np.all(np.isinf(got[beyond])) and not np.isnan(got).any()
+        for rest in ([1], [0, 1], [1, 2]):  # a token's results are its own
+            some = [i for i in range(M) if i % 3 in rest]
+            assert torch.equal(mb.int8_matmul(x[some], w), y[some])
