@@ -57,11 +57,11 @@
 //
 // The units of all sequences and heads are dealt out evenly to the resident
 // CTAs (two or three an SM), whatever the lengths: a CTA's share may begin and
-// end inside a sequence, and pass sequences without tokens.  Those parts (maximum, sum, unnormalised output) go to the workspace, two a
-// CTA at most, and a second kernel joins them in the order of the tokens, so
-// the result does not depend on the CTAs' timing.  Where the table holds few
-// tokens a sequence, a CTA takes a whole sequence's head instead and nothing
-// is joined.
+// end inside a sequence, and pass sequences without tokens.  Those parts (maximum,
+// sum, unnormalised output) go to the workspace, two a CTA at most, and a second
+// kernel joins them in the order of the tokens, so the result does not depend on
+// the CTAs' timing.  Where the table holds few tokens a sequence, a CTA takes a
+// whole sequence's head instead and nothing is joined.
 //
 // Measured: 8 bits stream at 88 % of the copy rate (one sequence of 65536 tokens
 // and 32 heads: 97 us for 86 us of bytes; 360 instructions a warp for 16 tokens

@@ -65,7 +65,8 @@ def test_no_module_at_all(tmp_path):
         if f.endswith(".py") or f == "libmemboost_b200.so":
             os.symlink(os.path.join(PKG, f), there / f)
     r = subprocess.run([sys.executable, "-c", "import memboost_b200"], cwd=str(tmp_path),
-                       capture_output=True, text=True, env=dict(os.environ, PYTHONPATH=str(tmp_path)))
+                       capture_output=True, text=True,
+                       env=dict(os.environ, PYTHONPATH=str(tmp_path)))
     assert r.returncode != 0 and "build it with" in r.stderr
 
 
